@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define FAROPE_ABI_VERSION 6
+#define FAROPE_ABI_VERSION 7
 
 typedef enum farope_dtype {
   FAROPE_F32 = 0,
@@ -50,7 +50,8 @@ typedef enum farope_status {
   FAROPE_ERR_SHAPE = 6,       /* batch/heads not positive or sizes overflow */
   FAROPE_ERR_LAUNCH = 7,      /* the HIP runtime rejected a kernel launch */
   FAROPE_ERR_ALIGN = 8,       /* a pointer is not aligned to its element size */
-  FAROPE_ERR_SCRATCH = 9      /* workspace elems > FAROPE_NOALLOC_MAX_ROWS (noalloc entry) */
+  FAROPE_ERR_SCRATCH = 9      /* workspace elems > FAROPE_NOALLOC_MAX_ROWS (noalloc entry), or a
+                                 workspace smaller than the call's */
 } farope_status;
 
 /* Rows (batch * heads * seq_len) the static workspace of
@@ -274,6 +275,106 @@ int farope_attn_bwd_noalloc(const farope_attn_desc* desc,
  * item.
  */
 int farope_tile_config(const farope_attn_desc* desc, int32_t which, int32_t out[4]);
+
+/*
+ * Attention over packed sequences and over a paged cache.  No counterpart in the
+ * reference, whose calls are dense [B, H, N, D] planes; rotation, scaling and
+ * softmax are those of the entry points above.
+ *
+ * tokens T of seqs B sequences lie behind each other: q, dout [T, heads, D] and
+ * k, v [T, kv_heads, D] with any element strides (stride[0..2] = t, h, d);
+ * outputs are contiguous.  heads is a multiple of kv_heads, and query head h
+ * reads key head h / (heads / kv_heads).  head_dim is 32, 64, 128 or 256; dtype
+ * is the tensors' and the products' type (fp32 tensors are computed in fp32).
+ *
+ * cu [B + 1] (device memory, int32): the sequences' first tokens in ascending
+ * order from 0 on, then the end of the last one.  Its values are read on the
+ * device alone, clamped to [0, T]; tokens from cu[B] on belong to no sequence: O and the
+ * gradients of their rows are zeros.  causal: token i sees tokens j <= i.
+ *
+ * cosp, sinp: contiguous fp32 tables [n_pos, D/2], 16-byte aligned, read as they are
+ * (not packed).  Token i of a sequence takes row i - has_cls, or positions[t] where
+ * positions (device memory, int32) is not NULL; a row below 0 is not rotated (the
+ * class token), one past the table takes its last row.
+ */
+typedef struct farope_seq_desc {
+  int32_t tokens;         /* T (0: nothing is done) */
+  int32_t seqs;           /* B >= 1 */
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t n_pos;
+  int32_t has_cls;
+  int32_t causal;
+  int32_t dtype;          /* farope_dtype */
+  float softmax_scale;
+} farope_seq_desc;
+
+/* 1 if the rows of a [T, heads, D] input can be streamed as they lie: contiguous
+ * channels, 16-byte aligned rows, a row stride of 0 or more, less than 2 GiB from the
+ * first row to the last.  Of V (and dout in the backward) the workspace holds a copy
+ * otherwise; every other input may have any strides. */
+int farope_seq_streams(const farope_seq_desc* desc, const void* x, const int64_t stride[3]);
+
+/* fp32 elements of the workspace of farope_seq_fwd (backward = 0) and farope_seq_bwd (1).
+ * v_streams, dout_streams: farope_seq_streams of V and dout (dout: backward only).
+ * The rotated K rows; the copy of V if it is kept; in the backward also the rotated
+ * Q rows, two fp32 values per query row and head, and the copy of dout if it is kept.
+ * 0 on an invalid descriptor. */
+size_t farope_seq_workspace_elems(const farope_seq_desc* desc, int32_t backward, int32_t v_streams, int32_t dout_streams);
+
+/* O [T, heads, D] and lse [heads, T] (fp32, natural log-sum-exp of the scaled logits).
+ * ws: ws_elems fp32 elements, 16-byte aligned; FAROPE_ERR_SCRATCH if they are too few. */
+int farope_seq_fwd(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3],
+                   const void* k, const int64_t k_stride[3], const void* v, const int64_t v_stride[3],
+                   const float* cosp, const float* sinp, const int32_t* positions, const int32_t* cu,
+                   void* o, float* lse, float* ws, size_t ws_elems, void* stream);
+
+/* dq [T, heads, D], dk and dv [T, kv_heads, D] from the forward's inputs, o and lse. */
+int farope_seq_bwd(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3],
+                   const void* k, const int64_t k_stride[3], const void* v, const int64_t v_stride[3],
+                   const void* o, const void* dout, const int64_t dout_stride[3], const float* lse,
+                   const float* cosp, const float* sinp, const int32_t* positions, const int32_t* cu,
+                   void* dq, void* dk, void* dv, float* ws, size_t ws_elems, void* stream);
+
+/*
+ * Paged cache of keys (rotated) and values: row r of page g, key head h, channel d at
+ * g*stride[0] + r*stride[1] + h*stride[2] + d elements (channels contiguous; base and
+ * strides 16-byte aligned).  Position i of sequence b is row i % page_rows of page
+ * page_table[b * table_stride + i / page_rows].  page_table and lengths [B] (int32)
+ * are read on the device alone.  A position past the max_pages entries of its
+ * sequence, or on a page number outside [0, pages), is not in the cache: it is not
+ * written, and attention leaves it out.  A length below 0 counts as 0.
+ */
+typedef struct farope_cache_desc {
+  void* k;
+  void* v;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int32_t pages;
+  int32_t page_rows;
+  int32_t max_pages;
+  int64_t table_stride;
+} farope_cache_desc;
+
+/* Writes the rotated k and v [T, kv_heads, D] of new tokens behind the lengths[b] rows that
+ * each sequence's cache holds (lengths is not changed).  cu NULL: token t is the next
+ * one of sequence t (tokens = seqs).  Rows go by position, lengths[b] + j - has_cls, or
+ * by positions [T].  A sequence of negative length is left out.  No two tokens of a call may share a row.  desc: heads, causal and
+ * softmax_scale are not read. */
+int farope_cache_append(const farope_seq_desc* desc, const void* k, const int64_t k_stride[3],
+                        const void* v, const int64_t v_stride[3], const float* cosp, const float* sinp,
+                        const int32_t* positions, const farope_cache_desc* cache, const int32_t* page_table,
+                        const int32_t* lengths, const int32_t* cu, void* stream);
+
+/* O [B, heads, D] of one query per sequence (tokens = seqs) over the lengths[b] rows of its
+ * cache, the last of which is its own: q is rotated by row lengths[b] - 1 - has_cls, or by
+ * positions [B].  A sequence with no rows in the cache has O = 0.  ws as above. */
+size_t farope_decode_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache);
+int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3], const float* cosp,
+                  const float* sinp, const int32_t* positions, const farope_cache_desc* cache,
+                  const int32_t* page_table, const int32_t* lengths, void* o, float* ws, size_t ws_elems,
+                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,311 @@
+"""GPU: attention over packed sequences (sdpa_rope_varlen) against 64 bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import seq_ref
+from tests._report import LINES
+from triton_fused_rope_flash_attn_amd import CosSinTable, sdpa_rope_varlen, sdpa_triton_fa_rope
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def starts(lens, device=DEV):
+    return torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=device)
+
+
+def inputs(T, H, Hkv, D, dtype, seed=0, views=False):
+    g = torch.Generator().manual_seed(seed)
+    if views:   # thirds of one projection's output
+        q, k, v = torch.randn(T, H + 2 * Hkv, D, generator=g).to(dtype).to(DEV).split([H, Hkv, Hkv], dim=1)
+    else:
+        q, k, v = (torch.randn(T, n, D, generator=g).to(dtype).to(DEV) for n in (H, Hkv, Hkv))
+    return q, k, v, torch.randn(T, H, D, generator=g).to(dtype).to(DEV)
+
+
+def grads(q, k, v, do, table, cu, **kw):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = sdpa_rope_varlen(*leaves, table, cu, **kw)
+    return dict(zip(("o", "dq", "dk", "dv"), (o.detach(), *torch.autograd.grad(o, leaves, do))))
+
+
+def compare(tag, got, ref, dtype):
+    worst = {n: seq_ref.check(n, got[n], ref, dtype) for n in got}
+    LINES.append(f"[varlen {tag}] " + " ".join(f"{n} {e:.2e}" for n, e in worst.items()))
+
+
+SHORT = [1, 0, 5, 0, 33]
+EDGES = [63, 64, 1, 65, 127, 128, 129]
+LONG = [197, 3, 577, 300]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,D,H,Hkv,lens,views", [
+    (BF16, 64, 4, 4, [1], False),
+    (BF16, 64, 6, 2, SHORT, True),
+    (BF16, 64, 3, 1, EDGES, False),
+    (BF16, 128, 4, 2, EDGES, True),
+    (BF16, 128, 8, 2, LONG, True),
+    (BF16, 32, 4, 1, EDGES, True),
+    (BF16, 256, 2, 1, EDGES, False),
+    (F16, 64, 12, 12, LONG, True),
+    (F16, 128, 7, 1, SHORT, False),
+    (F16, 32, 2, 2, LONG, False),
+    (F16, 256, 3, 3, SHORT, True),
+    (F32, 32, 2, 1, EDGES, False),
+    (F32, 64, 4, 2, EDGES, True),
+    (F32, 128, 2, 2, LONG, False),
+    (F32, 256, 2, 1, SHORT, True),
+])
+def test_varlen(dtype, D, H, Hkv, lens, views, causal):
+    T = sum(lens)
+    q, k, v, do = inputs(T, H, Hkv, D, dtype, seed=D + H, views=views)
+    table = seq_ref.Table(max(lens), D, DEV)
+    ref = seq_ref.varlen(q, k, v, do, table, starts(lens), causal, True)
+    got = grads(q, k, v, do, table, starts(lens), causal=causal)
+    compare(f"{dtype} D{D} H{H}/{Hkv} {lens} causal={causal}", got, ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_tokens_behind_the_last_sequence_are_zeros(dtype):
+    """... and what they hold, and what other sequences hold, reaches nothing."""
+    lens, T, D = [70, 0, 130], 333, 64
+    q, k, v, do = inputs(T, 4, 2, D, dtype)
+    table = seq_ref.Table(130, D, DEV)
+    ref = seq_ref.varlen(q[:200], k[:200], v[:200], do[:200], table, starts(lens), True, False)
+    for t in (q, k, v, do):
+        t[200:] = float("nan")
+    got = grads(q, k, v, do, table, starts(lens), has_cls=False)
+    for t in got.values():
+        assert (t[200:] == 0).all()
+    compare(f"behind the last {dtype}", {n: t[:200] for n, t in got.items()}, ref, dtype)
+    for t in (q, k, v, do):
+        t[:70] = float("inf")
+    again = grads(q, k, v, do, table, starts(lens), has_cls=False)
+    for n in got:
+        assert torch.equal(got[n][70:], again[n][70:]), n
+
+
+def test_all_sequences_empty():
+    q, k, v, do = inputs(9, 2, 2, 64, BF16)
+    got = grads(q, k, v, do, seq_ref.Table(4, 64, DEV), starts([0, 0]))
+    assert all((t == 0).all() for t in got.values())
+
+
+def test_no_tokens():
+    q, k, v, do = inputs(0, 2, 2, 64, BF16)
+    got = grads(q, k, v, do, seq_ref.Table(4, 64, DEV), starts([0]))
+    assert all(t.numel() == 0 for t in got.values())
+
+
+def _strided(kind, T, H, Hkv, D, dtype):
+    q, k, v, do = inputs(T, H, Hkv, D, dtype, seed=3)
+    if kind == "heads first":
+        return [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v, do)]
+    if kind == "channels apart":
+        return [torch.stack([t, t], dim=-1)[..., 1] for t in (q, k, v, do)]
+    if kind == "odd offset":   # rows not 16-byte aligned
+        flat = [torch.cat([t.new_zeros(1), t.reshape(-1)]) for t in (q, k, v, do)]
+        return [f[1:].view(t.shape) for f, t in zip(flat, (q, k, v, do))]
+    if kind == "one row":   # every token has the same k, v and dO row
+        return [q, *(t[:1].expand(T, -1, -1) for t in (k, v, do))]
+    if kind == "one head":
+        return [q[:, :1].expand(-1, H, -1), k[:, :1].expand(-1, Hkv, -1), v[:, :1].expand(-1, Hkv, -1), do[:, :1].expand(-1, H, -1)]
+    raise AssertionError(kind)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (F32, 64)])
+@pytest.mark.parametrize("kind", ["heads first", "channels apart", "odd offset", "one row", "one head"])
+def test_strides(kind, dtype, D):
+    lens = [130, 1, 77]
+    q, k, v, do = _strided(kind, sum(lens), 4, 2, D, dtype)
+    table = seq_ref.Table(130, D, DEV)
+    ref = seq_ref.varlen(q, k, v, do, table, starts(lens), True, True)
+    got = grads(q, k, v, do, table, starts(lens))
+    names = got if kind != "one row" else ("o", "dv")   # (equal keys: P's rows are exact, dQ and dK cancel to rounding)
+    compare(f"{kind} {dtype}", {n: got[n] for n in names}, ref, dtype)
+
+
+def test_gradient_of_a_sum():
+    """dO of o.sum(): one value expanded over the tensor."""
+    lens, D = [100, 61], 64
+    q, k, v, _ = inputs(161, 4, 2, D, BF16)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    table = seq_ref.Table(100, D, DEV)
+    sdpa_rope_varlen(*leaves, table, starts(lens)).sum().backward()
+    ref = seq_ref.varlen(q, k, v, torch.ones_like(q), table, starts(lens), True, True)
+    compare("sum", dict(dq=leaves[0].grad, dk=leaves[1].grad, dv=leaves[2].grad), ref, BF16)
+
+
+def test_positions_and_a_short_table():
+    lens, D = [50, 20], 64
+    q, k, v, do = inputs(70, 2, 1, D, F16)
+    table = seq_ref.Table(31, D, DEV)
+    pos = torch.randint(-2, 40, (70,), generator=torch.Generator().manual_seed(1), dtype=torch.int32).to(DEV)
+    ref = seq_ref.varlen(q, k, v, do, table, starts(lens), True, True, positions=pos)
+    compare("positions", grads(q, k, v, do, table, starts(lens), positions=pos), ref, F16)
+    ref = seq_ref.varlen(q, k, v, do, table, starts(lens), True, False)   # (rows 31 .. 49 take row 30)
+    compare("short table", grads(q, k, v, do, table, starts(lens), has_cls=False), ref, F16)
+
+
+@pytest.mark.parametrize("value", [3e4, -3e4])
+def test_large_logits(value):
+    """One key that takes every later row's whole softmax, and one that none looks at."""
+    lens, D = [140], 64
+    q, k, v, do = inputs(140, 2, 2, D, F32)
+    q[:, :, 0] = 8.0
+    k[3, :, 0] = value
+    table = seq_ref.Table(1, D, DEV)   # (row 0 turns by nothing)
+    ref = seq_ref.varlen(q, k, v, do, table, starts(lens), True, True)
+    got = grads(q, k, v, do, table, starts(lens))
+    # The backward takes P = exp2(s - LSE) with both at 4.3e4 (log2 units), where half a step of fp32
+    # is 2^-9: K's scaling, the product, its sum, LSE's two terms, its two conversions and the
+    # difference are 8 roundings, of 2^-9 ln 2 of P each.
+    assert seq_ref.rel(got["o"], ref["o"]) <= 32 * 2.0 ** -24
+    assert seq_ref.rel(got["dv"], ref["dv"]) <= 8 * 2.0 ** -9 * 0.6932
+    assert all(torch.isfinite(t).all() for t in got.values())
+
+
+def test_equals_the_dense_op():
+    """Not causal, equal lengths, one key head per query head: the dense op's values."""
+    B, H, side, D = 3, 4, 9, 64
+    N = side * side + 1
+    table = CosSinTable(100.0, side, D, device=DEV)
+    q, k, v, do = inputs(B * N, H, H, D, BF16)
+    dense = [t.view(B, N, H, D).transpose(1, 2).detach().requires_grad_() for t in (q, k, v)]
+    o = sdpa_triton_fa_rope(*dense, table)
+    want = [o.detach(), *torch.autograd.grad(o, dense, do.view(B, N, H, D).transpose(1, 2))]
+    got = grads(q, k, v, do, table, starts([N] * B), causal=False)
+    for (n, t), w in zip(got.items(), want):   # (each within its bound of the exact value)
+        w = w.transpose(1, 2).reshape(t.shape)
+        assert seq_ref.rel(t, w.double().cpu()) <= 2 * seq_ref.ROUNDINGS[n] * seq_ref.U[BF16], n
+
+
+def test_autocast():
+    lens, D = [90, 40], 64
+    q, k, v, do = inputs(130, 2, 1, D, F32)
+    table = seq_ref.Table(90, D, DEV)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    with torch.autocast("cuda", torch.bfloat16):
+        o = sdpa_rope_varlen(*leaves, table, starts(lens))
+    assert o.dtype == F32
+    g = torch.autograd.grad(o, leaves, do)
+    assert all(x.dtype == F32 for x in g)
+    # (the casts of q, k, v and dO are roundings too)
+    ref = seq_ref.varlen(*(t.detach().bfloat16() for t in (q, k, v)), do.bfloat16(), table, starts(lens), True, True)
+    compare("autocast", dict(zip(("o", "dq", "dk", "dv"), (o, *g))), ref, BF16)
+
+
+def test_gradient_against_differences():
+    """Central differences of the fp32 forward along random directions."""
+    lens, D, eps = [40, 25], 32, 1e-2
+    q, k, v, do = inputs(65, 4, 2, D, F32)
+    table = seq_ref.Table(40, D, DEV)
+    got = grads(q, k, v, do, table, starts(lens))
+    g = torch.Generator().manual_seed(5)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        x = [q, k, v]
+        d = torch.randn(x[i].shape, generator=g).to(DEV)
+        up, down = ([t + s * eps * d if j == i else t for j, t in enumerate(x)] for s in (1, -1))
+        f = [(sdpa_rope_varlen(*y, table, starts(lens)).double() * do.double()).sum().item() for y in (up, down)]
+        slope, want = (f[0] - f[1]) / (2 * eps), (got[name].double() * d.double()).sum().item()
+        # third derivatives of order 1 per term: eps^2 of the gradient's norm times the direction's
+        scale = got[name].double().norm().item() * d.double().norm().item()
+        assert abs(slope - want) <= 4 * eps ** 2 * scale + 1e-5 * scale, (name, slope, want)
+
+
+def test_repeats_are_equal_bit_for_bit():
+    lens, D = [257, 64, 100], 128
+    q, k, v, do = inputs(421, 8, 2, D, BF16, views=True)
+    table = seq_ref.Table(257, D, DEV)
+    first = grads(q, k, v, do, table, starts(lens))
+    for _ in range(3):
+        again = grads(q, k, v, do, table, starts(lens))
+        assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+def test_captured_and_replayed_with_other_lengths():
+    """One graph of forward and gradients; inputs and sequence starts change between replays."""
+    T, D = 300, 64
+    q, k, v, do = inputs(T, 4, 2, D, BF16)
+    table = seq_ref.Table(T, D, DEV)
+    cu = starts([100, 150, 20])
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    gdo = do.clone()
+
+    def step():
+        o = sdpa_rope_varlen(*leaves, table, cu)
+        return (o.detach(), *torch.autograd.grad(o, leaves, gdo))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed, lens in enumerate(([100, 150, 20], [0, 300, 0], [1, 1, 1], [130, 0, 170])):
+        x = inputs(T, 4, 2, D, BF16, seed=seed + 20)
+        with torch.no_grad():
+            for dst, src in zip((*leaves, gdo), x):
+                dst.copy_(src)
+            cu.copy_(starts(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = grads(*x, table, starts(lens))
+        for g, (n, w) in zip(out, want.items()):
+            assert torch.equal(g, w), (n, lens)
+
+
+def test_two_streams_at_once():
+    q, k, v, do = inputs(500, 4, 2, 64, BF16)
+    table = seq_ref.Table(300, 64, DEV)
+    cu = starts([300, 200])
+    want = grads(q, k, v, do, table, cu)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(grads(q, k, v, do, table, cu))
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(g[n], want[n]) for n in want)
+
+
+def test_starts_out_of_range_stay_inside():
+    """Values of cu_seqlens are clamped to the tensors: no error, nothing outside is touched."""
+    q, k, v, do = inputs(100, 2, 1, 64, BF16)
+    table = seq_ref.Table(100, 64, DEV)
+    want = grads(q, k, v, do, table, starts([60, 40]))
+    cu = torch.tensor([-5, 60, 1 << 30], dtype=torch.int32, device=DEV)
+    got = grads(q, k, v, do, table, cu)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+def test_compiles_fullgraph():
+    lens, D = [90, 40], 64
+    q, k, v, do = inputs(130, 2, 1, D, BF16)
+    table = CosSinTable(100.0, 10, D, device=DEV)
+    fn = torch.compile(lambda a, b, c, cu: sdpa_rope_varlen(a, b, c, table, cu) * 2, fullgraph=True, backend="aot_eager")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = fn(*leaves, starts(lens))
+    g = torch.autograd.grad(o, leaves, do)
+    want = grads(q, k, v, do * 2, table, starts(lens))
+    assert torch.equal(o, want["o"] * 2)
+    assert all(torch.equal(a, want[n]) for a, n in zip(g, ("dq", "dk", "dv")))
+
+
+def test_second_derivative_refused():
+    q, k, v, do = inputs(20, 1, 1, 64, F32)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = sdpa_rope_varlen(*leaves, seq_ref.Table(20, 64, DEV), starts([20]))
+    (dq,) = torch.autograd.grad(o, leaves[:1], do, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable again"):
+        dq.sum().backward()

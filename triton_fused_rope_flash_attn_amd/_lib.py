@@ -42,6 +42,13 @@ EXPORTS = (
     "farope_attn_bwd",
     "farope_attn_bwd_noalloc",
     "farope_tile_config",
+    "farope_seq_streams",
+    "farope_seq_workspace_elems",
+    "farope_seq_fwd",
+    "farope_seq_bwd",
+    "farope_cache_append",
+    "farope_decode_workspace_elems",
+    "farope_decode",
 )
 
 
@@ -59,6 +66,25 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class SeqDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("tokens", "seqs", "heads", "kv_heads", "head_dim", "n_pos", "has_cls", "causal",
+                                              "dtype")] + [("softmax_scale", ctypes.c_float)]
+
+
+class CacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("pages", ctypes.c_int32),
+        ("page_rows", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+    ]
+
+
+Stride3 = ctypes.c_int64 * 3
 Stride4 = ctypes.c_int64 * 4
 _P = ctypes.c_void_p
 _S = ctypes.POINTER(ctypes.c_int64)
@@ -66,6 +92,8 @@ _D = ctypes.POINTER(AttnDesc)
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _Z = ctypes.c_size_t
+_SD = ctypes.POINTER(SeqDesc)
+_CD = ctypes.POINTER(CacheDesc)
 
 _SIGNATURES = {
     "farope_abi_version": (ctypes.c_int, []),
@@ -92,6 +120,16 @@ _SIGNATURES = {
         [_D, _P, _S, _P, _S, _P, _S, _P, _S, _P, _P, _S, _P, _P, _Z, _P, _S, _P, _S, _P, _S, _P],
     ),
     "farope_tile_config": (ctypes.c_int, [_D, _I32, ctypes.POINTER(ctypes.c_int32)]),
+    "farope_seq_streams": (ctypes.c_int, [_SD, _P, _S]),
+    "farope_seq_workspace_elems": (_Z, [_SD, _I32, _I32, _I32]),
+    "farope_seq_fwd": (ctypes.c_int, [_SD, _P, _S, _P, _S, _P, _S, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "farope_seq_bwd": (
+        ctypes.c_int,
+        [_SD, _P, _S, _P, _S, _P, _S, _P, _P, _S, _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P],
+    ),
+    "farope_cache_append": (ctypes.c_int, [_SD, _P, _S, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P]),
+    "farope_decode_workspace_elems": (_Z, [_SD, _CD]),
+    "farope_decode": (ctypes.c_int, [_SD, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P, _Z, _P]),
 }
 
 _lib = None

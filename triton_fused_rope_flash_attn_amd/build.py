@@ -21,13 +21,14 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libfarope.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ["api.hip", "fwd.hip", "fwd_plane.hip", "fwd_stream.hip", "bwd.hip", "bwd_fused.hip", "bwd_keys.hip", "bwd_ds.hip", "bwd_stream.hip", "short.hip", "tail.hip"]
+SOURCES = ["api.hip", "fwd.hip", "fwd_plane.hip", "fwd_stream.hip", "bwd.hip", "bwd_fused.hip", "bwd_keys.hip", "bwd_ds.hip", "bwd_stream.hip", "short.hip", "tail.hip",
+           "seq_api.hip", "seq_prep.hip", "seq_fwd.hip", "seq_bwd.hip", "cache.hip", "decode.hip"]
 # Per-file code generation options.  fwd_plane.hip keeps its MFMA results in
 # VGPRs (they feed the softmax VALU directly) and its resident operand
 # fragments in AGPRs.
 EXTRA_FLAGS = {"fwd_plane.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 ARCH = "gfx950"
-OPS_SOURCE = "torch_ops.cpp"
+OPS_SOURCES = ["torch_ops.cpp", "torch_seq_ops.cpp"]
 OPS_PATH = os.path.join(PKG_DIR, "libfarope_torch.so")
 
 
@@ -67,21 +68,21 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"command failed ({res.returncode}): {' '.join(cmd)}\n{out}")
 
 
-def ops_commands(obj: str, out: str) -> list[list[str]]:
-    """Compile and link commands of the torch ops library (host code against
-    torch's headers; it finds libfarope.so next to itself)."""
+def ops_commands(objs: list[str], out: str) -> list[list[str]]:
+    """Compile commands, one per source, and the link command of the torch ops
+    library (host code against torch's headers; it finds libfarope.so next to itself)."""
     import torch
 
     tdir = os.path.dirname(torch.__file__)
     hipcc = _hipcc()
     rocm_inc = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(hipcc))), "include")
-    compile_ = [hipcc, "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+    compile_ = [[hipcc, "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                 f"-I{INCLUDE}", f"-I{tdir}/include", f"-I{tdir}/include/torch/csrc/api/include", f"-I{rocm_inc}",
-                "-Wno-deprecated-declarations", "-c", os.path.join(CSRC, OPS_SOURCE), "-o", obj]
-    link = [hipcc, "-shared", "-fPIC", obj, "-o", out, f"-L{PKG_DIR}", "-l:" + LIB_NAME, f"-L{tdir}/lib",
+                "-Wno-deprecated-declarations", "-c", os.path.join(CSRC, src), "-o", obj] for src, obj in zip(OPS_SOURCES, objs)]
+    link = [hipcc, "-shared", "-fPIC", *objs, "-o", out, f"-L{PKG_DIR}", "-l:" + LIB_NAME, f"-L{tdir}/lib",
             "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-Wl,-rpath,$ORIGIN"]
-    return [compile_, link]
+    return [*compile_, link]
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> str:
@@ -96,9 +97,9 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
             obj = os.path.join(tmp, src.replace(".hip", ".o"))
             objs.append(obj)
             cmds.append([hipcc, *flags, *EXTRA_FLAGS.get(src, []), "-c", os.path.join(CSRC, src), "-o", obj])
-        ops_obj, ops_out = os.path.join(tmp, "torch_ops.o"), OPS_PATH + ".tmp"
-        ops_compile, ops_link = ops_commands(ops_obj, ops_out)
-        cmds.append(ops_compile)
+        ops_objs, ops_out = [os.path.join(tmp, src.replace(".cpp", ".o")) for src in OPS_SOURCES], OPS_PATH + ".tmp"
+        *ops_compile, ops_link = ops_commands(ops_objs, ops_out)
+        cmds += ops_compile
         jobs = jobs or min(len(cmds), os.cpu_count() or 1, 16)
         with _cf.ThreadPoolExecutor(max_workers=jobs) as ex:
             for cmd, fut in zip(cmds, [ex.submit(_run, c) for c in cmds]):

@@ -652,12 +652,13 @@ const char* farope_strerror(int status) {
     case FAROPE_ERR_DTYPE: return "farope: unsupported dtype (float32, float16, bfloat16)";
     case FAROPE_ERR_TABLE:
       return "farope: RoPE table geometry does not match the call (rope_elems must be farope_rope_packed_elems(n_pos, head_dim / 2))";
-    case FAROPE_ERR_SHAPE: return "farope: batch/heads must be positive and B*H <= 2^30";
+    case FAROPE_ERR_SHAPE: return "farope: sizes must be positive (query heads a multiple of key heads), B*H <= 2^30 and within a launch's limits";
     case FAROPE_ERR_LAUNCH: return "farope: HIP kernel launch failed";
-    case FAROPE_ERR_ALIGN: return "farope: pointer not aligned to its element size";
+    case FAROPE_ERR_ALIGN: return "farope: pointer not aligned to its element size, or cache rows, tables, outputs or workspace not to 16 bytes";
     case FAROPE_ERR_SCRATCH:
       return "farope: the backward workspace (farope_attn_bwd_workspace_elems) exceeds the static workspace of farope_attn_bwd_noalloc "
-             "(FAROPE_NOALLOC_MAX_ROWS = 4194304); use farope_attn_bwd with a caller workspace";
+             "(FAROPE_NOALLOC_MAX_ROWS = 4194304); use farope_attn_bwd with a caller workspace.  Or: a caller's workspace is "
+             "smaller than the call's";
     default: return "farope: unknown status";
   }
 }

@@ -1,0 +1,249 @@
+// Packed sequences: what the kernels of attention over sequences of different
+// lengths share (seq_prep.hip, seq_fwd.hip, seq_bwd.hip, cache.hip, decode.hip).
+//
+// T tokens of B sequences lie behind each other; cu[0 .. B] are the sequences'
+// first tokens and the end of the last one.  Tokens from cu[B] on belong to no
+// sequence.  Tensors are [T, heads, D]; H query heads share Hkv key heads, query
+// head h reads key head h / (H / Hkv).
+#pragma once
+
+#include "common.h"
+#include "seq_params.h"
+
+namespace farope {
+
+// ---------------------------------------------------------------------------
+// Operand types.  16-bit tensors are computed in their own type.  fp32 tensors
+// are computed in fp32: v_mfma_f32_16x16x4_f32, whose lane group lg holds one
+// contraction index per instruction, so eight of them take the same operand
+// layout (8 values per lane) as one 16-bit instruction.
+// ---------------------------------------------------------------------------
+struct CompF32x {
+  typedef float S;
+  struct Frag { float v[8]; };
+  static __device__ __forceinline__ Frag make(const float (&x)[8]) {
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = x[e];
+    return f;
+  }
+  static __device__ __forceinline__ Frag lds(const float* p) {
+    Frag f;
+    __builtin_memcpy(&f.v[0], __builtin_assume_aligned(p, 16), 32);
+    return f;
+  }
+  static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], c, 0, 0, 0);
+    return c;
+  }
+};
+template <typename S> struct SeqComp;
+template <> struct SeqComp<bf16> { using C = Comp<DT_BF16>; };
+template <> struct SeqComp<f16> { using C = Comp<DT_F16>; };
+template <> struct SeqComp<float> { using C = CompF32x; };
+
+// ---------------------------------------------------------------------------
+// Streamed tiles: rows of D elements, unpadded, their 16-byte chunks XOR-swizzled
+// per row with period 16 (as in stream.h: 16-byte reads of 16 rows and the
+// transposed reads are free of bank conflicts).  A stage holds 64 rows, or 32
+// of more than 256 bytes; a 16-byte-per-lane load to LDS fills RPI of them.
+// ---------------------------------------------------------------------------
+template <typename S, int D> struct Tile {
+  static constexpr int ES = sizeof(S), RB = D * ES, CPR = RB / 16, EPC = 16 / ES;
+  static constexpr int SR = RB <= 256 ? 64 : 32;
+  static constexpr int RPI = CPR >= 64 ? 1 : 64 / CPR;
+  static constexpr int NI = SR / (kSeqNW * RPI);      // loads per wave and stage
+  static constexpr bool kSame = (kSeqNW * RPI) % 16 == 0;   // one swizzle pattern for all of them
+  static __device__ __forceinline__ int chunk_xor(int r) {
+    if constexpr (RB >= 256) return ((r >> 1) & 7) << 1;
+    else if constexpr (ES == 4) return ((r >> 1) & 3) << 1;   // (pairs of chunks stay adjacent)
+    else if constexpr (RB == 128) return ((((r >> 1) & 3) ^ ((r >> 2) & 2)) << 1) | ((r >> 3) & 1);
+    else return (r >> 2) & 3;
+  }
+  static __device__ __forceinline__ int at(int r, int col) {
+    return r * D + (((col / EPC) ^ chunk_xor(r)) * EPC) + (col % EPC);
+  }
+};
+
+template <typename S, int D> struct SeqStream {
+  using T = Tile<S, D>;
+  __amdgpu_buffer_rsrc_t rs;
+  unsigned voff[T::kSame ? 1 : T::NI];
+  unsigned row_b;     // bytes between rows
+  // lane offsets; the rows' bytes are row_b apart
+  __device__ __forceinline__ void lanes(int64_t stride, int wave, int lane) {
+    row_b = (unsigned)stride * T::ES;
+#pragma unroll
+    for (int g = 0; g < (T::kSame ? 1 : T::NI); ++g) {
+      const int r = (g * kSeqNW + wave) * T::RPI + lane / T::CPR;
+      voff[g] = (unsigned)r * row_b + (unsigned)(((lane % T::CPR) ^ T::chunk_xor(r)) * 16);
+    }
+  }
+  // rows [0, n) of a sequence's head; rows from n on read as zeros (unless rows overlap)
+  __device__ __forceinline__ void base(const S* p, int n) {
+    rs = make_rsrc(p, n > 0 ? (unsigned)(n - 1) * row_b + (unsigned)T::RB : 0u);
+  }
+  __device__ __forceinline__ void load(S* dst, int wave, int row0) const {
+#pragma unroll
+    for (int g = 0; g < T::NI; ++g) {
+      if constexpr (T::kSame)
+        lds_dma16(rs, dst + (wave + g * kSeqNW) * T::RPI * D, voff[0], (unsigned)(row0 + g * kSeqNW * T::RPI) * row_b);
+      else
+        lds_dma16(rs, dst + (wave + g * kSeqNW) * T::RPI * D, voff[g], (unsigned)row0 * row_b);
+    }
+  }
+};
+
+// 4 bytes per lane from a buffer straight into LDS (lane l lands at lds + 4 l).
+__device__ __forceinline__ void seq_dma4(__amdgpu_buffer_rsrc_t r, void* lds, unsigned voff, unsigned soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 4, voff, soff, 0, 0);
+}
+// 16 bytes per lane from the lane's own address straight into LDS (lane l lands at
+// lds + 16 l; lds is wave-uniform).
+__device__ __forceinline__ void seq_dma16(const void* src, void* lds) {
+  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)const_cast<void*>(src),
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+// Immediate of s_waitcnt that waits until at most n vector-memory loads are in flight.
+constexpr int vm_wait(int n) { return n > 63 ? vm_wait(63) : (n & 15) | ((n >> 4) << 14) | 0x0F70; }
+// A wave's own LDS buffers, without a workgroup barrier: its reads of a buffer have
+// returned before it is loaded again; reads come after the wait for the loads.
+__device__ __forceinline__ void wave_lds_reads_done() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+  asm volatile("" : : : "memory");
+}
+__device__ __forceinline__ void wave_lds_fence() { asm volatile("" : : : "memory"); }
+// This wave's LDS loads have landed, and so have every wave's behind the barrier.
+__device__ __forceinline__ void seq_stage_barrier() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+  lds_barrier();
+}
+
+// Operand fragments of a 32-row block of a staged tile: rows (row 16 h + lr, 8
+// channels 32 s + 8 lg) and columns (channel 16 d + lr of the rows that output
+// rows 4 lg + i of both halves are: k-slot 4 h + i is row 16 h + 4 lg + i).
+template <typename S, int D> struct FragAt {
+  using C = typename SeqComp<S>::C;
+  using T = Tile<S, D>;
+  int ao[D / 32], to[D / 16];
+  int lr, lg;
+  __device__ __forceinline__ void init(int lr_, int lg_) {
+    lr = lr_;
+    lg = lg_;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) ao[s] = T::at(lr, 32 * s + 8 * lg);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) to[d] = sizeof(S) == 2 ? T::at(4 * lg + (lr >> 2), 16 * d + 4 * (lr & 3)) : 0;
+  }
+  __device__ __forceinline__ typename C::Frag row(const S* block, int s, int h) const {
+    return C::lds(block + ao[s] + 16 * h * D);
+  }
+  __device__ __forceinline__ typename C::Frag col(const S* block, int d) const {
+    if constexpr (sizeof(S) == 2) {
+      return C::tr(block + to[d], block + to[d] + 16 * D);
+    } else {
+      typename C::Frag f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f.v[e] = block[T::at(16 * (e >> 2) + 4 * lg + (e & 3), 16 * d + lr)];
+      return f;
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Sequences and tiles.  Values of cu are clamped to [0, T], so no value of them
+// takes an access outside the tensors.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int cu_at(const int* __restrict__ cu, int i, int T) {
+  const int x = i == 0 ? 0 : cu[i];
+  return x < 0 ? 0 : x > T ? T : x;
+}
+
+struct SeqTile {
+  int seq;      // B: the tokens behind the last sequence
+  int start;    // first token of the sequence
+  int len;      // its tokens
+  int tile;     // tile of this workgroup within it (< 0: none)
+  int tiles;    // its tiles
+};
+
+// Workgroups come as slots of 2^lb rows: sequence i takes slots (cu[i] >> lb) + i on,
+// at least as many as it has tiles, so the grid needs T and B alone: no length
+// crosses to the host.  All 64 lanes search together (64 boundaries a step).
+__device__ __forceinline__ SeqTile find_tile(const int* __restrict__ cu, int B, int T, int lb, int slot, int lane) {
+  int lo = 0, n = B + 1;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, j = lane * step;
+    const bool le = j < n && (cu_at(cu, lo + (j < n ? j : 0), T) >> lb) + lo + j <= slot;
+    const int k = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(le) | 1ull);
+    lo += k * step;
+    n = n - k * step < step ? n - k * step : step;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  SeqTile t;
+  t.seq = lo;
+  t.start = cu_at(cu, lo, T);
+  const int end = lo < B ? cu_at(cu, lo + 1, T) : T;
+  t.len = end > t.start ? end - t.start : 0;
+  t.tiles = (t.len + (1 << lb) - 1) >> lb;
+  t.tile = slot - ((t.start >> lb) + lo);
+  if (t.tile >= t.tiles) t.tile = -1;
+  return t;
+}
+// Sequence of token t (B: none), for the 64 lanes of a wave whose tokens are near each other.
+__device__ __forceinline__ int find_seq(const int* __restrict__ cu, int B, int T, int first, int t, int lane) {
+  int lo = 0, n = B + 1;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, j = lane * step;
+    const bool le = j < n && cu_at(cu, lo + (j < n ? j : 0), T) <= first;
+    const int k = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(le) | 1ull);
+    lo += k * step;
+    n = n - k * step < step ? n - k * step : step;
+  }
+  while (lo < B && cu_at(cu, lo + 1, T) <= t) ++lo;
+  return lo;
+}
+
+// Table row of a token: `index` within its sequence, or the caller's position.  The
+// class token (has_cls, index 0) and negative positions are not rotated (row -1);
+// rows past the table take its last one.
+__device__ __forceinline__ int table_row(int index, int n_pos) { return index < n_pos ? index : n_pos - 1; }
+
+// cos and sin of pairs p0 .. p0 + 3 of a table row as rope_rotate8 takes them
+__device__ __forceinline__ void table_load4(const float* __restrict__ cosp, const float* __restrict__ sinp, int row, int d2,
+                                            int p0, float (&cs)[8]) {
+  if (row < 0) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) { cs[2 * p] = 1.f; cs[2 * p + 1] = 0.f; }
+    return;
+  }
+  const int64_t at = (int64_t)row * d2 + p0;
+  const f32x4 c = *reinterpret_cast<const f32x4*>(cosp + at), s = *reinterpret_cast<const f32x4*>(sinp + at);
+#pragma unroll
+  for (int p = 0; p < 4; ++p) { cs[2 * p] = c[p]; cs[2 * p + 1] = s[p]; }
+}
+
+// 8 channels of a row, as floats
+template <typename S>
+__device__ __forceinline__ void row8(const S* __restrict__ p, int64_t sd, bool vec, float (&x)[8]) { load8<S>(p, sd, vec, x); }
+
+// 8 channels to a contiguous row (16 or 32 bytes)
+template <typename S>
+__device__ __forceinline__ void put_row8(S* __restrict__ p, const float (&x)[8]) {
+  if constexpr (sizeof(S) == 4) {
+    f32x4 a, b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { a[e] = x[e]; b[e] = x[4 + e]; }
+    reinterpret_cast<f32x4*>(p)[0] = a;
+    reinterpret_cast<f32x4*>(p)[1] = b;
+  } else {
+    typedef S v8 __attribute__((ext_vector_type(8)));
+    v8 a;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = (S)x[e];
+    *reinterpret_cast<v8*>(p) = a;
+  }
+}
+
+}  // namespace farope

@@ -1,0 +1,434 @@
+// Backward of attention over packed sequences, from O, dO and the forward's LSE:
+//
+//   P = exp(s - LSE), delta_i = dO_i.O_i, dS = P * (dO V^T - delta)
+//   dV_j = sum_i P_ij dO_i             over the query heads of the key head
+//   dQ_i = R^T scale sum_j dS_ij R k_j
+//   dK_j = R^T scale sum_i dS_ij R q_i over the query heads of the key head
+//
+// Three launches:
+//   seq_prep_kernel   K-hat * c2 rows (c2 = scale * log2 e)
+//   seq_dq_kernel     query tiles: dQ; also -delta, -LSE * log2 e and the rotated Q rows
+//   seq_dkdv_kernel   key tiles: dK, dV, one pass over the group's query heads, so the
+//                     sums of shared key heads stay in registers and in one order
+// Both tile kernels stream their rows as the forward does (seq_fwd.hip).  No row of a
+// sequence reads another's: streams end at the sequence's last row.
+#include <type_traits>
+
+#include "seq.h"
+
+namespace farope {
+
+// Where a logit's -LSE2 (and dP's -delta) enters its sum: with 16-bit operands as the
+// accumulator's start; with fp32 ones at the end, so that the partial sums do not round
+// at LSE's size (dV at D 128, up to 577 tokens: off by 5.7e-7 of its norm, 1.6e-6 otherwise).
+template <typename S> __device__ __forceinline__ f32x4 first_sum(f32x4 x) { return sizeof(S) == 4 ? f32x4{0.f, 0.f, 0.f, 0.f} : x; }
+template <typename S> __device__ __forceinline__ void last_sum(f32x4& acc, f32x4 x) {
+  if constexpr (sizeof(S) == 4) acc += x;
+}
+
+// Gradient rows of a 16-row subtile: lane holds row `row`, channels 16d + 4lg + (0..3) of
+// each acc[d]; rows past the range of r drop.  turn: rotated back by the row of its token.
+template <typename S, int D>
+__device__ __forceinline__ void store_rows(const f32x4 (&acc)[D / 16], float factor, bool turn, const SeqParams& p, int table,
+                                           __amdgpu_buffer_rsrc_t r, unsigned off, int lg) {
+  f32x4 g[D / 16];
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) {
+    g[d] = acc[d] * factor;
+    if (turn && table >= 0) {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+      const int64_t at = (int64_t)table * (D / 2) + 8 * d + 2 * lg;
+      const f2 c = *reinterpret_cast<const f2*>(p.cosp + at), s = *reinterpret_cast<const f2*>(p.sinp + at);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float e = g[d][2 * k], o = g[d][2 * k + 1];
+        g[d][2 * k] = e * c[k] + o * s[k];
+        g[d][2 * k + 1] = o * c[k] - e * s[k];
+      }
+    }
+  }
+  if constexpr (sizeof(S) == 4) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) buf_store16(__builtin_bit_cast(u32x4, g[d]), r, off + (unsigned)(16 * d + 4 * lg) * 4u, 0u);
+  } else {
+    // lane groups lg and lg^1 trade halves so that each lane stores 8 consecutive channels
+#pragma unroll
+    for (int d0 = 0; d0 < D / 16; d0 += 2) {
+      u32x2 w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        typedef S s4 __attribute__((ext_vector_type(4)));
+        s4 a;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = (S)g[d0 + j][e];
+        __builtin_memcpy(&w[j], &a, 8);
+      }
+      u32x4 x;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const auto y = __builtin_amdgcn_permlane16_swap(w[0][k], w[1][k], false, false);
+        x[k] = y[0];
+        x[2 + k] = y[1];
+      }
+      buf_store16(x, r, off + (unsigned)(16 * (d0 + (lg & 1)) + 4 * (lg & 2)) * 2u, 0u);
+    }
+  }
+}
+
+// rows of zeros: tokens behind the last sequence
+template <typename S, int D>
+__device__ __forceinline__ void zero_rows(S* base, int64_t stride, int rows, int tid) {
+  for (int r = tid / (D / 8); r < rows; r += kSeqThreads / (D / 8)) {
+    const float z[8] = {};
+    put_row8<S>(base + (int64_t)r * stride + 8 * (tid % (D / 8)), z);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dQ of 64 QT query rows of one head.  S^T = K-hat Q-hat^T and dP^T = V dO^T per
+// 32-key block; their output rows are the k-slots of dQ-hat^T += K-hat^T dS^T.
+// ---------------------------------------------------------------------------
+template <typename S, int D, int QT>
+__global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 ? 2 : 3)
+seq_dq_kernel(const SeqParams p) {
+  using C = typename SeqComp<S>::C;
+  using Frag = typename C::Frag;
+  using T = Tile<S, D>;
+  constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, LB = QT == 2 ? 7 : 6;
+  __shared__ __attribute__((aligned(16))) S sK0[SR * D], sK1[SR * D], sV0[SR * D], sV1[SR * D];
+
+  const int tid = thread_id();
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  const int slot = p.slots - 1 - block_id() / p.H, hx = block_id() % p.H;   // (as in the forward)
+  const int kvh = hx % p.Hkv, head = kvh * (p.H / p.Hkv) + hx / p.Hkv;
+  const SeqTile tl = find_tile(p.cu, p.B, p.T, LB, slot, lane);
+  if (tl.tile < 0) return;
+  const int q0 = tl.tile << LB, rows = tl.len - q0 < (1 << LB) ? tl.len - q0 : 1 << LB;
+  const int64_t tok0 = tl.start + q0;
+  S* const dqb = static_cast<S*>(p.dq) + (tok0 * p.H + head) * D;
+  if (tl.seq == p.B) {
+    zero_rows<S, D>(dqb, (int64_t)p.H * D, rows, tid);
+    return;
+  }
+
+  SeqStream<S, D> srcK, srcV;
+  srcK.lanes(D, wave, lane);
+  srcK.base(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
+  if (p.vcopy) {
+    srcV.lanes(D, wave, lane);
+    srcV.base(static_cast<const S*>(p.vcopy) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
+  } else {
+    srcV.lanes(p.sv[0], wave, lane);
+    srcV.base(static_cast<const S*>(p.v) + tl.start * p.sv[0] + kvh * p.sv[1], tl.len);
+  }
+  srcK.load(sK0, wave, 0);
+  srcV.load(sV0, wave, 0);
+
+  const int row0 = wave * 16 * QT + lr;   // of the tile; subtile t: + 16 t
+  const int64_t hrow = (int64_t)head * p.T + tok0;
+  Frag qf[QT][KS], gf[QT][KS];
+  f32x4 nl4[QT], nd4[QT];
+  int seen[QT], trow[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t, rc = r < rows ? r : rows - 1;
+    const int64_t tok = tok0 + rc;
+    const S* qp = static_cast<const S*>(p.q) + tok * p.sq[0] + head * p.sq[1];
+    const S* gp = static_cast<const S*>(p.dout) + tok * p.sdo[0] + head * p.sdo[1];
+    const S* op = static_cast<const S*>(p.o) + (tok * p.H + head) * D;
+    seen[t] = p.causal ? q0 + rc + 1 : tl.len;
+    trow[t] = table_row(p.positions ? p.positions[tok] : q0 + rc - p.has_cls, p.n_pos);
+    float ds = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int c = 32 * s + 8 * lg;
+      float x[8], g[8], o[8], cs[8];
+      row8<S>(qp + c * p.sq[2], p.sq[2], p.vec_q, x);
+      row8<S>(gp + c * p.sdo[2], p.sdo[2], p.vec_do, g);
+      row8<S>(op + c, 1, true, o);
+      table_load4(p.cosp, p.sinp, trow[t], D / 2, c / 2, cs);
+      rope_rotate8(x, cs);
+      qf[t][s] = C::make(x);
+      gf[t][s] = C::make(g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ds += g[e] * o[e];
+      if (r < rows) {
+        put_row8<S>(static_cast<S*>(p.qhat) + (hrow + r) * D + c, x);
+        if (p.gcopy) put_row8<S>(static_cast<S*>(p.gcopy) + (hrow + r) * D + c, g);
+      }
+    }
+    const float nd = -group4_sum(ds), nl = -p.lse[hrow + rc] * kLog2e;
+    if (r < rows && lg == 0) {
+      p.nl[hrow + r] = nl;
+      p.nd[hrow + r] = nd;
+    }
+    nl4[t] = f32x4{nl, nl, nl, nl};
+    nd4[t] = f32x4{nd, nd, nd, nd};
+  }
+  const int w0 = q0 + wave * 16 * QT;   // the wave's first row (uniform)
+  const bool active = w0 < tl.len;
+  const int lo = p.causal ? w0 + 1 : tl.len;
+  const int hi = p.causal && w0 + 16 * QT < tl.len ? w0 + 16 * QT : tl.len;
+  const int last = p.causal && q0 + (1 << LB) < tl.len ? q0 + (1 << LB) : tl.len;
+  const int ns = (last + SR - 1) / SR;
+
+  f32x4 acc[QT][DT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  FragAt<S, D> at;
+  at.init(lr, lg);
+
+  auto block = [&](bool tail, int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
+    f32x4 sacc[QT][2], pacc[QT][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Frag a = at.row(k, s, h), b = at.row(v, s, h);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          sacc[t][h] = C::mma(a, qf[t][s], s == 0 ? first_sum<S>(nl4[t]) : sacc[t][h]);
+          pacc[t][h] = C::mma(b, gf[t][s], s == 0 ? first_sum<S>(nd4[t]) : pacc[t][h]);
+          if (s == KS - 1) {
+            last_sum<S>(sacc[t][h], nl4[t]);
+            last_sum<S>(pacc[t][h], nd4[t]);
+          }
+        }
+      }
+    Frag dsf[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const int lim = seen[t] - k0 - 4 * lg;
+      float ds[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = fast_exp2(sacc[t][h][i]) * pacc[t][h][i];
+          ds[4 * h + i] = !tail || 16 * h + i < lim ? y : 0.f;
+        }
+      dsf[t] = C::make(ds);   // (16-bit tensors: dS rounded to their type for the product)
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const Frag a = at.col(k, d);
+#pragma unroll
+      for (int t = 0; t < QT; ++t) acc[t][d] = C::mma(a, dsf[t], acc[t][d]);
+    }
+  };
+  auto stage = [&](int st, const S* __restrict__ k, const S* __restrict__ v, S* __restrict__ kn, S* __restrict__ vn)
+      __attribute__((always_inline)) {
+    seq_stage_barrier();
+    if (st + 1 < ns) {
+      srcK.load(kn, wave, (st + 1) * SR);
+      srcV.load(vn, wave, (st + 1) * SR);
+    }
+    const int k0 = st * SR;
+    if (active && k0 < hi) {
+      const bool tail = k0 + SR > lo;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        block(tail, k0 + 32 * j, k + 32 * j * D, v + 32 * j * D);
+    }
+  };
+  for (int st = 0; st < ns; st += 2) {
+    stage(st, sK0, sV0, sK1, sV1);
+    if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
+  }
+
+  const unsigned row_b = (unsigned)(p.H * D * (int)sizeof(S));
+  const auto rD = make_rsrc(dqb, (unsigned)(rows - 1) * row_b + T::RB);
+#pragma unroll
+  for (int t = 0; t < QT; ++t)   // (K-hat carries c2)
+    store_rows<S, D>(acc[t], p.scale / p.c2, true, p, trow[t], rD, (unsigned)(row0 + 16 * t) * row_b, lg);
+}
+
+// ---------------------------------------------------------------------------
+// dK and dV of 64 KT key rows of one key head.  Wave w owns KT 16-key subtiles:
+// its K-hat and V rows are operands in registers, dK-hat and dV accumulate in
+// registers over the stages of every query head of the group.
+// ---------------------------------------------------------------------------
+template <typename S, int D, int KT>
+__global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : 2) seq_dkdv_kernel(const SeqParams p) {
+  using C = typename SeqComp<S>::C;
+  using Frag = typename C::Frag;
+  using T = Tile<S, D>;
+  constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, LB = KT == 2 ? 7 : 6;
+  __shared__ __attribute__((aligned(16))) S sQ0[SR * D], sQ1[SR * D], sG0[SR * D], sG1[SR * D];
+  __shared__ __attribute__((aligned(16))) float sL0[64], sL1[64], sD0[64], sD1[64];
+
+  const int tid = thread_id();
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  // earlier keys (seen by more queries) come first in each sequence
+  const int slot = block_id() / p.Hkv, kvh = block_id() % p.Hkv, group = p.H / p.Hkv;
+  const SeqTile tl = find_tile(p.cu, p.B, p.T, LB, slot, lane);
+  if (tl.tile < 0) return;
+  const int k0 = tl.tile << LB, rows = tl.len - k0 < (1 << LB) ? tl.len - k0 : 1 << LB;
+  const int64_t tok0 = tl.start + k0;
+  S* const dkb = static_cast<S*>(p.dk) + (tok0 * p.Hkv + kvh) * D;
+  S* const dvb = static_cast<S*>(p.dv) + (tok0 * p.Hkv + kvh) * D;
+  if (tl.seq == p.B) {
+    zero_rows<S, D>(dkb, (int64_t)p.Hkv * D, rows, tid);
+    zero_rows<S, D>(dvb, (int64_t)p.Hkv * D, rows, tid);
+    return;
+  }
+
+  // stages of a query head: from the tile's first key on when causal
+  const int first = p.causal ? k0 / SR : 0, per = (tl.len + SR - 1) / SR - first, ns = per * group;
+  SeqStream<S, D> srcQ, srcG;
+  srcQ.lanes(D, wave, lane);
+  srcG.lanes(p.gcopy ? D : p.sdo[0], wave, lane);
+  int lh = -1, lst = per;   // the stage loaded next: head of the group, stage
+  __amdgpu_buffer_rsrc_t rStat = make_rsrc(p.nl, 0u);
+  auto load = [&](S* q, S* g, float* l, float* d) __attribute__((always_inline)) {
+    if (lst == per) {
+      lst = 0;
+      const int head = kvh * group + ++lh;
+      const int64_t hrow = (int64_t)head * p.T + tl.start;
+      srcQ.base(static_cast<const S*>(p.qhat) + hrow * D, tl.len);
+      srcG.base(p.gcopy ? static_cast<const S*>(p.gcopy) + hrow * D
+                        : static_cast<const S*>(p.dout) + tl.start * p.sdo[0] + head * p.sdo[1], tl.len);
+      rStat = make_rsrc((wave & 1 ? p.nd : p.nl) + hrow, (unsigned)tl.len * 4u);
+    }
+    const int r0 = (first + lst) * SR;
+    srcQ.load(q, wave, r0);
+    srcG.load(g, wave, r0);
+    // waves 0 and 1 also fetch the stage's -LSE2 and -delta (64 rows, of which SR count)
+    if (wave < 2) seq_dma4(rStat, wave ? d : l, (unsigned)lane * 4u, (unsigned)r0 * 4u);
+    ++lst;
+  };
+  load(sQ0, sG0, sL0, sD0);
+
+  const int row0 = wave * 16 * KT + lr;   // of the tile; subtile u: + 16 u
+  Frag kf[KT][KS], vf[KT][KS];
+  int trow[KT];
+#pragma unroll
+  for (int u = 0; u < KT; ++u) {
+    const int r = row0 + 16 * u, rc = r < rows ? r : rows - 1;
+    const int64_t tok = tok0 + rc;
+    const S* kp = static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D;
+    const S* vp = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1];
+    trow[u] = table_row(p.positions ? p.positions[tok] : k0 + rc - p.has_cls, p.n_pos);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int c = 32 * s + 8 * lg;
+      float x[8];
+      row8<S>(kp + c, 1, true, x);
+      kf[u][s] = C::make(x);
+      row8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
+      vf[u][s] = C::make(x);
+    }
+  }
+  const int w0 = k0 + wave * 16 * KT;   // the wave's first key (uniform)
+  const bool active = w0 < tl.len;
+  f32x4 dv[KT][DT], dk[KT][DT];
+#pragma unroll
+  for (int u = 0; u < KT; ++u)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dv[u][d] = dk[u][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  FragAt<S, D> at;
+  at.init(lr, lg);
+
+  // 32 queries from q0 on; tail: some of them do not exist or do not see all of the wave's keys
+  auto block = [&](bool tail, int q0, const S* __restrict__ q, const S* __restrict__ g, const float* __restrict__ l,
+                   const float* __restrict__ dl) __attribute__((always_inline)) {
+    f32x4 sacc[KT][2], pacc[KT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 nl = *reinterpret_cast<const f32x4*>(l + 16 * h + 4 * lg);
+      const f32x4 nd = *reinterpret_cast<const f32x4*>(dl + 16 * h + 4 * lg);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const Frag a = at.row(q, s, h), b = at.row(g, s, h);
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+          sacc[u][h] = C::mma(a, kf[u][s], s == 0 ? first_sum<S>(nl) : sacc[u][h]);
+          pacc[u][h] = C::mma(b, vf[u][s], s == 0 ? first_sum<S>(nd) : pacc[u][h]);
+          if (s == KS - 1) {
+            last_sum<S>(sacc[u][h], nl);
+            last_sum<S>(pacc[u][h], nd);
+          }
+        }
+      }
+    }
+    Frag pf[KT], dsf[KT];
+#pragma unroll
+    for (int u = 0; u < KT; ++u) {
+      // query q0 + 16 h + 4 lg + i exists and sees this lane's key
+      const int from = p.causal ? k0 + row0 + 16 * u - q0 - 4 * lg : -4 * lg, to = tl.len - q0 - 4 * lg;
+      float pv[8], ds[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = !tail || (16 * h + i >= from && 16 * h + i < to);
+          const float e = fast_exp2(sacc[u][h][i]);
+          pv[4 * h + i] = in ? e : 0.f;
+          ds[4 * h + i] = in ? e * pacc[u][h][i] : 0.f;
+        }
+      pf[u] = C::make(pv);    // (16-bit tensors: P and dS rounded to their type for the products)
+      dsf[u] = C::make(ds);
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const Frag ag = at.col(g, d), aq = at.col(q, d);
+#pragma unroll
+      for (int u = 0; u < KT; ++u) {
+        dv[u][d] = C::mma(ag, pf[u], dv[u][d]);
+        dk[u][d] = C::mma(aq, dsf[u], dk[u][d]);
+      }
+    }
+  };
+  int cst = 0;   // this stage within its head
+  auto stage = [&](int st, const S* __restrict__ q, const S* __restrict__ g, const float* __restrict__ l, const float* __restrict__ dl,
+                   S* __restrict__ qn, S* __restrict__ gn, float* __restrict__ ln, float* __restrict__ dn) __attribute__((always_inline)) {
+    seq_stage_barrier();
+    if (st + 1 < ns) load(qn, gn, ln, dn);
+    const int q0 = (first + cst) * SR;
+    cst = cst + 1 == per ? 0 : cst + 1;
+    if (!active || (p.causal && q0 + SR <= w0)) return;
+    const bool tail = q0 + SR > tl.len || (p.causal && q0 < w0 + 16 * KT);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      block(tail, q0 + 32 * j, q + 32 * j * D, g + 32 * j * D, l + 32 * j, dl + 32 * j);
+  };
+  for (int st = 0; st < ns; st += 2) {
+    stage(st, sQ0, sG0, sL0, sD0, sQ1, sG1, sL1, sD1);
+    if (st + 1 < ns) stage(st + 1, sQ1, sG1, sL1, sD1, sQ0, sG0, sL0, sD0);
+  }
+
+  const unsigned row_b = (unsigned)(p.Hkv * D * (int)sizeof(S));
+  const unsigned bytes = (unsigned)(rows - 1) * row_b + T::RB;
+  const auto rdK = make_rsrc(dkb, bytes), rdV = make_rsrc(dvb, bytes);
+#pragma unroll
+  for (int u = 0; u < KT; ++u) {
+    store_rows<S, D>(dk[u], p.scale, true, p, trow[u], rdK, (unsigned)(row0 + 16 * u) * row_b, lg);
+    store_rows<S, D>(dv[u], 1.f, false, p, trow[u], rdV, (unsigned)(row0 + 16 * u) * row_b, lg);
+  }
+}
+
+template <typename S, int D>
+static hipError_t bwd(const SeqParams& p0, hipStream_t st) {
+  hipError_t e = launch_seq_prep(p0, std::is_same<S, bf16>::value ? DT_BF16 : std::is_same<S, f16>::value ? DT_F16 : DT_F32, D, st);
+  if (e != hipSuccess) return e;
+  SeqParams p = p0;
+  p.slots = (int)seq_slots(p.T, p.B, 6);
+  hipLaunchKernelGGL((seq_dq_kernel<S, D, 1>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((seq_dkdv_kernel<S, D, 1>), dim3((unsigned)p.slots * p.Hkv), dim3(kSeqThreads), 0, st, p);
+  return hipGetLastError();
+}
+template <typename S>
+static hipError_t bwd_d(const SeqParams& p, int D, hipStream_t st) {
+  return D == 32 ? bwd<S, 32>(p, st) : D == 64 ? bwd<S, 64>(p, st) : D == 128 ? bwd<S, 128>(p, st) : bwd<S, 256>(p, st);
+}
+hipError_t launch_seq_bwd(const SeqParams& p, int dt, int D, hipStream_t st) {
+  return dt == DT_BF16 ? bwd_d<bf16>(p, D, st) : dt == DT_F16 ? bwd_d<f16>(p, D, st) : bwd_d<float>(p, D, st);
+}
+
+}  // namespace farope

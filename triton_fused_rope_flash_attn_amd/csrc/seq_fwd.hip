@@ -1,0 +1,260 @@
+// Forward of attention over packed sequences: O and the per-row log-sum-exp.
+//
+//   s_ij = scale (R q_i).(R k_j), j in i's sequence (causal: j <= i)
+//   O_i = sum_j exp(s_ij - m_i) v_j / l_i,   LSE_i = m_i + ln l_i
+//
+// seq_prep_kernel has written the rotated, scaled K rows; a workgroup of 4 waves
+// takes 64 or 128 query rows of one head and streams its sequence's K-hat and V
+// rows from memory straight to LDS, in double-buffered stages with one barrier
+// each, up to the last row that its queries see.
+#include <type_traits>
+
+#include "seq.h"
+
+namespace farope {
+
+constexpr float kSeqSlack = 8.0f;   // log2 units: P <= 2^8 between rescales
+
+// Wave w owns QT 16-query subtiles.  Logits are computed transposed, S^T = K-hat
+// Q-hat^T, so that their output rows (keys) are the k-slots of O^T += V^T P^T and P
+// never leaves registers.  The accumulators start at minus the running max, P =
+// exp2 of the product's output; O and the row sum are rescaled only when some logit
+// exceeds the running max by 2^8.
+template <typename S, int D, int QT>
+__global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 ? 2 : 3)
+seq_fwd_kernel(const SeqParams p) {
+  using C = typename SeqComp<S>::C;
+  using Frag = typename C::Frag;
+  using T = Tile<S, D>;
+  constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, LB = QT == 2 ? 7 : 6;
+  __shared__ __attribute__((aligned(16))) S sK0[SR * D], sK1[SR * D], sV0[SR * D], sV1[SR * D];
+
+  const int tid = thread_id();
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  // heads vary fastest, key heads before the query heads of a group: the workgroups of one
+  // key head meet on one XCD when Hkv is a multiple of 8; later rows (more keys) come first
+  const int slot = p.slots - 1 - block_id() / p.H, hx = block_id() % p.H;
+  const int kvh = hx % p.Hkv, head = kvh * (p.H / p.Hkv) + hx / p.Hkv;
+  const SeqTile tl = find_tile(p.cu, p.B, p.T, LB, slot, lane);
+  if (tl.tile < 0) return;
+  const int q0 = tl.tile << LB, rows = tl.len - q0 < (1 << LB) ? tl.len - q0 : 1 << LB;
+  S* const ob = static_cast<S*>(p.o) + ((int64_t)(tl.start + q0) * p.H + head) * D;
+  const unsigned o_row = (unsigned)(p.H * D * (int)sizeof(S));
+  const auto rO = make_rsrc(ob, (unsigned)(rows - 1) * o_row + T::RB);
+  const auto rL = make_rsrc(p.lse + (int64_t)head * p.T + tl.start + q0, (unsigned)rows * 4u);
+  const int row0 = wave * 16 * QT + lr;   // of the tile; subtile t: + 16 t
+
+  if (tl.seq == p.B) {   // tokens behind the last sequence: zeros
+    for (int r = tid / (D / 8); r < rows; r += kSeqThreads / (D / 8)) {
+      const float z[8] = {};
+      put_row8<S>(ob + (int64_t)r * p.H * D + 8 * (tid % (D / 8)), z);
+    }
+    if (tid < rows) p.lse[(int64_t)head * p.T + tl.start + q0 + tid] = 0.f;
+    return;
+  }
+
+  SeqStream<S, D> srcK, srcV;
+  srcK.lanes(D, wave, lane);
+  srcK.base(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
+  if (p.vcopy) {
+    srcV.lanes(D, wave, lane);
+    srcV.base(static_cast<const S*>(p.vcopy) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
+  } else {
+    srcV.lanes(p.sv[0], wave, lane);
+    srcV.base(static_cast<const S*>(p.v) + tl.start * p.sv[0] + kvh * p.sv[1], tl.len);
+  }
+  srcK.load(sK0, wave, 0);
+  srcV.load(sV0, wave, 0);
+
+  Frag qf[QT][KS];
+  int seen[QT];   // keys that the subtile's row of this lane sees
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int i = q0 + row0 + 16 * t, ic = i < tl.len ? i : tl.len - 1, tok = tl.start + ic;
+    seen[t] = p.causal ? ic + 1 : tl.len;
+    const S* qp = static_cast<const S*>(p.q) + tok * p.sq[0] + head * p.sq[1];
+    const int tr = table_row(p.positions ? p.positions[tok] : ic - p.has_cls, p.n_pos);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float x[8], cs[8];
+      row8<S>(qp + (32 * s + 8 * lg) * p.sq[2], p.sq[2], p.vec_q, x);
+      table_load4(p.cosp, p.sinp, tr, D / 2, 16 * s + 4 * lg, cs);
+      rope_rotate8(x, cs);
+      qf[t][s] = C::make(x);
+    }
+  }
+  const int w0 = q0 + wave * 16 * QT;   // the wave's first row (uniform)
+  const bool active = w0 < tl.len;
+  // every row of the wave sees keys below lo, none sees keys from hi on
+  const int lo = p.causal ? w0 + 1 : tl.len;
+  const int hi = p.causal && w0 + 16 * QT < tl.len ? w0 + 16 * QT : tl.len;
+  const int last = p.causal && q0 + (1 << LB) < tl.len ? q0 + (1 << LB) : tl.len;
+  const int ns = (last + SR - 1) / SR;
+
+  f32x4 acc[QT][DT];
+  float m_run[QT], l_run[QT];
+  f32x4 nm4[QT];       // minus the running max (0 before the first block)
+  float thr = -INFINITY;   // a value above it makes the block rescale
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    m_run[t] = -INFINITY;
+    l_run[t] = 0.f;
+    nm4[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  FragAt<S, D> at;
+  at.init(lr, lg);
+
+  // One stage's keys: the logit products, one test of the running max, then the
+  // probabilities and O products of its 32-key blocks.
+  auto blocks = [&](bool tail, int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
+    f32x4 sacc[NB][QT][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Frag a = at.row(k + 32 * j * D, s, h);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) sacc[j][t][h] = C::mma(a, qf[t][s], s == 0 ? nm4[t] : sacc[j][t][h]);
+        }
+    if (tail) {   // uniform: some row of the wave does not see all of these keys
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const int lim = seen[t] - k0 - 4 * lg;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sacc[j][t][h][i] = 32 * j + 16 * h + i < lim ? sacc[j][t][h][i] : -INFINITY;
+      }
+    }
+    float mx[QT], mxx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      mx[t] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 x = sacc[j][t][h];
+          mx[t] = fmaxf(mx[t], fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+        }
+      mxx = fmaxf(mxx, mx[t]);
+    }
+    if (__any(mxx > thr)) {
+      thr = kSeqSlack;
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const float old = m_run[t] == -INFINITY ? 0.f : m_run[t];
+        const float mnew = fmaxf(m_run[t], group4_max(mx[t]) + old);
+        const float alpha = fast_exp2(m_run[t] - mnew), sh = old - mnew;
+        m_run[t] = mnew;
+        l_run[t] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] *= alpha;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) sacc[j][t][h] += sh;
+        nm4[t] = f32x4{-mnew, -mnew, -mnew, -mnew};
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      Frag pf[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float x[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[4 * h + i] = fast_exp2(sacc[j][t][h][i]);
+        l_run[t] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        pf[t] = C::make(x);   // (16-bit tensors: P rounded to their type for the O product; the row sum is not)
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const Frag a = at.col(v + 32 * j * D, d);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) acc[t][d] = C::mma(a, pf[t], acc[t][d]);
+      }
+    }
+  };
+  auto stage = [&](int st, const S* __restrict__ k, const S* __restrict__ v, S* __restrict__ kn, S* __restrict__ vn)
+      __attribute__((always_inline)) {
+    seq_stage_barrier();
+    if (st + 1 < ns) {
+      srcK.load(kn, wave, (st + 1) * SR);
+      srcV.load(vn, wave, (st + 1) * SR);
+    }
+    const int k0 = st * SR;
+    if (active && k0 < hi) blocks(k0 + SR > lo, k0, k, v);
+  };
+  for (int st = 0; st < ns; st += 2) {
+    stage(st, sK0, sV0, sK1, sV1);
+    if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
+  }
+
+  // lane holds O[row][16d + 4lg + (0..3)]; rows past the tile drop
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int row = row0 + 16 * t;
+    const float l = group4_sum(l_run[t]);
+    const float inv = __builtin_amdgcn_rcpf(l);
+    if constexpr (sizeof(S) == 4) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const f32x4 x = acc[t][d] * inv;
+        buf_store16(__builtin_bit_cast(u32x4, x), rO, (unsigned)row * o_row + (unsigned)(16 * d + 4 * lg) * 4u, 0u);
+      }
+    } else {
+      // lane groups lg and lg^1 trade halves so that each lane stores 8 consecutive channels
+#pragma unroll
+      for (int d0 = 0; d0 < DT; d0 += 2) {
+        u32x2 w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          typedef S s4 __attribute__((ext_vector_type(4)));
+          s4 a;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) a[r] = (S)(acc[t][d0 + j][r] * inv);
+          __builtin_memcpy(&w[j], &a, 8);
+        }
+        u32x4 x;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const auto r = __builtin_amdgcn_permlane16_swap(w[0][k], w[1][k], false, false);
+          x[k] = r[0];
+          x[2 + k] = r[1];
+        }
+        buf_store16(x, rO, (unsigned)row * o_row + (unsigned)(16 * (d0 + (lg & 1)) + 4 * (lg & 2)) * 2u, 0u);
+      }
+    }
+    // (lanes lg != 0 write past the range)
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint((m_run[t] + fast_log2(l)) * kLn2), rL,
+                                          (unsigned)(lg == 0 ? row : 1 << LB) * 4u, 0u, 0);
+  }
+}
+
+template <typename S, int D, int QT>
+static hipError_t fwd(const SeqParams& p0, hipStream_t st) {
+  SeqParams p = p0;
+  p.slots = (int)seq_slots(p.T, p.B, QT == 2 ? 7 : 6);
+  hipLaunchKernelGGL((seq_fwd_kernel<S, D, QT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
+  return hipGetLastError();
+}
+template <typename S>
+static hipError_t fwd_d(const SeqParams& p, int D, hipStream_t st) {
+  if (sizeof(S) == 4) return D == 32 ? fwd<S, 32, 1>(p, st) : D == 64 ? fwd<S, 64, 1>(p, st) : D == 128 ? fwd<S, 128, 1>(p, st) : fwd<S, 256, 1>(p, st);
+  return D == 32 ? fwd<S, 32, 1>(p, st) : D == 64 ? fwd<S, 64, 1>(p, st) : D == 128 ? fwd<S, 128, 1>(p, st) : fwd<S, 256, 1>(p, st);
+}
+hipError_t launch_seq_fwd(const SeqParams& p, int dt, int D, hipStream_t st) {
+  return dt == DT_BF16 ? fwd_d<bf16>(p, D, st) : dt == DT_F16 ? fwd_d<f16>(p, D, st) : fwd_d<float>(p, D, st);
+}
+
+}  // namespace farope

@@ -1,0 +1,94 @@
+// Kernel argument blocks and launchers of attention over packed sequences and
+// over a paged cache (seq_api.hip calls them).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace farope {
+
+constexpr int kSeqNW = 4;                  // waves per workgroup
+constexpr int kSeqThreads = 64 * kSeqNW;
+
+// Token t, head h, channel d of an input: t*s[0] + h*s[1] + d*s[2] elements.
+struct SeqParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* dout;
+  int64_t sq[3], sk[3], sv[3], sdo[3];
+  int vec_q, vec_k, vec_v, vec_do;   // 16-byte access (seq_api.hip: vec_rows)
+  const float* cosp;                 // [n_pos, D/2]
+  const float* sinp;
+  const int* positions;              // [T] table rows, or null: by index
+  const int* cu;                     // [B + 1]
+  void* o;                           // [T, H, D]
+  float* lse;                        // [H, T], natural log
+  void* dq;                          // [T, H, D]
+  void* dk;                          // [T, Hkv, D]
+  void* dv;
+  // workspace
+  void* khat;                        // [Hkv, T, D]: rotated K rows times scale * log2 e
+  void* vcopy;                       // [Hkv, T, D]: V, where its own rows cannot be streamed (else null)
+  void* qhat;                        // [H, T, D]: rotated Q rows
+  void* gcopy;                       // [H, T, D]: dO, where its own rows cannot be streamed (else null)
+  float* nl;                         // [H, T]: -LSE * log2 e
+  float* nd;                         // [H, T]: -rowsum(dO * O)
+  int T, B, H, Hkv, n_pos, has_cls, causal;
+  float scale, c2;                   // softmax scale; times log2 e
+  int slots;                         // row slots of the launch (set by the launcher)
+};
+
+// A slot per 2^lb rows, one more per sequence, and the tokens behind the last one.
+inline int64_t seq_slots(int T, int B, int lb) { return (int64_t)(T >> lb) + B + 1; }
+
+hipError_t launch_seq_prep(const SeqParams& p, int dt, int D, hipStream_t st);
+hipError_t launch_seq_fwd(const SeqParams& p, int dt, int D, hipStream_t st);
+hipError_t launch_seq_bwd(const SeqParams& p, int dt, int D, hipStream_t st);
+
+// Paged cache: row r of page g, key head h: g*s[0] + r*s[1] + h*s[2] elements,
+// channels contiguous, every row 16-byte aligned.
+struct CacheParams {
+  void* kc;
+  void* vc;
+  int64_t skc[3], svc[3];
+  const int* pages;      // [B, max_pages]
+  int64_t spages;        // elements between its rows
+  const int* lengths;    // [B]
+  int n_pages, page, max_pages;
+};
+
+struct AppendParams {
+  const void* k;
+  const void* v;
+  int64_t sk[3], sv[3];
+  int vec_k, vec_v;
+  const float* cosp;
+  const float* sinp;
+  const int* positions;  // [T], or null
+  const int* cu;         // [B + 1], or null: token t is sequence t's
+  CacheParams c;
+  int T, B, Hkv, n_pos, has_cls;
+};
+hipError_t launch_cache_append(const AppendParams& p, int dt, int D, hipStream_t st);
+
+struct DecodeParams {
+  const void* q;
+  int64_t sq[3];         // sequence, head, channel
+  int vec_q;
+  const float* cosp;
+  const float* sinp;
+  const int* positions;  // [B], or null
+  CacheParams c;
+  void* o;               // [B, H, D]
+  float* sums;           // [B, H, parts, D]: the parts' unnormalised O (parts > 1)
+  float* stats;          // [B, H, parts, 2]: their max logit (log2 units) and row sum
+  int B, H, Hkv, n_pos, has_cls;
+  int parts;             // parts of a sequence's rows
+  int g_tiles;           // tiles of 16 query heads in a group
+  float c2;
+};
+// Parts of a call: see decode_parts in seq_api.hip.
+hipError_t launch_decode(const DecodeParams& p, int dt, int D, hipStream_t st);
+
+}  // namespace farope

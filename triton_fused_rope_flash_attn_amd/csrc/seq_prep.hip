@@ -1,0 +1,61 @@
+// Rotated key rows of packed sequences: what the forward's and the backward's
+// tiles stream.
+//
+// K-hat = scale * log2(e) * R(position) K, rounded once to the tensors' type, as
+// [Hkv, T, D]; and, where V's own rows cannot be streamed (channels not
+// contiguous, or rows not 16-byte aligned), V copied to the same layout.  A
+// thread takes 8 channels of one token and kPrepHeads key heads, so that their
+// loads are in flight together and share one read of the table row.
+#include "seq.h"
+
+namespace farope {
+
+constexpr int kPrepHeads = 4;
+
+template <typename S, int D>
+__global__ void __launch_bounds__(256) seq_prep_kernel(const SeqParams p, int n_grp) {
+  constexpr int CPR = D / 8, ROWS = 256 / CPR;
+  const int blk = block_id() / n_grp, h0 = (block_id() - blk * n_grp) * kPrepHeads;
+  const int tid = thread_id(), lane = tid & 63;
+  const int t0 = blk * ROWS, t = t0 + tid / CPR, c = 8 * (tid % CPR);
+  const int tc = t < p.T ? t : p.T - 1;
+  const int b = find_seq(p.cu, p.B, p.T, t0, tc, lane);
+  if (t >= p.T || b == p.B) return;   // (no tile reads tokens of no sequence)
+  const int row = table_row(p.positions ? p.positions[t] : t - cu_at(p.cu, b, p.T) - p.has_cls, p.n_pos);
+  float x[kPrepHeads][8], v[kPrepHeads][8];
+#pragma unroll
+  for (int i = 0; i < kPrepHeads; ++i) {
+    if (h0 + i >= p.Hkv) break;
+    row8<S>(static_cast<const S*>(p.k) + t * p.sk[0] + (h0 + i) * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x[i]);
+    if (p.vcopy) row8<S>(static_cast<const S*>(p.v) + t * p.sv[0] + (h0 + i) * p.sv[1] + c * p.sv[2], p.sv[2], p.vec_v, v[i]);
+  }
+  float cs[8];
+  table_load4(p.cosp, p.sinp, row, D / 2, c / 2, cs);
+#pragma unroll
+  for (int i = 0; i < kPrepHeads; ++i) {
+    if (h0 + i >= p.Hkv) break;
+    rope_rotate8(x[i], cs);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[i][e] *= p.c2;
+    const int64_t at = ((int64_t)(h0 + i) * p.T + t) * D + c;
+    put_row8<S>(static_cast<S*>(p.khat) + at, x[i]);
+    if (p.vcopy) put_row8<S>(static_cast<S*>(p.vcopy) + at, v[i]);
+  }
+}
+
+template <typename S, int D>
+static hipError_t prep(const SeqParams& p, hipStream_t st) {
+  const int rows = 256 / (D / 8), n_grp = (p.Hkv + kPrepHeads - 1) / kPrepHeads;
+  const int n_blk = (p.T + rows - 1) / rows;
+  hipLaunchKernelGGL((seq_prep_kernel<S, D>), dim3(n_blk * n_grp), dim3(256), 0, st, p, n_grp);
+  return hipGetLastError();
+}
+template <typename S>
+static hipError_t prep_d(const SeqParams& p, int D, hipStream_t st) {
+  return D == 32 ? prep<S, 32>(p, st) : D == 64 ? prep<S, 64>(p, st) : D == 128 ? prep<S, 128>(p, st) : prep<S, 256>(p, st);
+}
+hipError_t launch_seq_prep(const SeqParams& p, int dt, int D, hipStream_t st) {
+  return dt == DT_BF16 ? prep_d<bf16>(p, D, st) : dt == DT_F16 ? prep_d<f16>(p, D, st) : prep_d<float>(p, D, st);
+}
+
+}  // namespace farope

@@ -9,43 +9,12 @@
 // interpreter lock.  Small calls are bound by exactly that host work: a
 // training pass of 96 planes of 197 rows took 226 us around 43 us of kernels
 // with the Python kernels, 70 to 75 us with these (box to box).
-#include <ATen/ATen.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/DeviceGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/library.h>
-
-#include <sstream>
-
-#include "farope.h"
+#include "torch_util.h"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::variable_list;
+using namespace farope_torch;
 using Three = std::tuple<Tensor, Tensor, Tensor>;
-
-int dtype_code(at::ScalarType t) {
-  return t == at::kFloat ? FAROPE_F32 : t == at::kHalf ? FAROPE_F16 : t == at::kBFloat16 ? FAROPE_BF16 : -1;
-}
-std::string shape_str(const Tensor& t) {
-  std::ostringstream s;
-  s << '(';
-  for (int64_t i = 0; i < t.dim(); ++i) s << (i ? ", " : "") << t.size(i);
-  s << (t.dim() == 1 ? ",)" : ")");
-  return s.str();
-}
-std::string dtype_str(const Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return "torch.float32";
-    case at::kHalf: return "torch.float16";
-    case at::kBFloat16: return "torch.bfloat16";
-    case at::kDouble: return "torch.float64";
-    default: return std::string("torch.") + c10::toString(t.scalar_type());
-  }
-}
 
 void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
   TORCH_CHECK_VALUE(q.dim() == 4, "Q must be [B, H, N, D]; got shape ", shape_str(q));
@@ -82,18 +51,6 @@ farope_attn_desc make_desc(int64_t B, int64_t H, int64_t N, int64_t D, at::Scala
   d.compute_dtype = (int32_t)comp;
   d.softmax_scale = (float)scale;
   return d;
-}
-
-void check_rc(int rc, const char* what) {
-  TORCH_CHECK(rc == FAROPE_OK, what, ": ", farope_strerror(rc), " (status ", rc, ")");
-}
-
-const int64_t* strides(const Tensor& t) { return t.strides().data(); }
-float* floats(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr<float>() : nullptr; }
-void* data(const Tensor& t) { return t.numel() ? t.data_ptr() : nullptr; }
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
-Tensor workspace(const Tensor& like, size_t elems) {
-  return elems ? at::empty({(int64_t)elems}, like.options().dtype(at::kFloat)) : Tensor();
 }
 
 Three attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& rope, int64_t n_pos, bool has_cls,
@@ -276,12 +233,6 @@ struct AttnBwdNode : torch::autograd::Function<AttnBwdNode> {
                 "(the attention's gradients are not differentiable again).");
   }
 };
-
-bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
-  for (const Tensor* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
 
 Three attn_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& rope, c10::SymInt n_pos, bool has_cls,
                         double scale, c10::SymInt comp) {
