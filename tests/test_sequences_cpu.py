@@ -192,13 +192,17 @@ def test_c_entries_refuse_pointers_and_workspaces():
 
 
 def test_c_workspace_parts():
-    """K-hat; a copy of V and of dO where their rows cannot be streamed; Q-hat and two row values."""
+    """K-hat; a copy of V and of dO where their rows cannot be streamed; Q-hat and two row values;
+    where key tiles are few, the parts' sums of dK and dV."""
     lib = _lib.load()
-    d = _seq_desc(tokens=1000, heads=6, kv_heads=3, head_dim=128)
-    kv, q, row = 1000 * 3 * 128 // 2, 1000 * 6 * 128 // 2, (1000 * 6 + 63) // 64 * 64
-    size = lambda *a: lib.farope_seq_workspace_elems(ctypes.byref(d), *a)  # noqa: E731
-    assert size(0, 1, 1) == kv and size(0, 0, 1) == 2 * kv
-    assert size(1, 1, 1) == kv + q + 2 * row and size(1, 0, 0) == 2 * kv + 2 * q + 2 * row
+    d = _seq_desc(tokens=8000, heads=20, kv_heads=10, head_dim=128)
+    kv, q, row = 8000 * 10 * 128 // 2, 8000 * 20 * 128 // 2, 8000 * 20
+    size = lambda d, *a: lib.farope_seq_workspace_elems(ctypes.byref(d), *a)  # noqa: E731
+    assert size(d, 0, 1, 1) == kv and size(d, 0, 0, 1) == 2 * kv
+    assert size(d, 1, 1, 1) == kv + q + 2 * row and size(d, 1, 0, 0) == 2 * kv + 2 * q + 2 * row
+    d = _seq_desc(tokens=4096, seqs=1, heads=4, kv_heads=4, head_dim=128)   # 4 x 66 workgroups: 4 parts
+    n = 4096 * 4 * 128
+    assert size(d, 0, 1, 1) == n // 2 and size(d, 1, 1, 1) == n + 2 * 4096 * 4 + 2 * 4 * n
 
 
 @pytest.mark.parametrize("stride,ptr,ok", [

@@ -60,21 +60,50 @@ int check_sizes(const farope_seq_desc* d) {
   return token_blocks(d) > kMaxWorkgroups ? FAROPE_ERR_SHAPE : FAROPE_OK;
 }
 
+// Workgroups of a call over a paged cache that are resident at once (decode_kernel's registers):
+// one round of workers, whose shares are equal, is the fastest.  Measured (us, 512 / 768 / 1024
+// workgroups; "sequences x rows, key heads"), D 128: 1 x 32768, 8 37.5 / 43.4 / 46.0, 32 x 8192, 1
+// 35.5 / 44.6 / 41.5; D 64: 16 x 2048, 12 30.8 / 27.1 / 32.6; D 256, 256 / 512: 8 x 8192, 2 40 / 53.
+int64_t decode_wgs(const farope_seq_desc* d) {
+  const int row = d->head_dim * elem_size(d->dtype);
+  return (int64_t)kCus * (row <= 64 ? 4 : row == 128 ? 3 : row == 256 ? 2 : 1);
+}
+
 // Workspace, in fp32 elements, each part from a 256-byte boundary.
-struct Ws {
-  int64_t khat, vcopy, qhat, gcopy, nl, nd, total;
+constexpr int kMaxParts = 8;
+struct SeqWs {
+  int64_t khat, vcopy, qhat, gcopy, nl, nd, pk, pv, total;
 };
-Ws seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_streams) {
+// Parts that the queries of a key tile (64 rows) are divided into, joined by a launch of its
+// own: so many that about four workgroups per CU share the work, but none below a stage of
+// queries on average.  Measured (us, forward and backward, 1 / 2 / 4 parts; workgroups of
+// one part in brackets), D 128: 16384 tokens, 2 key heads [514] 3837 / 2839 / 2832, 4096, 4
+// [264] 713 / 523 / 432, 1024, 4 [72] 181 / 129 / 105, 8 x 1024, 8 [1096] 208 / 239 / 311; D 64:
+// 2048, 2 [68] 204 / 138 / 105, 4 x 2048, 8 [1064] 180 / 179 / 196; D 256: 2 x 4096, 8 [1048] 1251 /
+// 1347 / 1525; fp32, D 64: 3 up to 257, 4 [44] 100 / 79 / 72.
+int dkdv_parts(const farope_seq_desc* d) {
+  const int64_t wgs = seq_slots(d->tokens, d->seqs, 6) * d->kv_heads;
+  const int64_t stages = (int64_t)(d->heads / d->kv_heads) * (d->tokens / d->seqs / 64 + 1);
+  int64_t parts = (4 * kCus + wgs / 2) / wgs;
+  if (parts > kMaxParts) parts = kMaxParts;
+  if (parts > stages) parts = stages;
+  return parts < 1 ? 1 : (int)parts;
+}
+SeqWs seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_streams) {
   const int64_t es = elem_size(d->dtype), kv = (int64_t)d->tokens * d->kv_heads * d->head_dim * es / 4;
   const int64_t q = (int64_t)d->tokens * d->heads * d->head_dim * es / 4, rows = (int64_t)d->tokens * d->heads;
   auto al = [](int64_t x) { return (x + 63) & ~int64_t(63); };
-  Ws w{};
+  SeqWs w{};
   w.vcopy = al(kv);
   w.qhat = w.vcopy + (v_streams ? 0 : al(kv));
   w.gcopy = w.qhat + (backward ? al(q) : 0);
   w.nl = w.gcopy + (backward && !g_streams ? al(q) : 0);
   w.nd = w.nl + (backward ? al(rows) : 0);
-  w.total = w.nd + (backward ? al(rows) : 0);
+  const int parts = backward ? dkdv_parts(d) : 1;
+  const int64_t sums = parts > 1 ? al((int64_t)parts * d->tokens * d->kv_heads * d->head_dim) : 0;
+  w.pk = w.nd + (backward ? al(rows) : 0);
+  w.pv = w.pk + sums;
+  w.total = w.pv + sums;
   return w;
 }
 
@@ -126,19 +155,37 @@ CacheParams cache_params(const farope_cache_desc* c, const int32_t* table, const
   return p;
 }
 
-// Parts that a sequence's rows are divided into.  The lengths stay on the device, so the
-// rule goes by what a sequence can hold: enough parts for a few workgroups per CU, and
-// none smaller than 128 rows (a 32-row block per wave).
+// Workers among which a key head's cached rows are divided (decode.hip).  The lengths stay on
+// the device, so the rules go by the sequences' number and room.
 int decode_tiles(const farope_seq_desc* d) { return (d->heads / d->kv_heads + 15) / 16; }
-int decode_parts(const farope_seq_desc* d, const farope_cache_desc* c) {
-  const int64_t room = (int64_t)c->max_pages * c->page_rows, most = (room + 127) / 128;
-  const int64_t groups = (int64_t)d->seqs * d->kv_heads * decode_tiles(d);
-  int64_t parts = (3 * kCus + groups - 1) / groups;
-  if (parts > most) parts = most;
-  return parts < 1 ? 1 : (int)parts;
+// One worker per sequence, nothing to join, where a sequence's room is short, or up to 2048
+// rows where the sequences alone make several rounds (up to 1024, one).  Measured (us, even
+// shares / one per sequence): 1 x 197, 12 heads, D 64 11.1 / 6.9; 256 sequences up to 1024, 8
+// heads, D 128 104 / 89; 64 x 1024, 16 heads, D 64 66 / 59; 5 up to 1025, 8 heads, fp32 14.4 / 19.3.
+bool decode_direct(const farope_seq_desc* d, const farope_cache_desc* c) {
+  const int64_t room = (int64_t)c->max_pages * c->page_rows, wgs = (int64_t)d->seqs * d->kv_heads * decode_tiles(d);
+  return room <= 512 || (room <= 1024 && wgs >= decode_wgs(d)) || (room <= 2048 && wgs >= 2 * decode_wgs(d));
 }
-int64_t decode_ws(const farope_seq_desc* d, int parts) {
-  return parts == 1 ? 0 : (int64_t)d->seqs * d->heads * parts * (d->head_dim + 2);
+int decode_workers(const farope_seq_desc* d, const farope_cache_desc* c) {
+  if (decode_direct(d, c)) return d->seqs;
+  const int64_t heads = (int64_t)d->kv_heads * decode_tiles(d);
+  // (a worker has 128 rows at least)
+  const int64_t most = d->seqs * (((int64_t)c->max_pages * c->page_rows + 127) / 128);
+  const int64_t n = (decode_wgs(d) + heads - 1) / heads;
+  return (int)(n < most ? n : most);
+}
+// Workspace, in fp32 elements, each part from a 16-byte boundary: sums, their statistics, owners.
+struct DecodeWs {
+  int64_t stats, owners, total;
+};
+DecodeWs decode_ws(const farope_seq_desc* d, const farope_cache_desc* c) {
+  if (decode_direct(d, c)) return DecodeWs{};
+  const int64_t rows = ((int64_t)decode_workers(d, c) + d->seqs) * d->heads;
+  DecodeWs w{};
+  w.stats = rows * d->head_dim;
+  w.owners = (w.stats + 2 * rows + 3) & ~int64_t(3);
+  w.total = w.owners + 2 * (int64_t)d->seqs;
+  return w;
 }
 
 }  // namespace
@@ -164,7 +211,7 @@ int farope_seq_fwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
   FAROPE_TRY(check_ptr(lse, 4));
   FAROPE_TRY(check_ptr(ws, 16));
   const bool vs = streams(desc, v, v_stride);
-  const Ws w = seq_ws(desc, false, vs, true);
+  const SeqWs w = seq_ws(desc, false, vs, true);
   if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
   SeqParams p{};
   fill(p, desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu);
@@ -194,7 +241,7 @@ int farope_seq_bwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
   FAROPE_TRY(check_ptr(dv, 16));
   FAROPE_TRY(check_ptr(ws, 16));
   const bool vs = streams(desc, v, v_stride), gs = streams(desc, dout, dout_stride);
-  const Ws w = seq_ws(desc, true, vs, gs);
+  const SeqWs w = seq_ws(desc, true, vs, gs);
   if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
   SeqParams p{};
   fill(p, desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu);
@@ -210,6 +257,9 @@ int farope_seq_bwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
   p.gcopy = gs ? nullptr : ws + w.gcopy;
   p.nl = ws + w.nl;
   p.nd = ws + w.nd;
+  p.pk = ws + w.pk;
+  p.pv = ws + w.pv;
+  p.parts = dkdv_parts(desc);
   return launch_rc(launch_seq_bwd(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
 }
 
@@ -242,7 +292,7 @@ int farope_cache_append(const farope_seq_desc* desc, const void* k, const int64_
 
 size_t farope_decode_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache) {
   if (check_desc(desc, true) != FAROPE_OK || !cache || cache->max_pages < 1 || cache->page_rows < 1) return 0;
-  return (size_t)decode_ws(desc, decode_parts(desc, cache));
+  return (size_t)decode_ws(desc, cache).total;
 }
 
 int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3], const float* cosp, const float* sinp,
@@ -258,14 +308,13 @@ int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_st
   if (positions) FAROPE_TRY(check_ptr(positions, 4));
   FAROPE_TRY(check_cache(desc, cache, page_table, lengths));
   FAROPE_TRY(check_ptr(o, 16));
-  const int parts = decode_parts(desc, cache);
-  const int64_t need = decode_ws(desc, parts);
-  if (need) {
+  const DecodeWs w = decode_ws(desc, cache);
+  if (w.total) {
     FAROPE_TRY(check_ptr(ws, 16));
-    if ((int64_t)ws_elems < need) return FAROPE_ERR_SCRATCH;
+    if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
   }
-  const int64_t wgs = (int64_t)desc->seqs * desc->kv_heads * decode_tiles(desc) * parts;
-  if (wgs > kMaxWorkgroups || (int64_t)desc->seqs * desc->heads * desc->head_dim / 1024 + 1 > kMaxWorkgroups)
+  const int workers = decode_workers(desc, cache);
+  if ((int64_t)desc->kv_heads * decode_tiles(desc) * workers > kMaxWorkgroups || (int64_t)desc->seqs * desc->heads > kMaxWorkgroups)
     return FAROPE_ERR_SHAPE;
   DecodeParams p{};
   p.q = q;
@@ -275,9 +324,11 @@ int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_st
   p.c = cache_params(cache, page_table, lengths);
   p.o = o;
   p.sums = ws;
-  p.stats = need ? ws + (int64_t)desc->seqs * desc->heads * parts * desc->head_dim : nullptr;
+  p.stats = ws + w.stats;
+  p.owners = reinterpret_cast<int*>(ws + w.owners);
   p.B = desc->seqs; p.H = desc->heads; p.Hkv = desc->kv_heads; p.n_pos = desc->n_pos; p.has_cls = desc->has_cls;
-  p.parts = parts;
+  p.workers = workers;
+  p.direct = w.total == 0;
   p.g_tiles = decode_tiles(desc);
   p.c2 = desc->softmax_scale * 1.4426950408889634f;
   return launch_rc(launch_decode(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));

@@ -247,16 +247,18 @@ seq_dq_kernel(const SeqParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// dK and dV of 64 KT key rows of one key head.  Wave w owns KT 16-key subtiles:
-// its K-hat and V rows are operands in registers, dK-hat and dV accumulate in
-// registers over the stages of every query head of the group.
+// dK and dV of 64 key rows of one key head.  Wave w owns 16 of them: their K-hat and
+// V rows are operands in registers, dK-hat and dV accumulate in registers over the
+// stages of every query head of the group (parts > 1: over a part's equal share of
+// them).  128 keys per workgroup (D 32 and 64) measured the same within 3% for long
+// sequences and slower for short ones (64 up to 577, D 64: 146 / 163 us).
 // ---------------------------------------------------------------------------
-template <typename S, int D, int KT>
+template <typename S, int D>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : 2) seq_dkdv_kernel(const SeqParams p) {
   using C = typename SeqComp<S>::C;
   using Frag = typename C::Frag;
   using T = Tile<S, D>;
-  constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, LB = KT == 2 ? 7 : 6;
+  constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, LB = 6;
   __shared__ __attribute__((aligned(16))) S sQ0[SR * D], sQ1[SR * D], sG0[SR * D], sG1[SR * D];
   __shared__ __attribute__((aligned(16))) float sL0[64], sL1[64], sD0[64], sD1[64];
 
@@ -264,7 +266,8 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lr = lane & 15, lg = lane >> 4;
   // earlier keys (seen by more queries) come first in each sequence
-  const int slot = block_id() / p.Hkv, kvh = block_id() % p.Hkv, group = p.H / p.Hkv;
+  const int part = block_id() % p.parts, rest = block_id() / p.parts;
+  const int slot = rest / p.Hkv, kvh = rest % p.Hkv, group = p.H / p.Hkv;
   const SeqTile tl = find_tile(p.cu, p.B, p.T, LB, slot, lane);
   if (tl.tile < 0) return;
   const int k0 = tl.tile << LB, rows = tl.len - k0 < (1 << LB) ? tl.len - k0 : 1 << LB;
@@ -272,21 +275,24 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   S* const dkb = static_cast<S*>(p.dk) + (tok0 * p.Hkv + kvh) * D;
   S* const dvb = static_cast<S*>(p.dv) + (tok0 * p.Hkv + kvh) * D;
   if (tl.seq == p.B) {
+    if (p.parts > 1) return;   // (seq_join_kernel's)
     zero_rows<S, D>(dkb, (int64_t)p.Hkv * D, rows, tid);
     zero_rows<S, D>(dvb, (int64_t)p.Hkv * D, rows, tid);
     return;
   }
 
-  // stages of a query head: from the tile's first key on when causal
-  const int first = p.causal ? k0 / SR : 0, per = (tl.len + SR - 1) / SR - first, ns = per * group;
+  // stages of a query head: from the tile's first key on when causal; this part's share of all heads'
+  const int first = p.causal ? k0 / SR : 0, per = (tl.len + SR - 1) / SR - first;
+  const int64_t all = (int64_t)per * group;
+  const int begin = (int)(all * part / p.parts), ns = (int)(all * (part + 1) / p.parts) - begin;
   SeqStream<S, D> srcQ, srcG;
   srcQ.lanes(D, wave, lane);
   srcG.lanes(p.gcopy ? D : p.sdo[0], wave, lane);
-  int lh = -1, lst = per;   // the stage loaded next: head of the group, stage
+  int lh = begin / per - 1, lst = per, cst = begin % per;   // the stage loaded next: head of the group, stage
   __amdgpu_buffer_rsrc_t rStat = make_rsrc(p.nl, 0u);
   auto load = [&](S* q, S* g, float* l, float* d) __attribute__((always_inline)) {
     if (lst == per) {
-      lst = 0;
+      lst = lh < begin / per ? cst : 0;
       const int head = kvh * group + ++lh;
       const int64_t hrow = (int64_t)head * p.T + tl.start;
       srcQ.base(static_cast<const S*>(p.qhat) + hrow * D, tl.len);
@@ -301,42 +307,36 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
     if (wave < 2) seq_dma4(rStat, wave ? d : l, (unsigned)lane * 4u, (unsigned)r0 * 4u);
     ++lst;
   };
-  load(sQ0, sG0, sL0, sD0);
+  if (ns > 0) load(sQ0, sG0, sL0, sD0);
 
-  const int row0 = wave * 16 * KT + lr;   // of the tile; subtile u: + 16 u
-  Frag kf[KT][KS], vf[KT][KS];
-  int trow[KT];
+  const int row0 = wave * 16 + lr;   // of the tile
+  Frag kf[KS], vf[KS];
+  const int rc = row0 < rows ? row0 : rows - 1;
+  const int64_t tok = tok0 + rc;
+  const S* const kp = static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D;
+  const S* const vp = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1];
+  const int trow = table_row(p.positions ? p.positions[tok] : k0 + rc - p.has_cls, p.n_pos);
 #pragma unroll
-  for (int u = 0; u < KT; ++u) {
-    const int r = row0 + 16 * u, rc = r < rows ? r : rows - 1;
-    const int64_t tok = tok0 + rc;
-    const S* kp = static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D;
-    const S* vp = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1];
-    trow[u] = table_row(p.positions ? p.positions[tok] : k0 + rc - p.has_cls, p.n_pos);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int c = 32 * s + 8 * lg;
-      float x[8];
-      row8<S>(kp + c, 1, true, x);
-      kf[u][s] = C::make(x);
-      row8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
-      vf[u][s] = C::make(x);
-    }
+  for (int s = 0; s < KS; ++s) {
+    const int c = 32 * s + 8 * lg;
+    float x[8];
+    row8<S>(kp + c, 1, true, x);
+    kf[s] = C::make(x);
+    row8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
+    vf[s] = C::make(x);
   }
-  const int w0 = k0 + wave * 16 * KT;   // the wave's first key (uniform)
+  const int w0 = k0 + wave * 16;   // the wave's first key (uniform)
   const bool active = w0 < tl.len;
-  f32x4 dv[KT][DT], dk[KT][DT];
+  f32x4 dv[DT], dk[DT];
 #pragma unroll
-  for (int u = 0; u < KT; ++u)
-#pragma unroll
-    for (int d = 0; d < DT; ++d) dv[u][d] = dk[u][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < DT; ++d) dv[d] = dk[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   FragAt<S, D> at;
   at.init(lr, lg);
 
   // 32 queries from q0 on; tail: some of them do not exist or do not see all of the wave's keys
   auto block = [&](bool tail, int q0, const S* __restrict__ q, const S* __restrict__ g, const float* __restrict__ l,
                    const float* __restrict__ dl) __attribute__((always_inline)) {
-    f32x4 sacc[KT][2], pacc[KT][2];
+    f32x4 sacc[2], pacc[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const f32x4 nl = *reinterpret_cast<const f32x4*>(l + 16 * h + 4 * lg);
@@ -344,46 +344,32 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const Frag a = at.row(q, s, h), b = at.row(g, s, h);
-#pragma unroll
-        for (int u = 0; u < KT; ++u) {
-          sacc[u][h] = C::mma(a, kf[u][s], s == 0 ? first_sum<S>(nl) : sacc[u][h]);
-          pacc[u][h] = C::mma(b, vf[u][s], s == 0 ? first_sum<S>(nd) : pacc[u][h]);
-          if (s == KS - 1) {
-            last_sum<S>(sacc[u][h], nl);
-            last_sum<S>(pacc[u][h], nd);
-          }
-        }
+        sacc[h] = C::mma(a, kf[s], s == 0 ? first_sum<S>(nl) : sacc[h]);
+        pacc[h] = C::mma(b, vf[s], s == 0 ? first_sum<S>(nd) : pacc[h]);
       }
+      last_sum<S>(sacc[h], nl);
+      last_sum<S>(pacc[h], nd);
     }
-    Frag pf[KT], dsf[KT];
+    // query q0 + 16 h + 4 lg + i exists and sees this lane's key
+    const int from = p.causal ? k0 + row0 - q0 - 4 * lg : -4 * lg, to = tl.len - q0 - 4 * lg;
+    float pv[8], ds[8];
 #pragma unroll
-    for (int u = 0; u < KT; ++u) {
-      // query q0 + 16 h + 4 lg + i exists and sees this lane's key
-      const int from = p.causal ? k0 + row0 + 16 * u - q0 - 4 * lg : -4 * lg, to = tl.len - q0 - 4 * lg;
-      float pv[8], ds[8];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = !tail || (16 * h + i >= from && 16 * h + i < to);
-          const float e = fast_exp2(sacc[u][h][i]);
-          pv[4 * h + i] = in ? e : 0.f;
-          ds[4 * h + i] = in ? e * pacc[u][h][i] : 0.f;
-        }
-      pf[u] = C::make(pv);    // (16-bit tensors: P and dS rounded to their type for the products)
-      dsf[u] = C::make(ds);
-    }
+      for (int i = 0; i < 4; ++i) {
+        const bool in = !tail || (16 * h + i >= from && 16 * h + i < to);
+        const float e = fast_exp2(sacc[h][i]);
+        pv[4 * h + i] = in ? e : 0.f;
+        ds[4 * h + i] = in ? e * pacc[h][i] : 0.f;
+      }
+    const Frag pf = C::make(pv), dsf = C::make(ds);   // (16-bit tensors: P and dS rounded to their type for the products)
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const Frag ag = at.col(g, d), aq = at.col(q, d);
-#pragma unroll
-      for (int u = 0; u < KT; ++u) {
-        dv[u][d] = C::mma(ag, pf[u], dv[u][d]);
-        dk[u][d] = C::mma(aq, dsf[u], dk[u][d]);
-      }
+      dv[d] = C::mma(at.col(g, d), pf, dv[d]);
+      dk[d] = C::mma(at.col(q, d), dsf, dk[d]);
     }
   };
-  int cst = 0;   // this stage within its head
+  // (cst: this stage within its head)
   auto stage = [&](int st, const S* __restrict__ q, const S* __restrict__ g, const float* __restrict__ l, const float* __restrict__ dl,
                    S* __restrict__ qn, S* __restrict__ gn, float* __restrict__ ln, float* __restrict__ dn) __attribute__((always_inline)) {
     seq_stage_barrier();
@@ -391,7 +377,7 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
     const int q0 = (first + cst) * SR;
     cst = cst + 1 == per ? 0 : cst + 1;
     if (!active || (p.causal && q0 + SR <= w0)) return;
-    const bool tail = q0 + SR > tl.len || (p.causal && q0 < w0 + 16 * KT);
+    const bool tail = q0 + SR > tl.len || (p.causal && q0 < w0 + 16);
 #pragma unroll
     for (int j = 0; j < NB; ++j)
       block(tail, q0 + 32 * j, q + 32 * j * D, g + 32 * j * D, l + 32 * j, dl + 32 * j);
@@ -401,26 +387,78 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
     if (st + 1 < ns) stage(st + 1, sQ1, sG1, sL1, sD1, sQ0, sG0, sL0, sD0);
   }
 
+  if (p.parts > 1) {   // sums as they are, for seq_join_kernel
+    const int64_t at = (((int64_t)part * p.T + tok0) * p.Hkv + kvh) * D;
+    const unsigned row_b = (unsigned)(p.Hkv * D) * 4u, bytes = (unsigned)(rows - 1) * row_b + D * 4u;
+    const auto rpK = make_rsrc(p.pk + at, bytes), rpV = make_rsrc(p.pv + at, bytes);
+    store_rows<float, D>(dk, 1.f, false, p, 0, rpK, (unsigned)row0 * row_b, lg);
+    store_rows<float, D>(dv, 1.f, false, p, 0, rpV, (unsigned)row0 * row_b, lg);
+    return;
+  }
   const unsigned row_b = (unsigned)(p.Hkv * D * (int)sizeof(S));
   const unsigned bytes = (unsigned)(rows - 1) * row_b + T::RB;
   const auto rdK = make_rsrc(dkb, bytes), rdV = make_rsrc(dvb, bytes);
-#pragma unroll
-  for (int u = 0; u < KT; ++u) {
-    store_rows<S, D>(dk[u], p.scale, true, p, trow[u], rdK, (unsigned)(row0 + 16 * u) * row_b, lg);
-    store_rows<S, D>(dv[u], 1.f, false, p, trow[u], rdV, (unsigned)(row0 + 16 * u) * row_b, lg);
-  }
+  store_rows<S, D>(dk, p.scale, true, p, trow, rdK, (unsigned)row0 * row_b, lg);
+  store_rows<S, D>(dv, 1.f, false, p, trow, rdV, (unsigned)row0 * row_b, lg);
 }
 
+// dK and dV of the parts' sums, added in order; a thread takes 8 channels of one token
+// and key head.
+template <typename S, int D>
+__global__ void __launch_bounds__(256) seq_join_kernel(const SeqParams p) {
+  constexpr int CPR = D / 8, ROWS = 256 / CPR;
+  const int blk = block_id() / p.Hkv, kvh = block_id() % p.Hkv;
+  const int tid = thread_id(), t0 = blk * ROWS, t = t0 + tid / CPR, c = 8 * (tid % CPR);
+  const int tc = t < p.T ? t : p.T - 1;
+  const int b = find_seq(p.cu, p.B, p.T, t0, tc, tid & 63);
+  if (t >= p.T) return;
+  float k[8] = {}, v[8] = {};
+  const int64_t at = ((int64_t)t * p.Hkv + kvh) * D + c, step = (int64_t)p.T * p.Hkv * D;
+  if (b < p.B) {
+    for (int i = 0; i < p.parts; ++i) {
+      float x[8], y[8];
+      load8<float>(p.pk + i * step + at, 1, true, x);
+      load8<float>(p.pv + i * step + at, 1, true, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { k[e] += x[e]; v[e] += y[e]; }
+    }
+    const int row = table_row(p.positions ? p.positions[t] : t - cu_at(p.cu, b, p.T) - p.has_cls, p.n_pos);
+    float cs[8];
+    table_load4(p.cosp, p.sinp, row, D / 2, c / 2, cs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float e = k[2 * i] * p.scale, o = k[2 * i + 1] * p.scale;
+      k[2 * i] = e * cs[2 * i] + o * cs[2 * i + 1];
+      k[2 * i + 1] = o * cs[2 * i] - e * cs[2 * i + 1];
+    }
+  }
+  put_row8<S>(static_cast<S*>(p.dk) + at, k);
+  put_row8<S>(static_cast<S*>(p.dv) + at, v);
+}
+
+template <typename S, int D, int QT>
+static hipError_t dq(const SeqParams& p0, hipStream_t st) {
+  SeqParams p = p0;
+  p.slots = (int)seq_slots(p.T, p.B, QT == 2 ? 7 : 6);
+  hipLaunchKernelGGL((seq_dq_kernel<S, D, QT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
+  return hipGetLastError();
+}
 template <typename S, int D>
 static hipError_t bwd(const SeqParams& p0, hipStream_t st) {
   hipError_t e = launch_seq_prep(p0, std::is_same<S, bf16>::value ? DT_BF16 : std::is_same<S, f16>::value ? DT_F16 : DT_F32, D, st);
   if (e != hipSuccess) return e;
   SeqParams p = p0;
-  p.slots = (int)seq_slots(p.T, p.B, 6);
-  hipLaunchKernelGGL((seq_dq_kernel<S, D, 1>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
-  e = hipGetLastError();
+  if constexpr (sizeof(S) == 2)
+    e = seq_tile_rows(p.T, p.B, p.H, D, false) == 128 ? dq<S, D, 2>(p, st) : dq<S, D, 1>(p, st);
+  else
+    e = dq<S, D, 1>(p, st);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((seq_dkdv_kernel<S, D, 1>), dim3((unsigned)p.slots * p.Hkv), dim3(kSeqThreads), 0, st, p);
+  p.slots = (int)seq_slots(p.T, p.B, 6);
+  hipLaunchKernelGGL((seq_dkdv_kernel<S, D>), dim3((unsigned)p.slots * p.Hkv * p.parts), dim3(kSeqThreads), 0, st, p);
+  e = hipGetLastError();
+  if (e != hipSuccess || p.parts == 1) return e;
+  constexpr int rows = 256 / (D / 8);
+  hipLaunchKernelGGL((seq_join_kernel<S, D>), dim3((unsigned)((p.T + rows - 1) / rows) * p.Hkv), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 template <typename S>

@@ -248,10 +248,16 @@ static hipError_t fwd(const SeqParams& p0, hipStream_t st) {
   hipLaunchKernelGGL((seq_fwd_kernel<S, D, QT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
   return hipGetLastError();
 }
+template <typename S, int D>
+static hipError_t fwd_rows(const SeqParams& p, hipStream_t st) {
+  if constexpr (sizeof(S) == 2)
+    if (seq_tile_rows(p.T, p.B, p.H, D, false) == 128) return fwd<S, D, 2>(p, st);
+  return fwd<S, D, 1>(p, st);
+}
 template <typename S>
 static hipError_t fwd_d(const SeqParams& p, int D, hipStream_t st) {
-  if (sizeof(S) == 4) return D == 32 ? fwd<S, 32, 1>(p, st) : D == 64 ? fwd<S, 64, 1>(p, st) : D == 128 ? fwd<S, 128, 1>(p, st) : fwd<S, 256, 1>(p, st);
-  return D == 32 ? fwd<S, 32, 1>(p, st) : D == 64 ? fwd<S, 64, 1>(p, st) : D == 128 ? fwd<S, 128, 1>(p, st) : fwd<S, 256, 1>(p, st);
+  return D == 32 ? fwd_rows<S, 32>(p, st) : D == 64 ? fwd_rows<S, 64>(p, st)
+         : D == 128 ? fwd_rows<S, 128>(p, st) : fwd_rows<S, 256>(p, st);
 }
 hipError_t launch_seq_fwd(const SeqParams& p, int dt, int D, hipStream_t st) {
   return dt == DT_BF16 ? fwd_d<bf16>(p, D, st) : dt == DT_F16 ? fwd_d<f16>(p, D, st) : fwd_d<float>(p, D, st);

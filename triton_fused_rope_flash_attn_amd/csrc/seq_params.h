@@ -34,6 +34,9 @@ struct SeqParams {
   void* gcopy;                       // [H, T, D]: dO, where its own rows cannot be streamed (else null)
   float* nl;                         // [H, T]: -LSE * log2 e
   float* nd;                         // [H, T]: -rowsum(dO * O)
+  float* pk;                         // [parts, T, Hkv, D]: sums of the parts of dK / scale (rotated), parts > 1
+  float* pv;                         // and of dV
+  int parts;                         // parts of a key tile's queries
   int T, B, H, Hkv, n_pos, has_cls, causal;
   float scale, c2;                   // softmax scale; times log2 e
   int slots;                         // row slots of the launch (set by the launcher)
@@ -41,6 +44,21 @@ struct SeqParams {
 
 // A slot per 2^lb rows, one more per sequence, and the tokens behind the last one.
 inline int64_t seq_slots(int T, int B, int lb) { return (int64_t)(T >> lb) + B + 1; }
+
+// Rows per workgroup of the forward and of dQ, 128 (two 16-row subtiles per wave) or 64.  Two
+// subtiles halve the LDS reads per product, but cost workgroups, and products above the
+// diagonal.  16-bit tensors; measured (us, forward, 64 / 128 rows; "sequences x tokens, heads"),
+// D 128: 1 x 16384, 8 697 / 517, 24 up to 2048, 16 232 / 197, 8 x 1024, 8 53 / 46, 32 x 512, 16 96
+// / 85, 1 x 4096, 16 101 / 102, 1 x 2048, 16 46 / 52, 32 up to 512 (228 on average), 16 51 / 53; D
+// 64: 1 x 8192, 16 170 / 152, 1 x 4096, 16 57 / 70, 16 up to 2048, 16 99 / 104, 8 x 1024, 16 43 / 49;
+// D 32: 4 x 8192, 8 235 / 214, 4 x 2048, 8 34.8 / 36.3; D 256: 2 x 4096, 8 301 / 272, 8 x 512, 8 53 / 51.
+inline int seq_tile_rows(int T, int B, int H, int D, bool f32) {
+  const int64_t tiles = (int64_t)T * H / 128, mean = T / B;
+  if (f32) return 64;
+  if (D == 256) return tiles >= 256 ? 128 : 64;
+  if (D == 128) return tiles >= 512 && mean >= 256 ? 128 : 64;
+  return tiles >= 1024 && mean >= 4096 ? 128 : 64;
+}
 
 hipError_t launch_seq_prep(const SeqParams& p, int dt, int D, hipStream_t st);
 hipError_t launch_seq_fwd(const SeqParams& p, int dt, int D, hipStream_t st);
@@ -81,14 +99,16 @@ struct DecodeParams {
   const int* positions;  // [B], or null
   CacheParams c;
   void* o;               // [B, H, D]
-  float* sums;           // [B, H, parts, D]: the parts' unnormalised O (parts > 1)
-  float* stats;          // [B, H, parts, 2]: their max logit (log2 units) and row sum
+  float* sums;           // [workers + B, H, D]: unnormalised O of (worker, sequence) pairs
+  float* stats;          // [workers + B, H, 2]: their max logit (log2 units) and row sum
+  int* owners;           // [B, 2]: a sequence's first worker, and how many have a part of it
   int B, H, Hkv, n_pos, has_cls;
-  int parts;             // parts of a sequence's rows
+  int workers;           // workgroups of a key head and query tile
+  int direct;            // worker i has sequence i: nothing is joined
   int g_tiles;           // tiles of 16 query heads in a group
   float c2;
 };
-// Parts of a call: see decode_parts in seq_api.hip.
+// Workers of a call: decode_workers in seq_api.hip.
 hipError_t launch_decode(const DecodeParams& p, int dt, int D, hipStream_t st);
 
 }  // namespace farope
