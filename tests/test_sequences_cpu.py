@@ -181,11 +181,14 @@ def test_c_entries_refuse_descriptors(kw, rc):
 
 
 def test_c_entries_refuse_pointers_and_workspaces():
-    lib, d = _lib.load(), _seq_desc()
+    lib, d = _lib.load(), _seq_desc(tokens=1000)
     assert _fwd(d, q=None) == _lib.ERR_NULL and _fwd(d, cu=None) == _lib.ERR_NULL and _fwd(d, ws=None) == _lib.ERR_NULL
     assert _fwd(d, q=17) == _lib.ERR_ALIGN and _fwd(d, o=24) == _lib.ERR_ALIGN and _fwd(d, cos=20) == _lib.ERR_ALIGN
     n = lib.farope_seq_workspace_elems(ctypes.byref(d), 0, 1, 1)
-    assert n == 10 * 2 * 64 // 2 and _fwd(d, elems=n - 1) == _lib.ERR_SCRATCH
+    assert n > 0 and _fwd(d, elems=n - 1) == _lib.ERR_SCRATCH
+    short = _seq_desc()                                  # short sequences: K is rotated by the tiles
+    assert lib.farope_seq_workspace_elems(ctypes.byref(short), 0, 1, 1) == 0
+    assert lib.farope_seq_workspace_elems(ctypes.byref(short), 0, 0, 1) == 2 * 10 * 2 * 64 // 2
     assert lib.farope_seq_workspace_elems(ctypes.byref(_seq_desc(head_dim=48)), 0, 1, 1) == 0
     assert _fwd(_seq_desc(tokens=0)) == _lib.OK   # nothing to do
     assert lib.farope_seq_fwd(None, 16, S3, 16, S3, 16, S3, 16, 16, None, 16, 16, 16, 16, 0, None) == _lib.ERR_NULL

@@ -53,18 +53,6 @@ __device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
   const int lo = __builtin_amdgcn_ds_bpermute(4 * lane, (int)x), hi = __builtin_amdgcn_ds_bpermute(4 * lane, (int)(x >> 32));
   return (int64_t)((uint64_t)(unsigned)hi << 32 | (unsigned)lo);
 }
-// Inclusive sums over the wave's lanes: DPP shifts within each row of 16 lanes, then the
-// last lane of a row, and of half the wave, added to the rows behind.
-__device__ __forceinline__ unsigned wave_scan(unsigned x) {
-  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
-  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
-  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
-  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
-  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
-  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
-  return x;
-}
-
 template <typename S, int D>
 __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D * sizeof(S) <= 256 ? 2 : 1) decode_kernel(const DecodeParams p) {
   using T = Tile<S, D>;

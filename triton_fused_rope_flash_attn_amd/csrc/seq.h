@@ -191,6 +191,79 @@ __device__ __forceinline__ SeqTile find_tile(const int* __restrict__ cu, int B, 
   if (t.tile >= t.tiles) t.tile = -1;
   return t;
 }
+// Inclusive sums over the wave's lanes: DPP shifts within each row of 16 lanes, then the
+// last lane of a row, and of half the wave, added to the rows behind.
+__device__ __forceinline__ unsigned wave_scan(unsigned x) {
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
+  return x;
+}
+
+// The same, causal, in the order of the tiles' work: the r-th heaviest tile of the call for
+// r = slot (then the tokens behind the last sequence).  Level l holds the tiles with l
+// tiles of their sequence's keys before them (of its queries behind them: `keys`), one of
+// each sequence of more than l tiles.  The workgroups that start last are then the short ones.
+__device__ __forceinline__ SeqTile ordered_tile(const int* __restrict__ cu, int B, int T, int lb, int slot, int lane, bool keys) {
+  int nt[kOrderSeqs / 64];
+#pragma unroll
+  for (int k = 0; k < kOrderSeqs / 64; ++k) {
+    nt[k] = 0;
+    if (64 * k >= B) continue;
+    const int i = 64 * k + lane;
+    if (i < B) {
+      const int n = cu_at(cu, i + 1, T) - cu_at(cu, i, T);
+      nt[k] = n > 0 ? (n + (1 << lb) - 1) >> lb : 0;
+    }
+  }
+  auto from = [&](int l) {   // tiles of levels l and up
+    unsigned n = 0;
+#pragma unroll
+    for (int k = 0; k < kOrderSeqs / 64; ++k) n += nt[k] > l ? (unsigned)(nt[k] - l) : 0u;
+    return __builtin_amdgcn_readlane((int)wave_scan(n), 63);
+  };
+  SeqTile t;
+  const int tiles = from(0);
+  if (slot >= tiles) {
+    t.seq = B;
+    t.start = cu_at(cu, B, T);
+    t.len = T - t.start;
+    t.tiles = (t.len + (1 << lb) - 1) >> lb;
+    t.tile = slot - tiles < t.tiles ? slot - tiles : -1;
+    return t;
+  }
+  int l = 0, above = 0;   // the largest level l with from(l) > slot; above = from(l + 1)
+  for (int hi = tiles; hi - l > 1;) {
+    const int mid = (l + hi) >> 1, n = from(mid);
+    if (n > slot) l = mid; else { hi = mid; above = n; }
+  }
+  int j = slot - above;
+  t.seq = 0;
+#pragma unroll
+  for (int k = 0; k < kOrderSeqs / 64; ++k) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64(nt[k] > l);
+    const int n = __builtin_popcountll(m);
+    if (j >= 0 && j < n) {
+      const int below = __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0u));
+      t.seq = 64 * k + __builtin_ctzll(__builtin_amdgcn_ballot_w64((m >> lane & 1) && below == j));
+      t.tiles = __builtin_amdgcn_readlane(nt[k], t.seq & 63);
+    }
+    j -= n;
+  }
+  t.start = cu_at(cu, t.seq, T);
+  const int end = cu_at(cu, t.seq + 1, T);
+  t.len = end > t.start ? end - t.start : 0;
+  t.tile = keys ? t.tiles - 1 - l : l;
+  return t;
+}
+// A workgroup's tile of queries (keys: of keys), heavy ones first.
+__device__ __forceinline__ SeqTile work_tile(const SeqParams& p, int lb, int slot, int lane, bool keys) {
+  if (p.order) return ordered_tile(p.cu, p.B, p.T, lb, slot, lane, keys);
+  return find_tile(p.cu, p.B, p.T, lb, keys ? slot : p.slots - 1 - slot, lane);
+}
 // Sequence of token t (B: none), for the 64 lanes of a wave whose tokens are near each other.
 __device__ __forceinline__ int find_seq(const int* __restrict__ cu, int B, int T, int first, int t, int lane) {
   int lo = 0, n = B + 1;
@@ -224,6 +297,10 @@ __device__ __forceinline__ void table_load4(const float* __restrict__ cosp, cons
   for (int p = 0; p < 4; ++p) { cs[2 * p] = c[p]; cs[2 * p + 1] = s[p]; }
 }
 
+// 8 channels to a staged tile (one or two 16-byte chunks)
+template <typename S, int D>
+__device__ __forceinline__ void put_tile8(S* tile, int r, int col, const float (&x)[8]);
+
 // 8 channels of a row, as floats
 template <typename S>
 __device__ __forceinline__ void row8(const S* __restrict__ p, int64_t sd, bool vec, float (&x)[8]) { load8<S>(p, sd, vec, x); }
@@ -245,5 +322,42 @@ __device__ __forceinline__ void put_row8(S* __restrict__ p, const float (&x)[8])
     *reinterpret_cast<v8*>(p) = a;
   }
 }
+
+template <typename S, int D>
+__device__ __forceinline__ void put_tile8(S* tile, int r, int col, const float (&x)[8]) {
+  put_row8<S>(tile + Tile<S, D>::at(r, col), x);   // (fp32: pairs of chunks stay adjacent)
+}
+
+// K rows rotated on their way to LDS: a thread loads its 8-channel pieces of a stage and
+// their table entries early, and turns and stores them when the stage before has been
+// read.  For short sequences, whose rows few workgroups read: it takes the place of
+// seq_prep_kernel, whose launch and traffic they would notice.
+template <typename S, int D> struct RotStage {
+  using T = Tile<S, D>;
+  static constexpr int PPR = D / 8, N = T::SR * PPR / kSeqThreads;
+  Raw8<S> raw[N];
+  float cs[N][8];
+  __device__ __forceinline__ void load(const SeqParams& p, const SeqTile& tl, int kvh, int st, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = st * T::SR + (tid + kSeqThreads * i) / PPR, c = 8 * (tid % PPR);
+      const int rc = r < tl.len ? r : tl.len - 1;   // (keys past the end are masked)
+      const int64_t tok = tl.start + rc;
+      raw[i] = load_raw8<S>(static_cast<const S*>(p.k) + tok * p.sk[0] + kvh * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k);
+      table_load4(p.cosp, p.sinp, table_row(p.positions ? p.positions[tok] : rc - p.has_cls, p.n_pos), D / 2, c / 2, cs[i]);
+    }
+  }
+  __device__ __forceinline__ void store(const SeqParams& p, S* dst, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float x[8];
+      unpack8(raw[i], x);
+      rope_rotate8(x, cs[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= p.c2;
+      put_tile8<S, D>(dst, (tid + kSeqThreads * i) / PPR, 8 * (tid % PPR), x);
+    }
+  }
+};
 
 }  // namespace farope

@@ -89,12 +89,23 @@ int dkdv_parts(const farope_seq_desc* d) {
   if (parts > stages) parts = stages;
   return parts < 1 ? 1 : (int)parts;
 }
+// Short sequences: the tile kernels rotate K themselves.  Measured (us, rotated rows in a pass of
+// their own / rotated by the tiles; "sequences x tokens, heads", B backward too), D 64: 1 x 197, 12
+// 13.5 / 9.0, 4 x 197, 12 11.2 / 9.0, B 58 / 49, 64 x 100, 12 25.2 / 20.1, B 79 / 75, 1 x 400, 12 11.5 /
+// 12.4, 64 x 150, 12 B 103 / 104, 64 x 197, 12 36.0 / 36.8, 1 x 1024, 16 16 / 23; D 32: 128 up to 100, 8
+// B 91 / 81; D 128: 1 x 100, 8 11.4 / 9.4, 1 x 197, 12 13.0 / 13.3, 4 x 512, 16 23 / 28.
+bool rotates_itself(const farope_seq_desc* d, bool v_streams) {
+  if (!v_streams || d->head_dim > 128) return false;
+  const int mean = d->tokens / d->seqs;
+  if (d->head_dim == 128) return d->tokens <= 128;
+  return mean <= 128 || (mean <= 256 && d->tokens <= 1024);
+}
 SeqWs seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_streams) {
   const int64_t es = elem_size(d->dtype), kv = (int64_t)d->tokens * d->kv_heads * d->head_dim * es / 4;
   const int64_t q = (int64_t)d->tokens * d->heads * d->head_dim * es / 4, rows = (int64_t)d->tokens * d->heads;
   auto al = [](int64_t x) { return (x + 63) & ~int64_t(63); };
   SeqWs w{};
-  w.vcopy = al(kv);
+  w.vcopy = rotates_itself(d, v_streams) ? 0 : al(kv);
   w.qhat = w.vcopy + (v_streams ? 0 : al(kv));
   w.gcopy = w.qhat + (backward ? al(q) : 0);
   w.nl = w.gcopy + (backward && !g_streams ? al(q) : 0);
@@ -209,17 +220,17 @@ int farope_seq_fwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
   FAROPE_TRY(check_inputs(desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu));
   FAROPE_TRY(check_ptr(o, 16));
   FAROPE_TRY(check_ptr(lse, 4));
-  FAROPE_TRY(check_ptr(ws, 16));
   const bool vs = streams(desc, v, v_stride);
   const SeqWs w = seq_ws(desc, false, vs, true);
+  if (w.total) FAROPE_TRY(check_ptr(ws, 16));
   if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
   SeqParams p{};
   fill(p, desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu);
   p.o = o; p.lse = lse;
-  p.khat = ws;
+  p.khat = rotates_itself(desc, vs) ? nullptr : ws;
   p.vcopy = vs ? nullptr : ws + w.vcopy;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  FAROPE_TRY(launch_rc(launch_seq_prep(p, desc->dtype, desc->head_dim, st)));
+  if (p.khat) FAROPE_TRY(launch_rc(launch_seq_prep(p, desc->dtype, desc->head_dim, st)));
   return launch_rc(launch_seq_fwd(p, desc->dtype, desc->head_dim, st));
 }
 
@@ -251,7 +262,7 @@ int farope_seq_bwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
   p.o = const_cast<void*>(o);
   p.lse = const_cast<float*>(lse);
   p.dq = dq; p.dk = dk; p.dv = dv;
-  p.khat = ws;
+  p.khat = rotates_itself(desc, vs) ? nullptr : ws;
   p.vcopy = vs ? nullptr : ws + w.vcopy;
   p.qhat = ws + w.qhat;
   p.gcopy = gs ? nullptr : ws + w.gcopy;

@@ -5,7 +5,7 @@
 //   dQ_i = R^T scale sum_j dS_ij R k_j
 //   dK_j = R^T scale sum_i dS_ij R q_i over the query heads of the key head
 //
-// Three launches:
+// Three launches (short sequences: the last two, which then rotate K themselves):
 //   seq_prep_kernel   K-hat * c2 rows (c2 = scale * log2 e)
 //   seq_dq_kernel     query tiles: dQ; also -delta, -LSE * log2 e and the rotated Q rows
 //   seq_dkdv_kernel   key tiles: dK, dV, one pass over the group's query heads, so the
@@ -26,18 +26,19 @@ template <typename S> __device__ __forceinline__ void last_sum(f32x4& acc, f32x4
   if constexpr (sizeof(S) == 4) acc += x;
 }
 
-// Gradient rows of a 16-row subtile: lane holds row `row`, channels 16d + 4lg + (0..3) of
-// each acc[d]; rows past the range of r drop.  turn: rotated back by the row of its token.
-template <typename S, int D>
-__device__ __forceinline__ void store_rows(const f32x4 (&acc)[D / 16], float factor, bool turn, const SeqParams& p, int table,
-                                           __amdgpu_buffer_rsrc_t r, unsigned off, int lg) {
-  f32x4 g[D / 16];
+// Gradient rows of a 16-row subtile: lane holds row `row` (byte offset off), channels
+// c0 + 16d + 4lg + (0..3) of each acc[d]; rows past the range of r drop.  turn: rotated back by
+// the row of its token.
+template <typename S, int D, int N>
+__device__ __forceinline__ void store_tiles(const f32x4 (&acc)[N], int c0, float factor, bool turn, const SeqParams& p, int table,
+                                            __amdgpu_buffer_rsrc_t r, unsigned off, int lg) {
+  f32x4 g[N];
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d) {
+  for (int d = 0; d < N; ++d) {
     g[d] = acc[d] * factor;
     if (turn && table >= 0) {
       typedef float f2 __attribute__((ext_vector_type(2)));
-      const int64_t at = (int64_t)table * (D / 2) + 8 * d + 2 * lg;
+      const int64_t at = (int64_t)table * (D / 2) + c0 / 2 + 8 * d + 2 * lg;
       const f2 c = *reinterpret_cast<const f2*>(p.cosp + at), s = *reinterpret_cast<const f2*>(p.sinp + at);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -49,30 +50,41 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[D / 16], float fac
   }
   if constexpr (sizeof(S) == 4) {
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) buf_store16(__builtin_bit_cast(u32x4, g[d]), r, off + (unsigned)(16 * d + 4 * lg) * 4u, 0u);
+    for (int d = 0; d < N; ++d) buf_store16(__builtin_bit_cast(u32x4, g[d]), r, off + (unsigned)(c0 + 16 * d + 4 * lg) * 4u, 0u);
   } else {
-    // lane groups lg and lg^1 trade halves so that each lane stores 8 consecutive channels
+    u32x2 w[N];
 #pragma unroll
-    for (int d0 = 0; d0 < D / 16; d0 += 2) {
-      u32x2 w[2];
+    for (int d = 0; d < N; ++d) {
+      typedef S s4 __attribute__((ext_vector_type(4)));
+      s4 a;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        typedef S s4 __attribute__((ext_vector_type(4)));
-        s4 a;
+      for (int e = 0; e < 4; ++e) a[e] = (S)g[d][e];
+      __builtin_memcpy(&w[d], &a, 8);
+    }
+    if constexpr (N % 2) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = (S)g[d0 + j][e];
-        __builtin_memcpy(&w[j], &a, 8);
+      for (int d = 0; d < N; ++d)
+        __builtin_amdgcn_raw_buffer_store_b64(w[d], r, off + (unsigned)(c0 + 16 * d + 4 * lg) * 2u, 0u, 0);
+    } else {
+      // lane groups lg and lg^1 trade halves so that each lane stores 8 consecutive channels
+#pragma unroll
+      for (int d0 = 0; d0 < N; d0 += 2) {
+        u32x4 x;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const auto y = __builtin_amdgcn_permlane16_swap(w[d0][k], w[d0 + 1][k], false, false);
+          x[k] = y[0];
+          x[2 + k] = y[1];
+        }
+        buf_store16(x, r, off + (unsigned)(c0 + 16 * (d0 + (lg & 1)) + 4 * (lg & 2)) * 2u, 0u);
       }
-      u32x4 x;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const auto y = __builtin_amdgcn_permlane16_swap(w[0][k], w[1][k], false, false);
-        x[k] = y[0];
-        x[2 + k] = y[1];
-      }
-      buf_store16(x, r, off + (unsigned)(16 * (d0 + (lg & 1)) + 4 * (lg & 2)) * 2u, 0u);
     }
   }
+}
+template <typename S, int D>
+__device__ __forceinline__ void store_rows(const f32x4 (&acc)[D / 16], float factor, bool turn, const SeqParams& p, int table,
+                                           __amdgpu_buffer_rsrc_t r, unsigned off, int lg) {
+  store_tiles<S, D, D / 16>(acc, 0, factor, turn, p, table, r, off, lg);
 }
 
 // rows of zeros: tokens behind the last sequence
@@ -88,7 +100,7 @@ __device__ __forceinline__ void zero_rows(S* base, int64_t stride, int rows, int
 // dQ of 64 QT query rows of one head.  S^T = K-hat Q-hat^T and dP^T = V dO^T per
 // 32-key block; their output rows are the k-slots of dQ-hat^T += K-hat^T dS^T.
 // ---------------------------------------------------------------------------
-template <typename S, int D, int QT>
+template <typename S, int D, int QT, bool ROT>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 ? 2 : 3)
 seq_dq_kernel(const SeqParams p) {
   using C = typename SeqComp<S>::C;
@@ -100,9 +112,9 @@ seq_dq_kernel(const SeqParams p) {
   const int tid = thread_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lr = lane & 15, lg = lane >> 4;
-  const int slot = p.slots - 1 - block_id() / p.H, hx = block_id() % p.H;   // (as in the forward)
+  const int slot = block_id() / p.H, hx = block_id() % p.H;   // (as in the forward)
   const int kvh = hx % p.Hkv, head = kvh * (p.H / p.Hkv) + hx / p.Hkv;
-  const SeqTile tl = find_tile(p.cu, p.B, p.T, LB, slot, lane);
+  const SeqTile tl = work_tile(p, LB, slot, lane, false);
   if (tl.tile < 0) return;
   const int q0 = tl.tile << LB, rows = tl.len - q0 < (1 << LB) ? tl.len - q0 : 1 << LB;
   const int64_t tok0 = tl.start + q0;
@@ -113,16 +125,21 @@ seq_dq_kernel(const SeqParams p) {
   }
 
   SeqStream<S, D> srcK, srcV;
-  srcK.lanes(D, wave, lane);
-  srcK.base(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
-  if (p.vcopy) {
+  RotStage<S, D> rot;
+  if constexpr (ROT) {
+    rot.load(p, tl, kvh, 0, tid);
+  } else {
+    srcK.lanes(D, wave, lane);
+    srcK.base(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
+    srcK.load(sK0, wave, 0);
+  }
+  if (!ROT && p.vcopy) {
     srcV.lanes(D, wave, lane);
     srcV.base(static_cast<const S*>(p.vcopy) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
   } else {
     srcV.lanes(p.sv[0], wave, lane);
     srcV.base(static_cast<const S*>(p.v) + tl.start * p.sv[0] + kvh * p.sv[1], tl.len);
   }
-  srcK.load(sK0, wave, 0);
   srcV.load(sV0, wave, 0);
 
   const int row0 = wave * 16 * QT + lr;   // of the tile; subtile t: + 16 t
@@ -223,7 +240,8 @@ seq_dq_kernel(const SeqParams p) {
       __attribute__((always_inline)) {
     seq_stage_barrier();
     if (st + 1 < ns) {
-      srcK.load(kn, wave, (st + 1) * SR);
+      if constexpr (ROT) rot.load(p, tl, kvh, st + 1, tid);
+      else srcK.load(kn, wave, (st + 1) * SR);
       srcV.load(vn, wave, (st + 1) * SR);
     }
     const int k0 = st * SR;
@@ -233,7 +251,9 @@ seq_dq_kernel(const SeqParams p) {
       for (int j = 0; j < NB; ++j)
         block(tail, k0 + 32 * j, k + 32 * j * D, v + 32 * j * D);
     }
+    if (ROT && st + 1 < ns) rot.store(p, kn, tid);   // (read in the stage before this one)
   };
+  if constexpr (ROT) rot.store(p, sK0, tid);
   for (int st = 0; st < ns; st += 2) {
     stage(st, sK0, sV0, sK1, sV1);
     if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
@@ -268,7 +288,7 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   // earlier keys (seen by more queries) come first in each sequence
   const int part = block_id() % p.parts, rest = block_id() / p.parts;
   const int slot = rest / p.Hkv, kvh = rest % p.Hkv, group = p.H / p.Hkv;
-  const SeqTile tl = find_tile(p.cu, p.B, p.T, LB, slot, lane);
+  const SeqTile tl = work_tile(p, LB, slot, lane, true);
   if (tl.tile < 0) return;
   const int k0 = tl.tile << LB, rows = tl.len - k0 < (1 << LB) ? tl.len - k0 : 1 << LB;
   const int64_t tok0 = tl.start + k0;
@@ -313,14 +333,22 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   Frag kf[KS], vf[KS];
   const int rc = row0 < rows ? row0 : rows - 1;
   const int64_t tok = tok0 + rc;
-  const S* const kp = static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D;
   const S* const vp = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1];
   const int trow = table_row(p.positions ? p.positions[tok] : k0 + rc - p.has_cls, p.n_pos);
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     const int c = 32 * s + 8 * lg;
     float x[8];
-    row8<S>(kp + c, 1, true, x);
+    if (p.khat) {
+      row8<S>(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c, 1, true, x);
+    } else {
+      float cs[8];
+      row8<S>(static_cast<const S*>(p.k) + tok * p.sk[0] + kvh * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x);
+      table_load4(p.cosp, p.sinp, trow, D / 2, c / 2, cs);
+      rope_rotate8(x, cs);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= p.c2;
+    }
     kf[s] = C::make(x);
     row8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
     vf[s] = C::make(x);
@@ -402,6 +430,216 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   store_rows<S, D>(dv, 1.f, false, p, trow, rdV, (unsigned)row0 * row_b, lg);
 }
 
+// ---------------------------------------------------------------------------
+// The same for 16-bit tensors at head_dim 128, bound otherwise by the LDS reads of waves
+// that each need every query and dO row of a stage, both as rows and as columns.
+// Here wave w takes one half of a stage's 64 queries against one half of the 64 keys
+// (whose K-hat and V rows are operands in its registers) and leaves P and dS in LDS; then
+// it takes its 32 channels of dV^T += dO^T P and dK-hat^T += Q-hat^T dS.  P and dS lie in
+// LDS as the operands of those products.  LDS read per stage and wave: 40 KB instead of 64.
+// Measured (us, forward and backward, seq_dkdv_kernel / this): 16384 tokens, 2 key heads
+// 2696 / 2567, 24 up to 2048, 4 key heads 1094 / 1020, 8 x 4096, 8 1580 / 1501; at D 64 it is the
+// slower one (8192, 16 key heads 717 / 742).
+// ---------------------------------------------------------------------------
+template <typename S>
+__global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const SeqParams p) {
+  constexpr int D = 128;
+  using C = typename SeqComp<S>::C;
+  using Frag = typename C::Frag;
+  using T = Tile<S, D>;
+  constexpr int KS = D / 32, SR = T::SR, LB = 6, ND = D / 16 / kSeqNW;   // (ND: 16-channel tiles of a wave)
+  static_assert(SR == 64 && sizeof(S) == 2, "");
+  __shared__ __attribute__((aligned(16))) S sQ0[SR * D], sQ1[SR * D], sG0[SR * D], sG1[SR * D];
+  __shared__ __attribute__((aligned(16))) S sP[2 * 4 * 64 * 8], sS[2 * 4 * 64 * 8];   // [block][subtile][lane][slot]
+
+  const int tid = thread_id();
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  const int part = block_id() % p.parts, rest = block_id() / p.parts;
+  const int slot = rest / p.Hkv, kvh = rest % p.Hkv, group = p.H / p.Hkv;
+  const SeqTile tl = work_tile(p, LB, slot, lane, true);
+  if (tl.tile < 0) return;
+  const int k0 = tl.tile << LB, rows = tl.len - k0 < (1 << LB) ? tl.len - k0 : 1 << LB;
+  const int64_t tok0 = tl.start + k0;
+  S* const dkb = static_cast<S*>(p.dk) + (tok0 * p.Hkv + kvh) * D;
+  S* const dvb = static_cast<S*>(p.dv) + (tok0 * p.Hkv + kvh) * D;
+  if (tl.seq == p.B) {
+    if (p.parts > 1) return;   // (seq_join_kernel's)
+    zero_rows<S, D>(dkb, (int64_t)p.Hkv * D, rows, tid);
+    zero_rows<S, D>(dvb, (int64_t)p.Hkv * D, rows, tid);
+    return;
+  }
+
+  const int first = p.causal ? k0 / SR : 0, per = (tl.len + SR - 1) / SR - first;
+  const int64_t all = (int64_t)per * group;
+  const int begin = (int)(all * part / p.parts), ns = (int)(all * (part + 1) / p.parts) - begin;
+  SeqStream<S, D> srcQ, srcG;
+  srcQ.lanes(D, wave, lane);
+  srcG.lanes(p.gcopy ? D : p.sdo[0], wave, lane);
+  int head = kvh * group + begin / per - 1, lst = per;   // of the stage loaded next
+  const int start = begin % per;
+  bool fresh = true;
+  __amdgpu_buffer_rsrc_t rNl = make_rsrc(p.nl, 0u), rNd = make_rsrc(p.nd, 0u);
+  const int qh = wave & 1, kh = wave >> 1;   // the wave's halves of the queries and keys
+  u32x4 nl_next[2], nd_next[2];              // -LSE2 and -delta of queries 32 qh + 16 h + 4 lg + (0..3)
+  auto load = [&](S* q, S* g) __attribute__((always_inline)) {
+    if (lst == per) {
+      lst = fresh ? start : 0;
+      fresh = false;
+      ++head;
+      const int64_t hrow = (int64_t)head * p.T + tl.start;
+      srcQ.base(static_cast<const S*>(p.qhat) + hrow * D, tl.len);
+      srcG.base(p.gcopy ? static_cast<const S*>(p.gcopy) + hrow * D
+                        : static_cast<const S*>(p.dout) + tl.start * p.sdo[0] + head * p.sdo[1], tl.len);
+      rNl = make_rsrc(p.nl + hrow, (unsigned)tl.len * 4u);
+      rNd = make_rsrc(p.nd + hrow, (unsigned)tl.len * 4u);
+    }
+    const int r0 = (first + lst) * SR;
+    srcQ.load(q, wave, r0);
+    srcG.load(g, wave, r0);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned at = (unsigned)(r0 + 32 * qh + 16 * h + 4 * lg) * 4u;
+      nl_next[h] = __builtin_amdgcn_raw_buffer_load_b128(rNl, at, 0u, 0);
+      nd_next[h] = __builtin_amdgcn_raw_buffer_load_b128(rNd, at, 0u, 0);
+    }
+    ++lst;
+  };
+  if (ns > 0) load(sQ0, sG0);
+
+  Frag kf[2][KS], vf[2][KS];   // key 32 kh + 16 u + lr
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = 32 * kh + 16 * u + lr, rc = r < rows ? r : rows - 1;
+    const int64_t tok = tok0 + rc;
+    const S* const vp = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1];
+    const int trow = p.khat ? 0 : table_row(p.positions ? p.positions[tok] : k0 + rc - p.has_cls, p.n_pos);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int c = 32 * s + 8 * lg;
+      float x[8];
+      if (p.khat) {
+        row8<S>(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c, 1, true, x);
+      } else {
+        float cs[8];
+        row8<S>(static_cast<const S*>(p.k) + tok * p.sk[0] + kvh * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x);
+        table_load4(p.cosp, p.sinp, trow, D / 2, c / 2, cs);
+        rope_rotate8(x, cs);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= p.c2;
+      }
+      kf[u][s] = C::make(x);
+      row8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
+      vf[u][s] = C::make(x);
+    }
+  }
+  f32x4 dv[4][ND], dk[4][ND];
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dv[u][d] = dk[u][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  FragAt<S, D> at;
+  at.init(lr, lg);
+  const int d0 = wave * ND;
+  int to[ND];   // column reads of the wave's channels
+#pragma unroll
+  for (int d = 0; d < ND; ++d) to[d] = T::at(4 * lg + (lr >> 2), 16 * (d0 + d) + 4 * (lr & 3));
+  const int qrow = 32 * qh * D;
+  const int pw = ((4 * qh + 2 * kh) * 64 + lane) * 8;   // where the lane leaves its P and dS (subtile u, half h: + 512 u + 4 h)
+
+  int cst = start;   // this stage within its head
+  auto stage = [&](int st, const S* __restrict__ q, const S* __restrict__ g, S* __restrict__ qn, S* __restrict__ gn)
+      __attribute__((always_inline)) {
+    seq_stage_barrier();
+    f32x4 nl[2], nd[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      nl[h] = __builtin_bit_cast(f32x4, nl_next[h]);
+      nd[h] = __builtin_bit_cast(f32x4, nd_next[h]);
+    }
+    if (st + 1 < ns) load(qn, gn);
+    const int q0 = (first + cst) * SR;
+    cst = cst + 1 == per ? 0 : cst + 1;
+    const bool tail = q0 + SR > tl.len || (p.causal && q0 < k0 + 64);   // uniform
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 sacc[2], pacc[2];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const Frag a = C::lds(q + qrow + 16 * h * D + at.ao[s]), b = C::lds(g + qrow + 16 * h * D + at.ao[s]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          sacc[u] = C::mma(a, kf[u][s], s == 0 ? nl[h] : sacc[u]);
+          pacc[u] = C::mma(b, vf[u][s], s == 0 ? nd[h] : pacc[u]);
+        }
+      }
+      // query qi + i (of the sequence) exists and sees key k0 + 32 kh + 16 u + lr
+      const int qi = q0 + 32 * qh + 16 * h + 4 * lg, from = p.causal ? k0 + 32 * kh + lr - qi : -64, until = tl.len - qi;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        typedef S s4 __attribute__((ext_vector_type(4)));
+        s4 pv, ds;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = !tail || (i >= from + 16 * u && i < until);
+          const float e = fast_exp2(sacc[u][i]);
+          pv[i] = (S)(in ? e : 0.f);    // (P and dS rounded to the tensors' type for the products)
+          ds[i] = (S)(in ? e * pacc[u][i] : 0.f);
+        }
+        *reinterpret_cast<s4*>(sP + pw + 512 * u + 4 * h) = pv;
+        *reinterpret_cast<s4*>(sS + pw + 512 * u + 4 * h) = ds;
+      }
+    }
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      Frag ag[ND], aq[ND];
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        ag[d] = C::tr(g + 32 * j * D + to[d], g + 32 * j * D + to[d] + 16 * D);
+        aq[d] = C::tr(q + 32 * j * D + to[d], q + 32 * j * D + to[d] + 16 * D);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int o = ((4 * j + u) * 64 + lane) * 8;
+        const Frag pf = C::lds(sP + o), dsf = C::lds(sS + o);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          dv[u][d] = C::mma(ag[d], pf, dv[u][d]);
+          dk[u][d] = C::mma(aq[d], dsf, dk[u][d]);
+        }
+      }
+    }
+  };
+  for (int st = 0; st < ns; st += 2) {
+    stage(st, sQ0, sG0, sQ1, sG1);
+    if (st + 1 < ns) stage(st + 1, sQ1, sG1, sQ0, sG0);
+  }
+
+  // lane holds key 16 u + lr, channels 16 (d0 + d) + 4lg + (0..3)
+  const unsigned es = p.parts > 1 ? 4u : 2u, row_b = (unsigned)(p.Hkv * D) * es;
+  const unsigned bytes = (unsigned)(rows - 1) * row_b + D * es;
+  if (p.parts > 1) {   // sums as they are, for seq_join_kernel
+    const int64_t w = (((int64_t)part * p.T + tok0) * p.Hkv + kvh) * D;
+    const auto rK = make_rsrc(p.pk + w, bytes), rV = make_rsrc(p.pv + w, bytes);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const unsigned off = (unsigned)(16 * u + lr) * row_b;
+      store_tiles<float, D, ND>(dk[u], 16 * d0, 1.f, false, p, 0, rK, off, lg);
+      store_tiles<float, D, ND>(dv[u], 16 * d0, 1.f, false, p, 0, rV, off, lg);
+    }
+    return;
+  }
+  const auto rK = make_rsrc(dkb, bytes), rV = make_rsrc(dvb, bytes);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = 16 * u + lr, rc = r < rows ? r : rows - 1;
+    const int trow = table_row(p.positions ? p.positions[tok0 + rc] : k0 + rc - p.has_cls, p.n_pos);
+    store_tiles<S, D, ND>(dk[u], 16 * d0, p.scale, true, p, trow, rK, (unsigned)r * row_b, lg);
+    store_tiles<S, D, ND>(dv[u], 16 * d0, 1.f, false, p, trow, rV, (unsigned)r * row_b, lg);
+  }
+}
+
 // dK and dV of the parts' sums, added in order; a thread takes 8 channels of one token
 // and key head.
 template <typename S, int D>
@@ -436,25 +674,36 @@ __global__ void __launch_bounds__(256) seq_join_kernel(const SeqParams p) {
   put_row8<S>(static_cast<S*>(p.dv) + at, v);
 }
 
-template <typename S, int D, int QT>
+template <typename S, int D, int QT, bool ROT>
 static hipError_t dq(const SeqParams& p0, hipStream_t st) {
   SeqParams p = p0;
   p.slots = (int)seq_slots(p.T, p.B, QT == 2 ? 7 : 6);
-  hipLaunchKernelGGL((seq_dq_kernel<S, D, QT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
+  p.order = seq_order(p.T, p.B, D, p.causal);
+  hipLaunchKernelGGL((seq_dq_kernel<S, D, QT, ROT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
   return hipGetLastError();
 }
 template <typename S, int D>
 static hipError_t bwd(const SeqParams& p0, hipStream_t st) {
-  hipError_t e = launch_seq_prep(p0, std::is_same<S, bf16>::value ? DT_BF16 : std::is_same<S, f16>::value ? DT_F16 : DT_F32, D, st);
-  if (e != hipSuccess) return e;
   SeqParams p = p0;
-  if constexpr (sizeof(S) == 2)
-    e = seq_tile_rows(p.T, p.B, p.H, D, false) == 128 ? dq<S, D, 2>(p, st) : dq<S, D, 1>(p, st);
-  else
-    e = dq<S, D, 1>(p, st);
+  hipError_t e = hipSuccess;
+  if (p.khat) {
+    e = launch_seq_prep(p, std::is_same<S, bf16>::value ? DT_BF16 : std::is_same<S, f16>::value ? DT_F16 : DT_F32, D, st);
+    if (e != hipSuccess) return e;
+    if constexpr (sizeof(S) == 2)
+      e = seq_tile_rows(p.T, p.B, p.H, D, false) == 128 ? dq<S, D, 2, false>(p, st) : dq<S, D, 1, false>(p, st);
+    else
+      e = dq<S, D, 1, false>(p, st);
+  } else if constexpr (D <= 128) {
+    e = dq<S, D, 1, true>(p, st);
+  }
   if (e != hipSuccess) return e;
   p.slots = (int)seq_slots(p.T, p.B, 6);
-  hipLaunchKernelGGL((seq_dkdv_kernel<S, D>), dim3((unsigned)p.slots * p.Hkv * p.parts), dim3(kSeqThreads), 0, st, p);
+  p.order = seq_order(p.T, p.B, D, p.causal);
+  const dim3 grid((unsigned)p.slots * p.Hkv * p.parts);
+  if constexpr (sizeof(S) == 2 && D == 128)
+    hipLaunchKernelGGL((seq_dkdv_shared_kernel<S>), grid, dim3(kSeqThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL((seq_dkdv_kernel<S, D>), grid, dim3(kSeqThreads), 0, st, p);
   e = hipGetLastError();
   if (e != hipSuccess || p.parts == 1) return e;
   constexpr int rows = 256 / (D / 8);

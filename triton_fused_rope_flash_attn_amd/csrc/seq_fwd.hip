@@ -6,7 +6,8 @@
 // seq_prep_kernel has written the rotated, scaled K rows; a workgroup of 4 waves
 // takes 64 or 128 query rows of one head and streams its sequence's K-hat and V
 // rows from memory straight to LDS, in double-buffered stages with one barrier
-// each, up to the last row that its queries see.
+// each, up to the last row that its queries see.  Short sequences (ROT) have no
+// such pass: the workgroups rotate K themselves.
 #include <type_traits>
 
 #include "seq.h"
@@ -20,7 +21,7 @@ constexpr float kSeqSlack = 8.0f;   // log2 units: P <= 2^8 between rescales
 // never leaves registers.  The accumulators start at minus the running max, P =
 // exp2 of the product's output; O and the row sum are rescaled only when some logit
 // exceeds the running max by 2^8.
-template <typename S, int D, int QT>
+template <typename S, int D, int QT, bool ROT>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 ? 2 : 3)
 seq_fwd_kernel(const SeqParams p) {
   using C = typename SeqComp<S>::C;
@@ -34,9 +35,9 @@ seq_fwd_kernel(const SeqParams p) {
   const int lr = lane & 15, lg = lane >> 4;
   // heads vary fastest, key heads before the query heads of a group: the workgroups of one
   // key head meet on one XCD when Hkv is a multiple of 8; later rows (more keys) come first
-  const int slot = p.slots - 1 - block_id() / p.H, hx = block_id() % p.H;
+  const int slot = block_id() / p.H, hx = block_id() % p.H;
   const int kvh = hx % p.Hkv, head = kvh * (p.H / p.Hkv) + hx / p.Hkv;
-  const SeqTile tl = find_tile(p.cu, p.B, p.T, LB, slot, lane);
+  const SeqTile tl = work_tile(p, LB, slot, lane, false);
   if (tl.tile < 0) return;
   const int q0 = tl.tile << LB, rows = tl.len - q0 < (1 << LB) ? tl.len - q0 : 1 << LB;
   S* const ob = static_cast<S*>(p.o) + ((int64_t)(tl.start + q0) * p.H + head) * D;
@@ -55,16 +56,21 @@ seq_fwd_kernel(const SeqParams p) {
   }
 
   SeqStream<S, D> srcK, srcV;
-  srcK.lanes(D, wave, lane);
-  srcK.base(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
-  if (p.vcopy) {
+  RotStage<S, D> rot;
+  if constexpr (ROT) {
+    rot.load(p, tl, kvh, 0, tid);
+  } else {
+    srcK.lanes(D, wave, lane);
+    srcK.base(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
+    srcK.load(sK0, wave, 0);
+  }
+  if (!ROT && p.vcopy) {
     srcV.lanes(D, wave, lane);
     srcV.base(static_cast<const S*>(p.vcopy) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
   } else {
     srcV.lanes(p.sv[0], wave, lane);
     srcV.base(static_cast<const S*>(p.v) + tl.start * p.sv[0] + kvh * p.sv[1], tl.len);
   }
-  srcK.load(sK0, wave, 0);
   srcV.load(sV0, wave, 0);
 
   Frag qf[QT][KS];
@@ -189,12 +195,15 @@ seq_fwd_kernel(const SeqParams p) {
       __attribute__((always_inline)) {
     seq_stage_barrier();
     if (st + 1 < ns) {
-      srcK.load(kn, wave, (st + 1) * SR);
+      if constexpr (ROT) rot.load(p, tl, kvh, st + 1, tid);
+      else srcK.load(kn, wave, (st + 1) * SR);
       srcV.load(vn, wave, (st + 1) * SR);
     }
     const int k0 = st * SR;
     if (active && k0 < hi) blocks(k0 + SR > lo, k0, k, v);
+    if (ROT && st + 1 < ns) rot.store(p, kn, tid);   // (read in the stage before this one)
   };
+  if constexpr (ROT) rot.store(p, sK0, tid);
   for (int st = 0; st < ns; st += 2) {
     stage(st, sK0, sV0, sK1, sV1);
     if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
@@ -241,18 +250,21 @@ seq_fwd_kernel(const SeqParams p) {
   }
 }
 
-template <typename S, int D, int QT>
+template <typename S, int D, int QT, bool ROT>
 static hipError_t fwd(const SeqParams& p0, hipStream_t st) {
   SeqParams p = p0;
   p.slots = (int)seq_slots(p.T, p.B, QT == 2 ? 7 : 6);
-  hipLaunchKernelGGL((seq_fwd_kernel<S, D, QT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
+  p.order = seq_order(p.T, p.B, D, p.causal);
+  hipLaunchKernelGGL((seq_fwd_kernel<S, D, QT, ROT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
   return hipGetLastError();
 }
 template <typename S, int D>
 static hipError_t fwd_rows(const SeqParams& p, hipStream_t st) {
+  if constexpr (D <= 128)
+    if (!p.khat) return fwd<S, D, 1, true>(p, st);
   if constexpr (sizeof(S) == 2)
-    if (seq_tile_rows(p.T, p.B, p.H, D, false) == 128) return fwd<S, D, 2>(p, st);
-  return fwd<S, D, 1>(p, st);
+    if (seq_tile_rows(p.T, p.B, p.H, D, false) == 128) return fwd<S, D, 2, false>(p, st);
+  return fwd<S, D, 1, false>(p, st);
 }
 template <typename S>
 static hipError_t fwd_d(const SeqParams& p, int D, hipStream_t st) {

@@ -246,6 +246,9 @@ def _cache_attn_fake(q, k_cache, v_cache, cosp, sinp, page_table, lengths, posit
 
 
 _lib.load_torch_ops()   # (their kernels for GPU tensors, as in attention.py)
+_seq_fwd_op = torch.ops.farope.seq_fwd.default
+_append_op = torch.ops.farope.cache_append.default
+_attn_op = torch.ops.farope.cache_attn.default
 
 
 # ---------------------------------------------------------------------------
@@ -253,7 +256,9 @@ _lib.load_torch_ops()   # (their kernels for GPU tensors, as in attention.py)
 # ---------------------------------------------------------------------------
 def _tables(cos_sin):
     cosp, sinp = cos_sin.tables()
-    return cosp.contiguous(), sinp.contiguous()   # (no copy where they are)
+    if cosp.is_contiguous() and sinp.is_contiguous():
+        return cosp, sinp
+    return cosp.contiguous(), sinp.contiguous()
 
 
 def _scale(head_dim: int) -> float:
@@ -289,7 +294,7 @@ def sdpa_rope_varlen(
     if torch.is_autocast_enabled():
         comp = _sdpa_comp_dtype(Q)
         Q, K, V = Q.to(comp), K.to(comp), V.to(comp)
-    O = torch.ops.farope.seq_fwd(Q, K, V, cosp, sinp, cu_seqlens, positions, causal, has_cls, _scale(Q.shape[-1]))[0]
+    O = _seq_fwd_op(Q, K, V, cosp, sinp, cu_seqlens, positions, causal, has_cls, _scale(Q.shape[-1]))[0]
     return O if O.dtype == dtype else O.to(dtype)
 
 
@@ -323,7 +328,7 @@ def rope_cache_append(
     changes.  No two tokens of a call may share a row.  Not differentiable.
     """
     cosp, sinp = _tables(cos_sin)
-    torch.ops.farope.cache_append(K, V, cosp, sinp, k_cache, v_cache, page_table, lengths, cu_seqlens, positions, has_cls)
+    _append_op(K, V, cosp, sinp, k_cache, v_cache, page_table, lengths, cu_seqlens, positions, has_cls)
 
 
 def sdpa_rope_decode(
@@ -348,4 +353,4 @@ def sdpa_rope_decode(
     or on a page number that is no page of the cache are left out.  No gradients.
     """
     cosp, sinp = _tables(cos_sin)
-    return torch.ops.farope.cache_attn(Q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions, has_cls, _scale(Q.shape[-1]))
+    return _attn_op(Q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions, has_cls, _scale(Q.shape[-1]))
