@@ -259,10 +259,22 @@ __device__ __forceinline__ SeqTile ordered_tile(const int* __restrict__ cu, int 
   t.tile = keys ? t.tiles - 1 - l : l;
   return t;
 }
-// A workgroup's tile of queries (keys: of keys), heavy ones first.
-__device__ __forceinline__ SeqTile work_tile(const SeqParams& p, int lb, int slot, int lane, bool keys) {
-  if (p.order) return ordered_tile(p.cu, p.B, p.T, lb, slot, lane, keys);
-  return find_tile(p.cu, p.B, p.T, lb, keys ? slot : p.slots - 1 - slot, lane);
+// A workgroup's tile of queries (keys: of keys), the later ones first (the earlier), which
+// have more to do in a causal call: from the map that seq_prep_kernel has made, where
+// there is such a pass, so that the heads' workgroups of a slot read 16 bytes instead of
+// searching.
+__device__ __forceinline__ SeqTile slot_tile(const SeqParams& p, int lb, int slot, int lane, bool keys) {
+  const int* const map = keys ? p.map_k : p.map_q;
+  if (!map) return find_tile(p.cu, p.B, p.T, lb, keys ? slot : p.slots - 1 - slot, lane);
+  typedef int i4 __attribute__((ext_vector_type(4)));
+  const i4 m = reinterpret_cast<const i4*>(map)[slot];
+  SeqTile t;
+  t.seq = __builtin_amdgcn_readfirstlane(m[0]);
+  t.start = __builtin_amdgcn_readfirstlane(m[1]);
+  t.len = __builtin_amdgcn_readfirstlane(m[2]);
+  t.tile = __builtin_amdgcn_readfirstlane(m[3]);
+  t.tiles = (t.len + (1 << lb) - 1) >> lb;
+  return t;
 }
 // Sequence of token t (B: none), for the 64 lanes of a wave whose tokens are near each other.
 __device__ __forceinline__ int find_seq(const int* __restrict__ cu, int B, int T, int first, int t, int lane) {

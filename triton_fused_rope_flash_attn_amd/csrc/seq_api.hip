@@ -57,7 +57,8 @@ int check_sizes(const farope_seq_desc* d) {
   if (!offsets_fit(T, row)) return FAROPE_ERR_SHAPE;               // rows of the workspace
   if (d->heads * row > (int64_t(1) << 24)) return FAROPE_ERR_SHAPE;   // (a tile's rows of an output)
   if (seq_slots(d->tokens, d->seqs, 6) * d->heads > kMaxWorkgroups) return FAROPE_ERR_SHAPE;
-  return token_blocks(d) > kMaxWorkgroups ? FAROPE_ERR_SHAPE : FAROPE_OK;
+  // (with the workgroups that find the slots' tiles)
+  return token_blocks(d) + seq_slots(d->tokens, d->seqs, 6) > kMaxWorkgroups ? FAROPE_ERR_SHAPE : FAROPE_OK;
 }
 
 // Workgroups of a call over a paged cache that are resident at once (decode_kernel's registers):
@@ -72,7 +73,7 @@ int64_t decode_wgs(const farope_seq_desc* d) {
 // Workspace, in fp32 elements, each part from a 256-byte boundary.
 constexpr int kMaxParts = 8;
 struct SeqWs {
-  int64_t khat, vcopy, qhat, gcopy, nl, nd, pk, pv, total;
+  int64_t khat, vcopy, map_q, map_k, qhat, gcopy, nl, nd, pk, pv, total;
 };
 // Parts that the queries of a key tile (64 rows) are divided into, joined by a launch of its
 // own: so many that about four workgroups per CU share the work, but none below a stage of
@@ -105,8 +106,12 @@ SeqWs seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_str
   const int64_t q = (int64_t)d->tokens * d->heads * d->head_dim * es / 4, rows = (int64_t)d->tokens * d->heads;
   auto al = [](int64_t x) { return (x + 63) & ~int64_t(63); };
   SeqWs w{};
-  w.vcopy = rotates_itself(d, v_streams) ? 0 : al(kv);
-  w.qhat = w.vcopy + (v_streams ? 0 : al(kv));
+  const bool pass = !rotates_itself(d, v_streams);
+  const int64_t slots = pass ? al(4 * seq_slots(d->tokens, d->seqs, 6)) : 0;
+  w.vcopy = pass ? al(kv) : 0;
+  w.map_q = w.vcopy + (v_streams ? 0 : al(kv));
+  w.map_k = w.map_q + slots;
+  w.qhat = w.map_k + (backward ? slots : 0);
   w.gcopy = w.qhat + (backward ? al(q) : 0);
   w.nl = w.gcopy + (backward && !g_streams ? al(q) : 0);
   w.nd = w.nl + (backward ? al(rows) : 0);
@@ -116,6 +121,23 @@ SeqWs seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_str
   w.pv = w.pk + sums;
   w.total = w.pv + sums;
   return w;
+}
+
+void place(SeqParams& p, const farope_seq_desc* d, const SeqWs& w, float* ws, bool backward, bool v_streams, bool g_streams) {
+  if (!rotates_itself(d, v_streams)) {
+    p.khat = ws;
+    p.map_q = reinterpret_cast<int*>(ws + w.map_q);
+    if (backward) p.map_k = reinterpret_cast<int*>(ws + w.map_k);
+  }
+  if (!v_streams) p.vcopy = ws + w.vcopy;
+  if (!backward) return;
+  p.qhat = ws + w.qhat;
+  if (!g_streams) p.gcopy = ws + w.gcopy;
+  p.nl = ws + w.nl;
+  p.nd = ws + w.nd;
+  p.pk = ws + w.pk;
+  p.pv = ws + w.pv;
+  p.parts = dkdv_parts(d);
 }
 
 void fill(SeqParams& p, const farope_seq_desc* d, const void* q, const int64_t sq[3], const void* k, const int64_t sk[3],
@@ -227,10 +249,9 @@ int farope_seq_fwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
   SeqParams p{};
   fill(p, desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu);
   p.o = o; p.lse = lse;
-  p.khat = rotates_itself(desc, vs) ? nullptr : ws;
-  p.vcopy = vs ? nullptr : ws + w.vcopy;
+  place(p, desc, w, ws, false, vs, true);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p.khat) FAROPE_TRY(launch_rc(launch_seq_prep(p, desc->dtype, desc->head_dim, st)));
+  if (p.khat) FAROPE_TRY(launch_rc(launch_seq_prep(p, desc->dtype, desc->head_dim, false, st)));
   return launch_rc(launch_seq_fwd(p, desc->dtype, desc->head_dim, st));
 }
 
@@ -262,15 +283,7 @@ int farope_seq_bwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
   p.o = const_cast<void*>(o);
   p.lse = const_cast<float*>(lse);
   p.dq = dq; p.dk = dk; p.dv = dv;
-  p.khat = rotates_itself(desc, vs) ? nullptr : ws;
-  p.vcopy = vs ? nullptr : ws + w.vcopy;
-  p.qhat = ws + w.qhat;
-  p.gcopy = gs ? nullptr : ws + w.gcopy;
-  p.nl = ws + w.nl;
-  p.nd = ws + w.nd;
-  p.pk = ws + w.pk;
-  p.pv = ws + w.pv;
-  p.parts = dkdv_parts(desc);
+  place(p, desc, w, ws, true, vs, gs);
   return launch_rc(launch_seq_bwd(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
 }
 

@@ -114,7 +114,7 @@ seq_dq_kernel(const SeqParams p) {
   const int lr = lane & 15, lg = lane >> 4;
   const int slot = block_id() / p.H, hx = block_id() % p.H;   // (as in the forward)
   const int kvh = hx % p.Hkv, head = kvh * (p.H / p.Hkv) + hx / p.Hkv;
-  const SeqTile tl = work_tile(p, LB, slot, lane, false);
+  const SeqTile tl = slot_tile(p, LB, slot, lane, false);
   if (tl.tile < 0) return;
   const int q0 = tl.tile << LB, rows = tl.len - q0 < (1 << LB) ? tl.len - q0 : 1 << LB;
   const int64_t tok0 = tl.start + q0;
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   // earlier keys (seen by more queries) come first in each sequence
   const int part = block_id() % p.parts, rest = block_id() / p.parts;
   const int slot = rest / p.Hkv, kvh = rest % p.Hkv, group = p.H / p.Hkv;
-  const SeqTile tl = work_tile(p, LB, slot, lane, true);
+  const SeqTile tl = slot_tile(p, LB, slot, lane, true);
   if (tl.tile < 0) return;
   const int k0 = tl.tile << LB, rows = tl.len - k0 < (1 << LB) ? tl.len - k0 : 1 << LB;
   const int64_t tok0 = tl.start + k0;
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   const int lr = lane & 15, lg = lane >> 4;
   const int part = block_id() % p.parts, rest = block_id() / p.parts;
   const int slot = rest / p.Hkv, kvh = rest % p.Hkv, group = p.H / p.Hkv;
-  const SeqTile tl = work_tile(p, LB, slot, lane, true);
+  const SeqTile tl = slot_tile(p, LB, slot, lane, true);
   if (tl.tile < 0) return;
   const int k0 = tl.tile << LB, rows = tl.len - k0 < (1 << LB) ? tl.len - k0 : 1 << LB;
   const int64_t tok0 = tl.start + k0;
@@ -678,7 +678,6 @@ template <typename S, int D, int QT, bool ROT>
 static hipError_t dq(const SeqParams& p0, hipStream_t st) {
   SeqParams p = p0;
   p.slots = (int)seq_slots(p.T, p.B, QT == 2 ? 7 : 6);
-  p.order = seq_order(p.T, p.B, D, p.causal);
   hipLaunchKernelGGL((seq_dq_kernel<S, D, QT, ROT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
   return hipGetLastError();
 }
@@ -687,7 +686,7 @@ static hipError_t bwd(const SeqParams& p0, hipStream_t st) {
   SeqParams p = p0;
   hipError_t e = hipSuccess;
   if (p.khat) {
-    e = launch_seq_prep(p, std::is_same<S, bf16>::value ? DT_BF16 : std::is_same<S, f16>::value ? DT_F16 : DT_F32, D, st);
+    e = launch_seq_prep(p, std::is_same<S, bf16>::value ? DT_BF16 : std::is_same<S, f16>::value ? DT_F16 : DT_F32, D, true, st);
     if (e != hipSuccess) return e;
     if constexpr (sizeof(S) == 2)
       e = seq_tile_rows(p.T, p.B, p.H, D, false) == 128 ? dq<S, D, 2, false>(p, st) : dq<S, D, 1, false>(p, st);
@@ -698,7 +697,6 @@ static hipError_t bwd(const SeqParams& p0, hipStream_t st) {
   }
   if (e != hipSuccess) return e;
   p.slots = (int)seq_slots(p.T, p.B, 6);
-  p.order = seq_order(p.T, p.B, D, p.causal);
   const dim3 grid((unsigned)p.slots * p.Hkv * p.parts);
   if constexpr (sizeof(S) == 2 && D == 128)
     hipLaunchKernelGGL((seq_dkdv_shared_kernel<S>), grid, dim3(kSeqThreads), 0, st, p);

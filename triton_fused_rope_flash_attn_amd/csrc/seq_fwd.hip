@@ -37,7 +37,7 @@ seq_fwd_kernel(const SeqParams p) {
   // key head meet on one XCD when Hkv is a multiple of 8; later rows (more keys) come first
   const int slot = block_id() / p.H, hx = block_id() % p.H;
   const int kvh = hx % p.Hkv, head = kvh * (p.H / p.Hkv) + hx / p.Hkv;
-  const SeqTile tl = work_tile(p, LB, slot, lane, false);
+  const SeqTile tl = slot_tile(p, LB, slot, lane, false);
   if (tl.tile < 0) return;
   const int q0 = tl.tile << LB, rows = tl.len - q0 < (1 << LB) ? tl.len - q0 : 1 << LB;
   S* const ob = static_cast<S*>(p.o) + ((int64_t)(tl.start + q0) * p.H + head) * D;
@@ -254,7 +254,6 @@ template <typename S, int D, int QT, bool ROT>
 static hipError_t fwd(const SeqParams& p0, hipStream_t st) {
   SeqParams p = p0;
   p.slots = (int)seq_slots(p.T, p.B, QT == 2 ? 7 : 6);
-  p.order = seq_order(p.T, p.B, D, p.causal);
   hipLaunchKernelGGL((seq_fwd_kernel<S, D, QT, ROT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
   return hipGetLastError();
 }

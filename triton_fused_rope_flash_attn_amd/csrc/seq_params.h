@@ -32,6 +32,8 @@ struct SeqParams {
   void* vcopy;                       // [Hkv, T, D]: V, where its own rows cannot be streamed (else null)
   void* qhat;                        // [H, T, D]: rotated Q rows
   void* gcopy;                       // [H, T, D]: dO, where its own rows cannot be streamed (else null)
+  int* map_q;                        // [slots][4]: the tiles of the query kernels' workgroups (SeqTile); null: none
+  int* map_k;                        // and of the key kernel's
   float* nl;                         // [H, T]: -LSE * log2 e
   float* nd;                         // [H, T]: -rowsum(dO * O)
   float* pk;                         // [parts, T, Hkv, D]: sums of the parts of dK / scale (rotated), parts > 1
@@ -40,7 +42,6 @@ struct SeqParams {
   int T, B, H, Hkv, n_pos, has_cls, causal;
   float scale, c2;                   // softmax scale; times log2 e
   int slots;                         // row slots of the launch (set by the launcher)
-  int order;                         // tiles in the order of their work (ordered_tile; set by the launcher)
 };
 
 // A slot per 2^lb rows, one more per sequence, and the tokens behind the last one.
@@ -62,16 +63,17 @@ inline int seq_tile_rows(int T, int B, int H, int D, bool f32) {
 }
 
 // Whether the workgroups of a causal call come in the order of their work, over all sequences, not
-// sequence by sequence.  The search costs short sequences more than it gives.  Measured (us, by
-// sequence / by work; "sequences up to tokens, heads"), forward, D 128: 24 up to 2048, 16 214 / 194,
-// 8 up to 8192, 8 452 / 413; D 64: 4 up to 8192, 16 331 / 316, 16 up to 2048, 16 100 / 99, 64 up to
-// 577, 12 41 / 44.  Forward and backward: 1029 / 885, 2496 / 2115, 1546 / 1523, 435 / 444, 163 / 169.
+// sequence by sequence (whose tiles then read K and V from L2 one after the other: better for short
+// ones).  Measured (us, by sequence / by work; "sequences up to tokens (mean), heads"), forward, D
+// 128: 24 up to 2048 (943), 16 210 / 190, 8 up to 8192, 8 452 / 413, 32 up to 512 (228), 16 51 / 46; D 64: 16
+// up to 2048 (1124), 16 103 / 98, 8 x 1024, 16 43.8 / 41.7, 64 up to 577 (223), 12 40 / 49.  Forward
+// and backward: 1020 / 894, 2496 / 2115, 203 / 187, 426 / 421, 149 / 154; 200 up to 600 (224), 8 324 / 344.
 constexpr int kOrderSeqs = 256;   // (four sequences per lane of the search)
 inline int seq_order(int T, int B, int D, int causal) {
-  return causal && B > 1 && B <= kOrderSeqs && T / B >= (D >= 128 ? 512 : 2048);
+  return causal && B > 1 && B <= kOrderSeqs && T / B >= (D >= 128 ? 128 : 512);
 }
 
-hipError_t launch_seq_prep(const SeqParams& p, int dt, int D, hipStream_t st);
+hipError_t launch_seq_prep(const SeqParams& p, int dt, int D, bool backward, hipStream_t st);
 hipError_t launch_seq_fwd(const SeqParams& p, int dt, int D, hipStream_t st);
 hipError_t launch_seq_bwd(const SeqParams& p, int dt, int D, hipStream_t st);
 

@@ -5,18 +5,42 @@
 // [Hkv, T, D]; and, where V's own rows cannot be streamed (channels not
 // contiguous, or rows not 16-byte aligned), V copied to the same layout.  A
 // thread takes 8 channels of one token and kPrepHeads key heads, so that their
-// loads are in flight together and share one read of the table row.
+// loads are in flight together and share one read of the table row.  The first
+// workgroups also find the tiles of the slots that the kernels behind will take,
+// one slot a wave.
 #include "seq.h"
 
 namespace farope {
 
 constexpr int kPrepHeads = 4;
+struct SeqMaps {
+  int slots_q, slots_k, lb_q;   // slots of the query and key kernels; rows of a query slot: 2^lb_q
+  int blocks;                   // workgroups that fill the maps
+  int order;                    // tiles in the order of their work
+};
 
 template <typename S, int D>
-__global__ void __launch_bounds__(256) seq_prep_kernel(const SeqParams p, int n_grp) {
+__global__ void __launch_bounds__(256) seq_prep_kernel(const SeqParams p, const SeqMaps m, int n_grp) {
   constexpr int CPR = D / 8, ROWS = 256 / CPR;
-  const int blk = block_id() / n_grp, h0 = (block_id() - blk * n_grp) * kPrepHeads;
   const int tid = thread_id(), lane = tid & 63;
+  if (block_id() < m.blocks) {
+    int slot = 4 * block_id() + __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool keys = slot >= m.slots_q;
+    slot -= keys ? m.slots_q : 0;
+    if (keys && slot >= m.slots_k) return;
+    const int lb = keys ? 6 : m.lb_q;
+    const SeqTile t = m.order ? ordered_tile(p.cu, p.B, p.T, lb, slot, lane, keys)
+                              : find_tile(p.cu, p.B, p.T, lb, keys ? slot : m.slots_q - 1 - slot, lane);
+    int* const to = (keys ? p.map_k : p.map_q) + 4 * (int64_t)slot;
+    if (lane == 0) {
+      to[0] = t.seq;
+      to[1] = t.start;
+      to[2] = t.len;
+      to[3] = t.tile;
+    }
+    return;
+  }
+  const int id = block_id() - m.blocks, blk = id / n_grp, h0 = (id - blk * n_grp) * kPrepHeads;
   const int t0 = blk * ROWS, t = t0 + tid / CPR, c = 8 * (tid % CPR);
   const int tc = t < p.T ? t : p.T - 1;
   const int b = find_seq(p.cu, p.B, p.T, t0, tc, lane);
@@ -44,18 +68,24 @@ __global__ void __launch_bounds__(256) seq_prep_kernel(const SeqParams p, int n_
 }
 
 template <typename S, int D>
-static hipError_t prep(const SeqParams& p, hipStream_t st) {
+static hipError_t prep(const SeqParams& p, bool backward, hipStream_t st) {
+  SeqMaps m{};
+  m.order = seq_order(p.T, p.B, D, p.causal);
+  m.lb_q = seq_tile_rows(p.T, p.B, p.H, D, sizeof(S) == 4) == 128 ? 7 : 6;
+  m.slots_q = (int)seq_slots(p.T, p.B, m.lb_q);
+  m.slots_k = backward ? (int)seq_slots(p.T, p.B, 6) : 0;
+  m.blocks = (m.slots_q + m.slots_k + 3) / 4;
   const int rows = 256 / (D / 8), n_grp = (p.Hkv + kPrepHeads - 1) / kPrepHeads;
   const int n_blk = (p.T + rows - 1) / rows;
-  hipLaunchKernelGGL((seq_prep_kernel<S, D>), dim3(n_blk * n_grp), dim3(256), 0, st, p, n_grp);
+  hipLaunchKernelGGL((seq_prep_kernel<S, D>), dim3((unsigned)m.blocks + (unsigned)n_blk * n_grp), dim3(256), 0, st, p, m, n_grp);
   return hipGetLastError();
 }
 template <typename S>
-static hipError_t prep_d(const SeqParams& p, int D, hipStream_t st) {
-  return D == 32 ? prep<S, 32>(p, st) : D == 64 ? prep<S, 64>(p, st) : D == 128 ? prep<S, 128>(p, st) : prep<S, 256>(p, st);
+static hipError_t prep_d(const SeqParams& p, int D, bool b, hipStream_t st) {
+  return D == 32 ? prep<S, 32>(p, b, st) : D == 64 ? prep<S, 64>(p, b, st) : D == 128 ? prep<S, 128>(p, b, st) : prep<S, 256>(p, b, st);
 }
-hipError_t launch_seq_prep(const SeqParams& p, int dt, int D, hipStream_t st) {
-  return dt == DT_BF16 ? prep_d<bf16>(p, D, st) : dt == DT_F16 ? prep_d<f16>(p, D, st) : prep_d<float>(p, D, st);
+hipError_t launch_seq_prep(const SeqParams& p, int dt, int D, bool b, hipStream_t st) {
+  return dt == DT_BF16 ? prep_d<bf16>(p, D, b, st) : dt == DT_F16 ? prep_d<f16>(p, D, b, st) : prep_d<float>(p, D, b, st);
 }
 
 }  // namespace farope
