@@ -46,12 +46,13 @@ template <> struct SeqComp<float> { using C = CompF32x; };
 // ---------------------------------------------------------------------------
 // Streamed tiles: rows of D elements, unpadded, their 16-byte chunks XOR-swizzled
 // per row with period 16 (as in stream.h: 16-byte reads of 16 rows and the
-// transposed reads are free of bank conflicts).  A stage holds 64 rows, or 32
-// of more than 256 bytes; a 16-byte-per-lane load to LDS fills RPI of them.
+// transposed reads are free of bank conflicts).  A stage holds SR rows; a
+// 16-byte-per-lane load to LDS fills RPI of them.
 // ---------------------------------------------------------------------------
-template <typename S, int D> struct Tile {
+template <typename S, int D> constexpr int kStageRowsOf = D * sizeof(S) <= 256 ? 64 : 32;
+template <typename S, int D, int ROWS = kStageRowsOf<S, D>> struct Tile {
   static constexpr int ES = sizeof(S), RB = D * ES, CPR = RB / 16, EPC = 16 / ES;
-  static constexpr int SR = RB <= 256 ? 64 : 32;
+  static constexpr int SR = ROWS;
   static constexpr int RPI = CPR >= 64 ? 1 : 64 / CPR;
   static constexpr int NI = SR / (kSeqNW * RPI);      // loads per wave and stage
   static constexpr bool kSame = (kSeqNW * RPI) % 16 == 0;   // one swizzle pattern for all of them
@@ -66,8 +67,8 @@ template <typename S, int D> struct Tile {
   }
 };
 
-template <typename S, int D> struct SeqStream {
-  using T = Tile<S, D>;
+template <typename S, int D, int ROWS = kStageRowsOf<S, D>> struct SeqStream {
+  using T = Tile<S, D, ROWS>;
   __amdgpu_buffer_rsrc_t rs;
   unsigned voff[T::kSame ? 1 : T::NI];
   unsigned row_b;     // bytes between rows
@@ -344,8 +345,8 @@ __device__ __forceinline__ void put_tile8(S* tile, int r, int col, const float (
 // their table entries early, and turns and stores them when the stage before has been
 // read.  For short sequences, whose rows few workgroups read: it takes the place of
 // seq_prep_kernel, whose launch and traffic they would notice.
-template <typename S, int D> struct RotStage {
-  using T = Tile<S, D>;
+template <typename S, int D, int ROWS = kStageRowsOf<S, D>> struct RotStage {
+  using T = Tile<S, D, ROWS>;
   static constexpr int PPR = D / 8, N = T::SR * PPR / kSeqThreads;
   Raw8<S> raw[N];
   float cs[N][8];

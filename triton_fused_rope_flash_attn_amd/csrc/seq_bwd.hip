@@ -100,12 +100,14 @@ __device__ __forceinline__ void zero_rows(S* base, int64_t stride, int rows, int
 // dQ of 64 QT query rows of one head.  S^T = K-hat Q-hat^T and dP^T = V dO^T per
 // 32-key block; their output rows are the k-slots of dQ-hat^T += K-hat^T dS^T.
 // ---------------------------------------------------------------------------
+// (Keys of a stage: as in the forward.)
+template <typename S, int D> constexpr int kDqRows = sizeof(S) == 2 && D == 128 ? 32 : kStageRowsOf<S, D>;
 template <typename S, int D, int QT, bool ROT>
-__global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 ? 2 : 3)
+__global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 && (QT == 2 || ROT) ? 2 : 3)
 seq_dq_kernel(const SeqParams p) {
   using C = typename SeqComp<S>::C;
   using Frag = typename C::Frag;
-  using T = Tile<S, D>;
+  using T = Tile<S, D, kDqRows<S, D>>;
   constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, LB = QT == 2 ? 7 : 6;
   __shared__ __attribute__((aligned(16))) S sK0[SR * D], sK1[SR * D], sV0[SR * D], sV1[SR * D];
 
@@ -124,8 +126,8 @@ seq_dq_kernel(const SeqParams p) {
     return;
   }
 
-  SeqStream<S, D> srcK, srcV;
-  RotStage<S, D> rot;
+  SeqStream<S, D, T::SR> srcK, srcV;
+  RotStage<S, D, T::SR> rot;
   if constexpr (ROT) {
     rot.load(p, tl, kvh, 0, tid);
   } else {

@@ -49,17 +49,18 @@ inline int64_t seq_slots(int T, int B, int lb) { return (int64_t)(T >> lb) + B +
 
 // Rows per workgroup of the forward and of dQ, 128 (two 16-row subtiles per wave) or 64.  Two
 // subtiles halve the LDS reads per product, but cost workgroups, and products above the
-// diagonal.  16-bit tensors; measured (us, forward, 64 / 128 rows; "sequences x tokens, heads"),
-// D 128: 1 x 16384, 8 697 / 517, 24 up to 2048, 16 232 / 197, 8 x 1024, 8 53 / 46, 32 x 512, 16 96
-// / 85, 1 x 4096, 16 101 / 102, 1 x 2048, 16 46 / 52, 32 up to 512 (228 on average), 16 51 / 53; D
-// 64: 1 x 8192, 16 170 / 152, 1 x 4096, 16 57 / 70, 16 up to 2048, 16 99 / 104, 8 x 1024, 16 43 / 49;
-// D 32: 4 x 8192, 8 235 / 214, 4 x 2048, 8 34.8 / 36.3; D 256: 2 x 4096, 8 301 / 272, 8 x 512, 8 53 / 51.
+// diagonal.  16-bit tensors; measured (us, forward and backward, 64 / 128 rows; "sequences x
+// tokens, heads" and the call's 128-row tiles), D 128: 24 up to 2048, 16 [2828] 916 / 869, 1 x 16384, 8
+// [1024] 2702 / 2512, 4 up to 4096, 8 [676] 455 / 484, 1 x 4096, 16 [512] 422 / 467, 8 x 1024, 8 [512]
+// 164 / 175, 64 up to 200, 8 [308] 89 / 105.  Forward, D 64: 1 x 8192, 16 [1024] 170 / 152, 1 x 4096, 16
+// [512] 57 / 70, 16 up to 2048, 16 [2248] 99 / 104, 8 x 1024, 16 [1024] 43 / 49; D 32: 4 x 8192, 8 [2048]
+// 235 / 214, 4 x 2048, 8 [512] 34.8 / 36.3; D 256: 2 x 4096, 8 [512] 301 / 272, 8 x 512, 8 [256] 53 / 51.
 inline int seq_tile_rows(int T, int B, int H, int D, bool f32) {
   const int64_t tiles = (int64_t)T * H / 128, mean = T / B;
   if (f32) return 64;
   if (D == 256) return tiles >= 256 ? 128 : 64;
-  if (D == 128) return tiles >= 512 && mean >= 256 ? 128 : 64;
-  return tiles >= 1024 && mean >= 4096 ? 128 : 64;
+  if (D == 128) return tiles >= 4 * 256 && mean >= 256 ? 128 : 64;
+  return tiles >= 4 * 256 && mean >= 4096 ? 128 : 64;
 }
 
 // Whether the workgroups of a causal call come in the order of their work, over all sequences, not
