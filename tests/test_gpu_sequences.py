@@ -199,6 +199,22 @@ def test_autocast():
     compare("autocast", dict(zip(("o", "dq", "dk", "dv"), (o, *g))), ref, BF16)
 
 
+@pytest.mark.parametrize("dtype,D,causal", [(BF16, 64, True), (F16, 128, False), (BF16, 256, True)])
+def test_short_rows_do_not_feel_the_rounding_of_o(dtype, D, causal):
+    """V with a common offset: dP - delta cancels it, where delta does not come from O as stored
+    (u |dO| |O| = 64 u sqrt(D) here, dS of unit scale: several times dQ itself)."""
+    lens = [2, 17, 32, 1]
+    q, k, v, do = inputs(sum(lens), 4, 2, D, dtype)
+    v = (v.float() + 64.0).to(dtype)
+    table = seq_ref.Table(64, D, DEV)
+    ref = seq_ref.varlen(q, k, v, do, table, starts(lens), causal, True)
+    got = grads(q, k, v, do, table, starts(lens), causal=causal)
+    # dP's terms are 64 times dS's scale: sqrt(D) 64 units of 2^-24 of it
+    tol = seq_ref.ROUNDINGS["dq"] * seq_ref.U[dtype] + 64 * 64 * 2.0 ** -24
+    for n in ("dq", "dk"):
+        assert seq_ref.rel(got[n], ref[n]) <= tol, n
+
+
 def test_gradient_against_differences():
     """Central differences of the fp32 forward along random directions."""
     lens, D, eps = [40, 25], 32, 1e-2

@@ -100,14 +100,14 @@ __device__ __forceinline__ void zero_rows(S* base, int64_t stride, int rows, int
 // dQ of 64 QT query rows of one head.  S^T = K-hat Q-hat^T and dP^T = V dO^T per
 // 32-key block; their output rows are the k-slots of dQ-hat^T += K-hat^T dS^T.
 // ---------------------------------------------------------------------------
-// (Keys of a stage: as in the forward.)
-template <typename S, int D> constexpr int kDqRows = sizeof(S) == 2 && D == 128 ? 32 : kStageRowsOf<S, D>;
+// Keys of a stage: as in the forward (short sequences: 64, so that one stage holds them).
+template <typename S, int D, bool ROT> constexpr int kDqRows = sizeof(S) == 2 && D == 128 && !ROT ? 32 : kStageRowsOf<S, D>;
 template <typename S, int D, int QT, bool ROT>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 && (QT == 2 || ROT) ? 2 : 3)
 seq_dq_kernel(const SeqParams p) {
   using C = typename SeqComp<S>::C;
   using Frag = typename C::Frag;
-  using T = Tile<S, D, kDqRows<S, D>>;
+  using T = Tile<S, D, kDqRows<S, D, ROT>>;
   constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, LB = QT == 2 ? 7 : 6;
   __shared__ __attribute__((aligned(16))) S sK0[SR * D], sK1[SR * D], sV0[SR * D], sV1[SR * D];
 
@@ -256,9 +256,53 @@ seq_dq_kernel(const SeqParams p) {
     if (ROT && st + 1 < ns) rot.store(p, kn, tid);   // (read in the stage before this one)
   };
   if constexpr (ROT) rot.store(p, sK0, tid);
-  for (int st = 0; st < ns; st += 2) {
-    stage(st, sK0, sV0, sK1, sV1);
-    if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
+  // The only stage: delta = sum_j P_ij dP_ij, in fp32, while P and dP are in registers.  Rows that
+  // see few keys have an O as large as V, whose rounding as stored would be the largest error
+  // of a dS that cancels (sequences of two tokens, bf16: dQ off by 5e-3 of its norm from O dO).
+  auto whole = [&](const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
+    f32x4 prob[NB][2], pacc[NB][2];
+    const int lim = seen[0] - 4 * lg;
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          prob[j][h] = C::mma(at.row(k + 32 * j * D, s, h), qf[0][s], s == 0 ? first_sum<S>(nl4[0]) : prob[j][h]);
+          pacc[j][h] = C::mma(at.row(v + 32 * j * D, s, h), gf[0][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : pacc[j][h]);
+        }
+        last_sum<S>(prob[j][h], nl4[0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = 32 * j + 16 * h + i < lim;
+          prob[j][h][i] = in ? fast_exp2(prob[j][h][i]) : 0.f;
+          sum += in ? prob[j][h][i] * pacc[j][h][i] : 0.f;
+        }
+      }
+    const float delta = group4_sum(sum);
+    if (row0 < rows && lg == 0) p.nd[hrow + row0] = -delta;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      float ds[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          ds[4 * h + i] = 32 * j + 16 * h + i < lim ? prob[j][h][i] * (pacc[j][h][i] - delta) : 0.f;
+      const Frag dsf = C::make(ds);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[0][d] = C::mma(at.col(k + 32 * j * D, d), dsf, acc[0][d]);
+    }
+  };
+  if (QT == 1 && ns == 1) {   // (uniform)
+    seq_stage_barrier();
+    if (active) whole(sK0, sV0);
+  } else {
+    for (int st = 0; st < ns; st += 2) {
+      stage(st, sK0, sV0, sK1, sV1);
+      if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
+    }
   }
 
   const unsigned row_b = (unsigned)(p.H * D * (int)sizeof(S));

@@ -43,27 +43,29 @@ __global__ void __launch_bounds__(256) seq_prep_kernel(const SeqParams p, const 
   const int id = block_id() - m.blocks, blk = id / n_grp, h0 = (id - blk * n_grp) * kPrepHeads;
   const int t0 = blk * ROWS, t = t0 + tid / CPR, c = 8 * (tid % CPR);
   const int tc = t < p.T ? t : p.T - 1;
+  Raw8<S> k[kPrepHeads], v[kPrepHeads];   // (in flight while the token's sequence is found)
+#pragma unroll
+  for (int i = 0; i < kPrepHeads; ++i) {
+    const int h = h0 + i < p.Hkv ? h0 + i : p.Hkv - 1;
+    k[i] = load_raw8<S>(static_cast<const S*>(p.k) + tc * p.sk[0] + h * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k);
+    if (p.vcopy) v[i] = load_raw8<S>(static_cast<const S*>(p.v) + tc * p.sv[0] + h * p.sv[1] + c * p.sv[2], p.sv[2], p.vec_v);
+  }
   const int b = find_seq(p.cu, p.B, p.T, t0, tc, lane);
   if (t >= p.T || b == p.B) return;   // (no tile reads tokens of no sequence)
   const int row = table_row(p.positions ? p.positions[t] : t - cu_at(p.cu, b, p.T) - p.has_cls, p.n_pos);
-  float x[kPrepHeads][8], v[kPrepHeads][8];
-#pragma unroll
-  for (int i = 0; i < kPrepHeads; ++i) {
-    if (h0 + i >= p.Hkv) break;
-    row8<S>(static_cast<const S*>(p.k) + t * p.sk[0] + (h0 + i) * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x[i]);
-    if (p.vcopy) row8<S>(static_cast<const S*>(p.v) + t * p.sv[0] + (h0 + i) * p.sv[1] + c * p.sv[2], p.sv[2], p.vec_v, v[i]);
-  }
   float cs[8];
   table_load4(p.cosp, p.sinp, row, D / 2, c / 2, cs);
 #pragma unroll
   for (int i = 0; i < kPrepHeads; ++i) {
     if (h0 + i >= p.Hkv) break;
-    rope_rotate8(x[i], cs);
+    float x[8];
+    unpack8(k[i], x);
+    rope_rotate8(x, cs);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[i][e] *= p.c2;
+    for (int e = 0; e < 8; ++e) x[e] *= p.c2;
     const int64_t at = ((int64_t)(h0 + i) * p.T + t) * D + c;
-    put_row8<S>(static_cast<S*>(p.khat) + at, x[i]);
-    if (p.vcopy) put_row8<S>(static_cast<S*>(p.vcopy) + at, v[i]);
+    put_row8<S>(static_cast<S*>(p.khat) + at, x);
+    if (p.vcopy) *reinterpret_cast<Raw8<S>*>(static_cast<S*>(p.vcopy) + at) = v[i];
   }
 }
 
