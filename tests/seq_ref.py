@@ -53,14 +53,14 @@ def rotate(x, table, index, back=False):
     return torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2)
 
 
-def varlen(q, k, v, do, table, cu, causal, has_cls, positions=None):
+def varlen(q, k, v, do, table, cu, causal, has_cls, positions=None, scale=None):
     """{"o", "dq", "dk", "dv", "lse"} in 64 bits on the CPU; rows of no sequence are zeros.
     "dq+", "dk+": what the rows of dQ and dK may be off by where dS cancels."""
     u = U[q.dtype] if q.dtype in U else 0.0
     q, k, v = (t.detach().double().cpu() for t in (q, k, v))
     do = None if do is None else do.detach().double().cpu()
     T, H, D = q.shape
-    group, c = H // k.shape[1], 1.0 / math.sqrt(D)
+    group, c = H // k.shape[1], 1.0 / math.sqrt(D) if scale is None else scale
     out = {"o": torch.zeros_like(q), "dq": torch.zeros_like(q), "dk": torch.zeros_like(k), "dv": torch.zeros_like(v),
            "lse": torch.zeros(H, T, dtype=torch.float64), "dq+": torch.zeros(q.shape[:2], dtype=torch.float64),
            "dk+": torch.zeros(k.shape[:2], dtype=torch.float64)}
@@ -89,7 +89,7 @@ def varlen(q, k, v, do, table, cu, causal, has_cls, positions=None):
             gq[:, h] = ds @ kh[:, g]
             gk[:, g] += ds.t() @ qh[:, h]
             delta = (d * o).abs().sum(1, keepdim=True)
-            off = p * (64 * 2.0 ** -24 * (d.abs() @ v[a:b, g].abs().t() + delta) + u * delta) * c
+            off = p * (64 * 2.0 ** -24 * (d.abs() @ v[a:b, g].abs().t() + delta) + u * delta) * abs(c)
             out["dq+"][a:b, h] = (off @ kh[:, g].abs()).norm(dim=1)
             out["dk+"][a:b, g] += (off.t() @ qh[:, h].abs()).norm(dim=1)
         out["dq"][a:b] = rotate(gq, table, index, back=True)

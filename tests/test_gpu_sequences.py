@@ -215,6 +215,22 @@ def test_short_rows_do_not_feel_the_rounding_of_o(dtype, D, causal):
         assert seq_ref.rel(got[n], ref[n]) <= tol, n
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.25])
+@pytest.mark.parametrize("dtype,lens", [(F16, [40, 9]), (BF16, [300, 70]), (F32, [100, 3])])
+def test_softmax_scale_of_the_op(dtype, lens, scale):
+    """The op takes any scale; at 0 every key weighs the same and dQ and dK are zeros."""
+    T, D = sum(lens), 64
+    q, k, v, do = inputs(T, 4, 2, D, dtype, seed=9)
+    table = seq_ref.Table(300, D, DEV)
+    ref = seq_ref.varlen(q, k, v, do, table, starts(lens), True, True, scale=scale)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o, _ = torch.ops.farope.seq_fwd(*leaves, *table.tables(), starts(lens), None, True, True, scale)
+    got = dict(zip(("o", "dq", "dk", "dv"), (o.detach(), *torch.autograd.grad(o, leaves, do))))
+    if scale == 0:
+        assert (got.pop("dq") == 0).all() and (got.pop("dk") == 0).all()
+    compare(f"scale {scale} {dtype}", got, ref, dtype)
+
+
 def test_gradient_against_differences():
     """Central differences of the fp32 forward along random directions."""
     lens, D, eps = [40, 25], 32, 1e-2

@@ -308,8 +308,8 @@ seq_dq_kernel(const SeqParams p) {
   const unsigned row_b = (unsigned)(p.H * D * (int)sizeof(S));
   const auto rD = make_rsrc(dqb, (unsigned)(rows - 1) * row_b + T::RB);
 #pragma unroll
-  for (int t = 0; t < QT; ++t)   // (K-hat carries c2)
-    store_rows<S, D>(acc[t], p.scale / p.c2, true, p, trow[t], rD, (unsigned)(row0 + 16 * t) * row_b, lg);
+  for (int t = 0; t < QT; ++t)   // (K-hat carries scale * log2 e)
+    store_rows<S, D>(acc[t], kLn2, true, p, trow[t], rD, (unsigned)(row0 + 16 * t) * row_b, lg);
 }
 
 // ---------------------------------------------------------------------------
