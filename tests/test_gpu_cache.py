@@ -6,7 +6,7 @@ import torch
 
 from tests import seq_ref
 from tests._report import LINES
-from triton_fused_rope_flash_attn_amd import rope_cache_append, sdpa_rope_decode, sdpa_rope_varlen
+from triton_fused_rope_flash_attn_amd import CosSinTable, rope_cache_append, sdpa_rope_decode, sdpa_rope_varlen
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -303,6 +303,37 @@ def test_step_captured_and_replayed():
         el += 1
         assert torch.equal(out, sdpa_rope_decode(q, ek, ev, table, pages, el)), i
     assert torch.equal(kc, ek) and torch.equal(vc, ev)
+
+
+@pytest.mark.parametrize("one", [False, True], ids=["two caches", "halves of one tensor"])
+def test_step_compiles_fullgraph(one):
+    H, Hkv, D, page, B = 4, 2, 64, 16, 3
+    pages, n = page_table(B, 4)
+    table = CosSinTable(100.0, 8, D, device=DEV)
+    both = torch.stack(caches(n, page, Hkv, D, BF16))
+    q, k, v = (randn(B, h, D, dtype=BF16, seed=s) for h, s in ((H, 7), (Hkv, 8), (Hkv, 9)))
+    lengths = ints([0, 10, 40])
+
+    def step(q, k, v, kc, vc, lengths):
+        rope_cache_append(k, v, table, kc, vc, pages, lengths)
+        return sdpa_rope_decode(q, kc, vc, table, pages, lengths + 1) * 2
+
+    ek, ev = both[0].clone(), both[1].clone()
+    want = step(q, k, v, ek, ev, lengths)
+    kc, vc = (both[0], both[1]) if one else (both[0].clone(), both[1].clone())
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(q, k, v, kc, vc, lengths)
+    assert torch.equal(got, want) and torch.equal(kc, ek) and torch.equal(vc, ev)
+
+
+def test_pages_shared_by_sequences():
+    """Sequences that share the pages of a common beginning, and one read twice."""
+    page, D = 16, 64
+    pages, n = page_table(4, 40)
+    pages[1, :30] = pages[0, :30]
+    pages[2] = pages[0]
+    kc, vc = caches(n, page, 2, D, BF16)
+    q = randn(4, 8, D, dtype=BF16, seed=3)
+    run_decode("shared pages", q, kc, vc, seq_ref.Table(640, D, DEV), pages, ints([600, 500, 600, 640]))
 
 
 def test_two_streams_at_once():

@@ -283,8 +283,12 @@ def sdpa_rope_varlen(
     is computed in fp32; under autocast all three are cast to its dtype first).
     cu_seqlens: int32 ``[B + 1]`` on the GPU, the sequences' first tokens in ascending
     order from 0 on, then the end of the last; sequences may be empty.  Tokens behind
-    the last sequence come back as zeros, and so do their gradients.
-    causal: token i of a sequence sees its tokens 0 .. i, else all of them.
+    the last sequence come back as zeros, and so do their gradients, whatever they hold.
+    The first start counts as 0, the others are cut to 0 .. T; where they do not ascend,
+    the rows concerned hold no defined values.
+    causal: token i of a sequence sees its tokens 0 .. i, else all of them.  (What is not seen
+    weighs 0; within 63 tokens an infinity or NaN is still multiplied by that 0.  Rows of
+    other sequences enter no sum at all.)
     positions: int32 ``[T]`` table rows, instead of ``i - has_cls``.
 
     Returns O ``[T, H, D]`` of Q's dtype.  Gradients come back for Q, K and V.
