@@ -25,6 +25,11 @@ constexpr float kSeqSlack = 8.0f;   // log2 units: P <= 2^8 between rescales
 // never leaves registers.  The accumulators start at minus the running max, P =
 // exp2 of the product's output; O and the row sum are rescaled only when some logit
 // exceeds the running max by 2^8.
+//
+// 16-bit tensors: Q-hat, K-hat and P are rounded once to their type, as the products' operands.
+// Together with O's own rounding (1.6e-3 of its norm in bf16) that leaves 2.8e-3.  P as a pair of
+// values (hi + lo) measured 2.5e-3, Q-hat too 2.1e-3, at (us, one / P / both) 8 x 1024, 16 heads, D 64
+// 40 / 46 / 51, 64 up to 577, 12 heads, D 64 38 / 43 / 46, 16384 tokens, 8 heads, D 128 538 / 700 / 1573.
 template <typename S, int D, int QT, bool ROT>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : 3)
 seq_fwd_kernel(const SeqParams p) {
