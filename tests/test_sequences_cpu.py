@@ -180,6 +180,11 @@ def test_c_entries_refuse_descriptors(kw, rc):
                                       1 << 20, None) == rc
 
 
+def _map_elems(tokens, seqs):
+    """The tiles' places: 4 integers for each of (T >> 6) + B + 1 slots, in parts of 64."""
+    return -(-4 * ((tokens >> 6) + seqs + 1) // 64) * 64
+
+
 def test_c_entries_refuse_pointers_and_workspaces():
     lib, d = _lib.load(), _seq_desc(tokens=1000)
     assert _fwd(d, q=None) == _lib.ERR_NULL and _fwd(d, cu=None) == _lib.ERR_NULL and _fwd(d, ws=None) == _lib.ERR_NULL
@@ -188,24 +193,26 @@ def test_c_entries_refuse_pointers_and_workspaces():
     assert n > 0 and _fwd(d, elems=n - 1) == _lib.ERR_SCRATCH
     short = _seq_desc()                                  # short sequences: K is rotated by the tiles
     assert lib.farope_seq_workspace_elems(ctypes.byref(short), 0, 1, 1) == 0
-    assert lib.farope_seq_workspace_elems(ctypes.byref(short), 0, 0, 1) == 2 * 10 * 2 * 64 // 2
+    assert lib.farope_seq_workspace_elems(ctypes.byref(short), 0, 0, 1) == 2 * 10 * 2 * 64 // 2 + _map_elems(10, 2)
     assert lib.farope_seq_workspace_elems(ctypes.byref(_seq_desc(head_dim=48)), 0, 1, 1) == 0
     assert _fwd(_seq_desc(tokens=0)) == _lib.OK   # nothing to do
     assert lib.farope_seq_fwd(None, 16, S3, 16, S3, 16, S3, 16, 16, None, 16, 16, 16, 16, 0, None) == _lib.ERR_NULL
 
 
 def test_c_workspace_parts():
-    """K-hat; a copy of V and of dO where their rows cannot be streamed; Q-hat and two row values;
+    """K-hat and the tiles' places (the backward: of queries and of keys); a copy of V and of dO where their rows cannot be streamed; Q-hat and two row values;
     where key tiles are few, the parts' sums of dK and dV."""
     lib = _lib.load()
     d = _seq_desc(tokens=8000, heads=20, kv_heads=10, head_dim=128)
     kv, q, row = 8000 * 10 * 128 // 2, 8000 * 20 * 128 // 2, 8000 * 20
     size = lambda d, *a: lib.farope_seq_workspace_elems(ctypes.byref(d), *a)  # noqa: E731
-    assert size(d, 0, 1, 1) == kv and size(d, 0, 0, 1) == 2 * kv
-    assert size(d, 1, 1, 1) == kv + q + 2 * row and size(d, 1, 0, 0) == 2 * kv + 2 * q + 2 * row
+    m = _map_elems(8000, 2)
+    assert size(d, 0, 1, 1) == kv + m and size(d, 0, 0, 1) == 2 * kv + m
+    assert size(d, 1, 1, 1) == kv + 2 * m + q + 2 * row and size(d, 1, 0, 0) == 2 * kv + 2 * m + 2 * q + 2 * row
     d = _seq_desc(tokens=4096, seqs=1, heads=4, kv_heads=4, head_dim=128)   # 4 x 66 workgroups: 4 parts
     n = 4096 * 4 * 128
-    assert size(d, 0, 1, 1) == n // 2 and size(d, 1, 1, 1) == n + 2 * 4096 * 4 + 2 * 4 * n
+    m = _map_elems(4096, 1)
+    assert size(d, 0, 1, 1) == n // 2 + m and size(d, 1, 1, 1) == n + 2 * m + 2 * 4096 * 4 + 2 * 4 * n
 
 
 @pytest.mark.parametrize("stride,ptr,ok", [
