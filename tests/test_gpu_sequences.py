@@ -231,6 +231,26 @@ def test_softmax_scale_of_the_op(dtype, lens, scale):
     compare(f"scale {scale} {dtype}", got, ref, dtype)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,D,lens", [(BF16, 64, [1, 40, 1]), (F16, 128, [1, 1, 3]), (F16, 128, [300, 1, 700]), (BF16, 256, [1, 65]),
+                                          (F32, 32, [1, 1]), (F32, 64, [200, 1]), (BF16, 32, [1000, 1, 500])])
+def test_rows_that_see_one_key(dtype, D, lens, causal):
+    """P = 1 whatever the logit: dQ of the row is zero, and dK of a key that no other row sees."""
+    T = sum(lens)
+    q, k, v, do = inputs(T, 4, 2, D, dtype, seed=11)
+    table = seq_ref.Table(1000, D, DEV)
+    got = grads(q, k, v, do, table, starts(lens), causal=causal)
+    names = ("o", "dv") if max(lens) == 1 else tuple(got)   # (dQ and dK are zeros then)
+    ref = seq_ref.varlen(q, k, v, do, table, starts(lens), causal, True)
+    compare(f"one key {dtype} D{D} {lens}", {n: got[n] for n in names}, ref, dtype)
+    for a, n in zip(starts(lens, "cpu").tolist(), lens):
+        if causal or n == 1:
+            assert (got["dq"][a] == 0).all()
+        if n == 1:
+            assert (got["dk"][a] == 0).all()
+            assert torch.equal(got["o"][a], v[a].repeat_interleave(2, dim=0))
+
+
 def test_gradient_against_differences():
     """Central differences of the fp32 forward along random directions."""
     lens, D, eps = [40, 25], 32, 1e-2

@@ -100,6 +100,10 @@ __device__ __forceinline__ void zero_rows(S* base, int64_t stride, int rows, int
   }
 }
 
+// What the sums dS^T Q-hat are multiplied by: a sequence of one token has dS = 0, which the sums,
+// with -delta as their start, hold but for rounding.
+__device__ __forceinline__ float dk_factor(const SeqParams& p, int len) { return len == 1 ? 0.f : p.scale; }
+
 // ---------------------------------------------------------------------------
 // dQ of 64 QT query rows of one head.  S^T = K-hat Q-hat^T and dP^T = V dO^T per
 // 32-key block; their output rows are the k-slots of dQ-hat^T += K-hat^T dS^T.
@@ -224,7 +228,7 @@ seq_dq_kernel(const SeqParams p) {
     Frag dsf[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      const int lim = seen[t] - k0 - 4 * lg;
+      const int lim = (seen[t] > 1 ? seen[t] : 0) - k0 - 4 * lg;   // (a row that sees one key: P = 1, dS = 0)
       float ds[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -285,6 +289,7 @@ seq_dq_kernel(const SeqParams p) {
         }
       }
     const float delta = group4_sum(sum);
+    const int dlim = seen[0] > 1 ? lim : 0;   // (as in block)
     if (row0 < rows && lg == 0) p.nd[hrow + row0] = -delta;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
@@ -293,7 +298,7 @@ seq_dq_kernel(const SeqParams p) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          ds[4 * h + i] = 32 * j + 16 * h + i < lim ? prob[j][h][i] * (pacc[j][h][i] - delta) : 0.f;
+          ds[4 * h + i] = 32 * j + 16 * h + i < dlim ? prob[j][h][i] * (pacc[j][h][i] - delta) : 0.f;
       const Frag dsf = C::make(ds);
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[0][d] = C::mma(at.col(k + 32 * j * D, d), dsf, acc[0][d]);
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   const unsigned row_b = (unsigned)(p.Hkv * D * (int)sizeof(S));
   const unsigned bytes = (unsigned)(rows - 1) * row_b + T::RB;
   const auto rdK = make_rsrc(dkb, bytes), rdV = make_rsrc(dvb, bytes);
-  store_rows<S, D>(dk, p.scale, true, p, trow, rdK, (unsigned)row0 * row_b, lg);
+  store_rows<S, D>(dk, dk_factor(p, tl.len), true, p, trow, rdK, (unsigned)row0 * row_b, lg);
   store_rows<S, D>(dv, 1.f, false, p, trow, rdV, (unsigned)row0 * row_b, lg);
 }
 
@@ -689,7 +694,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   for (int u = 0; u < 4; ++u) {
     const int r = 16 * u + lr, rc = r < rows ? r : rows - 1;
     const int trow = table_row(p.positions ? p.positions[tok0 + rc] : k0 + rc - p.has_cls, p.n_pos);
-    store_tiles<S, D, ND>(dk[u], 16 * d0, p.scale, true, p, trow, rK, (unsigned)r * row_b, lg);
+    store_tiles<S, D, ND>(dk[u], 16 * d0, dk_factor(p, tl.len), true, p, trow, rK, (unsigned)r * row_b, lg);
     store_tiles<S, D, ND>(dv[u], 16 * d0, 1.f, false, p, trow, rV, (unsigned)r * row_b, lg);
   }
 }
@@ -714,12 +719,14 @@ __global__ void __launch_bounds__(256) seq_join_kernel(const SeqParams p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) { k[e] += x[e]; v[e] += y[e]; }
     }
-    const int row = table_row(p.positions ? p.positions[t] : t - cu_at(p.cu, b, p.T) - p.has_cls, p.n_pos);
+    const int start = cu_at(p.cu, b, p.T);
+    const int row = table_row(p.positions ? p.positions[t] : t - start - p.has_cls, p.n_pos);
+    const float factor = dk_factor(p, cu_at(p.cu, b + 1, p.T) - start);
     float cs[8];
     table_load4(p.cosp, p.sinp, row, D / 2, c / 2, cs);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float e = k[2 * i] * p.scale, o = k[2 * i + 1] * p.scale;
+      const float e = k[2 * i] * factor, o = k[2 * i + 1] * factor;
       k[2 * i] = e * cs[2 * i] + o * cs[2 * i + 1];
       k[2 * i + 1] = o * cs[2 * i] - e * cs[2 * i + 1];
     }
