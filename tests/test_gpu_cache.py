@@ -193,6 +193,30 @@ def test_append_prompts(dtype):
     run_append(k, v, seq_ref.Table(60, D, DEV), kc, vc, pages, ints(before), lens, cu_seqlens=cu, has_cls=False)
 
 
+def test_append_to_many_sequences():
+    """More sequences than a step of a wave's search covers, many of them without a token."""
+    page, D, B = 4, 32, 4300
+    g = torch.Generator().manual_seed(2)
+    lens, before = (torch.randint(0, 3, (B,), generator=g).tolist() for _ in range(2))
+    pages, n = page_table(B, 1)
+    kc, vc = caches(n, page, 1, D, BF16)
+    k, v = (randn(sum(lens), 1, D, dtype=BF16, seed=s) for s in (4, 5))
+    cu = ints([0, *torch.tensor(lens).cumsum(0).tolist()])
+    run_append(k, v, seq_ref.Table(8, D, DEV), kc, vc, pages, ints(before), lens, cu_seqlens=cu)
+
+
+@pytest.mark.parametrize("per", [4, 40])
+def test_decode_of_many_sequences(per):
+    """A thousand sequences, most of them short or empty: one worker each, and shares over all of them."""
+    page, D, B = 16, 32, 1100
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 12, (B,), generator=g)
+    lens[::97] = torch.randint(0, per * page + 1, (len(lens[::97]),), generator=g)
+    pages, n = page_table(B, per)
+    kc, vc = caches(n, page, 1, D, BF16)
+    run_decode(f"{B} sequences", randn(B, 2, D, dtype=BF16, seed=3), kc, vc, seq_ref.Table(700, D, DEV), pages, ints(lens.tolist()))
+
+
 def test_append_left_out():
     """Tokens past the page table, on no page of the cache, or of a negative length are not stored."""
     page, D = 16, 64

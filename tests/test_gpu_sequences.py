@@ -95,6 +95,33 @@ def test_all_sequences_empty():
     assert all((t == 0).all() for t in got.values())
 
 
+@pytest.mark.parametrize("dtype,D,B,low,high", [(BF16, 32, 4300, 0, 3), (F32, 64, 70, 0, 20), (F16, 128, 256, 120, 150), (BF16, 128, 257, 120, 150)])
+def test_many_sequences(dtype, D, B, low, high):
+    """More sequences than a step of a wave's search covers, and more than the order by work takes."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(low, high + 1, (B,), generator=g).tolist()
+    T = sum(lens) + 5
+    q, k, v, do = inputs(T, 2, 1, D, dtype, seed=13)
+    table = seq_ref.Table(200, D, DEV)
+    cu = starts(lens)
+    compare(f"{B} sequences {dtype} D{D}", grads(q, k, v, do, table, cu), seq_ref.varlen(q, k, v, do, table, cu, True, True), dtype)
+
+
+def test_rows_past_32_bits():
+    """Q, O, dO and dQ of more than 2^31 elements: the last sequences against 64 bits."""
+    H, Hkv, D, n = 256, 2, 128, 32
+    T = (1 << 31) // (H * D) // n * n + 2 * n
+    lens = [n] * (T // n - 1) + [n - 5]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, v, do = (torch.randn(T, h, D, generator=g, device=DEV, dtype=BF16) for h in (H, Hkv, Hkv, H))
+    table = seq_ref.Table(n, D, DEV)
+    got = grads(q, k, v, do, table, starts(lens))
+    a = T - 2 * n
+    ref = seq_ref.varlen(*(t[a:] for t in (q, k, v, do)), table, starts(lens[-2:]), True, True)
+    compare("past 32 bits", {m: got[m][a:] for m in got}, ref, BF16)
+    assert (got["o"][T - 5:] == 0).all() and (got["dq"][T - 5:] == 0).all()
+
+
 def test_no_tokens():
     q, k, v, do = inputs(0, 2, 2, 64, BF16)
     got = grads(q, k, v, do, seq_ref.Table(4, 64, DEV), starts([0]))
