@@ -349,6 +349,16 @@ def test_step_compiles_fullgraph(one):
     assert torch.equal(got, want) and torch.equal(kc, ek) and torch.equal(vc, ev)
 
 
+def test_ops_pass_opcheck():
+    page, D = 16, 64
+    pages, n = page_table(2, 3)
+    kc, vc = caches(n, page, 2, D, BF16)
+    q, k, v = (randn(2, h, D, dtype=BF16, seed=s) for h, s in ((4, 7), (2, 8), (2, 9)))
+    tables = seq_ref.Table(40, D, DEV).tables()
+    torch.library.opcheck(torch.ops.farope.cache_append.default, (k, v, *tables, kc, vc, pages, ints([0, 20]), None, None, True))
+    torch.library.opcheck(torch.ops.farope.cache_attn.default, (q, kc, vc, *tables, pages, ints([1, 21]), None, True, 0.125))
+
+
 def test_pages_shared_by_sequences():
     """Sequences that share the pages of a common beginning, and one read twice."""
     page, D = 16, 64

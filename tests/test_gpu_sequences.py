@@ -381,6 +381,13 @@ def test_compiles_fullgraph():
     assert all(torch.equal(a, want[n]) for a, n in zip(g, ("dq", "dk", "dv")))
 
 
+def test_op_passes_opcheck():
+    q, k, v, _ = inputs(40, 2, 1, 64, F16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    torch.library.opcheck(torch.ops.farope.seq_fwd.default,
+                          (*leaves, *seq_ref.Table(40, 64, DEV).tables(), starts([13, 20]), None, True, True, 0.125))
+
+
 def test_second_derivative_refused():
     q, k, v, do = inputs(20, 1, 1, 64, F32)
     leaves = [t.requires_grad_() for t in (q, k, v)]
