@@ -89,6 +89,42 @@ def test_tokens_behind_the_last_sequence_are_zeros(dtype):
         assert torch.equal(got[n][70:], again[n][70:]), n
 
 
+@pytest.mark.parametrize("dtype,D,H,Hkv,lens", [(BF16, 64, 2, 1, [100, 3]), (BF16, 64, 4, 4, [700, 130, 900]), (F16, 128, 4, 2, [90, 20]),
+                                                (F16, 128, 16, 4, [4100, 300, 700, 64, 2000, 1500]), (BF16, 256, 2, 1, [300, 70]),
+                                                (BF16, 32, 2, 2, [200]), (F32, 64, 2, 1, [140, 33]), (F32, 256, 1, 1, [70])])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_rows_do_not_feel_the_tokens_behind_them(dtype, D, H, Hkv, lens, value):
+    """Causal: K and V of some tokens not finite; the rows before them have the values that they have
+    without, the rows behind see them.  (V alone: channels that it does not touch stay as they are.)"""
+    T = sum(lens)
+    q, k, v, _ = inputs(T, H, Hkv, D, dtype, seed=17)
+    table, cu = seq_ref.Table(max(lens), D, DEV), starts(lens)
+    clean = sdpa_rope_varlen(q, k, v, table, cu)
+    at = [(a, i) for a, n in zip(cu.tolist(), lens) for i in (n * 5 // 8,)]
+    bad_v, bad_k = v.clone(), k.clone()
+    for a, i in at:
+        bad_v[a + i, :, 3] = value
+        bad_k[a + i] = value
+    behind = torch.zeros(T, dtype=torch.bool)
+    for (a, i), n in zip(at, lens):
+        behind[a + i:a + n] = True
+    behind = behind.to(DEV)
+    off = seq_ref.ROUNDINGS["o"] * seq_ref.U[dtype] if dtype != F32 else seq_ref.FP32_UNITS["o"] * seq_ref.U[dtype]
+    for kk in (k, bad_k):
+        got = sdpa_rope_varlen(q, kk, bad_v, table, cu)
+        assert torch.isfinite(got[~behind]).all()
+        # (such a row may be computed again in another order: two results, each within the bound)
+        err, size = (got[~behind].double() - clean[~behind].double()).norm(dim=-1), clean[~behind].double().norm(dim=-1)
+        assert (err <= 4 * off * (size + size.square().mean().sqrt())).all()
+        if kk is k:
+            assert not torch.isfinite(got[behind][..., 3]).any()
+            rest = torch.arange(D, device=DEV) != 3
+            assert torch.isfinite(got[..., rest]).all()
+            assert (got[behind][..., 3].isnan() | (got[behind][..., 3] == value)).all()
+        elif value != value:
+            assert not torch.isfinite(got[behind]).any()
+
+
 def test_all_sequences_empty():
     q, k, v, do = inputs(9, 2, 2, 64, BF16)
     got = grads(q, k, v, do, seq_ref.Table(4, 64, DEV), starts([0, 0]))

@@ -25,6 +25,83 @@ namespace farope {
 template <typename S, int D> constexpr int kFwdRows = sizeof(S) == 2 && D == 128 ? 32 : kStageRowsOf<S, D>;
 constexpr float kSeqSlack = 8.0f;   // log2 units: P <= 2^8 between rescales
 
+// Magnitude bits of x; 0x7f800000 and up are infinities and NaN.  (The kernels are compiled without
+// regard for NaN: the empty asm keeps the compiler from concluding that x is none.)
+__device__ __forceinline__ unsigned magnitude_bits(float x) {
+  unsigned u = __float_as_uint(x);
+  asm volatile("" : "+v"(u));
+  return u & 0x7fffffffu;
+}
+constexpr unsigned kInfBits = 0x7f800000u;
+
+// O of one row again, key by key and only over the keys that it sees: for the rows of a causal
+// call whose sums hold a NaN that may be 0 times an infinity or NaN of a V row behind them.
+// A lane takes channel pairs; m and l are the row's maximum and sum.  Slow, and rarely needed; what
+// finds such rows costs (us, without / with) 24 up to 2048, 16 heads, D 128 173 / 175, 64 up to 577, 12
+// heads, D 64 40.3 / 40.6, one of 16384, D 128 553 / 549.
+template <typename S, int D, bool ROT>
+__device__ __forceinline__ void row_again(const SeqParams& p, const SeqTile& tl, int head, int kvh, int i, float m, float l, int lane) {
+  constexpr int NP = D > 128 ? D / 128 : 1, AHEAD = 4;
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  auto turned = [&](const void* base, const int64_t* st, int64_t tok, int h, int index, int c) {
+    const S* const x = static_cast<const S*>(base) + tok * st[0] + h * st[1] + c * st[2];
+    const float a = (float)x[0], b = (float)x[st[2]];
+    const int row = table_row(p.positions ? p.positions[tok] : index - p.has_cls, p.n_pos);
+    const int64_t at = (int64_t)row * (D / 2) + c / 2;
+    const float co = row < 0 ? 1.f : p.cosp[at], si = row < 0 ? 0.f : p.sinp[at];
+    return f2{a * co - b * si, b * co + a * si};
+  };
+  const bool on = lane < D / 2;
+  f2 q[NP], acc[NP];
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    const f2 x = turned(p.q, p.sq, tl.start + i, head, i, on ? 2 * (lane + 64 * n) : 0);
+    q[n] = f2{(float)(S)x[0], (float)(S)x[1]};
+    acc[n] = f2{0.f, 0.f};
+  }
+  for (int j0 = 0; j0 <= i; j0 += AHEAD) {
+    float s[AHEAD];
+    f2 v[AHEAD][NP];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int j = j0 + u <= i ? j0 + u : i;
+      const int64_t tok = tl.start + j;
+      s[u] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        const int c = on ? 2 * (lane + 64 * n) : 0;
+        f2 k;
+        if constexpr (ROT) {
+          k = turned(p.k, p.sk, tok, kvh, j, c) * p.c2;
+          k = f2{(float)(S)k[0], (float)(S)k[1]};
+        } else {
+          const S* const x = static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c;
+          k = f2{(float)x[0], (float)x[1]};
+        }
+        s[u] += on ? q[n][0] * k[0] + q[n][1] * k[1] : 0.f;
+        const S* const y = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1] + c * p.sv[2];
+        v[u][n] = f2{(float)y[0], (float)y[p.sv[2]]};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) s[u] += __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (lane ^ d), __float_as_int(s[u])));
+      const float w = (float)(S)fast_exp2(s[u] - m);
+      if (j0 + u <= i)
+#pragma unroll
+        for (int n = 0; n < NP; ++n) acc[n] = f2{acc[n][0] + w * v[u][n][0], acc[n][1] + w * v[u][n][1]};
+    }
+  }
+  S* const o = static_cast<S*>(p.o) + ((int64_t)(tl.start + i) * p.H + head) * D;
+  if (on)
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      o[2 * (lane + 64 * n)] = (S)(acc[n][0] / l);
+      o[2 * (lane + 64 * n) + 1] = (S)(acc[n][1] / l);
+    }
+}
+
 // Wave w owns QT 16-query subtiles.  Logits are computed transposed, S^T = K-hat
 // Q-hat^T, so that their output rows (keys) are the k-slots of O^T += V^T P^T and P
 // never leaves registers.  The accumulators start at minus the running max, P =
@@ -224,10 +301,21 @@ seq_fwd_kernel(const SeqParams p) {
   }
 
   // lane holds O[row][16d + 4lg + (0..3)]; rows past the tile drop
+  unsigned again[QT];   // rows (bits) of the subtile that row_again takes
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int row = row0 + 16 * t;
     const float l = group4_sum(l_run[t]);
+    again[t] = 0;
+    if (p.causal) {   // (a sum is not finite if a term is not)
+      f32x4 x = acc[t][0];
+#pragma unroll
+      for (int d = 1; d < DT; ++d) x += acc[t][d];
+      const float sum = (x[0] + x[1]) + (x[2] + x[3]);
+      const uint64_t bad =
+          __builtin_amdgcn_ballot_w64(magnitude_bits(sum) >= kInfBits && magnitude_bits(l) - 1u < kInfBits - 1u && row < rows);
+      again[t] = (unsigned)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
+    }
     const float inv = __builtin_amdgcn_rcpf(l);
     if constexpr (sizeof(S) == 4) {
 #pragma unroll
@@ -261,6 +349,26 @@ seq_fwd_kernel(const SeqParams p) {
     // (lanes lg != 0 write past the range)
     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint((m_run[t] + fast_log2(l)) * kLn2), rL,
                                           (unsigned)(lg == 0 ? row : 1 << LB) * 4u, 0u, 0);
+  }
+  unsigned any = 0;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) any |= again[t];
+  if (any == 0) return;   // (uniform)
+  bool odd = false;       // some key that a row of the wave has met without seeing it holds one
+  for (int j = w0 + 1; j < ns * SR && j < tl.len; ++j)
+    for (int c = lane; c < D; c += 64)
+      odd |= magnitude_bits((float)static_cast<const S*>(p.v)[(tl.start + j) * p.sv[0] + kvh * p.sv[1] + c * p.sv[2]]) >= kInfBits;
+  if (!__any(odd)) return;
+  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the rows as stored above come first
+  asm volatile("" : : : "memory");
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const float l = group4_sum(l_run[t]);
+    for (unsigned left = again[t]; left; left &= left - 1) {
+      const int r = __builtin_ctz(left);
+      row_again<S, D, ROT>(p, tl, head, kvh, w0 + 16 * t + r, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run[t]), r)),
+                           __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l), r)), lane);
+    }
   }
 }
 

@@ -286,9 +286,9 @@ def sdpa_rope_varlen(
     the last sequence come back as zeros, and so do their gradients, whatever they hold.
     The first start counts as 0, the others are cut to 0 .. T; where they do not ascend,
     the rows concerned hold no defined values.
-    causal: token i of a sequence sees its tokens 0 .. i, else all of them.  (What is not seen
-    weighs 0; within 63 tokens an infinity or NaN is still multiplied by that 0.  Rows of
-    other sequences enter no sum at all.)
+    causal: token i of a sequence sees its tokens 0 .. i, else all of them.  What it does not
+    see does not reach O, infinities and NaN included.  (Gradients: an infinity or NaN of Q,
+    K or dO within 63 tokens of a row that has no part in it may reach it as 0 * NaN.)
     positions: int32 ``[T]`` table rows, instead of ``i - has_cls``.
 
     Returns O ``[T, H, D]`` of Q's dtype.  Gradients come back for Q, K and V.
