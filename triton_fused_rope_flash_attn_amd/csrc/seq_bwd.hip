@@ -15,7 +15,7 @@
 //
 // Bound as the forward is.  One sequence of 16384 tokens, 8 heads (2 of keys), D 128, causal: dQ
 // 750 us for its three products (1100 TFLOP/s), dK/dV 1230 for its four (895 TFLOP/s); 64
-// sequences up to 577, 12 heads, D 64: 41 and 43 us, of which waves wait 66% and 55%.
+// sequences up to 577, 12 heads, D 64: 41 and 43 us, of which waves wait 66% and 53%.
 #include <type_traits>
 
 #include "seq.h"
@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   // Last queries first: every tile of a sequence begins with the same rows, which then come from
   // L2.  Measured (us, forward and backward, first / last queries first): 16 sequences up to 2048
   // tokens, 16 heads (4 of keys), D 64 406 / 390, 64 up to 577, 12 143 / 140, 8 x 1024, 8, D 128 159 / 156,
-  // one sequence of 16384 2510 / 2494.
+  // one sequence of 16384 2510 / 2494
+  // (HBM reads of the kernel 1716 / 419 MB).
   const int first = p.causal ? k0 / SR : 0, per = (tl.len + SR - 1) / SR - first;
   const int64_t all = (int64_t)per * group;
   const int begin = (int)(all * part / p.parts), ns = (int)(all * (part + 1) / p.parts) - begin;

@@ -11,8 +11,8 @@
 //
 // Bound by the issue of matrix and vector instructions, which overlap between a SIMD's waves:
 // one sequence of 16384 tokens, 8 heads, D 128, causal 540 us (1020 TFLOP/s; matrix instructions run
-// in 50% of the cycles, vector ones in 40%).  Short sequences wait for latencies: 64 up to 577
-// tokens, 12 heads, D 64 25 us (206 TFLOP/s, waves waiting 56% of their time).
+// in 50% of the cycles, vector ones in 41%).  Short sequences wait for latencies: 64 up to 577
+// tokens, 12 heads, D 64 25 us (206 TFLOP/s, waves waiting 53% of their time).
 #include <type_traits>
 
 #include "seq.h"
