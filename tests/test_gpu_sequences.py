@@ -143,6 +143,17 @@ def test_many_sequences(dtype, D, B, low, high):
     compare(f"{B} sequences {dtype} D{D}", grads(q, k, v, do, table, cu), seq_ref.varlen(q, k, v, do, table, cu, True, True), dtype)
 
 
+@pytest.mark.parametrize("dtype,D,H,lens", [(F16, 32, 36, [4105]), (BF16, 64, 34, [4200]), (F16, 128, 64, [1500, 650]), (BF16, 256, 64, [700, 400])])
+def test_tiles_of_128_rows(dtype, D, H, lens):
+    """Calls large enough for the wider tiles; two of the heads against 64 bits."""
+    q, k, v, do = inputs(sum(lens), H, H, D, dtype, seed=19)
+    table, cu = seq_ref.Table(max(lens), D, DEV), starts(lens)
+    got = grads(q, k, v, do, table, cu)
+    heads = [1, H - 1]
+    ref = seq_ref.varlen(*(t[:, heads] for t in (q, k, v, do)), table, cu, True, True)
+    compare(f"128 rows {dtype} D{D}", {n: x[:, heads] for n, x in got.items()}, ref, dtype)
+
+
 def test_rows_past_32_bits():
     """Q, O, dO and dQ of more than 2^31 elements: the last sequences against 64 bits."""
     H, Hkv, D, n = 256, 2, 128, 32

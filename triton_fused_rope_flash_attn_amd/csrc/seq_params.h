@@ -54,11 +54,13 @@ inline int64_t seq_slots(int T, int B, int lb) { return (int64_t)(T >> lb) + B +
 // [1024] 2702 / 2512, 4 up to 4096, 8 [676] 455 / 484, 1 x 4096, 16 [512] 422 / 467, 8 x 1024, 8 [512]
 // 164 / 175, 64 up to 200, 8 [308] 89 / 105.  Forward, D 64: 1 x 8192, 16 [1024] 170 / 152, 1 x 4096, 16
 // [512] 57 / 70, 16 up to 2048, 16 [2248] 99 / 104, 8 x 1024, 16 [1024] 43 / 49; D 32: 4 x 8192, 8 [2048]
-// 235 / 214, 4 x 2048, 8 [512] 34.8 / 36.3; D 256: 2 x 4096, 8 [512] 301 / 272, 8 x 512, 8 [256] 53 / 51.
+// 235 / 214, 4 x 2048, 8 [512] 34.8 / 36.3.  D 256, forward and backward: 2 x 4096, 8 [512] 1242 / 1173, 16 x
+// 512, 8 [512] 333 / 331, 4 x 1024, 8 [256] 268 / 302, 64 up to 200 (77), 12 [462] 296 / 368, 125 up to 149 (54),
+// 8 [423] 292 / 365.
 inline int seq_tile_rows(int T, int B, int H, int D, bool f32) {
   const int64_t tiles = (int64_t)T * H / 128, mean = T / B;
   if (f32) return 64;
-  if (D == 256) return tiles >= 256 ? 128 : 64;
+  if (D == 256) return tiles >= 2 * 256 && mean >= 256 ? 128 : 64;
   if (D == 128) return tiles >= 4 * 256 && mean >= 256 ? 128 : 64;
   return tiles >= 4 * 256 && mean >= 4096 ? 128 : 64;
 }
