@@ -125,6 +125,15 @@ def test_rows_do_not_feel_the_tokens_behind_them(dtype, D, H, Hkv, lens, value):
             assert not torch.isfinite(got[behind]).any()
 
 
+def test_a_tensor_of_nan():
+    """V not a number from a token on: every row from it on, no row before it; nothing is searched for long."""
+    T, D = 20000, 64
+    q, k, v, _ = inputs(T, 2, 1, D, BF16, seed=23)
+    v[5001:] = float("nan")
+    o = sdpa_rope_varlen(q, k, v, seq_ref.Table(T, D, DEV), starts([T]))
+    assert o[5001:].isnan().all() and torch.isfinite(o[:5001]).all()
+
+
 def test_all_sequences_empty():
     q, k, v, do = inputs(9, 2, 2, 64, BF16)
     got = grads(q, k, v, do, seq_ref.Table(4, 64, DEV), starts([0, 0]))

@@ -36,7 +36,9 @@ constexpr unsigned kInfBits = 0x7f800000u;
 
 // O of one row again, key by key and only over the keys that it sees: for the rows of a causal
 // call whose sums hold a NaN that may be 0 times an infinity or NaN of a V row behind them.
-// A lane takes channel pairs; m and l are the row's maximum and sum.  Slow, and rarely needed; what
+// A lane takes channel pairs; m and l are the row's maximum and sum.  Rarely needed, and slow: one
+// infinity behind 9000 of 16384 tokens, 8 heads, D 128 takes the call from 0.55 to 80 ms (32 rows,
+// a quarter of a microsecond a key), a channel of NaN throughout to 156.  What
 // finds such rows costs (us, without / with) 24 up to 2048, 16 heads, D 128 173 / 175, 64 up to 577, 12
 // heads, D 64 40.3 / 40.6, one of 16384, D 128 553 / 549.
 template <typename S, int D, bool ROT>
@@ -354,11 +356,17 @@ seq_fwd_kernel(const SeqParams p) {
 #pragma unroll
   for (int t = 0; t < QT; ++t) any |= again[t];
   if (any == 0) return;   // (uniform)
-  bool odd = false;       // some key that a row of the wave has met without seeing it holds one
-  for (int j = w0 + 1; j < ns * SR && j < tl.len; ++j)
-    for (int c = lane; c < D; c += 64)
-      odd |= magnitude_bits((float)static_cast<const S*>(p.v)[(tl.start + j) * p.sv[0] + kvh * p.sv[1] + c * p.sv[2]]) >= kInfBits;
-  if (!__any(odd)) return;
+  // Some key that a row of the wave has met without seeing it holds one.  (Where the key that
+  // all of them see is NaN throughout, so is O, and rightly.)
+  auto v_bits = [&](int j, int c) {
+    return magnitude_bits((float)static_cast<const S*>(p.v)[(tl.start + j) * p.sv[0] + kvh * p.sv[1] + c * p.sv[2]]);
+  };
+  bool odd = false, some = false;
+  for (int c = lane; c < D; c += 64) {
+    some |= v_bits(w0, c) <= kInfBits;
+    for (int j = w0 + 1; j < ns * SR && j < tl.len; ++j) odd |= v_bits(j, c) >= kInfBits;
+  }
+  if (!__any(odd) || !__any(some)) return;
   __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the rows as stored above come first
   asm volatile("" : : : "memory");
 #pragma unroll
