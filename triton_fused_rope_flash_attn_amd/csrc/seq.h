@@ -127,26 +127,32 @@ __device__ __forceinline__ void seq_stage_barrier() {
 template <typename S, int D> struct FragAt {
   using C = typename SeqComp<S>::C;
   using T = Tile<S, D>;
-  int ao[D / 32], to[D / 16];
-  int lr, lg;
-  __device__ __forceinline__ void init(int lr_, int lg_) {
-    lr = lr_;
-    lg = lg_;
+  // Column reads: 16 bits, each tile's own; fp32, of rows 4 lg and 4 lg + 2 and the first four
+  // tiles: the swizzle is the same for the row behind an even one, for rows 16 apart and for
+  // tiles 4 apart (it moves chunks within 16), which are then constant steps.  (Held apart, each
+  // tile's and row's, they filled the registers: decode of 16 x 4096 rows, 2 key heads, D 256 126 us
+  // instead of 82; forward and backward of 51 x 290 tokens, 48 heads, D 128 1253 instead of 1140.)
+  static constexpr int NT = sizeof(S) == 2 ? D / 16 : D / 16 < 4 ? D / 16 : 4, NR = sizeof(S) == 2 ? 1 : 2;
+  int ao[D / 32], to[NT][NR];
+  __device__ __forceinline__ void init(int lr, int lg) {
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) ao[s] = T::at(lr, 32 * s + 8 * lg);
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) to[d] = sizeof(S) == 2 ? T::at(4 * lg + (lr >> 2), 16 * d + 4 * (lr & 3)) : 0;
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        to[d][r] = sizeof(S) == 2 ? T::at(4 * lg + (lr >> 2), 16 * d + 4 * (lr & 3)) : T::at(4 * lg + 2 * r, 16 * d + lr);
   }
   __device__ __forceinline__ typename C::Frag row(const S* block, int s, int h) const {
     return C::lds(block + ao[s] + 16 * h * D);
   }
   __device__ __forceinline__ typename C::Frag col(const S* block, int d) const {
     if constexpr (sizeof(S) == 2) {
-      return C::tr(block + to[d], block + to[d] + 16 * D);
+      return C::tr(block + to[d][0], block + to[d][0] + 16 * D);
     } else {
       typename C::Frag f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f.v[e] = block[T::at(16 * (e >> 2) + 4 * lg + (e & 3), 16 * d + lr)];
+      for (int e = 0; e < 8; ++e) f.v[e] = block[to[d & 3][(e >> 1) & 1] + (16 * (e >> 2) + (e & 1)) * D + 64 * (d >> 2)];
       return f;
     }
   }
