@@ -321,8 +321,8 @@ int farope_seq_streams(const farope_seq_desc* desc, const void* x, const int64_t
  * v_streams, dout_streams: farope_seq_streams of V and dout (dout: backward only).
  * The rotated K rows and the tiles' places, unless the sequences are short and V streams
  * (the tiles then rotate K themselves); the copy of V if it is kept; in the backward also
- * the rotated Q rows, two fp32 values per query row and head, the copy of dout if it is
- * kept, and, where key tiles are few, the partial sums of dk and dv.  Nothing in it is kept
+ * the rotated Q rows, two fp32 values per query row and head (three for fp16 at head_dim
+ * 128), the copy of dout if it is kept, and, where key tiles are few, the partial sums of dk and dv.  Nothing in it is kept
  * between calls.  0 on an invalid descriptor. */
 size_t farope_seq_workspace_elems(const farope_seq_desc* desc, int32_t backward, int32_t v_streams, int32_t dout_streams);
 

@@ -451,3 +451,37 @@ def test_second_derivative_refused():
     (dq,) = torch.autograd.grad(o, leaves[:1], do, create_graph=True)
     with pytest.raises(RuntimeError, match="not differentiable again"):
         dq.sum().backward()
+
+
+@pytest.mark.parametrize("D,H,Hkv,lens", [
+    (128, 2, 1, [4096]), (128, 64, 64, [1500, 650]), (64, 2, 1, [2048, 1000]), (64, 34, 34, [4200]), (32, 36, 36, [4105]),
+    (256, 2, 1, [1500]), (256, 64, 64, [700, 400]), (64, 4, 4, [100, 60, 1, 30]), (32, 4, 2, [30, 2, 17]), (128, 2, 2, [90, 20]),
+])
+@pytest.mark.parametrize("sizes", ["dO of 1e-4", "dO of 2e-5", "rows of dO apart", "large dO and V"])
+def test_fp16_gradients_over_its_range(D, H, Hkv, lens, sizes):
+    """dS = P (dP - delta) reaches the products with its eleven bits where P or dO is small, and does not
+    overflow where dO V is large.  The results as stored: half a step, 2^-25, of fp16's subnormals each."""
+    T, g = sum(lens), torch.Generator().manual_seed(27)
+    q, k, v, do = (t.float() for t in inputs(T, H, Hkv, D, F32, seed=29))
+    if sizes == "large dO and V":
+        q, k, v, do = 0.05 * q, 0.05 * k, 32 * v, 500 * do
+    elif sizes == "rows of dO apart":
+        do = do * (10.0 ** (6 * torch.rand(T, 1, 1, generator=g) - 4)).to(DEV)
+    else:
+        do = do * float(sizes[6:])
+    q, k, v, do = (t.to(F16) for t in (q, k, v, do))
+    table, cu = seq_ref.Table(max(lens), D, DEV), starts(lens)
+    got = grads(q, k, v, do, table, cu)
+    if H > 4:
+        heads = [H - 1]
+        got, (q, k, v, do) = {n: x[:, heads] for n, x in got.items()}, (t[:, heads] for t in (q, k, v, do))
+    ref = seq_ref.varlen(q, k, v, do, table, cu, True, True)
+    for n in ("dq", "dk", "dv"):
+        off = (got[n].double().cpu() - ref[n]).norm(dim=-1)
+        tol = seq_ref.ROUNDINGS[n] * seq_ref.U[F16]
+        stored = 2.0 ** -25 * D ** 0.5   # of a row
+        total = tol * ref[n].norm() + stored * off.numel() ** 0.5
+        assert off.norm() <= total, (n, float(off.norm() / total))
+        if n == "dq":   # each row by its own size
+            allowed = 2 * tol * ref[n].norm(dim=-1) + stored + ref["dq+"]
+            assert (off <= allowed).all(), (n, float((off / allowed).max()))

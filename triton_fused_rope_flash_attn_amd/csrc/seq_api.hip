@@ -73,7 +73,7 @@ int64_t decode_wgs(const farope_seq_desc* d) {
 // Workspace, in fp32 elements, each part from a 256-byte boundary.
 constexpr int kMaxParts = 8;
 struct SeqWs {
-  int64_t khat, vcopy, map_q, map_k, qhat, gcopy, nl, nd, pk, pv, total;
+  int64_t khat, vcopy, map_q, map_k, qhat, gcopy, nl, nd, ng, pk, pv, total;
 };
 // Parts that the queries of a key tile (64 rows) are divided into, joined by a launch of its
 // own: so many that about four workgroups per CU share the work, but none below a stage of
@@ -117,7 +117,8 @@ SeqWs seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_str
   w.nd = w.nl + (backward ? al(rows) : 0);
   const int parts = backward ? dkdv_parts(d) : 1;
   const int64_t sums = parts > 1 ? al((int64_t)parts * d->tokens * d->kv_heads * d->head_dim) : 0;
-  w.pk = w.nd + (backward ? al(rows) : 0);
+  w.ng = w.nd + (backward ? al(rows) : 0);
+  w.pk = w.ng + (backward && d->dtype == FAROPE_F16 && d->head_dim == 128 ? al(rows) : 0);
   w.pv = w.pk + sums;
   w.total = w.pv + sums;
   return w;
@@ -135,6 +136,7 @@ void place(SeqParams& p, const farope_seq_desc* d, const SeqWs& w, float* ws, bo
   if (!g_streams) p.gcopy = ws + w.gcopy;
   p.nl = ws + w.nl;
   p.nd = ws + w.nd;
+  p.ng = ws + w.ng;
   p.pk = ws + w.pk;
   p.pv = ws + w.pv;
   p.parts = dkdv_parts(d);

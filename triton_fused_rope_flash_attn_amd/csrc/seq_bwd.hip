@@ -7,7 +7,7 @@
 //
 // Three launches (short sequences: the last two, which then rotate K themselves):
 //   seq_prep_kernel   K-hat * c2 rows (c2 = scale * log2 e)
-//   seq_dq_kernel     query tiles: dQ; also -delta, -LSE * log2 e and the rotated Q rows
+//   seq_dq_kernel     query tiles: dQ; also -delta, -LSE * log2 e and the rotated Q rows (fp16, D 128: dO's norms)
 //   seq_dkdv_kernel   key tiles: dK, dV, one pass over the group's query heads, so the
 //                     sums of shared key heads stay in registers and in one order
 // Both tile kernels stream their rows as the forward does (seq_fwd.hip).  No row of a
@@ -28,6 +28,32 @@ namespace farope {
 template <typename S> __device__ __forceinline__ f32x4 first_sum(f32x4 x) { return sizeof(S) == 4 ? f32x4{0.f, 0.f, 0.f, 0.f} : x; }
 template <typename S> __device__ __forceinline__ void last_sum(f32x4& acc, f32x4 x) {
   if constexpr (sizeof(S) == 4) acc += x;
+}
+
+// fp16's normal values end at 2^-14 and its largest is 65504, while dS = P (dP - delta) of a row
+// of n keys is about |dO| |V| / n.  There the products take 2^ex dS, rounded once, with a power of two that
+// follows the values: where one passes the range, ex goes down and the sums held so far with it; the sums'
+// last factor takes it out (all of it exact).  Without (4096 tokens, D 128) a dO of 1e-4 left dQ and dK
+// off by 1.1e-2 of their norm, where rounding the exact ones to fp16 costs 2.7e-3 and 1.9e-3 (with: 2.8e-3
+// and 2.0e-3), and a dP past 65504 made them NaN.  Forward and backward take 0 to 6% longer for it (us, 24
+// up to 2048, 16 heads, D 128 858 / 880, 64 up to 577, 12 heads, D 64 153 / 158, 2 x 4096, 8 heads, D 256 1169 /
+// 1236).  bf16 has fp32's exponents and needs none.
+template <typename S> constexpr bool kFitDs = std::is_same<S, f16>::value;
+constexpr float kDsMost = 32768.f;
+constexpr int kExMost = 60, kExLeast = -100;
+__device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
+// The exponent that puts m >= 0 into [2^top, 2 * 2^top).
+__device__ __forceinline__ int fit_exponent(float m, int top) {
+  const int e = top + 127 - (int)(__float_as_uint(m) >> 23);
+  return e > kExMost ? kExMost : e < kExLeast ? kExLeast : e;
+}
+// |x|, or 0 where it is infinite or NaN (which no scale helps, and which must not take the others'); the empty asm
+// keeps the compiler, which builds without regard for NaN, from dropping the test.
+__device__ __forceinline__ float finite_size(float x) {
+  unsigned u = __float_as_uint(x);
+  asm volatile("" : "+v"(u));
+  u &= 0x7fffffffu;
+  return u < 0x7f800000u ? __uint_as_float(u) : 0.f;
 }
 
 // Gradient rows of a 16-row subtile: lane holds row `row` (byte offset off), channels
@@ -154,9 +180,12 @@ seq_dq_kernel(const SeqParams p) {
 
   const int row0 = wave * 16 * QT + lr;   // of the tile; subtile t: + 16 t
   const int64_t hrow = (int64_t)head * p.T + tok0;
+  const int last = p.causal && q0 + (1 << LB) < tl.len ? q0 + (1 << LB) : tl.len;
+  const int ns = (last + SR - 1) / SR;
   Frag qf[QT][KS], gf[QT][KS];
   f32x4 nl4[QT], nd4[QT];
   int seen[QT], trow[QT];
+  int ex[QT];   // kFitDs: P, and with it dS, carries 2^ex of its row
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int r = row0 + 16 * t, rc = r < rows ? r : rows - 1;
@@ -166,7 +195,7 @@ seq_dq_kernel(const SeqParams p) {
     const S* op = static_cast<const S*>(p.o) + (tok * p.H + head) * D;
     seen[t] = p.causal ? q0 + rc + 1 : tl.len;
     trow[t] = table_row(p.positions ? p.positions[tok] : q0 + rc - p.has_cls, p.n_pos);
-    float ds = 0.f;
+    float ds = 0.f, most = 0.f, size = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int c = 32 * s + 8 * lg;
@@ -179,26 +208,33 @@ seq_dq_kernel(const SeqParams p) {
       qf[t][s] = C::make(x);
       gf[t][s] = C::make(g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ds += g[e] * o[e];
+      for (int e = 0; e < 8; ++e) {
+        ds += g[e] * o[e];
+        if constexpr (kFitDs<S> && D == 128) size += g[e] * g[e];
+      }
+      if constexpr (kFitDs<S>) most = amax8(most, g);
       if (r < rows) {
         put_row8<S>(static_cast<S*>(p.qhat) + (hrow + r) * D + c, x);
         if (p.gcopy) put_row8<S>(static_cast<S*>(p.gcopy) + (hrow + r) * D + c, g);
       }
     }
     const float nd = -group4_sum(ds), nl = -p.lse[hrow + rc] * kLog2e;
+    const float norm = kFitDs<S> && D == 128 ? __builtin_sqrtf(group4_sum(size)) : 0.f;
     if (r < rows && lg == 0) {
       p.nl[hrow + r] = nl;
       p.nd[hrow + r] = nd;
+      if constexpr (kFitDs<S> && D == 128) p.ng[hrow + r] = norm;
     }
-    nl4[t] = f32x4{nl, nl, nl, nl};
+    // (at first the largest |dO| in [2^14, 2^15): dS is P |V| times that or a few times it)
+    ex[t] = kFitDs<S> && !(QT == 1 && ns == 1) ? fit_exponent(group4_max(most), 14) : 0;
+    const float nlx = nl + (float)ex[t];
+    nl4[t] = f32x4{nlx, nlx, nlx, nlx};
     nd4[t] = f32x4{nd, nd, nd, nd};
   }
   const int w0 = q0 + wave * 16 * QT;   // the wave's first row (uniform)
   const bool active = w0 < tl.len;
   const int lo = p.causal ? w0 + 1 : tl.len;
   const int hi = p.causal && w0 + 16 * QT < tl.len ? w0 + 16 * QT : tl.len;
-  const int last = p.causal && q0 + (1 << LB) < tl.len ? q0 + (1 << LB) : tl.len;
-  const int ns = (last + SR - 1) / SR;
 
   f32x4 acc[QT][DT];
 #pragma unroll
@@ -237,6 +273,20 @@ seq_dq_kernel(const SeqParams p) {
           const float y = fast_exp2(sacc[t][h][i]) * pacc[t][h][i];
           ds[4 * h + i] = !tail || 16 * h + i < lim ? y : 0.f;
         }
+      if constexpr (kFitDs<S>) {
+        const float most = amax8(0.f, ds);
+        if (__any(most > kDsMost)) {   // rows that pass it start again from 2^12
+          const float m = group4_max(most);
+          const int down = m > kDsMost ? fit_exponent(m, 12) : 0;
+          const float f = pow2(down);
+          ex[t] += down;
+          nl4[t] += (float)down;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ds[e] *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+        }
+      }
       dsf[t] = C::make(ds);   // (16-bit tensors: dS rounded to their type for the product)
     }
 #pragma unroll
@@ -291,6 +341,19 @@ seq_dq_kernel(const SeqParams p) {
     const float delta = group4_sum(sum);
     const int dlim = seen[0] > 1 ? lim : 0;   // (as in block)
     if (row0 < rows && lg == 0) p.nd[hrow + row0] = -delta;
+    float f = 1.f;
+    if constexpr (kFitDs<S>) {
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            most = fmaxf(most, 32 * j + 16 * h + i < dlim ? fabsf(prob[j][h][i] * (pacc[j][h][i] - delta)) : 0.f);
+      ex[0] = fit_exponent(group4_max(most), 14);
+      f = pow2(ex[0]);
+    }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       float ds[8];
@@ -298,7 +361,7 @@ seq_dq_kernel(const SeqParams p) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          ds[4 * h + i] = 32 * j + 16 * h + i < dlim ? prob[j][h][i] * (pacc[j][h][i] - delta) : 0.f;
+          ds[4 * h + i] = 32 * j + 16 * h + i < dlim ? prob[j][h][i] * (pacc[j][h][i] - delta) * f : 0.f;
       const Frag dsf = C::make(ds);
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[0][d] = C::mma(at.col(k + 32 * j * D, d), dsf, acc[0][d]);
@@ -318,7 +381,7 @@ seq_dq_kernel(const SeqParams p) {
   const auto rD = make_rsrc(dqb, (unsigned)(rows - 1) * row_b + T::RB);
 #pragma unroll
   for (int t = 0; t < QT; ++t)   // (K-hat carries scale * log2 e)
-    store_rows<S, D>(acc[t], kLn2, true, p, trow[t], rD, (unsigned)(row0 + 16 * t) * row_b, lg);
+    store_rows<S, D>(acc[t], kFitDs<S> ? __builtin_amdgcn_ldexpf(kLn2, -ex[t]) : kLn2, true, p, trow[t], rD, (unsigned)(row0 + 16 * t) * row_b, lg);
 }
 
 // ---------------------------------------------------------------------------
@@ -418,6 +481,8 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   f32x4 dv[DT], dk[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) dv[d] = dk[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int ex = kFitDs<S> ? kExMost : 0;   // the wave's dS and dK carry 2^ex
+  float fit = pow2(ex);
   FragAt<S, D> at;
   at.init(lr, lg);
 
@@ -450,6 +515,24 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
         pv[4 * h + i] = in ? e : 0.f;
         ds[4 * h + i] = in ? e * pacc[h][i] : 0.f;
       }
+    if constexpr (kFitDs<S>) {
+      const float most = amax8(0.f, ds) * fit;
+      if (__any(most > kDsMost)) {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_size(ds[e]));
+        const int to = fit_exponent(__uint_as_float(__builtin_amdgcn_readfirstlane(wave_max_bits(m))), 12);
+        if (to < ex) {
+          const float f = pow2(to - ex);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) dk[d] *= f;
+          ex = to;
+          fit = pow2(ex);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ds[e] *= fit;
+    }
     const Frag pf = C::make(pv), dsf = C::make(ds);   // (16-bit tensors: P and dS rounded to their type for the products)
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -479,14 +562,14 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
     const int64_t at = (((int64_t)part * p.T + tok0) * p.Hkv + kvh) * D;
     const unsigned row_b = (unsigned)(p.Hkv * D) * 4u, bytes = (unsigned)(rows - 1) * row_b + D * 4u;
     const auto rpK = make_rsrc(p.pk + at, bytes), rpV = make_rsrc(p.pv + at, bytes);
-    store_rows<float, D>(dk, 1.f, false, p, 0, rpK, (unsigned)row0 * row_b, lg);
+    store_rows<float, D>(dk, pow2(-ex), false, p, 0, rpK, (unsigned)row0 * row_b, lg);
     store_rows<float, D>(dv, 1.f, false, p, 0, rpV, (unsigned)row0 * row_b, lg);
     return;
   }
   const unsigned row_b = (unsigned)(p.Hkv * D * (int)sizeof(S));
   const unsigned bytes = (unsigned)(rows - 1) * row_b + T::RB;
   const auto rdK = make_rsrc(dkb, bytes), rdV = make_rsrc(dvb, bytes);
-  store_rows<S, D>(dk, dk_factor(p, tl.len), true, p, trow, rdK, (unsigned)row0 * row_b, lg);
+  store_rows<S, D>(dk, dk_factor(p, tl.len) * pow2(-ex), true, p, trow, rdK, (unsigned)row0 * row_b, lg);
   store_rows<S, D>(dv, 1.f, false, p, trow, rdV, (unsigned)row0 * row_b, lg);
 }
 
@@ -539,9 +622,10 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   int head = kvh * group + begin / per - 1, lst = per;   // of the stage loaded next
   const int start = begin % per;
   bool fresh = true;
-  __amdgpu_buffer_rsrc_t rNl = make_rsrc(p.nl, 0u), rNd = make_rsrc(p.nd, 0u);
+  __amdgpu_buffer_rsrc_t rNl = make_rsrc(p.nl, 0u), rNd = make_rsrc(p.nd, 0u), rNg = make_rsrc(p.nd, 0u);
   const int qh = wave & 1, kh = wave >> 1;   // the wave's halves of the queries and keys
   u32x4 nl_next[2], nd_next[2];              // -LSE2 and -delta of queries 32 qh + 16 h + 4 lg + (0..3)
+  unsigned ng_next = 0, na_next = 0;         // kFitDs: |dO| and -delta of query `lane`
   auto load = [&](S* q, S* g) __attribute__((always_inline)) {
     if (lst == per) {
       lst = fresh ? start : 0;
@@ -553,10 +637,15 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
                         : static_cast<const S*>(p.dout) + tl.start * p.sdo[0] + head * p.sdo[1], tl.len);
       rNl = make_rsrc(p.nl + hrow, (unsigned)tl.len * 4u);
       rNd = make_rsrc(p.nd + hrow, (unsigned)tl.len * 4u);
+      if constexpr (kFitDs<S>) rNg = make_rsrc(p.ng + hrow, (unsigned)tl.len * 4u);
     }
     const int r0 = (first + per - 1 - lst) * SR;
     srcQ.load(q, wave, r0);
     srcG.load(g, wave, r0);
+    if constexpr (kFitDs<S>) {
+      ng_next = __builtin_amdgcn_raw_buffer_load_b32(rNg, (unsigned)(r0 + lane) * 4u, 0u, 0);
+      na_next = __builtin_amdgcn_raw_buffer_load_b32(rNd, (unsigned)(r0 + lane) * 4u, 0u, 0);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const unsigned at = (unsigned)(r0 + 32 * qh + 16 * h + 4 * lg) * 4u;
@@ -568,8 +657,10 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   if (ns > 0) load(sQ0, sG0);
 
   Frag kf[2][KS], vf[2][KS];   // key 32 kh + 16 u + lr
+  float vmax = 0.f;            // kFitDs: the largest |V_j| of the tile
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
+    float size = 0.f;
     const int r = 32 * kh + 16 * u + lr, rc = r < rows ? r : rows - 1;
     const int64_t tok = tok0 + rc;
     const S* const vp = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1];
@@ -591,7 +682,24 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
       kf[u][s] = C::make(x);
       row8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
       vf[u][s] = C::make(x);
+      if constexpr (kFitDs<S>) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) size += x[e] * x[e];
+      }
     }
+    if constexpr (kFitDs<S>) vmax = fmaxf(vmax, finite_size(__builtin_sqrtf(group4_sum(size))));
+  }
+  // Every wave has to know the scale of the dS that it takes from the others, and LDS has no room for it
+  // (two workgroups fill the CU's).  So all of them derive it from the same numbers: |dS_ij| = P_ij |dP_ij -
+  // delta_i| <= |dO_i| max |V_j| + |delta_i|, over a stage's queries and the tile's keys.
+  int ex = kFitDs<S> ? kExMost : 0;
+  float fit = pow2(ex);
+  if constexpr (kFitDs<S>) {   // (sP is written behind the next barrier)
+    float* const share = reinterpret_cast<float*>(sP);
+    const unsigned most = wave_max_bits(vmax);
+    if (lane == 0) share[wave] = __uint_as_float(most);
+    lds_barrier();
+    vmax = fmaxf(fmaxf(share[0], share[1]), fmaxf(share[2], share[3]));
   }
   f32x4 dv[4][ND], dk[4][ND];
 #pragma unroll
@@ -616,6 +724,19 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
     for (int h = 0; h < 2; ++h) {
       nl[h] = __builtin_bit_cast(f32x4, nl_next[h]);
       nd[h] = __builtin_bit_cast(f32x4, nd_next[h]);
+    }
+    if constexpr (kFitDs<S>) {
+      const float bound = finite_size(__uint_as_float(ng_next)) * vmax + finite_size(__uint_as_float(na_next));
+      const int to = fit_exponent(__uint_as_float(__builtin_amdgcn_readfirstlane(wave_max_bits(finite_size(bound)))), 14);
+      if (to < ex) {   // (uniform)
+        const float f = pow2(to - ex);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) dk[u][d] *= f;
+        ex = to;
+        fit = pow2(ex);
+      }
     }
     if (st + 1 < ns) load(qn, gn);
     const int q0 = (first + per - 1 - cst) * SR;
@@ -644,7 +765,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
           const bool in = !tail || (i >= from + 16 * u && i < until);
           const float e = fast_exp2(sacc[u][i]);
           pv[i] = (S)(in ? e : 0.f);    // (P and dS rounded to the tensors' type for the products)
-          ds[i] = (S)(in ? e * pacc[u][i] : 0.f);
+          ds[i] = (S)(in ? kFitDs<S> ? e * pacc[u][i] * fit : e * pacc[u][i] : 0.f);
         }
         *reinterpret_cast<s4*>(sP + pw + 512 * u + 4 * h) = pv;
         *reinterpret_cast<s4*>(sS + pw + 512 * u + 4 * h) = ds;
@@ -685,7 +806,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const unsigned off = (unsigned)(16 * u + lr) * row_b;
-      store_tiles<float, D, ND>(dk[u], 16 * d0, 1.f, false, p, 0, rK, off, lg);
+      store_tiles<float, D, ND>(dk[u], 16 * d0, pow2(-ex), false, p, 0, rK, off, lg);
       store_tiles<float, D, ND>(dv[u], 16 * d0, 1.f, false, p, 0, rV, off, lg);
     }
     return;
@@ -695,7 +816,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   for (int u = 0; u < 4; ++u) {
     const int r = 16 * u + lr, rc = r < rows ? r : rows - 1;
     const int trow = table_row(p.positions ? p.positions[tok0 + rc] : k0 + rc - p.has_cls, p.n_pos);
-    store_tiles<S, D, ND>(dk[u], 16 * d0, dk_factor(p, tl.len), true, p, trow, rK, (unsigned)r * row_b, lg);
+    store_tiles<S, D, ND>(dk[u], 16 * d0, dk_factor(p, tl.len) * pow2(-ex), true, p, trow, rK, (unsigned)r * row_b, lg);
     store_tiles<S, D, ND>(dv[u], 16 * d0, 1.f, false, p, trow, rV, (unsigned)r * row_b, lg);
   }
 }

@@ -36,6 +36,7 @@ struct SeqParams {
   int* map_k;                        // and of the key kernel's
   float* nl;                         // [H, T]: -LSE * log2 e
   float* nd;                         // [H, T]: -rowsum(dO * O)
+  float* ng;                         // [H, T]: norms of dO's rows (fp16 at head_dim 128)
   float* pk;                         // [parts, T, Hkv, D]: sums of the parts of dK / scale (rotated), parts > 1
   float* pv;                         // and of dV
   int parts;                         // parts of a key tile's queries
