@@ -485,3 +485,29 @@ def test_fp16_gradients_over_its_range(D, H, Hkv, lens, sizes):
         if n == "dq":   # each row by its own size
             allowed = 2 * tol * ref[n].norm(dim=-1) + stored + ref["dq+"]
             assert (off <= allowed).all(), (n, float((off / allowed).max()))
+
+
+@pytest.mark.parametrize("dtype,D,H,short,long,causal", [
+    (BF16, 128, 4, [40, 50, 64, 33], [], True), (BF16, 128, 4, [40, 50, 64, 33], [], False), (BF16, 256, 2, [40, 64], [], True),
+    (BF16, 64, 4, [40, 50, 64, 33], [], True), (F32, 128, 2, [40, 64], [], True), (F32, 128, 2, [40, 60, 64, 1], [], False),
+    (BF16, 128, 32, [2, 17, 32, 1, 33, 64], [1100] * 6, True), (F16, 128, 32, [2, 17, 32, 1, 33, 64], [1100] * 6, False),
+    (BF16, 256, 32, [2, 17, 64], [900] * 3, True), (F16, 256, 32, [2, 17, 64], [900] * 3, False),
+    (F16, 64, 16, [2, 64], [13000], True), (F32, 256, 1, [3, 40, 64], [400], True), (BF16, 32, 16, [2, 64], [13000], True),
+])
+def test_short_rows_whatever_their_neighbours(dtype, D, H, short, long, causal):
+    """V with a common offset: the gradients of rows that see 64 keys at most do not feel the rounding of O, in
+    packs of every tile size (as in the test of short rows above; causal: a long sequence's first rows too)."""
+    lens = short + long
+    q, k, v, do = inputs(sum(lens), H, 2 if H > 2 else 1, D, dtype, seed=31)
+    v = (v.float() + 64.0).to(dtype)
+    table, cu = seq_ref.Table(max(lens), D, DEV), starts(lens)
+    got = grads(q, k, v, do, table, cu, causal=causal)
+    n = sum(short)
+    ref = seq_ref.varlen(*(t[:n] for t in (q, k, v, do)), table, starts(short), causal, True)
+    tol = seq_ref.ROUNDINGS["dq"] * seq_ref.U[dtype] + 64 * 64 * 2.0 ** -24 if dtype != F32 else 64 * 64 * 2.0 ** -24
+    for m in ("dq", "dk"):
+        assert seq_ref.rel(got[m][:n], ref[m]) <= tol, m
+    if long and causal:   # a first row of a long sequence depends on the rows before it alone
+        a = n + 64
+        ref = seq_ref.varlen(*(t[n:a] for t in (q, k, v, do)), table, starts([64]), True, True)
+        assert seq_ref.rel(got["dq"][n:a], ref["dq"]) <= tol

@@ -134,7 +134,7 @@ __device__ __forceinline__ float dk_factor(const SeqParams& p, int len) { return
 // dQ of 64 QT query rows of one head.  S^T = K-hat Q-hat^T and dP^T = V dO^T per
 // 32-key block; their output rows are the k-slots of dQ-hat^T += K-hat^T dS^T.
 // ---------------------------------------------------------------------------
-// Keys of a stage: as in the forward (short sequences: 64, so that one stage holds them).
+// Keys of a stage: as in the forward (short sequences: 64, so that one stage holds them).  Two stages hold 64 at least.
 template <typename S, int D, bool ROT> constexpr int kDqRows = sizeof(S) == 2 && D == 128 && !ROT ? 32 : kStageRowsOf<S, D>;
 template <typename S, int D, int QT, bool ROT>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 && (QT == 2 || ROT) ? 2 : 3)
@@ -180,8 +180,14 @@ seq_dq_kernel(const SeqParams p) {
 
   const int row0 = wave * 16 * QT + lr;   // of the tile; subtile t: + 16 t
   const int64_t hrow = (int64_t)head * p.T + tok0;
+  const int w0 = q0 + wave * 16 * QT;   // the wave's first row (uniform)
+  const bool active = w0 < tl.len;
+  const int lo = p.causal ? w0 + 1 : tl.len;
+  const int hi = p.causal && w0 + 16 * QT < tl.len ? w0 + 16 * QT : tl.len;
   const int last = p.causal && q0 + (1 << LB) < tl.len ? q0 + (1 << LB) : tl.len;
   const int ns = (last + SR - 1) / SR;
+  const bool few = q0 == 0 && (p.causal || tl.len <= 64);   // some rows of the tile see 64 keys at most
+  const bool mine = few && hi <= 64;                        // (uniform) and so do all of the wave's
   Frag qf[QT][KS], gf[QT][KS];
   f32x4 nl4[QT], nd4[QT];
   int seen[QT], trow[QT];
@@ -226,15 +232,11 @@ seq_dq_kernel(const SeqParams p) {
       if constexpr (kFitDs<S> && D == 128) p.ng[hrow + r] = norm;
     }
     // (at first the largest |dO| in [2^14, 2^15): dS is P |V| times that or a few times it)
-    ex[t] = kFitDs<S> && !(QT == 1 && ns == 1) ? fit_exponent(group4_max(most), 14) : 0;
+    ex[t] = kFitDs<S> && !mine ? fit_exponent(group4_max(most), 14) : 0;
     const float nlx = nl + (float)ex[t];
     nl4[t] = f32x4{nlx, nlx, nlx, nlx};
     nd4[t] = f32x4{nd, nd, nd, nd};
   }
-  const int w0 = q0 + wave * 16 * QT;   // the wave's first row (uniform)
-  const bool active = w0 < tl.len;
-  const int lo = p.causal ? w0 + 1 : tl.len;
-  const int hi = p.causal && w0 + 16 * QT < tl.len ? w0 + 16 * QT : tl.len;
 
   f32x4 acc[QT][DT];
 #pragma unroll
@@ -314,67 +316,106 @@ seq_dq_kernel(const SeqParams p) {
     if (ROT && st + 1 < ns) rot.store(p, kn, tid);   // (read in the stage before this one)
   };
   if constexpr (ROT) rot.store(p, sK0, tid);
-  // The only stage: delta = sum_j P_ij dP_ij, in fp32, while P and dP are in registers.  Rows that
-  // see few keys have an O as large as V, whose rounding as stored would be the largest error
-  // of a dS that cancels (sequences of two tokens, bf16: dQ off by 5e-3 of its norm from O dO).
-  auto whole = [&](const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
-    f32x4 prob[NB][2], pacc[NB][2];
-    const int lim = seen[0] - 4 * lg;
-    float sum = 0.f;
+  // Rows that see 64 keys at most, all of them in LDS: delta = sum_j P_ij dP_ij, in fp32, while P and dP
+  // are in registers.  Such rows have an O as large as V, whose rounding as stored would be the largest error
+  // of a dS that cancels (sequences of two tokens, bf16: dQ off by 5e-3 of its norm from O dO; V of 64 + N(0, 1):
+  // 0.16).  Key block j of 32 is at k[j], v[j].
+  auto whole = [&](const S* const (&k)[2], const S* const (&v)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+    for (int t = 0; t < QT; ++t) {
+      f32x4 prob[2][2], pacc[2][2];
+      const int lim = seen[t] - 4 * lg;
+      float sum = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int j = 0; j < 2; ++j) {
+        if (32 * j >= hi) {   // (uniform: no such keys, and nothing in LDS)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          prob[j][h] = C::mma(at.row(k + 32 * j * D, s, h), qf[0][s], s == 0 ? first_sum<S>(nl4[0]) : prob[j][h]);
-          pacc[j][h] = C::mma(at.row(v + 32 * j * D, s, h), gf[0][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : pacc[j][h]);
+          for (int h = 0; h < 2; ++h) prob[j][h] = pacc[j][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+          continue;
         }
-        last_sum<S>(prob[j][h], nl4[0]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = 32 * j + 16 * h + i < lim;
-          prob[j][h][i] = in ? fast_exp2(prob[j][h][i]) : 0.f;
-          sum += in ? prob[j][h][i] * pacc[j][h][i] : 0.f;
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            prob[j][h] = C::mma(at.row(k[j], s, h), qf[t][s], s == 0 ? first_sum<S>(nl4[t]) : prob[j][h]);
+            pacc[j][h] = C::mma(at.row(v[j], s, h), gf[t][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : pacc[j][h]);
+          }
+          last_sum<S>(prob[j][h], nl4[t]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool in = 32 * j + 16 * h + i < lim;
+            prob[j][h][i] = in ? fast_exp2(prob[j][h][i]) : 0.f;
+            sum += in ? prob[j][h][i] * pacc[j][h][i] : 0.f;
+          }
         }
       }
-    const float delta = group4_sum(sum);
-    const int dlim = seen[0] > 1 ? lim : 0;   // (as in block)
-    if (row0 < rows && lg == 0) p.nd[hrow + row0] = -delta;
-    float f = 1.f;
-    if constexpr (kFitDs<S>) {
-      float most = 0.f;
+      const float delta = group4_sum(sum);
+      const int dlim = seen[t] > 1 ? lim : 0;   // (as in block)
+      if (row0 + 16 * t < rows && lg == 0) p.nd[hrow + row0 + 16 * t] = -delta;
+      float f = 1.f;
+      if constexpr (kFitDs<S>) {
+        float most = 0.f;
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              most = fmaxf(most, 32 * j + 16 * h + i < dlim ? fabsf(prob[j][h][i] * (pacc[j][h][i] - delta)) : 0.f);
+        ex[t] = fit_exponent(group4_max(most), 14);
+        f = pow2(ex[t]);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (32 * j >= hi) continue;
+        float ds[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            most = fmaxf(most, 32 * j + 16 * h + i < dlim ? fabsf(prob[j][h][i] * (pacc[j][h][i] - delta)) : 0.f);
-      ex[0] = fit_exponent(group4_max(most), 14);
-      f = pow2(ex[0]);
-    }
+            ds[4 * h + i] = 32 * j + 16 * h + i < dlim ? prob[j][h][i] * (pacc[j][h][i] - delta) * f : 0.f;
+        const Frag dsf = C::make(ds);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      float ds[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          ds[4 * h + i] = 32 * j + 16 * h + i < dlim ? prob[j][h][i] * (pacc[j][h][i] - delta) * f : 0.f;
-      const Frag dsf = C::make(ds);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) acc[0][d] = C::mma(at.col(k + 32 * j * D, d), dsf, acc[0][d]);
+        for (int d = 0; d < DT; ++d) acc[t][d] = C::mma(at.col(k[j], d), dsf, acc[t][d]);
+      }
     }
   };
-  if (QT == 1 && ns == 1) {   // (uniform)
-    seq_stage_barrier();
-    if (active) whole(sK0, sV0);
-  } else {
-    for (int st = 0; st < ns; st += 2) {
-      stage(st, sK0, sV0, sK1, sV1);
-      if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
+  int from = 0;
+  if (few) {   // (uniform) the first two stages together
+    if (ns > 1) {
+      if constexpr (ROT) {
+        rot.load(p, tl, kvh, 1, tid);
+        rot.store(p, sK1, tid);
+      } else {
+        srcK.load(sK1, wave, SR);
+      }
+      srcV.load(sV1, wave, SR);
     }
+    seq_stage_barrier();
+    auto at_block = [&](const S* a, const S* b, int j) __attribute__((always_inline)) { return (j < NB ? a : b) + 32 * (j % NB) * D; };
+    if (mine) {
+      const S* const k[2] = {sK0, at_block(sK0, sK1, 1)};
+      const S* const v[2] = {sV0, at_block(sV0, sV1, 1)};
+      if (active) whole(k, v);
+    } else if (active) {
+#pragma unroll 1
+      for (int j = 0; j < 2 * NB && 32 * j < hi; ++j) block(true, 32 * j, at_block(sK0, sK1, j), at_block(sV0, sV1, j));
+    }
+    from = 2;
+    if (ns > 2) {
+      lds_barrier();   // (all waves have read them)
+      if constexpr (ROT) {
+        rot.load(p, tl, kvh, 2, tid);
+        rot.store(p, sK0, tid);
+      } else {
+        srcK.load(sK0, wave, 2 * SR);
+      }
+      srcV.load(sV0, wave, 2 * SR);
+    }
+  }
+  for (int st = from; st < ns; st += 2) {
+    stage(st, sK0, sV0, sK1, sV1);
+    if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
   }
 
   const unsigned row_b = (unsigned)(p.H * D * (int)sizeof(S));
