@@ -246,6 +246,20 @@ def test_c_cache_entries_refuse():
     assert n > 0 and decode(one, long, elems=n - 1) == _lib.ERR_SCRATCH and decode(one, long, ws=None) == _lib.ERR_NULL
 
 
+@pytest.mark.parametrize("D,dtype,most", [(128, _lib.BF16, 512), (256, _lib.F16, 256), (64, _lib.BF16, 768), (32, _lib.F16, 1024),
+                                          (128, _lib.F32, 256)])
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (3, 1), (4, 4), (5, 1), (6, 2), (7, 1), (11, 3), (12, 1), (3, 20), (600, 1)])
+def test_decode_workers_are_resident_at_once(kv_heads, group, D, dtype, most):
+    """Equal shares of the cached rows: one round of workgroups, no few of them behind it."""
+    heads, seqs, tiles = kv_heads * group, 4, -(-group // 16)
+    d = _seq_desc(tokens=seqs, seqs=seqs, heads=heads, kv_heads=kv_heads, head_dim=D, dtype=dtype)
+    n = _lib.load().farope_decode_workspace_elems(ctypes.byref(d), ctypes.byref(_cache_desc(max_pages=1 << 16)))
+    # sums [workers + seqs, heads, D], two statistics each, rounded up to 4; owners [seqs, 2]
+    workers = (n - 2 * seqs) // (heads * (D + 2)) - seqs
+    assert (workers + seqs) * heads * (D + 2) <= n - 2 * seqs < (workers + seqs) * heads * (D + 2) + 4
+    assert workers == max(1, most // (kv_heads * tiles))
+
+
 def test_slots_cover_every_tile():
     """The grid's rule: sequence i takes slots (cu[i] >> lb) + i on, at least as many as it has tiles."""
     g = torch.Generator().manual_seed(0)

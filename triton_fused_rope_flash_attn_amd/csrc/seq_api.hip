@@ -62,7 +62,9 @@ int check_sizes(const farope_seq_desc* d) {
 }
 
 // Workgroups of a call over a paged cache that are resident at once (decode_kernel's registers):
-// one round of workers, whose shares are equal, is the fastest.  Measured (us, 512 / 768 / 1024
+// one round of workers, whose shares are equal, is the fastest, so never more than these (a few more
+// start a whole share on an idle chip: 516 / 504 for 12 key heads, D 128, 2 x 32768 97 / 83; 264 / 252 at D
+// 256, 8 x 8192 209 / 156).  Measured (us, 512 / 768 / 1024
 // workgroups; "sequences x rows, key heads"), D 128: 1 x 32768, 8 37.5 / 43.4 / 46.0, 32 x 8192, 1
 // 35.5 / 44.6 / 41.5; D 64: 16 x 2048, 12 30.8 / 27.1 / 32.6; D 256, 256 / 512: 8 x 8192, 2 40 / 53.
 int64_t decode_wgs(const farope_seq_desc* d) {
@@ -206,7 +208,8 @@ int decode_workers(const farope_seq_desc* d, const farope_cache_desc* c) {
   const int64_t heads = (int64_t)d->kv_heads * decode_tiles(d);
   // (a worker has 128 rows at least)
   const int64_t most = d->seqs * (((int64_t)c->max_pages * c->page_rows + 127) / 128);
-  const int64_t n = (decode_wgs(d) + heads - 1) / heads;
+  int64_t n = decode_wgs(d) / heads;
+  if (n < 1) n = 1;
   return (int)(n < most ? n : most);
 }
 // Workspace, in fp32 elements, each part from a 16-byte boundary: sums, their statistics, owners.
