@@ -399,3 +399,20 @@ def test_gradients_are_refused():
     o = sdpa_rope_decode(k, kc, vc, table, pages, ints([1]))
     with pytest.raises(RuntimeError, match="no gradients"):
         o.sum().backward()
+
+
+@pytest.mark.parametrize("which", ["k", "v", "kc", "vc", "q"])
+def test_tangents_are_refused(which):
+    from torch.autograd import forward_ad
+
+    kc, vc = caches(3, 16, 2, 64, BF16)
+    pages, table = ints([[0, 1]]), seq_ref.Table(9, 64, DEV)
+    q, k, v = (randn(1, h, 64, dtype=BF16, seed=h) for h in (4, 2, 2))
+    with forward_ad.dual_level():
+        a = dict(q=q, k=k, v=v, kc=kc, vc=vc)
+        a[which] = forward_ad.make_dual(a[which], torch.ones_like(a[which]))
+        calls = [lambda: rope_cache_append(a["k"], a["v"], table, a["kc"], a["vc"], pages, ints([0]))] if which != "q" else []
+        calls += [lambda: sdpa_rope_decode(a["q"], a["kc"], a["vc"], table, pages, ints([1]))] if which in ("q", "kc", "vc") else []
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()

@@ -511,3 +511,21 @@ def test_short_rows_whatever_their_neighbours(dtype, D, H, short, long, causal):
         a = n + 64
         ref = seq_ref.varlen(*(t[n:a] for t in (q, k, v, do)), table, starts([64]), True, True)
         assert seq_ref.rel(got["dq"][n:a], ref["dq"]) <= tol
+
+
+@pytest.mark.parametrize("grad", [False, True], ids=["no_grad", "grad"])
+@pytest.mark.parametrize("which", ["Q", "K", "V", "table"])
+def test_tangents_are_refused(which, grad):
+    """Forward mode: no derivative is implemented, and none is dropped."""
+    from torch.autograd import forward_ad
+
+    q, k, v, _ = inputs(20, 2, 1, 64, BF16)
+    table = seq_ref.Table(20, 64, DEV)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        if which == "table":
+            table.cos = dual(table.cos)
+        x = [dual(t) if n == which else t for n, t in zip("QKV", (q, k, v))]
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            sdpa_rope_varlen(*x, table, starts([20]))
+    sdpa_rope_varlen(q, k, v, seq_ref.Table(20, 64, DEV), starts([20]))

@@ -89,3 +89,20 @@ def test_other_stream_and_dout_dtype(case):
     o, lse, res = torch.ops.farope.attn_fwd(q, k, v, *args)
     grads = torch.ops.farope.attn_bwd(do.float(), q, k, v, o, lse, *args, res)
     assert all(torch.equal(a, b) for a, b in zip(grads, want[1:]))
+
+
+@pytest.mark.parametrize("grad", [False, True], ids=["no_grad", "grad"])
+def test_tangents_are_refused(case, grad):
+    """Forward mode: no derivative is implemented, and none is dropped (dense planes and the packed projection)."""
+    from torch.autograd import forward_ad
+
+    from triton_fused_rope_flash_attn_amd import RoPEAttention
+
+    table, q, k, v, _ = case
+    layer = RoPEAttention(3 * D, 3, H_img=SIDE, device=DEV, dtype=torch.bfloat16)
+    x = torch.randn(2, N, 3 * D, device=DEV, dtype=torch.bfloat16)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: sdpa_triton_fa_rope(q, dual(k), v, table), lambda: layer(dual(x))):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()

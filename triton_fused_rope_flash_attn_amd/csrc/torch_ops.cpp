@@ -236,6 +236,7 @@ struct AttnBwdNode : torch::autograd::Function<AttnBwdNode> {
 
 Three attn_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& rope, c10::SymInt n_pos, bool has_cls,
                         double scale, c10::SymInt comp) {
+  refuse_tangents("attn_fwd", {&q, &k, &v, &rope});
   if (at::GradMode::is_enabled() && any_requires_grad({&q, &k, &v, &rope})) {
     const variable_list r = AttnFwdNode::apply(q, k, v, rope, n_pos, has_cls, scale, comp);
     return {r[0], r[1], r[2]};
@@ -247,6 +248,7 @@ Three attn_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const
 Three attn_bwd_autograd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
                         const Tensor& lse, const Tensor& rope, c10::SymInt n_pos, bool has_cls, double scale, c10::SymInt comp,
                         const Tensor& o_res) {
+  refuse_tangents("attn_bwd", {&dout, &q, &k, &v, &o, &lse, &rope, &o_res});
   if (at::GradMode::is_enabled() && any_requires_grad({&dout, &q, &k, &v, &o, &lse, &rope, &o_res})) {
     const variable_list r = AttnBwdNode::apply(dout, q, k, v, o, lse, rope, n_pos, has_cls, scale, comp, o_res);
     return {r[0], r[1], r[2]};
@@ -310,6 +312,7 @@ struct QkvBwdNode : torch::autograd::Function<QkvBwdNode> {
 
 Three attn_qkv_fwd_autograd(const Tensor& qkv, const Tensor& rope, c10::SymInt heads, c10::SymInt n_pos, bool has_cls,
                             double scale, c10::SymInt comp) {
+  refuse_tangents("attn_qkv_fwd", {&qkv, &rope});
   if (at::GradMode::is_enabled() && any_requires_grad({&qkv, &rope})) {
     const variable_list r = QkvFwdNode::apply(qkv, rope, heads, n_pos, has_cls, scale, comp);
     return {r[0], r[1], r[2]};
@@ -321,6 +324,7 @@ Three attn_qkv_fwd_autograd(const Tensor& qkv, const Tensor& rope, c10::SymInt h
 Tensor attn_qkv_bwd_autograd(const Tensor& dout, const Tensor& qkv, const Tensor& o, const Tensor& lse, const Tensor& rope,
                              c10::SymInt heads, c10::SymInt n_pos, bool has_cls, double scale, c10::SymInt comp,
                              const Tensor& o_res) {
+  refuse_tangents("attn_qkv_bwd", {&dout, &qkv, &o, &lse, &rope, &o_res});
   if (at::GradMode::is_enabled() && any_requires_grad({&dout, &qkv, &o, &lse, &rope, &o_res}))
     return QkvBwdNode::apply(dout, qkv, o, lse, rope, heads, n_pos, has_cls, scale, comp, o_res);
   at::AutoDispatchBelowADInplaceOrView below;

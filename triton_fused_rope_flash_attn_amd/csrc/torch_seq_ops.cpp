@@ -273,6 +273,7 @@ struct SeqFwdNode : torch::autograd::Function<SeqFwdNode> {
 };
 Two seq_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cosp, const Tensor& sinp, const Tensor& cu,
                      const Opt& positions, bool causal, bool has_cls, double scale) {
+  refuse_tangents("seq_fwd", {&q, &k, &v, &cosp, &sinp});
   if (at::GradMode::is_enabled() && any_requires_grad({&q, &k, &v})) {
     const variable_list r = SeqFwdNode::apply(q, k, v, cosp, sinp, cu, positions, causal, has_cls, scale);
     return {r[0], r[1]};
@@ -299,6 +300,7 @@ struct SeqBwdNode : torch::autograd::Function<SeqBwdNode> {
 Three seq_bwd_autograd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse,
                        const Tensor& cosp, const Tensor& sinp, const Tensor& cu, const Opt& positions, bool causal, bool has_cls,
                        double scale) {
+  refuse_tangents("seq_bwd", {&dout, &q, &k, &v, &o, &lse, &cosp, &sinp});
   if (at::GradMode::is_enabled() && any_requires_grad({&dout, &q, &k, &v, &o, &lse})) {
     const variable_list r = SeqBwdNode::apply(dout, q, k, v, o, lse, cosp, sinp, cu, positions, causal, has_cls, scale);
     return {r[0], r[1], r[2]};
@@ -310,6 +312,7 @@ Three seq_bwd_autograd(const Tensor& dout, const Tensor& q, const Tensor& k, con
 // A cache is no part of an autograd graph.
 void cache_append_autograd(const Tensor& k, const Tensor& v, const Tensor& cosp, const Tensor& sinp, Tensor kc, Tensor vc,
                            const Tensor& pages, const Tensor& lengths, const Opt& cu, const Opt& positions, bool has_cls) {
+  refuse_tangents("cache_append", {&k, &v, &kc, &vc, &cosp, &sinp});
   TORCH_CHECK(!at::GradMode::is_enabled() || !any_requires_grad({&k, &v, &kc, &vc}),
               "farope: appending to a cache is not differentiable; call it under torch.no_grad() or with detached tensors");
   {
@@ -334,6 +337,7 @@ struct CacheAttnNode : torch::autograd::Function<CacheAttnNode> {
 };
 Tensor cache_attn_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
                            const Tensor& pages, const Tensor& lengths, const Opt& positions, bool has_cls, double scale) {
+  refuse_tangents("cache_attn", {&q, &kc, &vc, &cosp, &sinp});
   if (at::GradMode::is_enabled() && any_requires_grad({&q, &kc, &vc}))
     return CacheAttnNode::apply(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale);
   at::AutoDispatchBelowADInplaceOrView below;

@@ -56,4 +56,11 @@ inline bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// None of the ops has a forward-mode derivative: a tangent is refused, whether gradients are enabled or not.
+inline void refuse_tangents(const char* op, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "farope: ", op,
+                " has no forward-mode derivative; detach the tangents of its inputs (torch.autograd.forward_ad)");
+}
+
 }  // namespace farope_torch
