@@ -416,3 +416,25 @@ def test_tangents_are_refused(which):
         for call in calls:
             with pytest.raises(RuntimeError, match="no forward-mode derivative"):
                 call()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_decode_many_small_weights(dtype):
+    """As in the packed call's test: one key, and 2^17 - 1 that weigh 2^-25 of it each; so many key heads (one,
+    expanded) that one worker takes a head's rows."""
+    N, D, H, page = 1 << 17, 32, 1024, 64
+    kc, vc = (torch.zeros(N // page, page, 1, D, dtype=dtype, device=DEV) for _ in range(2))
+    kc[0, 0, 0, 0] = 25.03125 * 0.693147 * D ** 0.5 / 8
+    vc[:] = 1.0
+    vc[0, 0] = -1.0
+    q = torch.zeros(1, H, D, dtype=dtype, device=DEV)
+    q[..., 0] = 8.0
+    w = (N - 1) * torch.exp(-8.0 * kc[0, 0, 0, 0].double() / D ** 0.5).item()
+    assert dtype == BF16 or w / (N - 1) < 2.0 ** -25
+    kc, vc = (t.expand(-1, -1, H, -1) for t in (kc, vc))
+    pages = torch.arange(N // page, dtype=torch.int32, device=DEV).view(1, -1)
+    got = sdpa_rope_decode(q, kc, vc, seq_ref.Table(1, D, DEV), pages, ints([N]))
+    u = seq_ref.U[dtype]
+    # the bound of run_decode; the logit in fp32 (log2 units, 25) and exp2: 32 units of 2^-24 of the weights
+    off = (got.double() - (w - 1) / (1 + w)).abs().max().item()
+    assert off <= u + 3 * u * u + 32 * 2.0 ** -24, off

@@ -529,3 +529,28 @@ def test_tangents_are_refused(which, grad):
         with pytest.raises(RuntimeError, match="no forward-mode derivative"):
             sdpa_rope_varlen(*x, table, starts([20]))
     sdpa_rope_varlen(q, k, v, seq_ref.Table(20, 64, DEV), starts([20]))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_many_small_weights(dtype):
+    """One key that weighs 2^25 times each of the others, 2^17 - 1 of them: together they are 0.4% of the row.
+    (Their weights are below the half of fp16's least value.)"""
+    T, D = 1 << 17, 32
+    q, k, v, do = (torch.zeros(T, 1, D, dtype=dtype, device=DEV) for _ in range(4))
+    logit = 25.03125 * 0.693147   # log2 units; q k / sqrt(D), in values that both types hold
+    q[..., 0] = 8.0
+    k[0, 0, 0] = logit * D ** 0.5 / 8
+    w = (T - 1) * torch.exp(-8.0 * k[0, 0, 0].double() / D ** 0.5).item()
+    assert dtype == BF16 or w / (T - 1) < 2.0 ** -25
+    v[:] = 1.0
+    v[0] = -1.0
+    do[:] = 0.25
+    got = grads(q, k, v, do, seq_ref.Table(1, D, DEV), starts([T]), causal=False)
+    u = seq_ref.U[dtype]
+    off = (got["o"].double() - (w - 1) / (1 + w)).abs().max().item()
+    # q-hat k-hat rounds as 25 * 2^-24 would (k-hat carries the scale: one rounding, u of the logit)
+    assert off <= 4 * u + 2 * w * (25 * 0.7 * u), off
+    each = 0.25 * T * (w / (T - 1)) / (1 + w)
+    off = (got["dv"][1:].double() - each).abs().max().item()
+    assert off <= (4 * u + 25 * 0.7 * u) * each + 2.0 ** -25, (off, each)
+    assert all(torch.isfinite(x).all() for x in got.values())

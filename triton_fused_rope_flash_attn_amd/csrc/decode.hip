@@ -233,9 +233,9 @@ __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D *
 #pragma unroll
       for (int h = 0; h < 2; ++h) mx = fmaxf(mx, fmaxf(fmaxf(sacc[h][0], sacc[h][1]), fmaxf(sacc[h][2], sacc[h][3])));
       if (__any(mx > thr)) {   // (as in the forward over packed sequences)
-        thr = 8.0f;
+        thr = kSeqSlack + kWeightUp<S>;
         const float old = m_run == -INFINITY ? 0.f : m_run;
-        const float mnew = fmaxf(m_run, group4_max(mx) + old);
+        const float mnew = fmaxf(m_run, group4_max(mx) + old - kWeightUp<S>);
         const float alpha = fast_exp2(m_run - mnew), sh = old - mnew;
         m_run = mnew;
         l_run *= alpha;

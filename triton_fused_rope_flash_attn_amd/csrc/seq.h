@@ -44,6 +44,16 @@ template <> struct SeqComp<f16> { using C = Comp<DT_F16>; };
 template <> struct SeqComp<float> { using C = CompF32x; };
 
 // ---------------------------------------------------------------------------
+// Softmax weights as operands of a product: P = exp2(s - m).  m is the row's running maximum, raised when a
+// logit passes it by kSeqSlack (log2 units).  fp16 rounds what is below 2^-25 to 0, and a key of a row of 2^17 that
+// far below the largest still counts in their sum (O of a row whose other keys weigh 2^-25 each was off
+// by 3.9e-3).  There m is kept kWeightUp below the maximum: P up to 2^7, 2^15 before m is raised, and down to 2^-32 of
+// the largest.  The weights of the backward are at most 1, and carry 2^kWeightUp alike.
+// ---------------------------------------------------------------------------
+template <typename S> constexpr float kWeightUp = std::is_same<S, f16>::value ? 7.0f : 0.0f;
+constexpr float kSeqSlack = 8.0f;
+
+// ---------------------------------------------------------------------------
 // Streamed tiles: rows of D elements, unpadded, their 16-byte chunks XOR-swizzled
 // per row with period 16 (as in stream.h: 16-byte reads of 16 rows and the
 // transposed reads are free of bank conflicts).  A stage holds SR rows; a

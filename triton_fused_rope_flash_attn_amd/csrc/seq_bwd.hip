@@ -227,7 +227,7 @@ seq_dq_kernel(const SeqParams p) {
     const float nd = -group4_sum(ds), nl = -p.lse[hrow + rc] * kLog2e;
     const float norm = kFitDs<S> && D == 128 ? __builtin_sqrtf(group4_sum(size)) : 0.f;
     if (r < rows && lg == 0) {
-      p.nl[hrow + r] = nl;
+      p.nl[hrow + r] = nl + kWeightUp<S>;
       p.nd[hrow + r] = nd;
       if constexpr (kFitDs<S> && D == 128) p.ng[hrow + r] = norm;
     }
@@ -599,19 +599,20 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
     if (st + 1 < ns) stage(st + 1, sQ1, sG1, sL1, sD1, sQ0, sG0, sL0, sD0);
   }
 
+  const float up = pow2(-(int)kWeightUp<S>);   // out of P
   if (p.parts > 1) {   // sums as they are, for seq_join_kernel
     const int64_t at = (((int64_t)part * p.T + tok0) * p.Hkv + kvh) * D;
     const unsigned row_b = (unsigned)(p.Hkv * D) * 4u, bytes = (unsigned)(rows - 1) * row_b + D * 4u;
     const auto rpK = make_rsrc(p.pk + at, bytes), rpV = make_rsrc(p.pv + at, bytes);
-    store_rows<float, D>(dk, pow2(-ex), false, p, 0, rpK, (unsigned)row0 * row_b, lg);
-    store_rows<float, D>(dv, 1.f, false, p, 0, rpV, (unsigned)row0 * row_b, lg);
+    store_rows<float, D>(dk, pow2(-ex) * up, false, p, 0, rpK, (unsigned)row0 * row_b, lg);
+    store_rows<float, D>(dv, up, false, p, 0, rpV, (unsigned)row0 * row_b, lg);
     return;
   }
   const unsigned row_b = (unsigned)(p.Hkv * D * (int)sizeof(S));
   const unsigned bytes = (unsigned)(rows - 1) * row_b + T::RB;
   const auto rdK = make_rsrc(dkb, bytes), rdV = make_rsrc(dvb, bytes);
-  store_rows<S, D>(dk, dk_factor(p, tl.len) * pow2(-ex), true, p, trow, rdK, (unsigned)row0 * row_b, lg);
-  store_rows<S, D>(dv, 1.f, false, p, trow, rdV, (unsigned)row0 * row_b, lg);
+  store_rows<S, D>(dk, dk_factor(p, tl.len) * pow2(-ex) * up, true, p, trow, rdK, (unsigned)row0 * row_b, lg);
+  store_rows<S, D>(dv, up, false, p, trow, rdV, (unsigned)row0 * row_b, lg);
 }
 
 // ---------------------------------------------------------------------------
@@ -768,7 +769,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
     }
     if constexpr (kFitDs<S>) {
       const float bound = finite_size(__uint_as_float(ng_next)) * vmax + finite_size(__uint_as_float(na_next));
-      const int to = fit_exponent(__uint_as_float(__builtin_amdgcn_readfirstlane(wave_max_bits(finite_size(bound)))), 14);
+      const int to = fit_exponent(__uint_as_float(__builtin_amdgcn_readfirstlane(wave_max_bits(finite_size(bound)))), 14 - (int)kWeightUp<S>);
       if (to < ex) {   // (uniform)
         const float f = pow2(to - ex);
 #pragma unroll
@@ -839,6 +840,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   }
 
   // lane holds key 16 u + lr, channels 16 (d0 + d) + 4lg + (0..3)
+  const float up = pow2(-(int)kWeightUp<S>);   // out of P
   const unsigned es = p.parts > 1 ? 4u : 2u, row_b = (unsigned)(p.Hkv * D) * es;
   const unsigned bytes = (unsigned)(rows - 1) * row_b + D * es;
   if (p.parts > 1) {   // sums as they are, for seq_join_kernel
@@ -847,8 +849,8 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const unsigned off = (unsigned)(16 * u + lr) * row_b;
-      store_tiles<float, D, ND>(dk[u], 16 * d0, pow2(-ex), false, p, 0, rK, off, lg);
-      store_tiles<float, D, ND>(dv[u], 16 * d0, 1.f, false, p, 0, rV, off, lg);
+      store_tiles<float, D, ND>(dk[u], 16 * d0, pow2(-ex) * up, false, p, 0, rK, off, lg);
+      store_tiles<float, D, ND>(dv[u], 16 * d0, up, false, p, 0, rV, off, lg);
     }
     return;
   }
@@ -857,8 +859,8 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   for (int u = 0; u < 4; ++u) {
     const int r = 16 * u + lr, rc = r < rows ? r : rows - 1;
     const int trow = table_row(p.positions ? p.positions[tok0 + rc] : k0 + rc - p.has_cls, p.n_pos);
-    store_tiles<S, D, ND>(dk[u], 16 * d0, dk_factor(p, tl.len) * pow2(-ex), true, p, trow, rK, (unsigned)r * row_b, lg);
-    store_tiles<S, D, ND>(dv[u], 16 * d0, 1.f, false, p, trow, rV, (unsigned)r * row_b, lg);
+    store_tiles<S, D, ND>(dk[u], 16 * d0, dk_factor(p, tl.len) * pow2(-ex) * up, true, p, trow, rK, (unsigned)r * row_b, lg);
+    store_tiles<S, D, ND>(dv[u], 16 * d0, up, false, p, trow, rV, (unsigned)r * row_b, lg);
   }
 }
 

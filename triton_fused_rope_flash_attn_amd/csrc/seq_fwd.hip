@@ -23,7 +23,6 @@ namespace farope {
 // of two.  Measured (us, forward, 64 / 32 keys): 24 sequences up to 2048 tokens, 16 heads 190 / 174,
 // 32 up to 512, 16 46 / 40, 8 x 1024, 8 46 / 41, 1 x 4096, 16 101 / 103, 1 x 16384, 8 517 / 527.
 template <typename S, int D> constexpr int kFwdRows = sizeof(S) == 2 && D == 128 ? 32 : kStageRowsOf<S, D>;
-constexpr float kSeqSlack = 8.0f;   // log2 units: P <= 2^8 between rescales
 
 // Magnitude bits of x; 0x7f800000 and up are infinities and NaN.  (The kernels are compiled without
 // regard for NaN: the empty asm keeps the compiler from concluding that x is none.)
@@ -36,7 +35,7 @@ constexpr unsigned kInfBits = 0x7f800000u;
 
 // O of one row again, key by key and only over the keys that it sees: for the rows of a causal
 // call whose sums hold a NaN that may be 0 times an infinity or NaN of a V row behind them.
-// A lane takes channel pairs; m and l are the row's maximum and sum.  Rarely needed, and slow: one
+// A lane takes channel pairs; m and l are the row's reference and sum.  Rarely needed, and slow: one
 // infinity behind 9000 of 16384 tokens, 8 heads, D 128 takes the call from 0.55 to 80 ms (32 rows,
 // a quarter of a microsecond a key), a channel of NaN throughout to 156.  What
 // finds such rows costs (us, without / with) 24 up to 2048, 16 heads, D 128 173 / 175, 64 up to 577, 12
@@ -108,7 +107,7 @@ __device__ __forceinline__ void row_again(const SeqParams& p, const SeqTile& tl,
 // Q-hat^T, so that their output rows (keys) are the k-slots of O^T += V^T P^T and P
 // never leaves registers.  The accumulators start at minus the running max, P =
 // exp2 of the product's output; O and the row sum are rescaled only when some logit
-// exceeds the running max by 2^8.
+// exceeds the running max by kSeqSlack.
 //
 // 16-bit tensors: Q-hat, K-hat and P are rounded once to their type, as the products' operands.
 // Together with O's own rounding (1.6e-3 of its norm in bf16) that leaves 2.8e-3.  P as a pair of
@@ -192,7 +191,7 @@ seq_fwd_kernel(const SeqParams p) {
   const int ns = (last + SR - 1) / SR;
 
   f32x4 acc[QT][DT];
-  float m_run[QT], l_run[QT];
+  float m_run[QT], l_run[QT];   // the running max (less kWeightUp) and sum
   f32x4 nm4[QT];       // minus the running max (0 before the first block)
   float thr = -INFINITY;   // a value above it makes the block rescale
 #pragma unroll
@@ -246,11 +245,11 @@ seq_fwd_kernel(const SeqParams p) {
       mxx = fmaxf(mxx, mx[t]);
     }
     if (__any(mxx > thr)) {
-      thr = kSeqSlack;
+      thr = kSeqSlack + kWeightUp<S>;
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         const float old = m_run[t] == -INFINITY ? 0.f : m_run[t];
-        const float mnew = fmaxf(m_run[t], group4_max(mx[t]) + old);
+        const float mnew = fmaxf(m_run[t], group4_max(mx[t]) + old - kWeightUp<S>);
         const float alpha = fast_exp2(m_run[t] - mnew), sh = old - mnew;
         m_run[t] = mnew;
         l_run[t] *= alpha;

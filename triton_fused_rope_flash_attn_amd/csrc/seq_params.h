@@ -34,7 +34,7 @@ struct SeqParams {
   void* gcopy;                       // [H, T, D]: dO, where its own rows cannot be streamed (else null)
   int* map_q;                        // [slots][4]: the tiles of the query kernels' workgroups (SeqTile); null: none
   int* map_k;                        // and of the key kernel's
-  float* nl;                         // [H, T]: -LSE * log2 e
+  float* nl;                         // [H, T]: -LSE * log2 e (fp16: and kWeightUp)
   float* nd;                         // [H, T]: -rowsum(dO * O)
   float* ng;                         // [H, T]: norms of dO's rows (fp16 at head_dim 128)
   float* pk;                         // [parts, T, Hkv, D]: sums of the parts of dK / scale (rotated), parts > 1
