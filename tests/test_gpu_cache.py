@@ -438,3 +438,33 @@ def test_decode_many_small_weights(dtype):
     # the bound of run_decode; the logit in fp32 (log2 units, 25) and exp2: 32 units of 2^-24 of the weights
     off = (got.double() - (w - 1) / (1 + w)).abs().max().item()
     assert off <= u + 3 * u * u + 32 * 2.0 ** -24, off
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype,D,H,Hkv,lens", [(BF16, 64, 16, 4, [300, 40]), (F16, 128, 32, 2, [130, 2]), (BF16, 128, 8, 8, [3000, 900]),
+                                                (F16, 64, 8, 2, [5000]), (BF16, 256, 4, 1, [600]), (F16, 32, 40, 2, [1500]), (F32, 64, 8, 2, [700, 90])])
+def test_decode_of_rows_that_are_not_finite(dtype, D, H, Hkv, lens, value):
+    """One channel of a K row (a logit of an infinity: a weight of 0, or of no value), then of a V row: the formula's
+    values, finite or not, in every head and channel."""
+    page = 16
+    pages, n = page_table(len(lens), -(-max(lens) // page))
+    kc, vc = caches(n, page, Hkv, D, dtype)
+    q = randn(len(lens), H, D, dtype=dtype, seed=3)
+    table = seq_ref.Table(max(lens), D, DEV)
+    for which in "KV":
+        bad = {"K": kc.clone(), "V": vc.clone()}
+        for b, m in enumerate(lens):
+            i = m * 5 // 8
+            bad[which][pages[b, i // page].item(), i % page, :, 5] = value
+        got = sdpa_rope_decode(q, bad["K"], bad["V"], table, pages, ints(lens)).double().cpu()
+        ref, _ = seq_ref.decode(q, bad["K"], bad["V"], table, pages, lens, True)
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)), which
+        assert torch.equal(got[torch.isinf(ref)], ref[torch.isinf(ref)]) and torch.equal(torch.isinf(got), torch.isinf(ref))
+        if which == "K" and value == value:
+            assert torch.isfinite(ref).any()
+        ok = torch.isfinite(ref)
+        # run_decode's bound, for the rows' finite channels (|V| up to 5: sum P |V| no larger)
+        u = seq_ref.U[dtype]
+        off = torch.where(ok, got - ref, 0.0).norm(dim=-1)
+        allowed = u * torch.where(ok, ref, 0.0).norm(dim=-1) + (32 * u if dtype == F32 else 3 * u * u + 32 * 2.0 ** -24) * 5 * D ** 0.5
+        assert (off <= allowed).all()

@@ -26,19 +26,32 @@ namespace farope {
 
 constexpr int kDecodeNW = 4;   // waves per worker, which take its blocks in turn
 
-// x = hi + lo in the operand type (fp32: hi alone)
+// x = hi + lo in the operand type (fp32: hi alone).  hi lies nearer to 0 than x, so that lo has its sign and is
+// not 0: the two products with an infinity of K or V then are the infinity that x times it is, not a NaN.  (Up
+// to what fp16 rounds to 0: weights of 2^-31 of the largest.)
 template <typename S> struct Split {
   using C = typename SeqComp<S>::C;
   static constexpr bool kTwo = sizeof(S) == 2;
   typename C::Frag hi, lo;
-  __device__ __forceinline__ void set(const float (&x)[8]) {
-    hi = C::make(x);
-    if constexpr (kTwo) {
-      float r[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = x[e] - (float)hi.v[e];
-      lo = C::make(r);
+  __device__ __forceinline__ void set(const float (&x)[8]) {   // (no -0)
+    if constexpr (!kTwo) {
+      hi = C::make(x);
+      return;
     }
+    float h[8], r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float below = __uint_as_float(__builtin_elementwise_sub_sat(__float_as_uint(x[e]), 1u));
+      if constexpr (std::is_same<S, f16>::value) h[e] = (float)__builtin_amdgcn_cvt_pkrtz(below, 0.f)[0];
+      else h[e] = __uint_as_float(__float_as_uint(below) & 0xffff0000u);
+      r[e] = x[e] - h[e];
+      if constexpr (std::is_same<S, f16>::value) {   // at least fp16's least value
+        const float least = __builtin_amdgcn_fmed3f(x[e], -0x1p-24f, 0x1p-24f);
+        r[e] = fabsf(r[e]) < fabsf(least) ? least : r[e];
+      }
+    }
+    hi = C::make(h);   // (exact)
+    lo = C::make(r);
   }
   __device__ __forceinline__ f32x4 mma(const typename C::Frag& a, f32x4 c) const {
     if constexpr (kTwo) c = C::mma(a, lo, c);
@@ -181,7 +194,7 @@ __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D *
         table_load4(p.cosp, p.sinp, tr, D / 2, 16 * s + 4 * lg, cs);
         rope_rotate8(x, cs);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = lr < nq ? x[e] * p.c2 : 0.f;
+        for (int e = 0; e < 8; ++e) x[e] = (lr < nq ? x[e] * p.c2 : 0.f) + 0.f;
         qf[s].set(x);
       }
     }

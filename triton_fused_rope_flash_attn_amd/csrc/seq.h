@@ -43,6 +43,15 @@ template <> struct SeqComp<bf16> { using C = Comp<DT_BF16>; };
 template <> struct SeqComp<f16> { using C = Comp<DT_F16>; };
 template <> struct SeqComp<float> { using C = CompF32x; };
 
+// Magnitude bits of x; 0x7f800000 and up are infinities and NaN.  (The kernels are compiled without
+// regard for NaN: the empty asm keeps the compiler from concluding that x is none.)
+__device__ __forceinline__ unsigned magnitude_bits(float x) {
+  unsigned u = __float_as_uint(x);
+  asm volatile("" : "+v"(u));
+  return u & 0x7fffffffu;
+}
+constexpr unsigned kInfBits = 0x7f800000u;
+
 // ---------------------------------------------------------------------------
 // Softmax weights as operands of a product: P = exp2(s - m).  m is the row's running maximum, raised when a
 // logit passes it by kSeqSlack (log2 units).  fp16 rounds what is below 2^-25 to 0, and a key of a row of 2^17 that

@@ -47,13 +47,10 @@ __device__ __forceinline__ int fit_exponent(float m, int top) {
   const int e = top + 127 - (int)(__float_as_uint(m) >> 23);
   return e > kExMost ? kExMost : e < kExLeast ? kExLeast : e;
 }
-// |x|, or 0 where it is infinite or NaN (which no scale helps, and which must not take the others'); the empty asm
-// keeps the compiler, which builds without regard for NaN, from dropping the test.
+// |x|, or 0 where it is infinite or NaN (which no scale helps, and which must not take the others')
 __device__ __forceinline__ float finite_size(float x) {
-  unsigned u = __float_as_uint(x);
-  asm volatile("" : "+v"(u));
-  u &= 0x7fffffffu;
-  return u < 0x7f800000u ? __uint_as_float(u) : 0.f;
+  const unsigned u = magnitude_bits(x);
+  return u < kInfBits ? __uint_as_float(u) : 0.f;
 }
 
 // Gradient rows of a 16-row subtile: lane holds row `row` (byte offset off), channels

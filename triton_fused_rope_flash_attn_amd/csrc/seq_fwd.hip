@@ -24,15 +24,6 @@ namespace farope {
 // 32 up to 512, 16 46 / 40, 8 x 1024, 8 46 / 41, 1 x 4096, 16 101 / 103, 1 x 16384, 8 517 / 527.
 template <typename S, int D> constexpr int kFwdRows = sizeof(S) == 2 && D == 128 ? 32 : kStageRowsOf<S, D>;
 
-// Magnitude bits of x; 0x7f800000 and up are infinities and NaN.  (The kernels are compiled without
-// regard for NaN: the empty asm keeps the compiler from concluding that x is none.)
-__device__ __forceinline__ unsigned magnitude_bits(float x) {
-  unsigned u = __float_as_uint(x);
-  asm volatile("" : "+v"(u));
-  return u & 0x7fffffffu;
-}
-constexpr unsigned kInfBits = 0x7f800000u;
-
 // O of one row again, key by key and only over the keys that it sees: for the rows of a causal
 // call whose sums hold a NaN that may be 0 times an infinity or NaN of a V row behind them.
 // A lane takes channel pairs; m and l are the row's reference and sum.  Rarely needed, and slow: one
