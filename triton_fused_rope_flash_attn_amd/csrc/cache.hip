@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendParams p,
 #pragma unroll
   for (int i = 0; i < kAppendHeads; ++i) {
     if (h0 + i >= p.Hkv) break;
-    row8<S>(static_cast<const S*>(p.k) + t * p.sk[0] + (h0 + i) * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x[i]);
+    load8<S>(static_cast<const S*>(p.k) + t * p.sk[0] + (h0 + i) * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x[i]);
     v[i] = load_raw8<S>(static_cast<const S*>(p.v) + t * p.sv[0] + (h0 + i) * p.sv[1] + c * p.sv[2], p.sv[2], p.vec_v);
   }
   float cs[8];

@@ -59,7 +59,7 @@ template <typename S> struct Split {
   }
 };
 
-// Blocks of sequence b: its rows, as far as its page list goes.
+// Rows of sequence b, as far as its page list goes, and their blocks of 32.
 __device__ __forceinline__ int cached_rows(const DecodeParams& p, int b) {
   const int64_t room = (int64_t)p.c.max_pages * p.c.page;
   const int len = p.c.lengths[b];
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D *
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         float x[8], cs[8];
-        row8<S>(qp + (32 * s + 8 * lg) * p.sq[2], p.sq[2], p.vec_q, x);
+        load8<S>(qp + (32 * s + 8 * lg) * p.sq[2], p.sq[2], p.vec_q, x);
         table_load4(p.cosp, p.sinp, tr, D / 2, 16 * s + 4 * lg, cs);
         rope_rotate8(x, cs);
 #pragma unroll

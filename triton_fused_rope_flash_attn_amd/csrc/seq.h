@@ -119,21 +119,6 @@ template <typename S, int D, int ROWS = kStageRowsOf<S, D>> struct SeqStream {
 __device__ __forceinline__ void seq_dma4(__amdgpu_buffer_rsrc_t r, void* lds, unsigned voff, unsigned soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 4, voff, soff, 0, 0);
 }
-// 16 bytes per lane from the lane's own address straight into LDS (lane l lands at
-// lds + 16 l; lds is wave-uniform).
-__device__ __forceinline__ void seq_dma16(const void* src, void* lds) {
-  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)const_cast<void*>(src),
-                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
-}
-// Immediate of s_waitcnt that waits until at most n vector-memory loads are in flight.
-constexpr int vm_wait(int n) { return n > 63 ? vm_wait(63) : (n & 15) | ((n >> 4) << 14) | 0x0F70; }
-// A wave's own LDS buffers, without a workgroup barrier: its reads of a buffer have
-// returned before it is loaded again; reads come after the wait for the loads.
-__device__ __forceinline__ void wave_lds_reads_done() {
-  __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
-  asm volatile("" : : : "memory");
-}
-__device__ __forceinline__ void wave_lds_fence() { asm volatile("" : : : "memory"); }
 // This wave's LDS loads have landed, and so have every wave's behind the barrier.
 __device__ __forceinline__ void seq_stage_barrier() {
   __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
@@ -338,10 +323,6 @@ __device__ __forceinline__ void table_load4(const float* __restrict__ cosp, cons
 // 8 channels to a staged tile (one or two 16-byte chunks)
 template <typename S, int D>
 __device__ __forceinline__ void put_tile8(S* tile, int r, int col, const float (&x)[8]);
-
-// 8 channels of a row, as floats
-template <typename S>
-__device__ __forceinline__ void row8(const S* __restrict__ p, int64_t sd, bool vec, float (&x)[8]) { load8<S>(p, sd, vec, x); }
 
 // 8 channels to a contiguous row (16 or 32 bytes)
 template <typename S>

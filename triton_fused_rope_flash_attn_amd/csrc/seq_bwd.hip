@@ -203,9 +203,9 @@ seq_dq_kernel(const SeqParams p) {
     for (int s = 0; s < KS; ++s) {
       const int c = 32 * s + 8 * lg;
       float x[8], g[8], o[8], cs[8];
-      row8<S>(qp + c * p.sq[2], p.sq[2], p.vec_q, x);
-      row8<S>(gp + c * p.sdo[2], p.sdo[2], p.vec_do, g);
-      row8<S>(op + c, 1, true, o);
+      load8<S>(qp + c * p.sq[2], p.sq[2], p.vec_q, x);
+      load8<S>(gp + c * p.sdo[2], p.sdo[2], p.vec_do, g);
+      load8<S>(op + c, 1, true, o);
       table_load4(p.cosp, p.sinp, trow[t], D / 2, c / 2, cs);
       rope_rotate8(x, cs);
       qf[t][s] = C::make(x);
@@ -501,17 +501,17 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
     const int c = 32 * s + 8 * lg;
     float x[8];
     if (p.khat) {
-      row8<S>(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c, 1, true, x);
+      load8<S>(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c, 1, true, x);
     } else {
       float cs[8];
-      row8<S>(static_cast<const S*>(p.k) + tok * p.sk[0] + kvh * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x);
+      load8<S>(static_cast<const S*>(p.k) + tok * p.sk[0] + kvh * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x);
       table_load4(p.cosp, p.sinp, trow, D / 2, c / 2, cs);
       rope_rotate8(x, cs);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= p.c2;
     }
     kf[s] = C::make(x);
-    row8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
+    load8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
     vf[s] = C::make(x);
   }
   const int w0 = k0 + wave * 16;   // the wave's first key (uniform)
@@ -709,17 +709,17 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
       const int c = 32 * s + 8 * lg;
       float x[8];
       if (p.khat) {
-        row8<S>(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c, 1, true, x);
+        load8<S>(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c, 1, true, x);
       } else {
         float cs[8];
-        row8<S>(static_cast<const S*>(p.k) + tok * p.sk[0] + kvh * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x);
+        load8<S>(static_cast<const S*>(p.k) + tok * p.sk[0] + kvh * p.sk[1] + c * p.sk[2], p.sk[2], p.vec_k, x);
         table_load4(p.cosp, p.sinp, trow, D / 2, c / 2, cs);
         rope_rotate8(x, cs);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= p.c2;
       }
       kf[u][s] = C::make(x);
-      row8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
+      load8<S>(vp + c * p.sv[2], p.sv[2], p.vec_v, x);
       vf[u][s] = C::make(x);
       if constexpr (kFitDs<S>) {
 #pragma unroll

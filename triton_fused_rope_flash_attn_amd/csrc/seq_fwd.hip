@@ -167,7 +167,7 @@ seq_fwd_kernel(const SeqParams p) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       float x[8], cs[8];
-      row8<S>(qp + (32 * s + 8 * lg) * p.sq[2], p.sq[2], p.vec_q, x);
+      load8<S>(qp + (32 * s + 8 * lg) * p.sq[2], p.sq[2], p.vec_q, x);
       table_load4(p.cosp, p.sinp, tr, D / 2, 16 * s + 4 * lg, cs);
       rope_rotate8(x, cs);
       qf[t][s] = C::make(x);
