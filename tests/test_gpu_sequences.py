@@ -554,3 +554,25 @@ def test_many_small_weights(dtype):
     off = (got["dv"][1:].double() - each).abs().max().item()
     assert off <= (4 * u + 25 * 0.7 * u) * each + 2.0 ** -25, (off, each)
     assert all(torch.isfinite(x).all() for x in got.values())
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype,D,H,Hkv", [(F16, 64, 2, 1), (F16, 128, 2, 1), (F16, 128, 48, 48), (F16, 256, 2, 2), (BF16, 128, 2, 1)])
+def test_one_row_of_do_that_is_not_finite(dtype, D, H, Hkv, value):
+    """Its own dQ row and the keys that it sees are not finite; the scale of the others' dS does not follow it."""
+    T, i = 700, 300
+    q, k, v, do = inputs(T, H, Hkv, D, dtype, seed=37)
+    do[i] = 0.0
+    table = seq_ref.Table(T, D, DEV)
+    heads = [0, H - 1] if H == Hkv else list(range(H))
+    keys = heads if H == Hkv else [0]
+    ref = seq_ref.varlen(q[:, heads], k[:, keys], v[:, keys], do[:, heads], table, starts([T]), True, True)
+    do[i] = value
+    got = grads(q, k, v, do, table, starts([T]))
+    assert not torch.isfinite(got["dq"][i]).any()
+    assert not torch.isfinite(got["dk"][:i + 1]).any() and not torch.isfinite(got["dv"][:i + 1]).any()
+    tol = {n: seq_ref.ROUNDINGS[n] * seq_ref.U[dtype] for n in ("dq", "dk", "dv")}
+    rows = torch.arange(T) != i
+    assert seq_ref.rel(got["dq"][:, heads][rows.to(DEV)], ref["dq"][rows]) <= tol["dq"]
+    assert seq_ref.rel(got["dk"][i + 1:][:, keys], ref["dk"][i + 1:]) <= tol["dk"]
+    assert seq_ref.rel(got["dv"][i + 64:][:, keys], ref["dv"][i + 64:]) <= tol["dv"]   # (0 times it, up to 63 tokens away)
