@@ -97,6 +97,9 @@ int dkdv_parts(const farope_seq_desc* d) {
 // 13.5 / 9.0, 4 x 197, 12 11.2 / 9.0, B 58 / 49, 64 x 100, 12 25.2 / 20.1, B 79 / 75, 1 x 400, 12 11.5 /
 // 12.4, 64 x 150, 12 B 103 / 104, 64 x 197, 12 36.0 / 36.8, 1 x 1024, 16 16 / 23; D 32: 128 up to 100, 8
 // B 91 / 81; D 128: 1 x 100, 8 11.4 / 9.4, 1 x 197, 12 13.0 / 13.3, 4 x 512, 16 23 / 28.
+// All of these are of like lengths.  The host knows the mean alone, which does not show one long sequence
+// beside many short ones: 8192 tokens and 100 of 1 to 30 (mean 96), 8 heads, D 64 take 224 us, B 688, where the
+// long one alone takes 100, B 428.
 bool rotates_itself(const farope_seq_desc* d, bool v_streams) {
   if (!v_streams || d->head_dim > 128) return false;
   const int mean = d->tokens / d->seqs;
@@ -199,6 +202,8 @@ int decode_tiles(const farope_seq_desc* d) { return (d->heads / d->kv_heads + 15
 // rows where the sequences alone make several rounds (up to 1024, one).  Measured (us, even
 // shares / one per sequence): 1 x 197, 12 heads, D 64 11.1 / 6.9; 256 sequences up to 1024, 8
 // heads, D 128 104 / 89; 64 x 1024, 16 heads, D 64 66 / 59; 5 up to 1025, 8 heads, fp32 14.4 / 19.3.
+// (So a short sequence in a wide table pays for the join: 197 rows, 12 heads, D 64 7 us with room for 197, 9 for
+// 512, 13 for 1024 to 131072.)
 bool decode_direct(const farope_seq_desc* d, const farope_cache_desc* c) {
   const int64_t room = (int64_t)c->max_pages * c->page_rows, wgs = (int64_t)d->seqs * d->kv_heads * decode_tiles(d);
   return room <= 512 || (room <= 1024 && wgs >= decode_wgs(d)) || (room <= 2048 && wgs >= 2 * decode_wgs(d));

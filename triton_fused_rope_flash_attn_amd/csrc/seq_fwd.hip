@@ -20,7 +20,7 @@
 namespace farope {
 
 // Keys of a stage: at head_dim 128 in 16 bits 32, which lets three workgroups run on a CU instead
-// of two.  Measured (us, forward, 64 / 32 keys): 24 sequences up to 2048 tokens, 16 heads 190 / 174,
+// of two.  Measured (us, forward, 64 / 32 keys): 24 sequences up to 2048 tokens (mean 943), 16 heads 190 / 174,
 // 32 up to 512, 16 46 / 40, 8 x 1024, 8 46 / 41, 1 x 4096, 16 101 / 103, 1 x 16384, 8 517 / 527.
 template <typename S, int D> constexpr int kFwdRows = sizeof(S) == 2 && D == 128 ? 32 : kStageRowsOf<S, D>;
 
@@ -29,7 +29,7 @@ template <typename S, int D> constexpr int kFwdRows = sizeof(S) == 2 && D == 128
 // A lane takes channel pairs; m and l are the row's reference and sum.  Rarely needed, and slow: one
 // infinity behind 9000 of 16384 tokens, 8 heads, D 128 takes the call from 0.55 to 80 ms (32 rows,
 // a quarter of a microsecond a key), a channel of NaN throughout to 156.  What
-// finds such rows costs (us, without / with) 24 up to 2048, 16 heads, D 128 173 / 175, 64 up to 577, 12
+// finds such rows costs (us, without / with) 24 up to 2048 (mean 943), 16 heads, D 128 173 / 175, 64 up to 577, 12
 // heads, D 64 40.3 / 40.6, one of 16384, D 128 553 / 549.
 template <typename S, int D, bool ROT>
 __device__ __forceinline__ void row_again(const SeqParams& p, const SeqTile& tl, int head, int kvh, int i, float m, float l, int lane) {

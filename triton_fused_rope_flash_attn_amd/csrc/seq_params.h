@@ -50,7 +50,8 @@ inline int64_t seq_slots(int T, int B, int lb) { return (int64_t)(T >> lb) + B +
 
 // Rows per workgroup of the forward and of dQ, 128 (two 16-row subtiles per wave) or 64.  Two
 // subtiles halve the LDS reads per product, but cost workgroups, and products above the
-// diagonal.  16-bit tensors; measured (us, forward and backward, 64 / 128 rows; "sequences x
+// diagonal.  ("24 up to 2048": here and beside the kernels lengths drawn down to a 16th of the longest, on a
+// logarithmic scale; these have a mean of 943.)  16-bit tensors; measured (us, forward and backward, 64 / 128 rows; "sequences x
 // tokens, heads" and the call's 128-row tiles), D 128: 24 up to 2048, 16 [2828] 916 / 869, 1 x 16384, 8
 // [1024] 2702 / 2512, 4 up to 4096, 8 [676] 455 / 484, 1 x 4096, 16 [512] 422 / 467, 8 x 1024, 8 [512]
 // 164 / 175, 64 up to 200, 8 [308] 89 / 105.  Forward, D 64: 1 x 8192, 16 [1024] 170 / 152, 1 x 4096, 16

@@ -353,6 +353,9 @@ def sdpa_rope_decode(
     new token's own among them.  Q is rotated by table row ``lengths[b] - 1 - has_cls``, or by
     positions[b] (int32 ``[B]``).
 
+    How the rows are divided goes by the page table's width (lengths stay on the GPU): for short
+    sequences a view of its first columns, as many as they need, is faster.
+
     Returns O ``[B, H, D]``.  A sequence without rows has O = 0; rows past the page table
     or on a page number that is no page of the cache are left out.  No gradients.
     """
