@@ -381,6 +381,38 @@ int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_st
                   const int32_t* page_table, const int32_t* lengths, void* o, float* ws, size_t ws_elems,
                   void* stream);
 
+/*
+ * Rows and pages of a cache that are there.  Rows move as they are: of desc seqs, kv_heads,
+ * head_dim and dtype are read.
+ *
+ * farope_cache_accept: of the drafted tokens that were appended behind the lengths[b] rows of
+ * sequence b, those that path [B, path_cols] (device memory, int32, rows path_stride elements
+ * apart) names in its leading entries of 0 or more stay: row lengths[b] + i becomes what row
+ * lengths[b] + path[b][i] was before the call.  new_lengths [B] gets lengths[b] plus their number.
+ * A row whose own or whose source's position is not in the cache stays as it is, and so does a sequence
+ * of negative length.  No row may be two sequences'.  path_cols is at most 2048.
+ */
+int farope_cache_accept(const farope_seq_desc* desc, const farope_cache_desc* cache, const int32_t* page_table,
+                        const int32_t* lengths, const int32_t* path, int64_t path_stride, int32_t path_cols,
+                        int32_t* new_lengths, void* stream);
+
+/* farope_cache_fork: place b of the batch goes on from where place parents[b] is (p; a number outside
+ * [0, seqs) empties the place).  page_table and lengths are written in place, and so are refs
+ * [pages]: how many entries of page tables hold each page; one that is 0 is free.  With n = lengths[p] rows,
+ * cut to 0 .. max_pages * page_rows, and full = n / page_rows:
+ *   entries below full are p's: the pages are shared;
+ *   entries from full on are p's where no place before b has the same parent and refs of the page is 1;
+ *   the other ones below ceil((n + room[b]) / page_rows) (room NULL or negative: 0) get pages that were free
+ *   before the call, in order of place and entry, lowest page first, or -1 where there are no more;
+ *   the rest are -1.
+ * Where entry full is a new page, the n % page_rows rows in use of p's page are copied to it.
+ * missing [1]: pages wanted and not there.  ws: farope_cache_fork_workspace_elems fp32 elements, 16-byte
+ * aligned.  seqs > 1: the rows of page_table do not overlap. */
+size_t farope_cache_fork_workspace_elems(int32_t seqs, const farope_cache_desc* cache);
+int farope_cache_fork(const farope_seq_desc* desc, const farope_cache_desc* cache, int32_t* page_table, int32_t* lengths,
+                      int32_t* refs, const int32_t* parents, const int32_t* room, int32_t* missing, float* ws,
+                      size_t ws_elems, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -231,6 +231,36 @@ DecodeWs decode_ws(const farope_seq_desc* d, const farope_cache_desc* c) {
   return w;
 }
 
+// The cache of a call that moves rows as they are: no queries, no tables.
+int check_rows(const farope_seq_desc* d) {
+  if (!d) return FAROPE_ERR_NULL;
+  if (d->seqs < 1 || d->kv_heads < 1) return FAROPE_ERR_SHAPE;
+  if (d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256) return FAROPE_ERR_HEAD_DIM;
+  if (d->dtype != FAROPE_F32 && d->dtype != FAROPE_F16 && d->dtype != FAROPE_BF16) return FAROPE_ERR_DTYPE;
+  return (int64_t)d->kv_heads * d->head_dim > (int64_t(1) << 24) ? FAROPE_ERR_SHAPE : FAROPE_OK;
+}
+int row_chunks(const farope_seq_desc* d) { return d->head_dim * elem_size(d->dtype) / 16; }
+constexpr int kMaxPath = 2048;   // columns of a path (cache_accept_kernel: 8 rows a thread)
+
+// Workspace, in fp32 elements, each part from a 16-byte boundary.
+struct ForkWs {
+  int64_t free, table, wanted, len, from, list, total;
+};
+int fork_chunks(const farope_cache_desc* c) { return (c->pages + kForkChunk - 1) / kForkChunk; }
+ForkWs fork_ws(int32_t seqs, const farope_cache_desc* c) {
+  auto al = [](int64_t x) { return (x + 3) & ~int64_t(3); };
+  const int64_t chunks = fork_chunks(c), entries = (int64_t)seqs * c->max_pages;
+  ForkWs w{};
+  w.free = chunks * (kForkChunk / 32);
+  w.table = w.free + al(chunks);
+  w.wanted = w.table + al(entries);
+  w.len = w.wanted + al(seqs);
+  w.from = w.len + al(seqs);
+  w.list = w.from + al(seqs);
+  w.total = w.list + al(entries < c->pages ? entries : c->pages);
+  return w;
+}
+
 }  // namespace
 
 extern "C" {
@@ -366,6 +396,57 @@ int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_st
   p.g_tiles = decode_tiles(desc);
   p.c2 = desc->softmax_scale * 1.4426950408889634f;
   return launch_rc(launch_decode(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
+}
+
+int farope_cache_accept(const farope_seq_desc* desc, const farope_cache_desc* cache, const int32_t* page_table,
+                        const int32_t* lengths, const int32_t* path, int64_t path_stride, int32_t path_cols, int32_t* new_lengths,
+                        void* stream) {
+  FAROPE_TRY(check_rows(desc));
+  FAROPE_TRY(check_cache(desc, cache, page_table, lengths));
+  if (path_cols < 0 || path_cols > kMaxPath || path_stride < 0) return FAROPE_ERR_SHAPE;
+  if (path_cols) FAROPE_TRY(check_ptr(path, 4));
+  FAROPE_TRY(check_ptr(new_lengths, 4));
+  AcceptParams p{};
+  p.c = cache_params(cache, page_table, lengths);
+  p.path = path; p.spath = path_stride; p.cols = path_cols;
+  p.out = new_lengths;
+  p.B = desc->seqs; p.Hkv = desc->kv_heads; p.es = elem_size(desc->dtype); p.cpr = row_chunks(desc);
+  if ((int64_t)p.B * 2 * p.Hkv * p.cpr > kMaxWorkgroups) return FAROPE_ERR_SHAPE;   // (one chunk a workgroup at least)
+  return launch_rc(launch_cache_accept(p, static_cast<hipStream_t>(stream)));
+}
+
+size_t farope_cache_fork_workspace_elems(int32_t seqs, const farope_cache_desc* cache) {
+  if (seqs < 1 || !cache || cache->pages < 1 || cache->max_pages < 1) return 0;
+  return (size_t)fork_ws(seqs, cache).total;
+}
+
+int farope_cache_fork(const farope_seq_desc* desc, const farope_cache_desc* cache, int32_t* page_table, int32_t* lengths,
+                      int32_t* refs, const int32_t* parents, const int32_t* room, int32_t* missing, float* ws, size_t ws_elems,
+                      void* stream) {
+  FAROPE_TRY(check_rows(desc));
+  FAROPE_TRY(check_cache(desc, cache, page_table, lengths));
+  if (desc->seqs > 1 && cache->table_stride < cache->max_pages) return FAROPE_ERR_SHAPE;   // (rows are written)
+  FAROPE_TRY(check_ptr(refs, 4));
+  FAROPE_TRY(check_ptr(parents, 4));
+  if (room) FAROPE_TRY(check_ptr(room, 4));
+  FAROPE_TRY(check_ptr(missing, 4));
+  FAROPE_TRY(check_ptr(ws, 16));
+  const ForkWs w = fork_ws(desc->seqs, cache);
+  if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
+  ForkParams p{};
+  p.c = cache_params(cache, page_table, lengths);
+  p.pages = page_table; p.lengths = lengths; p.refs = refs; p.parents = parents; p.room = room; p.missing = missing;
+  int32_t* const ints = reinterpret_cast<int32_t*>(ws);
+  p.bits = reinterpret_cast<uint64_t*>(ws);
+  p.free = ints + w.free; p.table = ints + w.table; p.wanted = ints + w.wanted; p.len = ints + w.len; p.from = ints + w.from;
+  p.list = ints + w.list;
+  p.chunks = fork_chunks(cache);
+  p.B = desc->seqs; p.Hkv = desc->kv_heads; p.es = elem_size(desc->dtype); p.cpr = row_chunks(desc);
+  const int64_t row = (int64_t)p.Hkv * p.cpr, chunks = 2 * (int64_t)p.c.page * row;
+  if ((int64_t)p.B * p.c.max_pages > INT32_MAX || (int64_t)p.c.page * row > INT32_MAX ||
+      (chunks / 2048 + 2) * p.B > kMaxWorkgroups || (int64_t)p.B + p.chunks > kMaxWorkgroups)
+    return FAROPE_ERR_SHAPE;
+  return launch_rc(launch_cache_fork(p, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -129,4 +129,37 @@ struct DecodeParams {
 // Workers of a call: decode_workers in seq_api.hip.
 hipError_t launch_decode(const DecodeParams& p, int dt, int D, hipStream_t st);
 
+// Rows and pages of a cache that are there (cache_pages.hip).  Rows are copied as bytes: es per
+// element, cpr 16-byte chunks a row of one head.
+struct AcceptParams {
+  CacheParams c;
+  const int* path;       // [B, cols] drafted tokens, -1 behind the last accepted one
+  int64_t spath;         // elements between its rows
+  int* out;              // [B]: the new lengths
+  int B, Hkv, cols, es, cpr;
+};
+hipError_t launch_cache_accept(const AcceptParams& p, hipStream_t st);
+
+struct ForkParams {
+  CacheParams c;
+  int* pages;            // c.pages and c.lengths, which the call writes
+  int* lengths;
+  int* refs;             // [pages of the cache]: how many entries of page tables hold a page
+  const int* parents;    // [B]: the place that place b continues
+  const int* room;       // [B]: rows to reserve behind the new length, or null
+  int* missing;          // [1]: pages wanted and not there
+  // workspace
+  uint64_t* bits;        // [chunks * 16]: free pages
+  int* free;             // [chunks]: how many
+  int* table;            // [B, max_pages]: the new page table, entries that want a page marked
+  int* wanted;           // [B]: how many do
+  int* len;              // [B]: the new lengths
+  int* from;             // [B]: the page whose rows are copied to the first page wanted, or -1
+  int* list;             // pages given out
+  int chunks;            // of kForkChunk pages
+  int B, Hkv, es, cpr;
+};
+constexpr int kForkChunk = 1024;   // pages a workgroup looks through
+hipError_t launch_cache_fork(const ForkParams& p, hipStream_t st);
+
 }  // namespace farope

@@ -1,6 +1,6 @@
 // Native kernels of the torch ops over packed sequences and over a paged cache:
-// farope::seq_fwd, seq_bwd, cache_append and cache_attn (defined in sequences.py,
-// which also refuses CPU tensors).  As in torch_ops.cpp: argument checks,
+// farope::seq_fwd, seq_bwd, cache_append, cache_attn (defined in sequences.py),
+// cache_accept and cache_fork (pages.py), which also refuse CPU tensors.  As in torch_ops.cpp: argument checks,
 // allocation and the C ABI call without the interpreter, and a native autograd
 // node.  Nothing is read back from the device: sequence starts, lengths and page
 // numbers are the kernels' to check.
@@ -215,6 +215,55 @@ Tensor cache_attn(const Tensor& q, const Tensor& kc, const Tensor& vc, const Ten
   return o;
 }
 
+// A cache whose rows move as they are (x: its first page, [rows, Hkv, D]), and the call's descriptor.
+std::pair<farope_cache_desc, farope_seq_desc> check_rows(const Tensor& kc, const Tensor& vc, const Tensor& pages,
+                                                         const Tensor& lengths) {
+  TORCH_CHECK_VALUE(kc.dim() == 4 && kc.size(0) >= 1 && kc.size(2) >= 1,
+                    "farope: the caches must be [pages, page_rows, Hkv, D]; got ", shape_str(kc));
+  check_head_dim(kc.size(3));
+  check_first(kc);
+  const farope_cache_desc c = check_cache(kc, vc, pages, lengths, kc.size(2), kc.select(0, 0));
+  farope_seq_desc d{};
+  d.seqs = to32(pages.size(0));
+  d.heads = d.kv_heads = to32(kc.size(2));
+  d.head_dim = to32(kc.size(3));
+  d.dtype = dtype_code(kc.scalar_type());
+  return {c, d};
+}
+
+Tensor cache_accept(Tensor kc, Tensor vc, const Tensor& pages, const Tensor& lengths, const Tensor& path) {
+  const auto [c, d] = check_rows(kc, vc, pages, lengths);
+  TORCH_CHECK_TYPE(path.scalar_type() == at::kInt, "farope: path must be int32; got ", dtype_str(path));
+  TORCH_CHECK_VALUE(path.dim() == 2 && path.size(0) == d.seqs && (path.size(1) <= 1 || path.stride(1) == 1),
+                    "farope: path must be [B, columns] with B=", d.seqs, ", its rows contiguous; got shape ", shape_str(path));
+  TORCH_CHECK_VALUE(path.size(1) <= 2048, "farope: path has at most 2048 columns; got ", path.size(1));
+  TORCH_CHECK(path.device() == kc.device(), "farope: path must be on the other tensors' device");
+  const c10::DeviceGuard guard(kc.device());
+  const Tensor out = at::empty({d.seqs}, lengths.options());
+  if (d.seqs == 0) return out;
+  check_rc(farope_cache_accept(&d, &c, pages.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), path.data_ptr<int32_t>(),
+                               path.stride(0), (int32_t)path.size(1), out.data_ptr<int32_t>(), stream_of(kc)),
+           "farope_cache_accept");
+  return out;
+}
+
+Tensor cache_fork(Tensor kc, Tensor vc, Tensor pages, Tensor lengths, Tensor refs, const Tensor& parents, const Opt& room) {
+  const auto [c, d] = check_rows(kc, vc, pages, lengths);
+  TORCH_CHECK_VALUE(d.seqs <= 1 || pages.stride(0) >= pages.size(1), "farope: the rows of page_table must not overlap");
+  check_ints(refs, "refs", kc.size(0), kc);
+  check_ints(parents, "parents", d.seqs, kc);
+  if (room) check_ints(*room, "room", d.seqs, kc);
+  const c10::DeviceGuard guard(kc.device());
+  const Tensor missing = d.seqs ? at::empty({1}, lengths.options()) : at::zeros({1}, lengths.options());
+  if (d.seqs == 0) return missing;
+  const Tensor ws = workspace(kc, farope_cache_fork_workspace_elems(d.seqs, &c));
+  check_rc(farope_cache_fork(&d, &c, pages.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), refs.data_ptr<int32_t>(),
+                             parents.data_ptr<int32_t>(), ints(room), missing.data_ptr<int32_t>(), floats(ws),
+                             ws.defined() ? ws.numel() : 0, stream_of(kc)),
+           "farope_cache_fork");
+  return missing;
+}
+
 // ---------------------------------------------------------------------------
 // Autograd
 // ---------------------------------------------------------------------------
@@ -309,6 +358,11 @@ Three seq_bwd_autograd(const Tensor& dout, const Tensor& q, const Tensor& k, con
   return bwd_op().call(dout, q, k, v, o, lse, cosp, sinp, cu, positions, causal, has_cls, scale);
 }
 
+void bump(std::initializer_list<Tensor*> ts) {
+  for (Tensor* t : ts)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // A cache is no part of an autograd graph.
 void cache_append_autograd(const Tensor& k, const Tensor& v, const Tensor& cosp, const Tensor& sinp, Tensor kc, Tensor vc,
                            const Tensor& pages, const Tensor& lengths, const Opt& cu, const Opt& positions, bool has_cls) {
@@ -319,8 +373,36 @@ void cache_append_autograd(const Tensor& k, const Tensor& v, const Tensor& cosp,
     at::AutoDispatchBelowADInplaceOrView below;
     append_op().call(k, v, cosp, sinp, kc, vc, pages, lengths, cu, positions, has_cls);
   }
-  for (Tensor* t : {&kc, &vc})
-    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  bump({&kc, &vc});
+}
+
+using AcceptSig = Tensor(Tensor, Tensor, const Tensor&, const Tensor&, const Tensor&);
+using ForkSig = Tensor(Tensor, Tensor, Tensor, Tensor, Tensor, const Tensor&, const Opt&);
+Tensor cache_accept_autograd(Tensor kc, Tensor vc, const Tensor& pages, const Tensor& lengths, const Tensor& path) {
+  refuse_tangents("cache_accept", {&kc, &vc});
+  TORCH_CHECK(!at::GradMode::is_enabled() || !any_requires_grad({&kc, &vc}),
+              "farope: moving rows of a cache is not differentiable; call it under torch.no_grad() or with detached tensors");
+  static const auto op = find<AcceptSig>("farope::cache_accept");
+  Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = op.call(kc, vc, pages, lengths, path);
+  }
+  bump({&kc, &vc});
+  return out;
+}
+Tensor cache_fork_autograd(Tensor kc, Tensor vc, Tensor pages, Tensor lengths, Tensor refs, const Tensor& parents, const Opt& room) {
+  refuse_tangents("cache_fork", {&kc, &vc});
+  TORCH_CHECK(!at::GradMode::is_enabled() || !any_requires_grad({&kc, &vc}),
+              "farope: copying pages of a cache is not differentiable; call it under torch.no_grad() or with detached tensors");
+  static const auto op = find<ForkSig>("farope::cache_fork");
+  Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = op.call(kc, vc, pages, lengths, refs, parents, room);
+  }
+  bump({&kc, &vc, &pages, &lengths, &refs});
+  return out;
 }
 
 struct CacheAttnNode : torch::autograd::Function<CacheAttnNode> {
@@ -351,6 +433,8 @@ TORCH_LIBRARY_IMPL(farope, CUDA, m) {
   m.impl("seq_bwd", seq_bwd);
   m.impl("cache_append", cache_append);
   m.impl("cache_attn", cache_attn);
+  m.impl("cache_accept", cache_accept);
+  m.impl("cache_fork", cache_fork);
 }
 
 TORCH_LIBRARY_IMPL(farope, AutogradCUDA, m) {
@@ -358,4 +442,6 @@ TORCH_LIBRARY_IMPL(farope, AutogradCUDA, m) {
   m.impl("seq_bwd", seq_bwd_autograd);
   m.impl("cache_append", cache_append_autograd);
   m.impl("cache_attn", cache_attn_autograd);
+  m.impl("cache_accept", cache_accept_autograd);
+  m.impl("cache_fork", cache_fork_autograd);
 }
