@@ -381,6 +381,20 @@ int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_st
                   const int32_t* page_table, const int32_t* lengths, void* o, float* ws, size_t ws_elems,
                   void* stream);
 
+/* O [T, heads, D] of several new tokens per sequence over its cache, whose rows they have been
+ * appended to: token j of sequence b is row lengths[b] + j (lengths: the rows before the new tokens, as
+ * in farope_cache_append), q is rotated by row lengths[b] + j - has_cls, or by positions [T].
+ * It sees rows 0 .. lengths[b] - 1, and of the new tokens' rows those i < tree_cols with
+ * tree[t * tree_stride + i] != 0 (device memory, bytes; t is the token's place in q), or, where tree
+ * is NULL, rows up to its own.  A token that sees no row that is in the cache has O = 0, as have all
+ * tokens of a sequence of negative length and those behind the last sequence.  desc: causal is not read.
+ * ws: farope_tree_workspace_elems fp32 elements, 16-byte aligned. */
+size_t farope_tree_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache);
+int farope_tree(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3], const float* cosp,
+                const float* sinp, const int32_t* positions, const farope_cache_desc* cache,
+                const int32_t* page_table, const int32_t* lengths, const int32_t* cu, const uint8_t* tree,
+                int64_t tree_stride, int32_t tree_cols, void* o, float* ws, size_t ws_elems, void* stream);
+
 /*
  * Rows and pages of a cache that are there.  Rows move as they are: of desc seqs, kv_heads,
  * head_dim and dtype are read.

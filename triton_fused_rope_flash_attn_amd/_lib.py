@@ -49,6 +49,8 @@ EXPORTS = (
     "farope_cache_append",
     "farope_decode_workspace_elems",
     "farope_decode",
+    "farope_tree_workspace_elems",
+    "farope_tree",
     "farope_cache_accept",
     "farope_cache_fork_workspace_elems",
     "farope_cache_fork",
@@ -133,8 +135,10 @@ _SIGNATURES = {
     "farope_cache_append": (ctypes.c_int, [_SD, _P, _S, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P]),
     "farope_decode_workspace_elems": (_Z, [_SD, _CD]),
     "farope_decode": (ctypes.c_int, [_SD, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P, _Z, _P]),
-    "farope_cache_accept": (ctypes.c_int, [_SD, _CD, _P, _P, _P, ctypes.c_int64, ctypes.c_int32, _P, _P]),
-    "farope_cache_fork_workspace_elems": (_Z, [ctypes.c_int32, _CD]),
+    "farope_tree_workspace_elems": (_Z, [_SD, _CD]),
+    "farope_tree": (ctypes.c_int, [_SD, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P, _I64, _I32, _P, _P, _Z, _P]),
+    "farope_cache_accept": (ctypes.c_int, [_SD, _CD, _P, _P, _P, _I64, _I32, _P, _P]),
+    "farope_cache_fork_workspace_elems": (_Z, [_I32, _CD]),
     "farope_cache_fork": (ctypes.c_int, [_SD, _CD, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
 }
 

@@ -67,10 +67,6 @@ __device__ __forceinline__ int cached_rows(const DecodeParams& p, int b) {
 }
 __device__ __forceinline__ int cached_blocks(const DecodeParams& p, int b) { return (int)(((int64_t)cached_rows(p, b) + 31) >> 5); }
 
-__device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
-  const int lo = __builtin_amdgcn_ds_bpermute(4 * lane, (int)x), hi = __builtin_amdgcn_ds_bpermute(4 * lane, (int)(x >> 32));
-  return (int64_t)((uint64_t)(unsigned)hi << 32 | (unsigned)lo);
-}
 template <typename S, int D>
 __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D * sizeof(S) <= 256 ? 2 : 1) decode_kernel(const DecodeParams p) {
   using T = Tile<S, D>;

@@ -202,6 +202,11 @@ __device__ __forceinline__ SeqTile find_tile(const int* __restrict__ cu, int B, 
   if (t.tile >= t.tiles) t.tile = -1;
   return t;
 }
+// x of another lane
+__device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
+  const int lo = __builtin_amdgcn_ds_bpermute(4 * lane, (int)x), hi = __builtin_amdgcn_ds_bpermute(4 * lane, (int)(x >> 32));
+  return (int64_t)((uint64_t)(unsigned)hi << 32 | (unsigned)lo);
+}
 // Inclusive sums over the wave's lanes: DPP shifts within each row of 16 lanes, then the
 // last lane of a row, and of half the wave, added to the rows behind.
 __device__ __forceinline__ unsigned wave_scan(unsigned x) {

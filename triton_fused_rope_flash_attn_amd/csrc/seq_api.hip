@@ -231,6 +231,39 @@ DecodeWs decode_ws(const farope_seq_desc* d, const farope_cache_desc* c) {
   return w;
 }
 
+// Several new tokens per sequence over a cache (tree.hip).  The host knows the sequences' number, their
+// mean of new tokens and their room alone.
+int tree_group(const farope_seq_desc* d) { return d->heads / d->kv_heads; }
+int tree_rows(const farope_seq_desc* d) {
+  return d->dtype != FAROPE_F32 && (int64_t)d->tokens * tree_group(d) / d->seqs > 64 ? 128 : 64;
+}
+int64_t tree_slots(const farope_seq_desc* d) { return (int64_t)d->tokens * tree_group(d) / tree_rows(d) + d->seqs + 1; }
+int tree_stage(const farope_seq_desc* d) { return d->head_dim * elem_size(d->dtype) <= 256 ? 64 : 32; }
+bool tree_direct(const farope_seq_desc* d, const farope_cache_desc* c) {
+  return (int64_t)c->max_pages * c->page_rows <= 512;
+}
+int tree_workers(const farope_seq_desc* d, const farope_cache_desc* c) {
+  const int64_t room = ((int64_t)c->max_pages * c->page_rows + tree_stage(d) - 1) / tree_stage(d);
+  const int64_t wgs = (int64_t)kCus * (d->head_dim * elem_size(d->dtype) <= 256 ? 2 : 1);
+  int64_t n = wgs / d->kv_heads;
+  if (n < 1) n = 1;
+  const int64_t most = tree_slots(d) * ((room + kTreeLeast - 1) / kTreeLeast);
+  return (int)(n < most ? n : most);
+}
+// Workspace, in fp32 elements, each part from a 16-byte boundary: sums, their statistics, owners.
+struct TreeWs {
+  int64_t stats, owners, total;
+};
+TreeWs tree_ws(const farope_seq_desc* d, const farope_cache_desc* c) {
+  if (tree_direct(d, c)) return TreeWs{};
+  const int64_t rows = 2 * (int64_t)tree_workers(d, c) * d->kv_heads * tree_rows(d);
+  TreeWs w{};
+  w.stats = rows * d->head_dim;
+  w.owners = w.stats + 2 * rows;
+  w.total = w.owners + 4 * tree_slots(d);
+  return w;
+}
+
 // The cache of a call that moves rows as they are: no queries, no tables.
 int check_rows(const farope_seq_desc* d) {
   if (!d) return FAROPE_ERR_NULL;
@@ -396,6 +429,55 @@ int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_st
   p.g_tiles = decode_tiles(desc);
   p.c2 = desc->softmax_scale * 1.4426950408889634f;
   return launch_rc(launch_decode(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
+}
+
+size_t farope_tree_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache) {
+  if (check_desc(desc, true) != FAROPE_OK || !cache || cache->max_pages < 1 || cache->page_rows < 1) return 0;
+  return (size_t)tree_ws(desc, cache).total;
+}
+
+int farope_tree(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3], const float* cosp, const float* sinp,
+                const int32_t* positions, const farope_cache_desc* cache, const int32_t* page_table, const int32_t* lengths,
+                const int32_t* cu, const uint8_t* tree, int64_t tree_stride, int32_t tree_cols, void* o, float* ws, size_t ws_elems,
+                void* stream) {
+  FAROPE_TRY(check_desc(desc, true));
+  if (desc->tokens == 0) return FAROPE_OK;
+  if (!q_stride) return FAROPE_ERR_NULL;
+  const int es = elem_size(desc->dtype);
+  FAROPE_TRY(check_ptr(q, es));
+  FAROPE_TRY(check_ptr(cosp, 16));
+  FAROPE_TRY(check_ptr(sinp, 16));
+  if (positions) FAROPE_TRY(check_ptr(positions, 4));
+  FAROPE_TRY(check_cache(desc, cache, page_table, lengths));
+  FAROPE_TRY(check_ptr(cu, 4));
+  if (tree && (tree_cols < 0 || tree_stride < 0)) return FAROPE_ERR_SHAPE;
+  FAROPE_TRY(check_ptr(o, 16));
+  const TreeWs w = tree_ws(desc, cache);
+  if (w.total) {
+    FAROPE_TRY(check_ptr(ws, 16));
+    if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
+  }
+  TreeParams p{};
+  p.q = q;
+  for (int i = 0; i < 3; ++i) p.sq[i] = q_stride[i];
+  p.vec_q = vec_rows(q, q_stride, es);
+  p.cosp = cosp; p.sinp = sinp; p.positions = positions; p.cu = cu;
+  p.tree = tree; p.stree = tree_stride; p.cols = tree_cols;
+  p.c = cache_params(cache, page_table, lengths);
+  p.o = o;
+  p.sums = ws;
+  p.stats = ws + w.stats;
+  p.owners = reinterpret_cast<int*>(ws + w.owners);
+  p.T = desc->tokens; p.B = desc->seqs; p.H = desc->heads; p.Hkv = desc->kv_heads; p.n_pos = desc->n_pos; p.has_cls = desc->has_cls;
+  p.rows = tree_rows(desc);
+  // (rows of a key head in 32 bits, with a tile's more; workgroups of the join: 16 rows each)
+  if ((int64_t)p.T * p.H > INT32_MAX - 256 || tree_slots(desc) * p.Hkv * (p.rows / 16) > kMaxWorkgroups) return FAROPE_ERR_SHAPE;
+  p.slots = (int)tree_slots(desc);
+  p.workers = tree_workers(desc, cache);
+  p.direct = w.total == 0;
+  p.c2 = desc->softmax_scale * 1.4426950408889634f;
+  if (!p.direct && (int64_t)p.workers * p.Hkv > kMaxWorkgroups) return FAROPE_ERR_SHAPE;
+  return launch_rc(launch_tree(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
 }
 
 int farope_cache_accept(const farope_seq_desc* desc, const farope_cache_desc* cache, const int32_t* page_table,

@@ -129,6 +129,32 @@ struct DecodeParams {
 // Workers of a call: decode_workers in seq_api.hip.
 hipError_t launch_decode(const DecodeParams& p, int dt, int D, hipStream_t st);
 
+struct TreeParams {
+  const void* q;
+  int64_t sq[3];         // token, head, channel
+  int vec_q;
+  const float* cosp;
+  const float* sinp;
+  const int* positions;  // [T], or null
+  const int* cu;         // [B + 1]
+  const uint8_t* tree;   // [T, cols]: the drafted tokens of its sequence that a token sees, or null: those up to itself
+  int64_t stree;         // elements between its rows
+  int cols;
+  CacheParams c;         // lengths: rows before the new tokens
+  void* o;               // [T, H, D]
+  float* sums;           // [2 * workers, Hkv, rows, D]: unnormalised O of a share's first and last piece
+  float* stats;          // [2 * workers, Hkv, rows, 2]: their max logit (log2 units) and row sum
+  int* owners;           // [slots, 4]: a tile's first worker, how many have a part of it, which piece the first one's is
+  int T, B, H, Hkv, n_pos, has_cls;
+  int rows;              // of a tile: 64 or 128
+  int slots;             // row slots of the call
+  int workers;           // workgroups of a key head
+  int direct;            // a workgroup a slot: nothing is joined
+  float c2;
+};
+constexpr int kTreeLeast = 2;   // stages of a worker's share at least
+hipError_t launch_tree(const TreeParams& p, int dt, int D, hipStream_t st);
+
 // Rows and pages of a cache that are there (cache_pages.hip).  Rows are copied as bytes: es per
 // element, cpr 16-byte chunks a row of one head.
 struct AcceptParams {

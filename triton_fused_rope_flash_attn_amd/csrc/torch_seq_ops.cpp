@@ -1,5 +1,5 @@
 // Native kernels of the torch ops over packed sequences and over a paged cache:
-// farope::seq_fwd, seq_bwd, cache_append, cache_attn (defined in sequences.py),
+// farope::seq_fwd, seq_bwd, cache_append, cache_attn, cache_tree (defined in sequences.py),
 // cache_accept and cache_fork (pages.py), which also refuse CPU tensors.  As in torch_ops.cpp: argument checks,
 // allocation and the C ABI call without the interpreter, and a native autograd
 // node.  Nothing is read back from the device: sequence starts, lengths and page
@@ -215,6 +215,42 @@ Tensor cache_attn(const Tensor& q, const Tensor& kc, const Tensor& vc, const Ten
   return o;
 }
 
+Tensor cache_tree(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
+                  const Tensor& pages, const Tensor& lengths, const Tensor& cu, const Opt& tree, const Opt& positions, bool has_cls,
+                  double scale) {
+  check_heads(q, "Q", "[T, H, D]");
+  check_head_dim(q.size(2));
+  check_first(q);
+  TORCH_CHECK_VALUE(kc.dim() == 4 && kc.size(2) >= 1 && q.size(1) >= 1 && q.size(1) % kc.size(2) == 0,
+                    "farope: query heads must be a multiple of the cache's key heads; got ", shape_str(q), " and ", shape_str(kc));
+  check_tables(cosp, sinp, q.size(2), q);
+  const farope_cache_desc c = check_cache(kc, vc, pages, lengths, kc.size(2), q);
+  check_cu(cu, q);
+  TORCH_CHECK_VALUE(cu.size(0) == pages.size(0) + 1, "farope: cu_seqlens must hold the page table's ", pages.size(0),
+                    " sequences; got ", cu.size(0), " elements");
+  const bool drafted = tree && tree->defined();
+  if (drafted) {
+    TORCH_CHECK_TYPE(tree->scalar_type() == at::kBool, "farope: tree must be bool; got ", dtype_str(*tree));
+    TORCH_CHECK_VALUE(tree->dim() == 2 && tree->size(0) == q.size(0) && (tree->size(1) <= 1 || tree->stride(1) == 1),
+                      "farope: tree must be [T, columns] with T=", q.size(0), ", its rows contiguous; got shape ", shape_str(*tree));
+    TORCH_CHECK(tree->device() == q.device(), "farope: tree must be on the other tensors' device");
+  }
+  if (positions) check_ints(*positions, "positions", q.size(0), q);
+  const c10::DeviceGuard guard(q.device());
+  const Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  if (q.size(0) == 0) return o;
+  const farope_seq_desc d = make_desc(q.size(0), pages.size(0), q.size(1), kc.size(2), q, cosp, true, has_cls, scale);
+  const Tensor ws = workspace(q, farope_tree_workspace_elems(&d, &c));
+  // (a tree without columns is one all the same: no token sees a new one)
+  static const uint8_t none = 0;
+  const uint8_t* sees = !drafted ? nullptr : tree->numel() ? reinterpret_cast<const uint8_t*>(tree->data_ptr<bool>()) : &none;
+  check_rc(farope_tree(&d, q.data_ptr(), strides(q), floats(cosp), floats(sinp), ints(positions), &c, pages.data_ptr<int32_t>(),
+                       lengths.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), sees, drafted ? tree->stride(0) : 0,
+                       drafted ? to32(tree->size(1)) : 0, o.data_ptr(), floats(ws), ws.defined() ? ws.numel() : 0, stream_of(q)),
+           "farope_tree");
+  return o;
+}
+
 // A cache whose rows move as they are (x: its first page, [rows, Hkv, D]), and the call's descriptor.
 std::pair<farope_cache_desc, farope_seq_desc> check_rows(const Tensor& kc, const Tensor& vc, const Tensor& pages,
                                                          const Tensor& lengths) {
@@ -426,6 +462,34 @@ Tensor cache_attn_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, 
   return attn_op().call(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale);
 }
 
+using TreeSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                       const Tensor&, const Opt&, const Opt&, bool, double);
+const c10::TypedOperatorHandle<TreeSig>& tree_op() {
+  static const auto op = find<TreeSig>("farope::cache_tree");
+  return op;
+}
+struct CacheTreeNode : torch::autograd::Function<CacheTreeNode> {
+  static Tensor forward(torch::autograd::AutogradContext*, const Tensor& q, const Tensor& kc, const Tensor& vc,
+                        const Tensor& cosp, const Tensor& sinp, const Tensor& pages, const Tensor& lengths, const Tensor& cu,
+                        const Opt& tree, const Opt& positions, bool has_cls, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return tree_op().call(q, kc, vc, cosp, sinp, pages, lengths, cu, tree, positions, has_cls, scale);
+  }
+  static variable_list backward(torch::autograd::AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "Trying to backward through farope.cache_tree.default but no autograd formula was registered "
+                       "(attention over a cache has no gradients).");
+  }
+};
+Tensor cache_tree_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
+                           const Tensor& pages, const Tensor& lengths, const Tensor& cu, const Opt& tree, const Opt& positions,
+                           bool has_cls, double scale) {
+  refuse_tangents("cache_tree", {&q, &kc, &vc, &cosp, &sinp});
+  if (at::GradMode::is_enabled() && any_requires_grad({&q, &kc, &vc}))
+    return CacheTreeNode::apply(q, kc, vc, cosp, sinp, pages, lengths, cu, tree, positions, has_cls, scale);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return tree_op().call(q, kc, vc, cosp, sinp, pages, lengths, cu, tree, positions, has_cls, scale);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(farope, CUDA, m) {
@@ -433,6 +497,7 @@ TORCH_LIBRARY_IMPL(farope, CUDA, m) {
   m.impl("seq_bwd", seq_bwd);
   m.impl("cache_append", cache_append);
   m.impl("cache_attn", cache_attn);
+  m.impl("cache_tree", cache_tree);
   m.impl("cache_accept", cache_accept);
   m.impl("cache_fork", cache_fork);
 }
@@ -442,6 +507,7 @@ TORCH_LIBRARY_IMPL(farope, AutogradCUDA, m) {
   m.impl("seq_bwd", seq_bwd_autograd);
   m.impl("cache_append", cache_append_autograd);
   m.impl("cache_attn", cache_attn_autograd);
+  m.impl("cache_tree", cache_tree_autograd);
   m.impl("cache_accept", cache_accept_autograd);
   m.impl("cache_fork", cache_fork_autograd);
 }

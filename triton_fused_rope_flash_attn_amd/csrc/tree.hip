@@ -1,0 +1,578 @@
+// Attention of several new tokens per sequence over its paged cache: a tree of
+// drafted tokens, or a chain of them (a prompt in chunks).
+//
+//   q-hat = R(position) q;  O_j = softmax(scale q-hat_j K^T) V over the rows that token j of its sequence sees: the
+//   `lengths` cached before the new tokens, and of the new ones' rows, which lie behind them, those that
+//   tree[j] names (chain: rows 0 .. j).  K is cached rotated.  A token that sees no row has O = 0.
+//
+// A key head's query rows (tokens times the heads of its group, head fastest) are taken in tiles of
+// 64 or 128, whose 4 waves have 16 or 32 of them each, and the cache's rows in stages, gathered through the page
+// table from memory straight to LDS, double-buffered, one barrier a stage.  The stages of all tiles of all
+// sequences are divided evenly over the workers (workgroups) of a key head, as in decode.hip: a
+// worker's share may end inside a tile and run on in the next; of tiles that several workers share
+// these leave unnormalised sums, which tree_join_kernel joins.
+//
+// Few rows are bound by memory (the cache is read once a tile), many by the issue of matrix and vector
+// instructions, as the forward over packed sequences.
+#include <type_traits>
+
+#include "seq.h"
+
+namespace farope {
+
+// What a sequence has: its tokens, rows cached before them, rows in the cache with them, tiles, stages of a tile.
+struct TreeSeq {
+  int start, m, len, n, tiles, blocks;
+};
+template <int ROWS, int SR>
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
+  TreeSeq s;
+  s.start = cu_at(p.cu, b, p.T);
+  const int end = cu_at(p.cu, b + 1, p.T);
+  s.m = end > s.start ? end - s.start : 0;
+  s.len = p.c.lengths[b];
+  const int64_t room = (int64_t)p.c.max_pages * p.c.page, all = (int64_t)s.len + s.m;
+  const int64_t n = s.len < 0 ? 0 : all < room ? all : room;
+  s.n = n < INT32_MAX - 255 ? (int)n : INT32_MAX - 255;   // (so that a stage's last row has a number)
+  s.tiles = (int)(((int64_t)s.m * (p.H / p.Hkv) + ROWS - 1) / ROWS);
+  s.blocks = s.n > 0 ? (s.n + SR - 1) / SR : 1;   // (a tile without rows is visited too, for its zeros)
+  return s;
+}
+
+__device__ __forceinline__ int64_t wave_scan64(int64_t x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int64_t y = shfl64(x, lane - d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ int64_t lane64(int64_t x, int l) {
+  return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)x, l));
+}
+
+// The tile of a slot: sequence i takes slots (cu[i] * group >> lb) + i on, as in find_tile (seq.h).
+__device__ __forceinline__ void find_rows(const TreeParams& p, int lb, int slot, int lane, int& seq, int& tile) {
+  const int group = p.H / p.Hkv;
+  int lo = 0, n = p.B + 1;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, j = lane * step;
+    const bool le = j < n && ((cu_at(p.cu, lo + (j < n ? j : 0), p.T) * group) >> lb) + lo + j <= slot;
+    const int k = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(le) | 1ull);
+    lo += k * step;
+    n = n - k * step < step ? n - k * step : step;
+  }
+  seq = __builtin_amdgcn_readfirstlane(lo);
+  tile = slot - (((cu_at(p.cu, seq, p.T) * group) >> lb) + seq);
+}
+
+// 16 bytes per lane from memory straight into LDS (lane l lands at lds + 16 l); off lanes write nothing.
+__device__ __forceinline__ void gather16(const void* from, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)from,
+                                   (__attribute__((address_space(3))) unsigned*)lds, 16, 0, 0);
+}
+
+// O (or the sums) of one row of a tile again, row by row of the cache and only over those that it sees: for
+// rows whose sums hold an infinity or a NaN, which may be 0 times a value of a row that they do not see, or of one
+// that they see with a weight that rounds to 0.  m: the row's reference; out: `factor` times the sums,
+// rounded where they are O.  A lane takes channel pairs.  Rarely needed, and slow.
+template <typename S, int D>
+__device__ __forceinline__ void tree_row_again(const TreeParams& p, const TreeSeq& s, int b, int kvh, int head, int j, int seen,
+                                               int from, int to, float m, float factor, void* out, bool is_o, int lane) {
+  constexpr int NP = D > 128 ? D / 128 : 1;
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const bool on = lane < D / 2;
+  const int64_t tok = s.start + j, index = (int64_t)s.len + j - p.has_cls;
+  const int tr = table_row(p.positions ? p.positions[tok] : (int)(index < INT32_MAX ? index : INT32_MAX), p.n_pos);
+  f2 q[NP], acc[NP];
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    const int c = on ? 2 * (lane + 64 * n) : 0;
+    const S* const x = static_cast<const S*>(p.q) + tok * p.sq[0] + head * p.sq[1] + c * p.sq[2];
+    const float x0 = (float)x[0], x1 = (float)x[p.sq[2]];
+    const int64_t at = (int64_t)tr * (D / 2) + c / 2;
+    const float co = tr < 0 ? 1.f : p.cosp[at], si = tr < 0 ? 0.f : p.sinp[at];
+    q[n] = f2{(float)(S)((x0 * co - x1 * si) * p.c2), (float)(S)((x1 * co + x0 * si) * p.c2)};
+    acc[n] = f2{0.f, 0.f};
+  }
+  for (int r = from; r < to; ++r) {
+    if (p.tree ? r >= s.len && (r - s.len >= p.cols || !p.tree[tok * p.stree + r - s.len]) : r >= seen) continue;
+    const int place = r / p.c.page, g = p.c.pages[b * p.c.spages + place];
+    if (g < 0 || g >= p.c.n_pages) continue;
+    const int64_t in = r - (int64_t)place * p.c.page;
+    const S* const k = static_cast<const S*>(p.c.kc) + g * p.c.skc[0] + in * p.c.skc[1] + kvh * p.c.skc[2];
+    const S* const v = static_cast<const S*>(p.c.vc) + g * p.c.svc[0] + in * p.c.svc[1] + kvh * p.c.svc[2];
+    float x = 0.f;
+    f2 y[NP];
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const int c = on ? 2 * (lane + 64 * n) : 0;
+      x += on ? q[n][0] * (float)k[c] + q[n][1] * (float)k[c + 1] : 0.f;
+      y[n] = f2{(float)v[c], (float)v[c + 1]};
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x += __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (lane ^ d), __float_as_int(x)));
+    const float w = (float)(S)fast_exp2(x - m);
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) acc[n][e] += (magnitude_bits(y[n][e]) >= kInfBits ? fmaxf(w, 0x1p-126f) : w) * y[n][e];
+  }
+#pragma unroll
+  for (int n = 0; n < NP; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int c = 2 * (lane + 64 * n) + e;
+      const float x = acc[n][e] * factor;
+      if (!on) continue;
+      if (is_o) static_cast<S*>(out)[c] = (S)x;
+      else static_cast<float*>(out)[c] = x;
+    }
+}
+
+template <typename S, int D, int QT>
+__global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tree_kernel(const TreeParams p) {
+  using C = typename SeqComp<S>::C;
+  using Frag = typename C::Frag;
+  using T = Tile<S, D>;
+  constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, ROWS = 64 * QT, LB = QT == 2 ? 7 : 6;
+  constexpr uint64_t kAll = SR == 64 ? ~0ull : 0xffffffffull;
+  __shared__ __attribute__((aligned(16))) S sK0[SR * D], sK1[SR * D], sV0[SR * D], sV1[SR * D];
+
+  const int tid = thread_id();
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  const int worker = block_id() / p.Hkv, kvh = block_id() % p.Hkv, group = p.H / p.Hkv;
+
+  // this worker's stages [at, stop) of all, from stage `first` of tile `tile` of sequence b on; `before`: the
+  // stages of the tiles before that one
+  int b = 0, tile = 0, first = 0, which = 0;
+  int64_t at = 0, stop = 0, before = 0, size = 1;
+  if (p.direct) {
+    find_rows(p, LB, worker, lane, b, tile);
+    if (b == p.B) {   // tokens behind the last sequence: zeros
+      const int start = cu_at(p.cu, b, p.T), rows = (p.T - start) * group, r0 = tile * ROWS;
+      for (int r = r0 + tid / (D / 8); r < rows && r < r0 + ROWS; r += kSeqThreads / (D / 8)) {
+        const float z[8] = {};
+        put_row8<S>(static_cast<S*>(p.o) + ((int64_t)(start + r / group) * p.H + kvh * group + r % group) * D + 8 * (tid % (D / 8)), z);
+      }
+      return;
+    }
+    const TreeSeq s = tree_seq<ROWS, SR>(p, b);
+    if (tile >= s.tiles) return;
+  } else {
+    int64_t all = 0, n = 0, sum = 0;
+    for (int i = 0; i < p.B; i += 64) {
+      n = 0;
+      if (i + lane < p.B) {
+        const TreeSeq s = tree_seq<ROWS, SR>(p, i + lane);
+        n = (int64_t)s.tiles * s.blocks;
+      }
+      sum = wave_scan64(n, lane);
+      all += lane64(sum, 63);
+    }
+    const int64_t even = (all + p.workers - 1) / p.workers;
+    size = even > kTreeLeast ? even : kTreeLeast;
+    at = worker * size;
+    if (at >= all) return;
+    stop = at + size < all ? at + size : all;
+    b = -1;
+    for (int i = 0; i < p.B; i += 64) {   // (some sequence holds stage `at`)
+      if (p.B > 64) {
+        n = 0;
+        if (i + lane < p.B) {
+          const TreeSeq s = tree_seq<ROWS, SR>(p, i + lane);
+          n = (int64_t)s.tiles * s.blocks;
+        }
+        sum = wave_scan64(n, lane);
+      }
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > at);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        b = i + l;
+        before += lane64(sum, l) - lane64(n, l);
+        break;
+      }
+      before += lane64(sum, 63);
+    }
+    if (b < 0) return;
+    const TreeSeq s = tree_seq<ROWS, SR>(p, b);
+    tile = (int)((at - before) / s.blocks);
+    before += (int64_t)tile * s.blocks;
+    first = (int)(at - before);
+  }
+
+  FragAt<S, D> frag;
+  frag.init(lr, lg);
+
+  for (;;) {
+    const TreeSeq s = tree_seq<ROWS, SR>(p, b);
+    const int stages = p.direct || stop - at > s.blocks - first ? s.blocks : first + (int)(stop - at);   // this piece: [first, stages)
+    const int r0 = tile * ROWS, rows = s.m * group - r0 < ROWS ? s.m * group - r0 : ROWS;
+    const bool chain = !p.tree;
+    // rows of the cache that the tile's last token sees (a tree's: all); stages behind them hold nothing for it
+    auto seen_by = [&](int row) {   // (int64: a length may be any number)
+      const int64_t x = chain ? (int64_t)s.len + (r0 + row) / group + 1 : s.n;
+      return x < s.n ? (int)x : s.n;
+    };
+    const int last = (seen_by(rows - 1) + SR - 1) / SR, end = stages < last ? stages : last;
+
+    // lane l: row l of a stage: page and row in it
+    const int* const pages = p.c.pages + b * p.c.spages;
+    struct Ids { int page, row; };
+    auto fetch = [&](int st) __attribute__((always_inline)) {
+      Ids id{-1, 0};
+      const int64_t r = (int64_t)st * SR + lane;
+      if (st < end && lane < SR && r < s.n) {
+        const unsigned place = (unsigned)r / (unsigned)p.c.page;
+        id.page = pages[place];
+        id.row = (int)((unsigned)r - place * (unsigned)p.c.page);
+      }
+      return id;
+    };
+    uint64_t rows_in = 0;   // rows (bits) of the loaded stage that exist
+    auto load = [&](const Ids& id, S* __restrict__ kd, S* __restrict__ vd) __attribute__((always_inline)) {
+      const bool in = id.page >= 0 && id.page < p.c.n_pages;
+      rows_in = __builtin_amdgcn_ballot_w64(in);
+      const int64_t g = in ? id.page : 0, r = in ? id.row : 0;   // (the others read page 0's first row)
+      const int64_t ko = g * p.c.skc[0] + r * p.c.skc[1], vo = g * p.c.svc[0] + r * p.c.svc[1];
+      const S* const kb = static_cast<const S*>(p.c.kc) + kvh * p.c.skc[2];
+      const S* const vb = static_cast<const S*>(p.c.vc) + kvh * p.c.svc[2];
+#pragma unroll
+      for (int i = 0; i < T::NI; ++i) {
+        const int rw = (i * kSeqNW + wave) * T::RPI + lane / T::CPR, ch = ((lane % T::CPR) ^ T::chunk_xor(rw)) * T::EPC;
+        gather16(kb + shfl64(ko, rw) + ch, kd + (i * kSeqNW + wave) * T::RPI * D);
+      }
+#pragma unroll
+      for (int i = 0; i < T::NI; ++i) {
+        const int rw = (i * kSeqNW + wave) * T::RPI + lane / T::CPR, ch = ((lane % T::CPR) ^ T::chunk_xor(rw)) * T::EPC;
+        S* const to = vd + (i * kSeqNW + wave) * T::RPI * D;
+        const S* const from = vb + shfl64(vo, rw) + ch;
+        if (rows_in == kAll) {   // uniform
+          gather16(from, to);
+        } else if (rows_in >> rw & 1) {
+          gather16(from, to);
+        } else {   // V rows that do not exist are zeros: their weights are
+          *reinterpret_cast<u32x4*>(to + lane * T::EPC) = u32x4{0u, 0u, 0u, 0u};
+        }
+      }
+    };
+
+    const int row0 = wave * 16 * QT + lr;   // of the tile; subtile t: + 16 t
+    const int w0 = wave * 16 * QT, w1 = w0 + 16 * QT < rows ? w0 + 16 * QT - 1 : rows - 1;
+    const bool active = w0 < rows;
+    // every row of the wave sees rows below lo of the cache, none sees rows from hi on
+    const int lo = chain ? seen_by(active ? w0 : 0) : s.len < s.n ? s.len : s.n, hi = seen_by(active ? w1 : 0);
+    Frag qf[QT][KS];
+    int seen[QT];                // chain: rows that the lane's row of the subtile sees
+    const uint8_t* sees[QT];     // tree: its row of the tree
+    f32x4 acc[QT][DT];
+    float m_run[QT], l_run[QT];
+    {
+      Ids next = fetch(first);
+      if (first < end) load(next, sK0, sV0);
+      next = fetch(first + 1);
+      {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const int r = row0 + 16 * t < rows ? row0 + 16 * t : rows - 1, j = (r0 + r) / group, h = kvh * group + (r0 + r) % group;
+          const int64_t tok = s.start + j, index = (int64_t)s.len + j - p.has_cls;
+          seen[t] = seen_by(r);
+          sees[t] = p.tree + tok * p.stree;
+          const int tr = table_row(p.positions ? p.positions[tok] : (int)(index < INT32_MAX ? index : INT32_MAX), p.n_pos);
+          const S* const qp = static_cast<const S*>(p.q) + tok * p.sq[0] + h * p.sq[1];
+#pragma unroll
+          for (int c = 0; c < KS; ++c) {
+            float x[8], cs[8];
+            load8<S>(qp + (32 * c + 8 * lg) * p.sq[2], p.sq[2], p.vec_q, x);
+            table_load4(p.cosp, p.sinp, tr, D / 2, 16 * c + 4 * lg, cs);
+            rope_rotate8(x, cs);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= p.c2;
+            qf[t][c] = C::make(x);   // (16-bit tensors: rounded once, with the scale)
+          }
+        }
+      }
+      float thr = -INFINITY;   // a value above it makes the stage rescale
+      f32x4 nm4[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        m_run[t] = -INFINITY;
+        l_run[t] = 0.f;
+        nm4[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+
+      auto blocks = [&](bool tail, uint64_t have, int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
+        f32x4 sacc[NB][QT][2];
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const Frag a = frag.row(k + 32 * j * D, c, h);
+#pragma unroll
+              for (int t = 0; t < QT; ++t) sacc[j][t][h] = C::mma(a, qf[t][c], c == 0 ? nm4[t] : sacc[j][t][h]);
+            }
+        if (tail) {   // uniform: some row of the wave does not see all of these rows
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int e = 32 * j + 16 * h + 4 * lg + i, key = k0 + e;
+                  bool in = have >> e & 1;
+                  if (chain) {
+                    in = in && key < seen[t];
+                  } else if (in && key >= s.len) {
+                    in = key - s.len < p.cols && sees[t][key - s.len] != 0;
+                  }
+                  sacc[j][t][h][i] = in ? sacc[j][t][h][i] : -INFINITY;
+                }
+          }
+        }
+        float mx[QT], mxx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          mx[t] = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const f32x4 x = sacc[j][t][h];
+              mx[t] = fmaxf(mx[t], fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+            }
+          mxx = fmaxf(mxx, mx[t]);
+        }
+        if (__any(mxx > thr)) {   // (as in the forward over packed sequences)
+          thr = kSeqSlack + kWeightUp<S>;
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            const float old = m_run[t] == -INFINITY ? 0.f : m_run[t];
+            const float mnew = fmaxf(m_run[t], group4_max(mx[t]) + old - kWeightUp<S>);
+            const bool none = mnew == -INFINITY;   // the row has seen nothing yet
+            const float alpha = none ? 1.f : fast_exp2(m_run[t] - mnew), sh = none ? 0.f : old - mnew, nm = none ? 0.f : -mnew;
+            m_run[t] = mnew;
+            thr = none ? -INFINITY : thr;
+            l_run[t] *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[t][d] *= alpha;
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) sacc[j][t][h] += sh;
+            nm4[t] = f32x4{nm, nm, nm, nm};
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          Frag pf[QT];
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            float x[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[4 * h + i] = fast_exp2(sacc[j][t][h][i]);
+            l_run[t] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            pf[t] = C::make(x);   // (16-bit tensors: P rounded to their type for the O product; the row sum is not)
+          }
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const Frag a = frag.col(v + 32 * j * D, d);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) acc[t][d] = C::mma(a, pf[t], acc[t][d]);
+          }
+        }
+      };
+      auto stage = [&](int st, const S* __restrict__ k, const S* __restrict__ v, S* __restrict__ kn, S* __restrict__ vn)
+          __attribute__((always_inline)) {
+        seq_stage_barrier();
+        const uint64_t have = rows_in;
+        if (st + 1 < end) {
+          load(next, kn, vn);
+          next = fetch(st + 2);
+        }
+        const int k0 = st * SR;
+        if (active && k0 < hi) blocks(have != kAll || k0 + SR > lo, have, k0, k, v);
+      };
+      for (int st = first; st < end; st += 2) {
+        stage(st, sK0, sV0, sK1, sV1);
+        if (st + 1 < end) stage(st + 1, sK1, sV1, sK0, sV0);
+      }
+    }
+
+    const bool whole = first == 0 && stages == s.blocks;   // the tile is this worker's alone
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const int row = row0 + 16 * t;
+      const float l = group4_sum(l_run[t]);
+      if (whole) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const int j = (r0 + row) / group, h = kvh * group + (r0 + row) % group;
+        S* const o = static_cast<S*>(p.o) + ((int64_t)(s.start + j) * p.H + h) * D;
+#pragma unroll
+        for (int d0 = 0; d0 < DT; d0 += 2) {
+          if constexpr (sizeof(S) == 4) {
+#pragma unroll
+            for (int d = d0; d < d0 + 2; ++d) {
+              const f32x4 x = acc[t][d] * inv;
+              if (row < rows) *reinterpret_cast<f32x4*>(o + 16 * d + 4 * lg) = x;
+            }
+          } else {
+            // lane groups lg and lg^1 trade halves so that each lane stores 8 consecutive channels
+            u32x2 w[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              typedef S s4 __attribute__((ext_vector_type(4)));
+              s4 a;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a[e] = (S)(acc[t][d0 + k][e] * inv);
+              __builtin_memcpy(&w[k], &a, 8);
+            }
+            u32x4 x;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const auto y = __builtin_amdgcn_permlane16_swap(w[0][k], w[1][k], false, false);
+              x[k] = y[0];
+              x[2 + k] = y[1];
+            }
+            if (row < rows) *reinterpret_cast<u32x4*>(o + 16 * (d0 + (lg & 1)) + 4 * (lg & 2)) = x;
+          }
+        }
+      } else if (row < rows) {
+        // (the first piece of a share and its last one: no other piece is a part of a tile)
+        const int64_t at_row = ((int64_t)(2 * worker + which) * p.Hkv + kvh) * ROWS + row;
+        if (m_run[t] > -INFINITY) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.sums + at_row * D + 16 * d + 4 * lg) = acc[t][d];
+        }
+        if (lg == 0) {
+          p.stats[2 * at_row] = m_run[t];
+          p.stats[2 * at_row + 1] = l;
+        }
+      }
+    }
+    // rows (bits) whose sums are not finite (a sum is not if a term is not) while their weights' sum is
+    unsigned odd[QT], any = 0;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      f32x4 x = acc[t][0];
+#pragma unroll
+      for (int d = 1; d < DT; ++d) x += acc[t][d];
+      const float sum = (x[0] + x[1]) + (x[2] + x[3]);
+      const uint64_t bad = __builtin_amdgcn_ballot_w64(magnitude_bits(sum) >= kInfBits && row0 + 16 * t < rows);
+      const uint64_t fine = __builtin_amdgcn_ballot_w64(magnitude_bits(group4_sum(l_run[t])) - 1u < kInfBits - 1u);
+      odd[t] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & fine) & 0xffffu;
+      any |= odd[t];
+    }
+    if (any) {   // (uniform)
+      __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the rows as stored above come first
+      asm volatile("" : : : "memory");
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const float l = group4_sum(l_run[t]);
+        for (unsigned left = odd[t]; left; left &= left - 1) {
+          const int i = __builtin_ctz(left), row = w0 + 16 * t + i, j = (r0 + row) / group, h = kvh * group + (r0 + row) % group;
+          const float m = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run[t]), i));
+          const float li = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l), i));
+          void* const out = whole ? static_cast<void*>(static_cast<S*>(p.o) + ((int64_t)(s.start + j) * p.H + h) * D)
+                                  : static_cast<void*>(p.sums + (((int64_t)(2 * worker + which) * p.Hkv + kvh) * ROWS + row) * D);
+          tree_row_again<S, D>(p, s, b, kvh, h, j, seen_by(row), first * SR, end * SR < s.n ? end * SR : s.n, m, whole ? 1.f / li : 1.f,
+                               out, whole, lane);
+        }
+      }
+    }
+    if (p.direct) return;
+    // the join's: the tile's first worker, how many have a part of it, and which piece the first one's is
+    if (first == 0 && tid == 0 && kvh == 0) {
+      int* const own = p.owners + 4 * ((int64_t)((s.start * group) >> LB) + b + tile);
+      own[0] = worker;
+      own[1] = (int)((before + s.blocks - 1) / size) - worker + 1;
+      own[2] = which;
+    }
+    at += stages - first;
+    if (at >= stop) return;
+    before += s.blocks;
+    first = 0;
+    which = 1;
+    if (++tile == s.tiles) {
+      tile = 0;
+      do {   // (stages are left, so a sequence with tokens follows)
+        if (++b == p.B) return;
+      } while (cu_at(p.cu, b + 1, p.T) <= cu_at(p.cu, b, p.T));
+    }
+    lds_barrier();   // (the last stage has been read)
+  }
+}
+
+// O of the tiles that more than one worker had a part of, and zeros of the tokens behind the last
+// sequence.  A workgroup takes 16 rows of a tile; a thread 4 channels of one.
+template <typename S, int D, int QT>
+__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
+  constexpr int ROWS = 64 * QT, LB = QT == 2 ? 7 : 6, SUB = ROWS / 16, Q = D / 4;
+  const int tid = thread_id(), lane = tid & 63;
+  const int sub = block_id() % SUB, rest = block_id() / SUB, kvh = rest % p.Hkv, slot = rest / p.Hkv, group = p.H / p.Hkv;
+  int b, tile;
+  find_rows(p, LB, slot, lane, b, tile);
+  const int start = cu_at(p.cu, b, p.T), end = b < p.B ? cu_at(p.cu, b + 1, p.T) : p.T;
+  const int rows = (end > start ? end - start : 0) * group - tile * ROWS;   // (of this tile and those behind it)
+  if (rows <= 16 * sub) return;
+  int w0 = 0, n = 0, which = 0;
+  if (b < p.B) {
+    w0 = p.owners[4 * (int64_t)slot];
+    n = p.owners[4 * (int64_t)slot + 1];
+    which = p.owners[4 * (int64_t)slot + 2];
+    // finished by its worker; or, where starts do not ascend, no worker's
+    if (n <= 1 || w0 < 0 || n > p.workers || w0 > p.workers - n || (which & ~1)) return;
+  }
+  for (int u = tid; u < 16 * Q; u += 256) {
+    const int row = 16 * sub + u / Q, c = 4 * (u % Q);
+    if (row >= rows) break;
+    auto at = [&](int i) { return ((int64_t)(2 * (w0 + i) + (i ? 0 : which)) * p.Hkv + kvh) * ROWS + row; };
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < n; ++i) m = fmaxf(m, p.stats[2 * at(i)]);
+    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < n; ++i) {
+      const float mi = p.stats[2 * at(i)];
+      if (mi == -INFINITY) continue;
+      const float a = fmaxf(fast_exp2(mi - m), 0x1p-126f);   // (an infinite sum stays one)
+      l += a * p.stats[2 * at(i) + 1];
+      x += a * *reinterpret_cast<const f32x4*>(p.sums + at(i) * D + c);
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int r = tile * ROWS + row;
+    const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+    store4<S>(static_cast<S*>(p.o) + ((int64_t)(start + r / group) * p.H + kvh * group + r % group) * D + c, 1, true, y);
+  }
+}
+
+template <typename S, int D, int QT>
+static hipError_t tree(const TreeParams& p, hipStream_t st) {
+  constexpr int SUB = 4 * QT;
+  hipLaunchKernelGGL((tree_kernel<S, D, QT>), dim3((unsigned)p.Hkv * (unsigned)(p.direct ? p.slots : p.workers)), dim3(kSeqThreads), 0, st, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.direct) return e;
+  hipLaunchKernelGGL((tree_join_kernel<S, D, QT>), dim3((unsigned)p.slots * p.Hkv * SUB), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+template <typename S, int D>
+static hipError_t tree_rows(const TreeParams& p, hipStream_t st) {
+  if constexpr (sizeof(S) == 2)
+    if (p.rows == 128) return tree<S, D, 2>(p, st);
+  return tree<S, D, 1>(p, st);
+}
+template <typename S>
+static hipError_t tree_d(const TreeParams& p, int D, hipStream_t st) {
+  return D == 32 ? tree_rows<S, 32>(p, st) : D == 64 ? tree_rows<S, 64>(p, st) : D == 128 ? tree_rows<S, 128>(p, st) : tree_rows<S, 256>(p, st);
+}
+hipError_t launch_tree(const TreeParams& p, int dt, int D, hipStream_t st) {
+  return dt == DT_BF16 ? tree_d<bf16>(p, D, st) : dt == DT_F16 ? tree_d<f16>(p, D, st) : tree_d<float>(p, D, st);
+}
+
+}  // namespace farope

@@ -7,7 +7,8 @@ decoder), with the same tables, rotation and class-token convention:
 * ``sdpa_rope_varlen``   attention over packed sequences of different lengths,
                          causal or not, with shared key heads; forward and gradients;
 * ``rope_cache_append``  new keys (rotated on the way) and values into a paged cache;
-* ``sdpa_rope_decode``   one new token per sequence over its cached keys.
+* ``sdpa_rope_decode``   one new token per sequence over its cached keys;
+* ``sdpa_rope_tree``     several new tokens per sequence over them: a drafted tree, or a chunk of a prompt.
 
 The reference has no counterpart: its calls are dense [B, H, N, D] planes.
 
@@ -22,7 +23,7 @@ the device, and a captured call reads their new values when it is replayed.
 Their values are therefore not refused; each function says what it does with
 those that make no sense, and none reads or writes outside its tensors.
 
-The work is done by four ``torch.library`` ops with native GPU kernels
+The work is done by five ``torch.library`` ops with native GPU kernels
 (csrc/torch_seq_ops.cpp), one call into libfarope.so each, on the current stream of
 the tensors' device.  There is no CPU fallback: CPU tensors raise.
 """
@@ -35,7 +36,7 @@ import torch
 from . import _lib
 from .attention import _check_device, _sdpa_comp_dtype
 
-__all__ = ["sdpa_rope_varlen", "rope_cache_append", "sdpa_rope_decode"]
+__all__ = ["sdpa_rope_varlen", "rope_cache_append", "sdpa_rope_decode", "sdpa_rope_tree"]
 
 HEAD_DIMS = (32, 64, 128, 256)
 
@@ -245,10 +246,48 @@ def _cache_attn_fake(q, k_cache, v_cache, cosp, sinp, page_table, lengths, posit
     return q.new_empty(tuple(q.shape))
 
 
+@torch.library.custom_op("farope::cache_tree", mutates_args=())
+def _cache_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cosp: torch.Tensor, sinp: torch.Tensor,
+                page_table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor, tree: Optional[torch.Tensor],
+                positions: Optional[torch.Tensor], has_cls: bool, softmax_scale: float) -> torch.Tensor:
+    """-> O [T, H, D]."""
+    _check_tree(q, k_cache, v_cache, cosp, sinp, page_table, lengths, cu, tree, positions)
+    _check_device(q)
+    _lib.require_torch_ops()
+
+
+def _check_tree(q, k_cache, v_cache, cosp, sinp, page_table, lengths, cu, tree, positions):
+    _check_first(q, "Q", "[T, H, D]")
+    if k_cache.dim() != 4 or k_cache.shape[2] < 1 or q.shape[1] < 1 or q.shape[1] % k_cache.shape[2]:
+        raise ValueError("farope: query heads must be a multiple of the cache's key heads; got "
+                         f"{tuple(q.shape)} and {tuple(k_cache.shape)}")
+    _check_tables(cosp, sinp, q)
+    _check_cache(k_cache, v_cache, page_table, lengths, k_cache.shape[2], q)
+    _check_cu(cu, q)
+    if cu.shape[0] != page_table.shape[0] + 1:
+        raise ValueError(f"farope: cu_seqlens must hold the page table's {page_table.shape[0]} sequences; got {cu.shape[0]} elements")
+    if tree is not None:
+        if tree.dtype != torch.bool:
+            raise TypeError(f"farope: tree must be bool; got {tree.dtype}")
+        if tree.dim() != 2 or tree.shape[0] != q.shape[0] or (tree.shape[1] > 1 and tree.stride(1) != 1):
+            raise ValueError(f"farope: tree must be [T, columns] with T={q.shape[0]}, its rows contiguous; got shape {tuple(tree.shape)}")
+        if tree.device != q.device:
+            raise RuntimeError("farope: tree must be on the other tensors' device")
+    if positions is not None:
+        _check_ints(positions, "positions", q.shape[0], q)
+
+
+@_cache_tree.register_fake
+def _cache_tree_fake(q, k_cache, v_cache, cosp, sinp, page_table, lengths, cu, tree, positions, has_cls, softmax_scale):
+    _check_tree(q, k_cache, v_cache, cosp, sinp, page_table, lengths, cu, tree, positions)
+    return q.new_empty(tuple(q.shape))
+
+
 _lib.load_torch_ops()   # (their kernels for GPU tensors, as in attention.py)
 _seq_fwd_op = torch.ops.farope.seq_fwd.default
 _append_op = torch.ops.farope.cache_append.default
 _attn_op = torch.ops.farope.cache_attn.default
+_tree_op = torch.ops.farope.cache_tree.default
 
 
 # ---------------------------------------------------------------------------
@@ -361,3 +400,38 @@ def sdpa_rope_decode(
     """
     cosp, sinp = _tables(cos_sin)
     return _attn_op(Q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions, has_cls, _scale(Q.shape[-1]))
+
+
+def sdpa_rope_tree(
+    Q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    cos_sin,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    *,
+    tree: Optional[torch.Tensor] = None,
+    has_cls: bool = True,
+    positions: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of several new tokens per sequence over its paged cache: a tree of drafted tokens
+    that is to be verified, or, without ``tree``, a chain of tokens, such as a chunk of a prompt.
+
+    The new tokens have been appended (``rope_cache_append`` with the same page_table, lengths,
+    cu_seqlens and positions).  Q: ``[T, H, D]`` of the cache's dtype, any strides, packed as
+    cu_seqlens (int32 ``[B + 1]``) says; caches and page_table as in ``rope_cache_append``;
+    lengths: int32 ``[B]``, the rows of each sequence's cache before the new tokens.
+    tree: bool ``[T, columns]``, rows contiguous: token t sees the i-th new token of its sequence where ``tree[t, i]``
+    (its ancestors and itself), and every row before them; without it the new tokens up to itself.  What it does not
+    see does not reach O, infinities and NaN included.
+    Q is rotated by table row ``lengths[b] + j - has_cls`` for the j-th token, or by positions[t] (int32
+    ``[T]``): a tree's tokens take the rows of their depths, so that accepted ones (``rope_cache_accept``)
+    are where a chain would have put them.
+
+    Returns O ``[T, H, D]``.  A token that sees no row has O = 0, and so have tokens behind the last
+    sequence and those of a sequence of negative length; rows past the page table or on a page number that is no page
+    of the cache are left out.  No gradients.
+    """
+    cosp, sinp = _tables(cos_sin)
+    return _tree_op(Q, k_cache, v_cache, cosp, sinp, page_table, lengths, cu_seqlens, tree, positions, has_cls, _scale(Q.shape[-1]))
