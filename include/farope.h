@@ -381,6 +381,16 @@ int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_st
                   const int32_t* page_table, const int32_t* lengths, void* o, float* ws, size_t ws_elems,
                   void* stream);
 
+/* The same with a window: the last `window` rows of each sequence count, the new token's own among
+ * them, and its first `sinks` rows.  window is at least 1, sinks 0 or more.  The rows between them are not
+ * read: their pages may be given back. */
+size_t farope_decode_window_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache, int32_t window,
+                                            int32_t sinks);
+int farope_decode_window(const farope_seq_desc* desc, int32_t window, int32_t sinks, const void* q,
+                         const int64_t q_stride[3], const float* cosp, const float* sinp, const int32_t* positions,
+                         const farope_cache_desc* cache, const int32_t* page_table, const int32_t* lengths, void* o,
+                         float* ws, size_t ws_elems, void* stream);
+
 /* O [T, heads, D] of several new tokens per sequence over its cache, whose rows they have been
  * appended to: token j of sequence b is row lengths[b] + j (lengths: the rows before the new tokens, as
  * in farope_cache_append), q is rotated by row lengths[b] + j - has_cls, or by positions [T].

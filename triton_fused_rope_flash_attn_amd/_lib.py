@@ -49,6 +49,8 @@ EXPORTS = (
     "farope_cache_append",
     "farope_decode_workspace_elems",
     "farope_decode",
+    "farope_decode_window_workspace_elems",
+    "farope_decode_window",
     "farope_tree_workspace_elems",
     "farope_tree",
     "farope_cache_accept",
@@ -135,6 +137,8 @@ _SIGNATURES = {
     "farope_cache_append": (ctypes.c_int, [_SD, _P, _S, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P]),
     "farope_decode_workspace_elems": (_Z, [_SD, _CD]),
     "farope_decode": (ctypes.c_int, [_SD, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P, _Z, _P]),
+    "farope_decode_window_workspace_elems": (_Z, [_SD, _CD, _I32, _I32]),
+    "farope_decode_window": (ctypes.c_int, [_SD, _I32, _I32, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P, _Z, _P]),
     "farope_tree_workspace_elems": (_Z, [_SD, _CD]),
     "farope_tree": (ctypes.c_int, [_SD, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P, _I64, _I32, _P, _P, _Z, _P]),
     "farope_cache_accept": (ctypes.c_int, [_SD, _CD, _P, _P, _P, _I64, _I32, _P, _P]),

@@ -10,6 +10,9 @@
 // that lies in one worker's share is finished there; of the others the workers leave
 // unnormalised sums, which decode_join_kernel joins.
 //
+// With a window (WIN) a sequence's blocks are those of its first rows that stay visible and of its last rows;
+// the blocks between them are not read.
+//
 // The products run on MFMA with the 16 query heads as columns.  Their rate is far
 // from binding, so 16-bit tensors keep fp32 accuracy where it costs no memory: q-hat
 // and P enter as a pair of 16-bit values (x = hi + lo), K and V are exact as cached.
@@ -65,9 +68,28 @@ __device__ __forceinline__ int cached_rows(const DecodeParams& p, int b) {
   const int len = p.c.lengths[b];
   return len < 0 ? 0 : len > room ? (int)room : len;
 }
-__device__ __forceinline__ int cached_blocks(const DecodeParams& p, int b) { return (int)(((int64_t)cached_rows(p, b) + 31) >> 5); }
+// With a window rows [0, sinks) and from `from` on count: blocks from `skip` on lie `gap` blocks further on.
+struct Cached {
+  int len, from, blocks, skip, gap;
+};
+template <bool WIN>
+__device__ __forceinline__ Cached cached(const DecodeParams& p, int b) {
+  Cached c;
+  c.len = cached_rows(p, b);
+  c.blocks = (int)(((int64_t)c.len + 31) >> 5);
+  c.from = c.skip = c.gap = 0;
+  if constexpr (WIN) {
+    c.from = c.len > p.window ? c.len - p.window : 0;
+    c.skip = (int)(((int64_t)(p.sinks < c.from ? p.sinks : c.from) + 31) >> 5);
+    c.gap = (c.from >> 5) > c.skip ? (c.from >> 5) - c.skip : 0;
+    c.blocks -= c.gap;
+  }
+  return c;
+}
+template <bool WIN>
+__device__ __forceinline__ int cached_blocks(const DecodeParams& p, int b) { return cached<WIN>(p, b).blocks; }
 
-template <typename S, int D>
+template <typename S, int D, bool WIN>
 __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D * sizeof(S) <= 256 ? 2 : 1) decode_kernel(const DecodeParams p) {
   using T = Tile<S, D>;
   using Frag = typename SeqComp<S>::C::Frag;
@@ -94,7 +116,7 @@ __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D *
     int64_t all = 0;
     unsigned n = 0, sum = 0;
     for (int i = 0; i < p.B; i += 64) {   // (blocks of 64 sequences: less than 2^32)
-      n = i + lane < p.B ? (unsigned)cached_blocks(p, i + lane) : 0u;
+      n = i + lane < p.B ? (unsigned)cached_blocks<WIN>(p, i + lane) : 0u;
       sum = wave_scan(n);
       all += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
     }
@@ -106,7 +128,7 @@ __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D *
     b = -1;
     for (int i = 0; i < p.B; i += 64) {   // (some sequence holds block `at`)
       if (p.B > 64) {
-        n = i + lane < p.B ? (unsigned)cached_blocks(p, i + lane) : 0u;
+        n = i + lane < p.B ? (unsigned)cached_blocks<WIN>(p, i + lane) : 0u;
         sum = wave_scan(n);
       }
       const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > at);
@@ -130,7 +152,8 @@ __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D *
   const int vrow = lane >> 2, vch = lane & 3;    // V chunks of a lane: rows vrow + 16 h, 16-byte chunks vch + 4 j
 
   for (;;) {
-    const int len = cached_rows(p, b), blocks = (int)(((int64_t)len + 31) >> 5);
+    const Cached cr = cached<WIN>(p, b);
+    const int len = cr.len, blocks = cr.blocks;
     const int end = p.direct || stop - at > blocks - first ? blocks : first + (int)(stop - at);
 
     // lane l (and l + 32): row 32 blk + l of the sequence: element offsets in the caches, whether it exists
@@ -139,8 +162,9 @@ __global__ void __launch_bounds__(64 * kDecodeNW, D * sizeof(S) <= 128 ? 3 : D *
     auto fetch = [&](int blk) __attribute__((always_inline)) {
       Ids id{-1, 0};
       if (blk < end) {
-        const unsigned r = 32u * (unsigned)blk + (unsigned)(lane & 31);
-        if (r < (unsigned)len) {
+        unsigned r = 32u * (unsigned)blk + (unsigned)(lane & 31);
+        if (WIN && blk >= cr.skip) r += 32u * (unsigned)cr.gap;
+        if (r < (unsigned)len && (!WIN || r >= (unsigned)cr.from || r < (unsigned)p.sinks)) {
           const unsigned place = r / (unsigned)p.c.page;
           id.page = pages[place];
           id.row = (int)(r - place * (unsigned)p.c.page);
@@ -340,7 +364,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeParams p) 
   __shared__ float sl[GR];
   const int tid = thread_id(), lane = tid & 63;
   const int b = block_id() / p.H, h = block_id() % p.H;
-  const int blocks = cached_blocks(p, b);
+  const int blocks = cached_blocks<false>(p, b);   // (only whether there are any)
   S* const o = static_cast<S*>(p.o) + ((int64_t)b * p.H + h) * D;
   if (blocks == 0) {
     if (tid < D / 8) {
@@ -379,13 +403,17 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeParams p) 
   store4<S>(o + c, 1, true, y);
 }
 
-template <typename S, int D>
-static hipError_t decode(const DecodeParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((decode_kernel<S, D>), dim3((unsigned)(p.Hkv * p.g_tiles) * (unsigned)p.workers), dim3(64 * kDecodeNW), 0, st, p);
+template <typename S, int D, bool WIN>
+static hipError_t decode_rows(const DecodeParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((decode_kernel<S, D, WIN>), dim3((unsigned)(p.Hkv * p.g_tiles) * (unsigned)p.workers), dim3(64 * kDecodeNW), 0, st, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.direct) return e;
   hipLaunchKernelGGL((decode_join_kernel<S, D>), dim3((unsigned)p.B * p.H), dim3(256), 0, st, p);
   return hipGetLastError();
+}
+template <typename S, int D>
+static hipError_t decode(const DecodeParams& p, hipStream_t st) {
+  return p.window ? decode_rows<S, D, true>(p, st) : decode_rows<S, D, false>(p, st);
 }
 template <typename S>
 static hipError_t decode_d(const DecodeParams& p, int D, hipStream_t st) {

@@ -204,15 +204,21 @@ int decode_tiles(const farope_seq_desc* d) { return (d->heads / d->kv_heads + 15
 // heads, D 128 104 / 89; 64 x 1024, 16 heads, D 64 66 / 59; 5 up to 1025, 8 heads, fp32 14.4 / 19.3.
 // (So a short sequence in a wide table pays for the join: 197 rows, 12 heads, D 64 7 us with room for 197, 9 for
 // 512, 13 for 1024 to 131072.)
-bool decode_direct(const farope_seq_desc* d, const farope_cache_desc* c) {
-  const int64_t room = (int64_t)c->max_pages * c->page_rows, wgs = (int64_t)d->seqs * d->kv_heads * decode_tiles(d);
+// (With a window the rules go by the rows that it leaves.)
+int64_t decode_room(const farope_cache_desc* c, int32_t window, int32_t sinks) {
+  const int64_t room = (int64_t)c->max_pages * c->page_rows;
+  const int64_t rows = window ? ((int64_t)window + 31) / 32 * 32 + 32 + ((int64_t)sinks + 31) / 32 * 32 : room;
+  return rows < room ? rows : room;
+}
+bool decode_direct(const farope_seq_desc* d, const farope_cache_desc* c, int32_t window, int32_t sinks) {
+  const int64_t room = decode_room(c, window, sinks), wgs = (int64_t)d->seqs * d->kv_heads * decode_tiles(d);
   return room <= 512 || (room <= 1024 && wgs >= decode_wgs(d)) || (room <= 2048 && wgs >= 2 * decode_wgs(d));
 }
-int decode_workers(const farope_seq_desc* d, const farope_cache_desc* c) {
-  if (decode_direct(d, c)) return d->seqs;
+int decode_workers(const farope_seq_desc* d, const farope_cache_desc* c, int32_t window, int32_t sinks) {
+  if (decode_direct(d, c, window, sinks)) return d->seqs;
   const int64_t heads = (int64_t)d->kv_heads * decode_tiles(d);
   // (a worker has 128 rows at least)
-  const int64_t most = d->seqs * (((int64_t)c->max_pages * c->page_rows + 127) / 128);
+  const int64_t most = d->seqs * ((decode_room(c, window, sinks) + 127) / 128);
   int64_t n = decode_wgs(d) / heads;
   if (n < 1) n = 1;
   return (int)(n < most ? n : most);
@@ -221,14 +227,58 @@ int decode_workers(const farope_seq_desc* d, const farope_cache_desc* c) {
 struct DecodeWs {
   int64_t stats, owners, total;
 };
-DecodeWs decode_ws(const farope_seq_desc* d, const farope_cache_desc* c) {
-  if (decode_direct(d, c)) return DecodeWs{};
-  const int64_t rows = ((int64_t)decode_workers(d, c) + d->seqs) * d->heads;
+DecodeWs decode_ws(const farope_seq_desc* d, const farope_cache_desc* c, int32_t window, int32_t sinks) {
+  if (decode_direct(d, c, window, sinks)) return DecodeWs{};
+  const int64_t rows = ((int64_t)decode_workers(d, c, window, sinks) + d->seqs) * d->heads;
   DecodeWs w{};
   w.stats = rows * d->head_dim;
   w.owners = (w.stats + 2 * rows + 3) & ~int64_t(3);
   w.total = w.owners + 2 * (int64_t)d->seqs;
   return w;
+}
+
+// A window that holds every row that a sequence can have is none.
+int32_t decode_window(const farope_cache_desc* c, int32_t window) {
+  return window >= (int64_t)c->max_pages * c->page_rows ? 0 : window;
+}
+int decode_call(const farope_seq_desc* desc, int32_t window, int32_t sinks, const void* q, const int64_t q_stride[3],
+                const float* cosp, const float* sinp, const int32_t* positions, const farope_cache_desc* cache,
+                const int32_t* page_table, const int32_t* lengths, void* o, float* ws, size_t ws_elems, void* stream) {
+  FAROPE_TRY(check_desc(desc, true));
+  if (desc->tokens != desc->seqs) return FAROPE_ERR_SHAPE;
+  if (!q_stride) return FAROPE_ERR_NULL;
+  const int es = elem_size(desc->dtype);
+  FAROPE_TRY(check_ptr(q, es));
+  FAROPE_TRY(check_ptr(cosp, 16));
+  FAROPE_TRY(check_ptr(sinp, 16));
+  if (positions) FAROPE_TRY(check_ptr(positions, 4));
+  FAROPE_TRY(check_cache(desc, cache, page_table, lengths));
+  FAROPE_TRY(check_ptr(o, 16));
+  const DecodeWs w = decode_ws(desc, cache, window, sinks);
+  if (w.total) {
+    FAROPE_TRY(check_ptr(ws, 16));
+    if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
+  }
+  const int workers = decode_workers(desc, cache, window, sinks);
+  if ((int64_t)desc->kv_heads * decode_tiles(desc) * workers > kMaxWorkgroups || (int64_t)desc->seqs * desc->heads > kMaxWorkgroups)
+    return FAROPE_ERR_SHAPE;
+  DecodeParams p{};
+  p.q = q;
+  for (int i = 0; i < 3; ++i) p.sq[i] = q_stride[i];
+  p.vec_q = vec_rows(q, q_stride, es);
+  p.cosp = cosp; p.sinp = sinp; p.positions = positions;
+  p.c = cache_params(cache, page_table, lengths);
+  p.o = o;
+  p.sums = ws;
+  p.stats = ws + w.stats;
+  p.owners = reinterpret_cast<int*>(ws + w.owners);
+  p.B = desc->seqs; p.H = desc->heads; p.Hkv = desc->kv_heads; p.n_pos = desc->n_pos; p.has_cls = desc->has_cls;
+  p.workers = workers;
+  p.direct = w.total == 0;
+  p.window = window; p.sinks = sinks;
+  p.g_tiles = decode_tiles(desc);
+  p.c2 = desc->softmax_scale * 1.4426950408889634f;
+  return launch_rc(launch_decode(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
 }
 
 // Several new tokens per sequence over a cache (tree.hip).  The host knows the sequences' number, their
@@ -389,48 +439,30 @@ int farope_cache_append(const farope_seq_desc* desc, const void* k, const int64_
 
 size_t farope_decode_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache) {
   if (check_desc(desc, true) != FAROPE_OK || !cache || cache->max_pages < 1 || cache->page_rows < 1) return 0;
-  return (size_t)decode_ws(desc, cache).total;
+  return (size_t)decode_ws(desc, cache, 0, 0).total;
+}
+
+size_t farope_decode_window_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache, int32_t window,
+                                            int32_t sinks) {
+  if (check_desc(desc, true) != FAROPE_OK || !cache || cache->max_pages < 1 || cache->page_rows < 1 || window < 1 || sinks < 0)
+    return 0;
+  return (size_t)decode_ws(desc, cache, decode_window(cache, window), sinks).total;
 }
 
 int farope_decode(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3], const float* cosp, const float* sinp,
                   const int32_t* positions, const farope_cache_desc* cache, const int32_t* page_table, const int32_t* lengths,
                   void* o, float* ws, size_t ws_elems, void* stream) {
-  FAROPE_TRY(check_desc(desc, true));
-  if (desc->tokens != desc->seqs) return FAROPE_ERR_SHAPE;
-  if (!q_stride) return FAROPE_ERR_NULL;
-  const int es = elem_size(desc->dtype);
-  FAROPE_TRY(check_ptr(q, es));
-  FAROPE_TRY(check_ptr(cosp, 16));
-  FAROPE_TRY(check_ptr(sinp, 16));
-  if (positions) FAROPE_TRY(check_ptr(positions, 4));
-  FAROPE_TRY(check_cache(desc, cache, page_table, lengths));
-  FAROPE_TRY(check_ptr(o, 16));
-  const DecodeWs w = decode_ws(desc, cache);
-  if (w.total) {
-    FAROPE_TRY(check_ptr(ws, 16));
-    if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
-  }
-  const int workers = decode_workers(desc, cache);
-  if ((int64_t)desc->kv_heads * decode_tiles(desc) * workers > kMaxWorkgroups || (int64_t)desc->seqs * desc->heads > kMaxWorkgroups)
-    return FAROPE_ERR_SHAPE;
-  DecodeParams p{};
-  p.q = q;
-  for (int i = 0; i < 3; ++i) p.sq[i] = q_stride[i];
-  p.vec_q = vec_rows(q, q_stride, es);
-  p.cosp = cosp; p.sinp = sinp; p.positions = positions;
-  p.c = cache_params(cache, page_table, lengths);
-  p.o = o;
-  p.sums = ws;
-  p.stats = ws + w.stats;
-  p.owners = reinterpret_cast<int*>(ws + w.owners);
-  p.B = desc->seqs; p.H = desc->heads; p.Hkv = desc->kv_heads; p.n_pos = desc->n_pos; p.has_cls = desc->has_cls;
-  p.workers = workers;
-  p.direct = w.total == 0;
-  p.g_tiles = decode_tiles(desc);
-  p.c2 = desc->softmax_scale * 1.4426950408889634f;
-  return launch_rc(launch_decode(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
+  return decode_call(desc, 0, 0, q, q_stride, cosp, sinp, positions, cache, page_table, lengths, o, ws, ws_elems, stream);
 }
 
+int farope_decode_window(const farope_seq_desc* desc, int32_t window, int32_t sinks, const void* q, const int64_t q_stride[3],
+                         const float* cosp, const float* sinp, const int32_t* positions, const farope_cache_desc* cache,
+                         const int32_t* page_table, const int32_t* lengths, void* o, float* ws, size_t ws_elems, void* stream) {
+  if (window < 1 || sinks < 0) return FAROPE_ERR_SHAPE;
+  if (!cache) return FAROPE_ERR_NULL;
+  return decode_call(desc, decode_window(cache, window), sinks, q, q_stride, cosp, sinp, positions, cache, page_table, lengths, o, ws,
+                     ws_elems, stream);
+}
 size_t farope_tree_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache) {
   if (check_desc(desc, true) != FAROPE_OK || !cache || cache->max_pages < 1 || cache->page_rows < 1) return 0;
   return (size_t)tree_ws(desc, cache).total;

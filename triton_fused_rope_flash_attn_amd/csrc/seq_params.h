@@ -123,6 +123,7 @@ struct DecodeParams {
   int B, H, Hkv, n_pos, has_cls;
   int workers;           // workgroups of a key head and query tile
   int direct;            // worker i has sequence i: nothing is joined
+  int window, sinks;     // rows that count: the last `window` and the first `sinks`; window 0: all
   int g_tiles;           // tiles of 16 query heads in a group
   float c2;
 };

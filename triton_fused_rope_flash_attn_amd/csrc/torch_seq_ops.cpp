@@ -53,6 +53,11 @@ int32_t to32(int64_t x) {
   return (int32_t)x;
 }
 
+void check_window(int64_t window, int64_t sinks) {
+  TORCH_CHECK_VALUE(window >= 1 && window <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX,
+                    "farope: window must be at least 1 and sinks at least 0, both in 32 bits; got ", window, " and ", sinks);
+}
+
 farope_seq_desc make_desc(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, const Tensor& x, const Tensor& cosp,
                           bool causal, bool has_cls, double scale) {
   farope_seq_desc d;
@@ -191,8 +196,10 @@ void cache_append(const Tensor& k, const Tensor& v, const Tensor& cosp, const Te
            "farope_cache_append");
 }
 
-Tensor cache_attn(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
-                  const Tensor& pages, const Tensor& lengths, const Opt& positions, bool has_cls, double scale) {
+// (window 0: none)
+Tensor cache_attn_rows(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
+                       const Tensor& pages, const Tensor& lengths, const Opt& positions, bool has_cls, double scale, int64_t window,
+                       int64_t sinks) {
   check_heads(q, "Q", "[B, H, D]");
   check_head_dim(q.size(2));
   check_first(q);
@@ -207,12 +214,29 @@ Tensor cache_attn(const Tensor& q, const Tensor& kc, const Tensor& vc, const Ten
   const Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   if (q.size(0) == 0) return o;
   const farope_seq_desc d = make_desc(q.size(0), q.size(0), q.size(1), kc.size(2), q, cosp, true, has_cls, scale);
-  const Tensor ws = workspace(q, farope_decode_workspace_elems(&d, &c));
-  check_rc(farope_decode(&d, q.data_ptr(), strides(q), floats(cosp), floats(sinp), ints(positions), &c,
-                         pages.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), o.data_ptr(), floats(ws),
-                         ws.defined() ? ws.numel() : 0, stream_of(q)),
-           "farope_decode");
+  const int32_t win = to32(window), first = to32(sinks);
+  const Tensor ws = workspace(q, win ? farope_decode_window_workspace_elems(&d, &c, win, first) : farope_decode_workspace_elems(&d, &c));
+  const size_t n = ws.defined() ? ws.numel() : 0;
+  if (win)
+    check_rc(farope_decode_window(&d, win, first, q.data_ptr(), strides(q), floats(cosp), floats(sinp), ints(positions), &c,
+                                  pages.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), o.data_ptr(), floats(ws), n, stream_of(q)),
+             "farope_decode_window");
+  else
+    check_rc(farope_decode(&d, q.data_ptr(), strides(q), floats(cosp), floats(sinp), ints(positions), &c, pages.data_ptr<int32_t>(),
+                           lengths.data_ptr<int32_t>(), o.data_ptr(), floats(ws), n, stream_of(q)),
+             "farope_decode");
   return o;
+}
+
+Tensor cache_attn(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
+                  const Tensor& pages, const Tensor& lengths, const Opt& positions, bool has_cls, double scale) {
+  return cache_attn_rows(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale, 0, 0);
+}
+Tensor cache_attn_window(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
+                         const Tensor& pages, const Tensor& lengths, const Opt& positions, bool has_cls, double scale,
+                         int64_t window, int64_t sinks) {
+  check_window(window, sinks);
+  return cache_attn_rows(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale, window, sinks);
 }
 
 Tensor cache_tree(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
@@ -311,6 +335,8 @@ using AppendSig = void(const Tensor&, const Tensor&, const Tensor&, const Tensor
                        const Opt&, const Opt&, bool);
 using AttnSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                        const Opt&, bool, double);
+using AttnWindowSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                             const Opt&, bool, double, int64_t, int64_t);
 template <typename Sig> c10::TypedOperatorHandle<Sig> find(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
 }
@@ -328,6 +354,10 @@ const c10::TypedOperatorHandle<AppendSig>& append_op() {
 }
 const c10::TypedOperatorHandle<AttnSig>& attn_op() {
   static const auto op = find<AttnSig>("farope::cache_attn");
+  return op;
+}
+const c10::TypedOperatorHandle<AttnWindowSig>& attn_window_op() {
+  static const auto op = find<AttnWindowSig>("farope::cache_attn_window");
   return op;
 }
 
@@ -441,12 +471,14 @@ Tensor cache_fork_autograd(Tensor kc, Tensor vc, Tensor pages, Tensor lengths, T
   return out;
 }
 
+// A pass over a cache that has no gradients.
 struct CacheAttnNode : torch::autograd::Function<CacheAttnNode> {
   static Tensor forward(torch::autograd::AutogradContext*, const Tensor& q, const Tensor& kc, const Tensor& vc,
                         const Tensor& cosp, const Tensor& sinp, const Tensor& pages, const Tensor& lengths, const Opt& positions,
-                        bool has_cls, double scale) {
+                        bool has_cls, double scale, std::optional<int64_t> window, int64_t sinks) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return attn_op().call(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale);
+    return window ? attn_window_op().call(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale, *window, sinks)
+                  : attn_op().call(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale);
   }
   static variable_list backward(torch::autograd::AutogradContext*, variable_list) {
     TORCH_CHECK(false, "Trying to backward through farope.cache_attn.default but no autograd formula was registered "
@@ -457,9 +489,18 @@ Tensor cache_attn_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, 
                            const Tensor& pages, const Tensor& lengths, const Opt& positions, bool has_cls, double scale) {
   refuse_tangents("cache_attn", {&q, &kc, &vc, &cosp, &sinp});
   if (at::GradMode::is_enabled() && any_requires_grad({&q, &kc, &vc}))
-    return CacheAttnNode::apply(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale);
+    return CacheAttnNode::apply(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale, std::optional<int64_t>(), (int64_t)0);
   at::AutoDispatchBelowADInplaceOrView below;
   return attn_op().call(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale);
+}
+Tensor cache_attn_window_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cosp, const Tensor& sinp,
+                                  const Tensor& pages, const Tensor& lengths, const Opt& positions, bool has_cls, double scale,
+                                  int64_t window, int64_t sinks) {
+  refuse_tangents("cache_attn_window", {&q, &kc, &vc, &cosp, &sinp});
+  if (at::GradMode::is_enabled() && any_requires_grad({&q, &kc, &vc}))
+    return CacheAttnNode::apply(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale, std::optional<int64_t>(window), sinks);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return attn_window_op().call(q, kc, vc, cosp, sinp, pages, lengths, positions, has_cls, scale, window, sinks);
 }
 
 using TreeSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
@@ -497,6 +538,7 @@ TORCH_LIBRARY_IMPL(farope, CUDA, m) {
   m.impl("seq_bwd", seq_bwd);
   m.impl("cache_append", cache_append);
   m.impl("cache_attn", cache_attn);
+  m.impl("cache_attn_window", cache_attn_window);
   m.impl("cache_tree", cache_tree);
   m.impl("cache_accept", cache_accept);
   m.impl("cache_fork", cache_fork);
@@ -507,6 +549,7 @@ TORCH_LIBRARY_IMPL(farope, AutogradCUDA, m) {
   m.impl("seq_bwd", seq_bwd_autograd);
   m.impl("cache_append", cache_append_autograd);
   m.impl("cache_attn", cache_attn_autograd);
+  m.impl("cache_attn_window", cache_attn_window_autograd);
   m.impl("cache_tree", cache_tree_autograd);
   m.impl("cache_accept", cache_accept_autograd);
   m.impl("cache_fork", cache_fork_autograd);

@@ -113,6 +113,11 @@ def _check_cache(k_cache, v_cache, page_table, lengths, kv_heads, x):
     _check_ints(lengths, "lengths", page_table.shape[0], x)
 
 
+def _check_window(window, sinks):
+    if not (1 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31):
+        raise ValueError(f"farope: window must be at least 1 and sinks at least 0, both in 32 bits; got {window} and {sinks}")
+
+
 def _check_seq(q, k, v, cosp, sinp, cu, positions):
     if q.dim() != 3:
         raise ValueError(f"Q must be [T, H, D]; got shape {tuple(q.shape)}")
@@ -246,6 +251,24 @@ def _cache_attn_fake(q, k_cache, v_cache, cosp, sinp, page_table, lengths, posit
     return q.new_empty(tuple(q.shape))
 
 
+@torch.library.custom_op("farope::cache_attn_window", mutates_args=())
+def _cache_attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cosp: torch.Tensor, sinp: torch.Tensor,
+                       page_table: torch.Tensor, lengths: torch.Tensor, positions: Optional[torch.Tensor], has_cls: bool,
+                       softmax_scale: float, window: int, sinks: int) -> torch.Tensor:
+    """-> O [B, H, D]."""
+    _check_window(window, sinks)
+    _check_attn(q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions)
+    _check_device(q)
+    _lib.require_torch_ops()
+
+
+@_cache_attn_window.register_fake
+def _cache_attn_window_fake(q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions, has_cls, softmax_scale, window, sinks):
+    _check_window(window, sinks)
+    _check_attn(q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions)
+    return q.new_empty(tuple(q.shape))
+
+
 @torch.library.custom_op("farope::cache_tree", mutates_args=())
 def _cache_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cosp: torch.Tensor, sinp: torch.Tensor,
                 page_table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor, tree: Optional[torch.Tensor],
@@ -287,6 +310,7 @@ _lib.load_torch_ops()   # (their kernels for GPU tensors, as in attention.py)
 _seq_fwd_op = torch.ops.farope.seq_fwd.default
 _append_op = torch.ops.farope.cache_append.default
 _attn_op = torch.ops.farope.cache_attn.default
+_attn_window_op = torch.ops.farope.cache_attn_window.default
 _tree_op = torch.ops.farope.cache_tree.default
 
 
@@ -384,6 +408,8 @@ def sdpa_rope_decode(
     *,
     has_cls: bool = True,
     positions: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> torch.Tensor:
     """Attention of one new token per sequence over its paged cache.
 
@@ -392,6 +418,10 @@ def sdpa_rope_decode(
     new token's own among them.  Q is rotated by table row ``lengths[b] - 1 - has_cls``, or by
     positions[b] (int32 ``[B]``).
 
+    window, sinks: the token sees the last ``window`` rows (at least 1: its own) and the first ``sinks`` ones alone,
+    as in ``sdpa_rope_varlen``; the rows between them are not read, and their pages may be
+    given back.
+
     How the rows are divided goes by the page table's width (lengths stay on the GPU): for short
     sequences a view of its first columns, as many as they need, is faster.
 
@@ -399,7 +429,8 @@ def sdpa_rope_decode(
     or on a page number that is no page of the cache are left out.  No gradients.
     """
     cosp, sinp = _tables(cos_sin)
-    return _attn_op(Q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions, has_cls, _scale(Q.shape[-1]))
+    args = (Q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions, has_cls, _scale(Q.shape[-1]))
+    return _attn_op(*args) if window is None else _attn_window_op(*args, window, sinks)
 
 
 def sdpa_rope_tree(
