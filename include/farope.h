@@ -340,6 +340,20 @@ int farope_seq_bwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
                    const float* cosp, const float* sinp, const int32_t* positions, const int32_t* cu,
                    void* dq, void* dk, void* dv, float* ws, size_t ws_elems, void* stream);
 
+/* The same with a window: token i of a sequence sees tokens j <= i with i - j < window, and those with
+ * j < sinks.  window is at least 1, sinks 0 or more; desc: causal is not read. */
+size_t farope_seq_window_workspace_elems(const farope_seq_desc* desc, int32_t window, int32_t sinks, int32_t backward,
+                                         int32_t v_streams, int32_t dout_streams);
+int farope_seq_window_fwd(const farope_seq_desc* desc, int32_t window, int32_t sinks, const void* q,
+                          const int64_t q_stride[3], const void* k, const int64_t k_stride[3], const void* v,
+                          const int64_t v_stride[3], const float* cosp, const float* sinp, const int32_t* positions,
+                          const int32_t* cu, void* o, float* lse, float* ws, size_t ws_elems, void* stream);
+int farope_seq_window_bwd(const farope_seq_desc* desc, int32_t window, int32_t sinks, const void* q,
+                          const int64_t q_stride[3], const void* k, const int64_t k_stride[3], const void* v,
+                          const int64_t v_stride[3], const void* o, const void* dout, const int64_t dout_stride[3],
+                          const float* lse, const float* cosp, const float* sinp, const int32_t* positions,
+                          const int32_t* cu, void* dq, void* dk, void* dv, float* ws, size_t ws_elems, void* stream);
+
 /*
  * Paged cache of keys (rotated) and values: row r of page g, key head h, channel d at
  * g*stride[0] + r*stride[1] + h*stride[2] + d elements (channels contiguous; base and

@@ -46,6 +46,9 @@ EXPORTS = (
     "farope_seq_workspace_elems",
     "farope_seq_fwd",
     "farope_seq_bwd",
+    "farope_seq_window_workspace_elems",
+    "farope_seq_window_fwd",
+    "farope_seq_window_bwd",
     "farope_cache_append",
     "farope_decode_workspace_elems",
     "farope_decode",
@@ -133,6 +136,12 @@ _SIGNATURES = {
     "farope_seq_bwd": (
         ctypes.c_int,
         [_SD, _P, _S, _P, _S, _P, _S, _P, _P, _S, _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P],
+    ),
+    "farope_seq_window_workspace_elems": (_Z, [_SD, _I32, _I32, _I32, _I32, _I32]),
+    "farope_seq_window_fwd": (ctypes.c_int, [_SD, _I32, _I32, _P, _S, _P, _S, _P, _S, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "farope_seq_window_bwd": (
+        ctypes.c_int,
+        [_SD, _I32, _I32, _P, _S, _P, _S, _P, _S, _P, _P, _S, _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P],
     ),
     "farope_cache_append": (ctypes.c_int, [_SD, _P, _S, _P, _S, _P, _P, _P, _CD, _P, _P, _P, _P]),
     "farope_decode_workspace_elems": (_Z, [_SD, _CD]),

@@ -275,6 +275,27 @@ __device__ __forceinline__ SeqTile ordered_tile(const int* __restrict__ cu, int 
   t.tile = keys ? t.tiles - 1 - l : l;
   return t;
 }
+// Stages of SR keys that a tile of queries [q0, end) reads: with a window (WIN) the ones that hold sinks,
+// then, `gap` further on, those of its rows' windows.
+template <bool WIN, int SR> struct KeyStages {
+  int n, sink, gap;
+  __device__ __forceinline__ KeyStages(const SeqParams& p, int q0, int end, int len) {
+    const int last = p.causal && end < len ? end : len;
+    n = (last + SR - 1) / SR;
+    sink = gap = 0;
+    if constexpr (WIN) {
+      const int low = q0 + 1 > p.window ? q0 + 1 - p.window : 0;   // the first key of the first row's window
+      sink = ((p.sinks < low ? p.sinks : low) + SR - 1) / SR;
+      gap = low / SR > sink ? low / SR - sink : 0;
+      n -= gap;
+    }
+  }
+  // stage st of the tile: which of the sequence's
+  __device__ __forceinline__ int at(int st) const { return WIN && st >= sink ? st + gap : st; }
+};
+// Whether some key of [k0, k0 + n) is none that a row with the window [from, ..] sees
+__device__ __forceinline__ bool past_window(const SeqParams& p, int k0, int n, int from) { return k0 < from && k0 + n > p.sinks; }
+
 // A workgroup's tile of queries (keys: of keys), the later ones first (the earlier), which
 // have more to do in a causal call: from the map that seq_prep_kernel has made, where
 // there is such a pass, so that the heads' workgroups of a slot read 16 bytes instead of

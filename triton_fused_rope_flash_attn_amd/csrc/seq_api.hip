@@ -72,10 +72,25 @@ int64_t decode_wgs(const farope_seq_desc* d) {
   return (int64_t)kCus * (row <= 64 ? 4 : row == 128 ? 3 : row == 256 ? 2 : 1);
 }
 
+// Token i sees j <= i with i - j < window or j < sinks; window 0: as the descriptor says.
+struct Window {
+  int32_t window, sinks;
+};
+// A window that holds every row that a sequence can have is none.
+Window window_of(const farope_seq_desc* d, int32_t window, int32_t sinks) {
+  if (window >= d->tokens) return Window{0, 0};
+  return Window{window, sinks < d->tokens ? sinks : d->tokens};
+}
+farope_seq_desc causal_desc(const farope_seq_desc* d) {
+  farope_seq_desc c = *d;
+  c.causal = 1;
+  return c;
+}
+
 // Workspace, in fp32 elements, each part from a 256-byte boundary.
 constexpr int kMaxParts = 8;
 struct SeqWs {
-  int64_t khat, vcopy, map_q, map_k, qhat, gcopy, nl, nd, ng, pk, pv, total;
+  int64_t khat, vcopy, map_q, map_k, qhat, gcopy, nl, nd, ng, pk, pv, spk, spv, total;
 };
 // Parts that the queries of a key tile (64 rows) are divided into, joined by a launch of its
 // own: so many that about four workgroups per CU share the work, but none below a stage of
@@ -84,9 +99,11 @@ struct SeqWs {
 // [264] 713 / 523 / 432, 1024, 4 [72] 181 / 129 / 105, 8 x 1024, 8 [1096] 208 / 239 / 311; D 64:
 // 2048, 2 [68] 204 / 138 / 105, 4 x 2048, 8 [1064] 180 / 179 / 196; D 256: 2 x 4096, 8 [1048] 1251 /
 // 1347 / 1525; fp32, D 64: 3 up to 257, 4 [44] 100 / 79 / 72.
-int dkdv_parts(const farope_seq_desc* d) {
+int dkdv_parts(const farope_seq_desc* d, Window win) {
   const int64_t wgs = seq_slots(d->tokens, d->seqs, 6) * d->kv_heads;
-  const int64_t stages = (int64_t)(d->heads / d->kv_heads) * (d->tokens / d->seqs / 64 + 1);
+  int64_t rows = d->tokens / d->seqs;   // queries that see a key
+  if (win.window && rows > win.window) rows = win.window;
+  const int64_t stages = (int64_t)(d->heads / d->kv_heads) * (rows / 64 + 1);
   int64_t parts = (4 * kCus + wgs / 2) / wgs;
   if (parts > kMaxParts) parts = kMaxParts;
   if (parts > stages) parts = stages;
@@ -106,7 +123,19 @@ bool rotates_itself(const farope_seq_desc* d, bool v_streams) {
   if (d->head_dim == 128) return d->tokens <= 128;
   return mean <= 128 || (mean <= 256 && d->tokens <= 1024);
 }
-SeqWs seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_streams) {
+// Key tiles with sinks, which every later query sees: parts of their queries, so that one has about the
+// work of another tile, whose queries are those of a window (0: they are not divided).
+constexpr int kMaxSinkParts = 64;
+int sink_tiles(Window win) { return win.window ? (int)(((int64_t)win.sinks + 63) / 64) : 0; }
+int sink_parts(const farope_seq_desc* d, Window win) {
+  if (!sink_tiles(win)) return 0;
+  const int64_t n = d->tokens / d->seqs / ((int64_t)win.window + 128);
+  return n < 2 ? 0 : n < kMaxSinkParts ? (int)n : kMaxSinkParts;
+}
+int64_t sink_workgroups(const farope_seq_desc* d, Window win) {
+  return (int64_t)d->seqs * sink_tiles(win) * sink_parts(d, win) * d->kv_heads;
+}
+SeqWs seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_streams, Window win) {
   const int64_t es = elem_size(d->dtype), kv = (int64_t)d->tokens * d->kv_heads * d->head_dim * es / 4;
   const int64_t q = (int64_t)d->tokens * d->heads * d->head_dim * es / 4, rows = (int64_t)d->tokens * d->heads;
   auto al = [](int64_t x) { return (x + 63) & ~int64_t(63); };
@@ -120,16 +149,22 @@ SeqWs seq_ws(const farope_seq_desc* d, bool backward, bool v_streams, bool g_str
   w.gcopy = w.qhat + (backward ? al(q) : 0);
   w.nl = w.gcopy + (backward && !g_streams ? al(q) : 0);
   w.nd = w.nl + (backward ? al(rows) : 0);
-  const int parts = backward ? dkdv_parts(d) : 1;
+  const int parts = backward ? dkdv_parts(d, win) : 1;
   const int64_t sums = parts > 1 ? al((int64_t)parts * d->tokens * d->kv_heads * d->head_dim) : 0;
   w.ng = w.nd + (backward ? al(rows) : 0);
   w.pk = w.ng + (backward && d->dtype == FAROPE_F16 && d->head_dim == 128 ? al(rows) : 0);
   w.pv = w.pk + sums;
-  w.total = w.pv + sums;
+  w.spk = w.pv + sums;
+  const int64_t sink_sums = backward ? al(sink_workgroups(d, win) * 64 * d->head_dim) : 0;
+  w.spv = w.spk + sink_sums;
+  w.total = w.spv + sink_sums;
   return w;
 }
 
-void place(SeqParams& p, const farope_seq_desc* d, const SeqWs& w, float* ws, bool backward, bool v_streams, bool g_streams) {
+void place(SeqParams& p, const farope_seq_desc* d, const SeqWs& w, float* ws, bool backward, bool v_streams, bool g_streams,
+           Window win) {
+  p.window = win.window;
+  p.sinks = win.sinks;
   if (!rotates_itself(d, v_streams)) {
     p.khat = ws;
     p.map_q = reinterpret_cast<int*>(ws + w.map_q);
@@ -144,7 +179,11 @@ void place(SeqParams& p, const farope_seq_desc* d, const SeqWs& w, float* ws, bo
   p.ng = ws + w.ng;
   p.pk = ws + w.pk;
   p.pv = ws + w.pv;
-  p.parts = dkdv_parts(d);
+  p.parts = dkdv_parts(d, win);
+  p.spk = ws + w.spk;
+  p.spv = ws + w.spv;
+  p.sink_tiles = sink_tiles(win);
+  p.sink_parts = sink_parts(d, win);
 }
 
 void fill(SeqParams& p, const farope_seq_desc* d, const void* q, const int64_t sq[3], const void* k, const int64_t sk[3],
@@ -174,6 +213,60 @@ int check_inputs(const farope_seq_desc* d, const void* q, const int64_t* sq, con
   FAROPE_TRY(check_ptr(sinp, 16));
   if (positions) FAROPE_TRY(check_ptr(positions, 4));
   return check_ptr(cu, 4);
+}
+
+int seq_fwd_call(const farope_seq_desc* desc, Window win, const void* q, const int64_t q_stride[3], const void* k,
+                   const int64_t k_stride[3], const void* v, const int64_t v_stride[3], const float* cosp, const float* sinp,
+                   const int32_t* positions, const int32_t* cu, void* o, float* lse, float* ws, size_t ws_elems, void* stream) {
+  FAROPE_TRY(check_desc(desc, true));
+  if (desc->tokens == 0) return FAROPE_OK;
+  FAROPE_TRY(check_inputs(desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu));
+  FAROPE_TRY(check_ptr(o, 16));
+  FAROPE_TRY(check_ptr(lse, 4));
+  const bool vs = streams(desc, v, v_stride);
+  const SeqWs w = seq_ws(desc, false, vs, true, win);
+  if (w.total) FAROPE_TRY(check_ptr(ws, 16));
+  if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
+  SeqParams p{};
+  fill(p, desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu);
+  p.o = o; p.lse = lse;
+  place(p, desc, w, ws, false, vs, true, win);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p.khat) FAROPE_TRY(launch_rc(launch_seq_prep(p, desc->dtype, desc->head_dim, false, st)));
+  return launch_rc(launch_seq_fwd(p, desc->dtype, desc->head_dim, st));
+}
+
+int seq_bwd_call(const farope_seq_desc* desc, Window win, const void* q, const int64_t q_stride[3], const void* k,
+                   const int64_t k_stride[3], const void* v, const int64_t v_stride[3], const void* o, const void* dout,
+                   const int64_t dout_stride[3], const float* lse, const float* cosp, const float* sinp,
+                   const int32_t* positions, const int32_t* cu, void* dq, void* dk, void* dv, float* ws, size_t ws_elems,
+                   void* stream) {
+  FAROPE_TRY(check_desc(desc, true));
+  if (desc->tokens == 0) return FAROPE_OK;
+  FAROPE_TRY(check_inputs(desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu));
+  if (!dout_stride) return FAROPE_ERR_NULL;
+  const int es = elem_size(desc->dtype);
+  FAROPE_TRY(check_ptr(dout, es));
+  FAROPE_TRY(check_ptr(o, 16));
+  FAROPE_TRY(check_ptr(lse, 4));
+  FAROPE_TRY(check_ptr(dq, 16));
+  FAROPE_TRY(check_ptr(dk, 16));
+  FAROPE_TRY(check_ptr(dv, 16));
+  FAROPE_TRY(check_ptr(ws, 16));
+  const bool vs = streams(desc, v, v_stride), gs = streams(desc, dout, dout_stride);
+  if (seq_slots(desc->tokens, desc->seqs, 6) * desc->kv_heads * kMaxParts + sink_workgroups(desc, win) > INT32_MAX) return FAROPE_ERR_SHAPE;
+  const SeqWs w = seq_ws(desc, true, vs, gs, win);
+  if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
+  SeqParams p{};
+  fill(p, desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu);
+  p.dout = dout;
+  for (int i = 0; i < 3; ++i) p.sdo[i] = dout_stride[i];
+  p.vec_do = vec_rows(dout, dout_stride, es);
+  p.o = const_cast<void*>(o);
+  p.lse = const_cast<float*>(lse);
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  place(p, desc, w, ws, true, vs, gs, win);
+  return launch_rc(launch_seq_bwd(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
 }
 
 int check_cache(const farope_seq_desc* d, const farope_cache_desc* c, const int32_t* table, const int32_t* lengths) {
@@ -354,28 +447,19 @@ int farope_seq_streams(const farope_seq_desc* desc, const void* x, const int64_t
 
 size_t farope_seq_workspace_elems(const farope_seq_desc* desc, int32_t backward, int32_t v_streams, int32_t dout_streams) {
   if (check_desc(desc, true) != FAROPE_OK) return 0;
-  return (size_t)seq_ws(desc, backward != 0, v_streams != 0, dout_streams != 0).total;
+  return (size_t)seq_ws(desc, backward != 0, v_streams != 0, dout_streams != 0, Window{0, 0}).total;
+}
+
+size_t farope_seq_window_workspace_elems(const farope_seq_desc* desc, int32_t window, int32_t sinks, int32_t backward,
+                                         int32_t v_streams, int32_t dout_streams) {
+  if (check_desc(desc, true) != FAROPE_OK || window < 1 || sinks < 0) return 0;
+  return (size_t)seq_ws(desc, backward != 0, v_streams != 0, dout_streams != 0, window_of(desc, window, sinks)).total;
 }
 
 int farope_seq_fwd(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3], const void* k,
                    const int64_t k_stride[3], const void* v, const int64_t v_stride[3], const float* cosp, const float* sinp,
                    const int32_t* positions, const int32_t* cu, void* o, float* lse, float* ws, size_t ws_elems, void* stream) {
-  FAROPE_TRY(check_desc(desc, true));
-  if (desc->tokens == 0) return FAROPE_OK;
-  FAROPE_TRY(check_inputs(desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu));
-  FAROPE_TRY(check_ptr(o, 16));
-  FAROPE_TRY(check_ptr(lse, 4));
-  const bool vs = streams(desc, v, v_stride);
-  const SeqWs w = seq_ws(desc, false, vs, true);
-  if (w.total) FAROPE_TRY(check_ptr(ws, 16));
-  if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
-  SeqParams p{};
-  fill(p, desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu);
-  p.o = o; p.lse = lse;
-  place(p, desc, w, ws, false, vs, true);
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p.khat) FAROPE_TRY(launch_rc(launch_seq_prep(p, desc->dtype, desc->head_dim, false, st)));
-  return launch_rc(launch_seq_fwd(p, desc->dtype, desc->head_dim, st));
+  return seq_fwd_call(desc, Window{0, 0}, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu, o, lse, ws, ws_elems, stream);
 }
 
 int farope_seq_bwd(const farope_seq_desc* desc, const void* q, const int64_t q_stride[3], const void* k,
@@ -383,31 +467,27 @@ int farope_seq_bwd(const farope_seq_desc* desc, const void* q, const int64_t q_s
                    const int64_t dout_stride[3], const float* lse, const float* cosp, const float* sinp,
                    const int32_t* positions, const int32_t* cu, void* dq, void* dk, void* dv, float* ws, size_t ws_elems,
                    void* stream) {
+  return seq_bwd_call(desc, Window{0, 0}, q, q_stride, k, k_stride, v, v_stride, o, dout, dout_stride, lse, cosp, sinp, positions, cu, dq, dk, dv, ws, ws_elems, stream);
+}
+
+int farope_seq_window_fwd(const farope_seq_desc* desc, int32_t window, int32_t sinks, const void* q, const int64_t q_stride[3], const void* k,
+                          const int64_t k_stride[3], const void* v, const int64_t v_stride[3], const float* cosp, const float* sinp,
+                          const int32_t* positions, const int32_t* cu, void* o, float* lse, float* ws, size_t ws_elems, void* stream) {
   FAROPE_TRY(check_desc(desc, true));
-  if (desc->tokens == 0) return FAROPE_OK;
-  FAROPE_TRY(check_inputs(desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu));
-  if (!dout_stride) return FAROPE_ERR_NULL;
-  const int es = elem_size(desc->dtype);
-  FAROPE_TRY(check_ptr(dout, es));
-  FAROPE_TRY(check_ptr(o, 16));
-  FAROPE_TRY(check_ptr(lse, 4));
-  FAROPE_TRY(check_ptr(dq, 16));
-  FAROPE_TRY(check_ptr(dk, 16));
-  FAROPE_TRY(check_ptr(dv, 16));
-  FAROPE_TRY(check_ptr(ws, 16));
-  const bool vs = streams(desc, v, v_stride), gs = streams(desc, dout, dout_stride);
-  const SeqWs w = seq_ws(desc, true, vs, gs);
-  if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
-  SeqParams p{};
-  fill(p, desc, q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu);
-  p.dout = dout;
-  for (int i = 0; i < 3; ++i) p.sdo[i] = dout_stride[i];
-  p.vec_do = vec_rows(dout, dout_stride, es);
-  p.o = const_cast<void*>(o);
-  p.lse = const_cast<float*>(lse);
-  p.dq = dq; p.dk = dk; p.dv = dv;
-  place(p, desc, w, ws, true, vs, gs);
-  return launch_rc(launch_seq_bwd(p, desc->dtype, desc->head_dim, static_cast<hipStream_t>(stream)));
+  if (window < 1 || sinks < 0) return FAROPE_ERR_SHAPE;
+  const farope_seq_desc causal = causal_desc(desc);
+  return seq_fwd_call(&causal, window_of(desc, window, sinks), q, q_stride, k, k_stride, v, v_stride, cosp, sinp, positions, cu, o, lse, ws, ws_elems, stream);
+}
+
+int farope_seq_window_bwd(const farope_seq_desc* desc, int32_t window, int32_t sinks, const void* q, const int64_t q_stride[3], const void* k,
+                          const int64_t k_stride[3], const void* v, const int64_t v_stride[3], const void* o, const void* dout,
+                          const int64_t dout_stride[3], const float* lse, const float* cosp, const float* sinp,
+                          const int32_t* positions, const int32_t* cu, void* dq, void* dk, void* dv, float* ws, size_t ws_elems,
+                          void* stream) {
+  FAROPE_TRY(check_desc(desc, true));
+  if (window < 1 || sinks < 0) return FAROPE_ERR_SHAPE;
+  const farope_seq_desc causal = causal_desc(desc);
+  return seq_bwd_call(&causal, window_of(desc, window, sinks), q, q_stride, k, k_stride, v, v_stride, o, dout, dout_stride, lse, cosp, sinp, positions, cu, dq, dk, dv, ws, ws_elems, stream);
 }
 
 int farope_cache_append(const farope_seq_desc* desc, const void* k, const int64_t k_stride[3], const void* v,

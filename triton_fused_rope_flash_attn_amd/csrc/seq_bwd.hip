@@ -123,9 +123,12 @@ __device__ __forceinline__ void zero_rows(S* base, int64_t stride, int rows, int
   }
 }
 
+// A window of one token and no sinks: every row sees itself alone.
+template <bool WIN> __device__ __forceinline__ bool sees_itself(const SeqParams& p) { return WIN && p.window == 1 && p.sinks == 0; }
 // What the sums dS^T Q-hat are multiplied by: a sequence of one token has dS = 0, which the sums,
 // with -delta as their start, hold but for rounding.
-__device__ __forceinline__ float dk_factor(const SeqParams& p, int len) { return len == 1 ? 0.f : p.scale; }
+template <bool WIN>
+__device__ __forceinline__ float dk_factor(const SeqParams& p, int len) { return len == 1 || sees_itself<WIN>(p) ? 0.f : p.scale; }
 
 // ---------------------------------------------------------------------------
 // dQ of 64 QT query rows of one head.  S^T = K-hat Q-hat^T and dP^T = V dO^T per
@@ -133,7 +136,7 @@ __device__ __forceinline__ float dk_factor(const SeqParams& p, int len) { return
 // ---------------------------------------------------------------------------
 // Keys of a stage: as in the forward (short sequences: 64, so that one stage holds them).  Two stages hold 64 at least.
 template <typename S, int D, bool ROT> constexpr int kDqRows = sizeof(S) == 2 && D == 128 && !ROT ? 32 : kStageRowsOf<S, D>;
-template <typename S, int D, int QT, bool ROT>
+template <typename S, int D, int QT, bool ROT, bool WIN>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : D == 128 && (QT == 2 || ROT) ? 2 : 3)
 seq_dq_kernel(const SeqParams p) {
   using C = typename SeqComp<S>::C;
@@ -157,14 +160,15 @@ seq_dq_kernel(const SeqParams p) {
     return;
   }
 
+  const KeyStages<WIN, SR> ks(p, q0, q0 + (1 << LB), tl.len);
   SeqStream<S, D, T::SR> srcK, srcV;
   RotStage<S, D, T::SR> rot;
   if constexpr (ROT) {
-    rot.load(p, tl, kvh, 0, tid);
+    rot.load(p, tl, kvh, ks.at(0), tid);
   } else {
     srcK.lanes(D, wave, lane);
     srcK.base(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
-    srcK.load(sK0, wave, 0);
+    srcK.load(sK0, wave, ks.at(0) * SR);
   }
   if (!ROT && p.vcopy) {
     srcV.lanes(D, wave, lane);
@@ -173,7 +177,7 @@ seq_dq_kernel(const SeqParams p) {
     srcV.lanes(p.sv[0], wave, lane);
     srcV.base(static_cast<const S*>(p.v) + tl.start * p.sv[0] + kvh * p.sv[1], tl.len);
   }
-  srcV.load(sV0, wave, 0);
+  srcV.load(sV0, wave, ks.at(0) * SR);
 
   const int row0 = wave * 16 * QT + lr;   // of the tile; subtile t: + 16 t
   const int64_t hrow = (int64_t)head * p.T + tok0;
@@ -181,9 +185,10 @@ seq_dq_kernel(const SeqParams p) {
   const bool active = w0 < tl.len;
   const int lo = p.causal ? w0 + 1 : tl.len;
   const int hi = p.causal && w0 + 16 * QT < tl.len ? w0 + 16 * QT : tl.len;
-  const int last = p.causal && q0 + (1 << LB) < tl.len ? q0 + (1 << LB) : tl.len;
-  const int ns = (last + SR - 1) / SR;
-  const bool few = q0 == 0 && (p.causal || tl.len <= 64);   // some rows of the tile see 64 keys at most
+  const int ns = ks.n;
+  const bool few = !WIN && q0 == 0 && (p.causal || tl.len <= 64);   // some rows of the tile see 64 keys at most
+  // (with a window: they may be anywhere, and have their delta from a pass of its own over the tile's keys)
+  const bool twice = WIN && (q0 == 0 || p.window <= 64 - p.sinks);
   const bool mine = few && hi <= 64;                        // (uniform) and so do all of the wave's
   Frag qf[QT][KS], gf[QT][KS];
   f32x4 nl4[QT], nd4[QT];
@@ -243,6 +248,10 @@ seq_dq_kernel(const SeqParams p) {
   FragAt<S, D> at;
   at.init(lr, lg);
 
+  // key 16 h + i of the lane's part of a block is one that its row of the subtile sees; lim: those behind its keys
+  auto sees = [&](int e, int lim, int k0) __attribute__((always_inline)) {
+    return e < lim && (!WIN || e >= lim - p.window || e < p.sinks - k0 - 4 * lg);
+  };
   auto block = [&](bool tail, int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
     f32x4 sacc[QT][2], pacc[QT][2];
 #pragma unroll
@@ -263,14 +272,15 @@ seq_dq_kernel(const SeqParams p) {
     Frag dsf[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      const int lim = (seen[t] > 1 ? seen[t] : 0) - k0 - 4 * lg;   // (a row that sees one key: P = 1, dS = 0)
+      // (a row that sees one key: P = 1, dS = 0)
+      const int lim = (seen[t] > 1 && !sees_itself<WIN>(p) ? seen[t] : 0) - k0 - 4 * lg;
       float ds[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float y = fast_exp2(sacc[t][h][i]) * pacc[t][h][i];
-          ds[4 * h + i] = !tail || 16 * h + i < lim ? y : 0.f;
+          ds[4 * h + i] = !tail || sees(16 * h + i, lim, k0) ? y : 0.f;
         }
       if constexpr (kFitDs<S>) {
         const float most = amax8(0.f, ds);
@@ -295,20 +305,44 @@ seq_dq_kernel(const SeqParams p) {
       for (int t = 0; t < QT; ++t) acc[t][d] = C::mma(a, dsf[t], acc[t][d]);
     }
   };
-  auto stage = [&](int st, const S* __restrict__ k, const S* __restrict__ v, S* __restrict__ kn, S* __restrict__ vn)
+  // sum_j P_ij dP_ij of a block's keys (delta, in fp32)
+  float sum[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) sum[t] = 0.f;
+  auto sum_block = [&](int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const int lim = seen[t] - k0 - 4 * lg;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x4 sacc, pacc;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          sacc = C::mma(at.row(k, s, h), qf[t][s], s == 0 ? first_sum<S>(nl4[t]) : sacc);
+          pacc = C::mma(at.row(v, s, h), gf[t][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : pacc);
+        }
+        last_sum<S>(sacc, nl4[t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[t] += sees(16 * h + i, lim, k0) ? fast_exp2(sacc[i]) * pacc[i] : 0.f;
+      }
+    }
+  };
+  auto stage = [&](int st, bool sums, const S* __restrict__ k, const S* __restrict__ v, S* __restrict__ kn, S* __restrict__ vn)
       __attribute__((always_inline)) {
     seq_stage_barrier();
     if (st + 1 < ns) {
-      if constexpr (ROT) rot.load(p, tl, kvh, st + 1, tid);
-      else srcK.load(kn, wave, (st + 1) * SR);
-      srcV.load(vn, wave, (st + 1) * SR);
+      if constexpr (ROT) rot.load(p, tl, kvh, ks.at(st + 1), tid);
+      else srcK.load(kn, wave, ks.at(st + 1) * SR);
+      srcV.load(vn, wave, ks.at(st + 1) * SR);
     }
-    const int k0 = st * SR;
-    if (active && k0 < hi) {
-      const bool tail = k0 + SR > lo;
+    const int k0 = ks.at(st) * SR;
+    if (active && k0 < hi && (!WIN || k0 + SR > w0 + 1 - p.window || k0 < p.sinks)) {
+      const bool tail = k0 + SR > lo || (WIN && past_window(p, k0, SR, hi - p.window));
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-        block(tail, k0 + 32 * j, k + 32 * j * D, v + 32 * j * D);
+      for (int j = 0; j < NB; ++j) {
+        if (WIN && sums) sum_block(k0 + 32 * j, k + 32 * j * D, v + 32 * j * D);
+        else block(tail, k0 + 32 * j, k + 32 * j * D, v + 32 * j * D);
+      }
     }
     if (ROT && st + 1 < ns) rot.store(p, kn, tid);   // (read in the stage before this one)
   };
@@ -410,9 +444,32 @@ seq_dq_kernel(const SeqParams p) {
       srcV.load(sV0, wave, 2 * SR);
     }
   }
+  if constexpr (WIN) {
+    if (twice) {   // (uniform)
+#pragma unroll 1
+      for (int st = 0; st < ns; st += 2) {
+        stage(st, true, sK0, sV0, sK1, sV1);
+        if (st + 1 < ns) stage(st + 1, true, sK1, sV1, sK0, sV0);
+      }
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {   // (P carries 2^ex)
+        const float nd = -group4_sum(sum[t]) * (kFitDs<S> ? pow2(-ex[t]) : 1.f);
+        if (row0 + 16 * t < rows && lg == 0) p.nd[hrow + row0 + 16 * t] = nd;
+        nd4[t] = f32x4{nd, nd, nd, nd};
+      }
+      lds_barrier();   // (all waves have read the last stages)
+      if constexpr (ROT) {
+        rot.load(p, tl, kvh, ks.at(0), tid);
+        rot.store(p, sK0, tid);
+      } else {
+        srcK.load(sK0, wave, ks.at(0) * SR);
+      }
+      srcV.load(sV0, wave, ks.at(0) * SR);
+    }
+  }
   for (int st = from; st < ns; st += 2) {
-    stage(st, sK0, sV0, sK1, sV1);
-    if (st + 1 < ns) stage(st + 1, sK1, sV1, sK0, sV0);
+    stage(st, false, sK0, sV0, sK1, sV1);
+    if (st + 1 < ns) stage(st + 1, false, sK1, sV1, sK0, sV0);
   }
 
   const unsigned row_b = (unsigned)(p.H * D * (int)sizeof(S));
@@ -422,6 +479,58 @@ seq_dq_kernel(const SeqParams p) {
     store_rows<S, D>(acc[t], kFitDs<S> ? __builtin_amdgcn_ldexpf(kLn2, -ex[t]) : kLn2, true, p, trow[t], rD, (unsigned)(row0 + 16 * t) * row_b, lg);
 }
 
+// Queries from the returned one on do not see keys [first, last] (a key: first = last).
+template <bool WIN>
+__device__ __forceinline__ int key_reach(const SeqParams& p, int len, int first, int last) {
+  return WIN && first >= p.sinks && len - last > p.window ? last + p.window : len;
+}
+
+// A workgroup's key tile, key head and part of the queries.  With a window all queries behind them see the sinks, so
+// their tiles have many times the others' work: the workgroups of the launch's front divide it into parts
+// of their own, and the others leave it to them.
+template <bool WIN> struct KeyTile {
+  SeqTile tl;
+  int part, parts, kvh;
+  bool sinks;   // the sums go to p.spk and p.spv
+  bool sums;
+  __device__ __forceinline__ KeyTile(const SeqParams& p, int lane) {
+    int id = block_id();
+    sinks = false;
+    if constexpr (WIN) {
+      const int front = p.B * p.sink_tiles * p.sink_parts * p.Hkv;
+      if (id < front) {
+        sinks = sums = true;
+        parts = p.sink_parts;
+        part = id % parts;
+        id /= parts;
+        kvh = id % p.Hkv;
+        id /= p.Hkv;
+        tl.tile = id % p.sink_tiles;
+        tl.seq = id / p.sink_tiles;
+        tl.start = cu_at(p.cu, tl.seq, p.T);
+        const int end = cu_at(p.cu, tl.seq + 1, p.T);
+        tl.len = end > tl.start ? end - tl.start : 0;
+        tl.tiles = (tl.len + 63) >> 6;
+        if (tl.tile >= tl.tiles) tl.tile = -1;
+        return;
+      }
+      id -= front;
+    }
+    parts = p.parts;
+    sums = parts > 1;
+    part = id % parts;
+    id /= parts;
+    kvh = id % p.Hkv;
+    tl = slot_tile(p, 6, id / p.Hkv, lane, true);
+    if (WIN && p.sink_parts && tl.seq < p.B && tl.tile < p.sink_tiles) tl.tile = -1;
+  }
+  // the first row of the sums (in rows of D)
+  __device__ __forceinline__ int64_t sums_at(const SeqParams& p, int64_t tok0) const {
+    if (sinks) return ((((int64_t)part * p.B + tl.seq) * p.sink_tiles + tl.tile) * 64) * p.Hkv + kvh;
+    return ((int64_t)part * p.T + tok0) * p.Hkv + kvh;
+  }
+};
+
 // ---------------------------------------------------------------------------
 // dK and dV of 64 key rows of one key head.  Wave w owns 16 of them: their K-hat and
 // V rows are operands in registers, dK-hat and dV accumulate in registers over the
@@ -429,7 +538,7 @@ seq_dq_kernel(const SeqParams p) {
 // them).  128 keys per workgroup (D 32 and 64) measured the same within 3% for long
 // sequences and slower for short ones (64 up to 577, D 64: 146 / 163 us).
 // ---------------------------------------------------------------------------
-template <typename S, int D>
+template <typename S, int D, bool WIN>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : 2) seq_dkdv_kernel(const SeqParams p) {
   using C = typename SeqComp<S>::C;
   using Frag = typename C::Frag;
@@ -442,16 +551,16 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lr = lane & 15, lg = lane >> 4;
   // earlier keys (seen by more queries) come first in each sequence
-  const int part = block_id() % p.parts, rest = block_id() / p.parts;
-  const int slot = rest / p.Hkv, kvh = rest % p.Hkv, group = p.H / p.Hkv;
-  const SeqTile tl = slot_tile(p, LB, slot, lane, true);
+  const KeyTile<WIN> kt(p, lane);
+  const int part = kt.part, parts = kt.parts, kvh = kt.kvh, group = p.H / p.Hkv;
+  const SeqTile tl = kt.tl;
   if (tl.tile < 0) return;
   const int k0 = tl.tile << LB, rows = tl.len - k0 < (1 << LB) ? tl.len - k0 : 1 << LB;
   const int64_t tok0 = tl.start + k0;
   S* const dkb = static_cast<S*>(p.dk) + (tok0 * p.Hkv + kvh) * D;
   S* const dvb = static_cast<S*>(p.dv) + (tok0 * p.Hkv + kvh) * D;
   if (tl.seq == p.B) {
-    if (p.parts > 1) return;   // (seq_join_kernel's)
+    if (parts > 1) return;   // (seq_join_kernel's)
     zero_rows<S, D>(dkb, (int64_t)p.Hkv * D, rows, tid);
     zero_rows<S, D>(dvb, (int64_t)p.Hkv * D, rows, tid);
     return;
@@ -463,9 +572,9 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   // tokens, 16 heads (4 of keys), D 64 406 / 390, 64 up to 577, 12 143 / 140, 8 x 1024, 8, D 128 159 / 156,
   // one sequence of 16384 2510 / 2494
   // (HBM reads of the kernel 1716 / 419 MB).
-  const int first = p.causal ? k0 / SR : 0, per = (tl.len + SR - 1) / SR - first;
+  const int first = p.causal ? k0 / SR : 0, per = (key_reach<WIN>(p, tl.len, k0, k0 + 63) + SR - 1) / SR - first;
   const int64_t all = (int64_t)per * group;
-  const int begin = (int)(all * part / p.parts), ns = (int)(all * (part + 1) / p.parts) - begin;
+  const int begin = (int)(all * part / parts), ns = (int)(all * (part + 1) / parts) - begin;
   SeqStream<S, D> srcQ, srcG;
   srcQ.lanes(D, wave, lane);
   srcG.lanes(p.gcopy ? D : p.sdo[0], wave, lane);
@@ -516,6 +625,10 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   }
   const int w0 = k0 + wave * 16;   // the wave's first key (uniform)
   const bool active = w0 < tl.len;
+  // queries from here on do not see the lane's key, some of the wave's keys, any of them
+  const int qend = key_reach<WIN>(p, tl.len, k0 + row0, k0 + row0);
+  const int qfull = WIN ? w0 + 16 <= p.sinks ? tl.len : key_reach<WIN>(p, tl.len, p.sinks > w0 ? p.sinks : w0, w0) : tl.len;
+  const int qlast = key_reach<WIN>(p, tl.len, w0, w0 + 15);
   f32x4 dv[DT], dk[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) dv[d] = dk[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -542,7 +655,7 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
       last_sum<S>(pacc[h], nd);
     }
     // query q0 + 16 h + 4 lg + i exists and sees this lane's key
-    const int from = p.causal ? k0 + row0 - q0 - 4 * lg : -4 * lg, to = tl.len - q0 - 4 * lg;
+    const int from = p.causal ? k0 + row0 - q0 - 4 * lg : -4 * lg, to = qend - q0 - 4 * lg;
     float pv[8], ds[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -585,8 +698,8 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
     if (st + 1 < ns) load(qn, gn, ln, dn);
     const int q0 = (first + per - 1 - cst) * SR;
     cst = cst + 1 == per ? 0 : cst + 1;
-    if (!active || (p.causal && q0 + SR <= w0)) return;
-    const bool tail = q0 + SR > tl.len || (p.causal && q0 < w0 + 16);
+    if (!active || (p.causal && q0 + SR <= w0) || (WIN && q0 >= qlast)) return;
+    const bool tail = q0 + SR > qfull || (p.causal && q0 < w0 + 16);
 #pragma unroll
     for (int j = 0; j < NB; ++j)
       block(tail, q0 + 32 * j, q + 32 * j * D, g + 32 * j * D, l + 32 * j, dl + 32 * j);
@@ -597,10 +710,10 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   }
 
   const float up = pow2(-(int)kWeightUp<S>);   // out of P
-  if (p.parts > 1) {   // sums as they are, for seq_join_kernel
-    const int64_t at = (((int64_t)part * p.T + tok0) * p.Hkv + kvh) * D;
+  if (kt.sums) {   // sums as they are, for seq_join_kernel
+    const int64_t at = kt.sums_at(p, tok0) * D;
     const unsigned row_b = (unsigned)(p.Hkv * D) * 4u, bytes = (unsigned)(rows - 1) * row_b + D * 4u;
-    const auto rpK = make_rsrc(p.pk + at, bytes), rpV = make_rsrc(p.pv + at, bytes);
+    const auto rpK = make_rsrc((kt.sinks ? p.spk : p.pk) + at, bytes), rpV = make_rsrc((kt.sinks ? p.spv : p.pv) + at, bytes);
     store_rows<float, D>(dk, pow2(-ex) * up, false, p, 0, rpK, (unsigned)row0 * row_b, lg);
     store_rows<float, D>(dv, up, false, p, 0, rpV, (unsigned)row0 * row_b, lg);
     return;
@@ -608,7 +721,7 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
   const unsigned row_b = (unsigned)(p.Hkv * D * (int)sizeof(S));
   const unsigned bytes = (unsigned)(rows - 1) * row_b + T::RB;
   const auto rdK = make_rsrc(dkb, bytes), rdV = make_rsrc(dvb, bytes);
-  store_rows<S, D>(dk, dk_factor(p, tl.len) * pow2(-ex) * up, true, p, trow, rdK, (unsigned)row0 * row_b, lg);
+  store_rows<S, D>(dk, dk_factor<WIN>(p, tl.len) * pow2(-ex) * up, true, p, trow, rdK, (unsigned)row0 * row_b, lg);
   store_rows<S, D>(dv, up, false, p, trow, rdV, (unsigned)row0 * row_b, lg);
 }
 
@@ -623,7 +736,7 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
 // 2696 / 2567, 24 up to 2048, 4 key heads 1094 / 1020, 8 x 4096, 8 1580 / 1501; at D 64 it is the
 // slower one (8192, 16 key heads 717 / 742).
 // ---------------------------------------------------------------------------
-template <typename S>
+template <typename S, bool WIN>
 __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const SeqParams p) {
   constexpr int D = 128;
   using C = typename SeqComp<S>::C;
@@ -637,24 +750,24 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   const int tid = thread_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lr = lane & 15, lg = lane >> 4;
-  const int part = block_id() % p.parts, rest = block_id() / p.parts;
-  const int slot = rest / p.Hkv, kvh = rest % p.Hkv, group = p.H / p.Hkv;
-  const SeqTile tl = slot_tile(p, LB, slot, lane, true);
+  const KeyTile<WIN> kt(p, lane);
+  const int part = kt.part, parts = kt.parts, kvh = kt.kvh, group = p.H / p.Hkv;
+  const SeqTile tl = kt.tl;
   if (tl.tile < 0) return;
   const int k0 = tl.tile << LB, rows = tl.len - k0 < (1 << LB) ? tl.len - k0 : 1 << LB;
   const int64_t tok0 = tl.start + k0;
   S* const dkb = static_cast<S*>(p.dk) + (tok0 * p.Hkv + kvh) * D;
   S* const dvb = static_cast<S*>(p.dv) + (tok0 * p.Hkv + kvh) * D;
   if (tl.seq == p.B) {
-    if (p.parts > 1) return;   // (seq_join_kernel's)
+    if (parts > 1) return;   // (seq_join_kernel's)
     zero_rows<S, D>(dkb, (int64_t)p.Hkv * D, rows, tid);
     zero_rows<S, D>(dvb, (int64_t)p.Hkv * D, rows, tid);
     return;
   }
 
-  const int first = p.causal ? k0 / SR : 0, per = (tl.len + SR - 1) / SR - first;
+  const int first = p.causal ? k0 / SR : 0, per = (key_reach<WIN>(p, tl.len, k0, k0 + 63) + SR - 1) / SR - first;
   const int64_t all = (int64_t)per * group;
-  const int begin = (int)(all * part / p.parts), ns = (int)(all * (part + 1) / p.parts) - begin;
+  const int begin = (int)(all * part / parts), ns = (int)(all * (part + 1) / parts) - begin;
   SeqStream<S, D> srcQ, srcG;
   srcQ.lanes(D, wave, lane);
   srcG.lanes(p.gcopy ? D : p.sdo[0], wave, lane);
@@ -754,6 +867,11 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   const int qrow = 32 * qh * D;
   const int pw = ((4 * qh + 2 * kh) * 64 + lane) * 8;   // where the lane leaves its P and dS (subtile u, half h: + 512 u + 4 h)
 
+  int qend[2];   // queries from here on do not see the lane's key
+#pragma unroll
+  for (int u = 0; u < 2; ++u) qend[u] = key_reach<WIN>(p, tl.len, k0 + 32 * kh + 16 * u + lr, k0 + 32 * kh + 16 * u + lr);
+  // ... some of the tile's keys
+  const int qfull = WIN ? k0 + 64 <= p.sinks ? tl.len : key_reach<WIN>(p, tl.len, p.sinks > k0 ? p.sinks : k0, k0) : tl.len;
   int cst = start;   // this stage within its head
   auto stage = [&](int st, const S* __restrict__ q, const S* __restrict__ g, S* __restrict__ qn, S* __restrict__ gn)
       __attribute__((always_inline)) {
@@ -780,7 +898,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
     if (st + 1 < ns) load(qn, gn);
     const int q0 = (first + per - 1 - cst) * SR;
     cst = cst + 1 == per ? 0 : cst + 1;
-    const bool tail = q0 + SR > tl.len || (p.causal && q0 < k0 + 64);   // uniform
+    const bool tail = q0 + SR > qfull || (p.causal && q0 < k0 + 64);   // uniform
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       f32x4 sacc[2], pacc[2];
@@ -794,14 +912,14 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
         }
       }
       // query qi + i (of the sequence) exists and sees key k0 + 32 kh + 16 u + lr
-      const int qi = q0 + 32 * qh + 16 * h + 4 * lg, from = p.causal ? k0 + 32 * kh + lr - qi : -64, until = tl.len - qi;
+      const int qi = q0 + 32 * qh + 16 * h + 4 * lg, from = p.causal ? k0 + 32 * kh + lr - qi : -64;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         typedef S s4 __attribute__((ext_vector_type(4)));
         s4 pv, ds;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool in = !tail || (i >= from + 16 * u && i < until);
+          const bool in = !tail || (i >= from + 16 * u && i < qend[u] - qi);
           const float e = fast_exp2(sacc[u][i]);
           pv[i] = (S)(in ? e : 0.f);    // (P and dS rounded to the tensors' type for the products)
           ds[i] = (S)(in ? kFitDs<S> ? e * pacc[u][i] * fit : e * pacc[u][i] : 0.f);
@@ -838,11 +956,11 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
 
   // lane holds key 16 u + lr, channels 16 (d0 + d) + 4lg + (0..3)
   const float up = pow2(-(int)kWeightUp<S>);   // out of P
-  const unsigned es = p.parts > 1 ? 4u : 2u, row_b = (unsigned)(p.Hkv * D) * es;
+  const unsigned es = kt.sums ? 4u : 2u, row_b = (unsigned)(p.Hkv * D) * es;
   const unsigned bytes = (unsigned)(rows - 1) * row_b + D * es;
-  if (p.parts > 1) {   // sums as they are, for seq_join_kernel
-    const int64_t w = (((int64_t)part * p.T + tok0) * p.Hkv + kvh) * D;
-    const auto rK = make_rsrc(p.pk + w, bytes), rV = make_rsrc(p.pv + w, bytes);
+  if (kt.sums) {   // sums as they are, for seq_join_kernel
+    const int64_t w = kt.sums_at(p, tok0) * D;
+    const auto rK = make_rsrc((kt.sinks ? p.spk : p.pk) + w, bytes), rV = make_rsrc((kt.sinks ? p.spv : p.pv) + w, bytes);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const unsigned off = (unsigned)(16 * u + lr) * row_b;
@@ -856,14 +974,14 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   for (int u = 0; u < 4; ++u) {
     const int r = 16 * u + lr, rc = r < rows ? r : rows - 1;
     const int trow = table_row(p.positions ? p.positions[tok0 + rc] : k0 + rc - p.has_cls, p.n_pos);
-    store_tiles<S, D, ND>(dk[u], 16 * d0, dk_factor(p, tl.len) * pow2(-ex) * up, true, p, trow, rK, (unsigned)r * row_b, lg);
+    store_tiles<S, D, ND>(dk[u], 16 * d0, dk_factor<WIN>(p, tl.len) * pow2(-ex) * up, true, p, trow, rK, (unsigned)r * row_b, lg);
     store_tiles<S, D, ND>(dv[u], 16 * d0, up, false, p, trow, rV, (unsigned)r * row_b, lg);
   }
 }
 
 // dK and dV of the parts' sums, added in order; a thread takes 8 channels of one token
 // and key head.
-template <typename S, int D>
+template <typename S, int D, bool WIN>
 __global__ void __launch_bounds__(256) seq_join_kernel(const SeqParams p) {
   constexpr int CPR = D / 8, ROWS = 256 / CPR;
   const int blk = block_id() / p.Hkv, kvh = block_id() % p.Hkv;
@@ -872,18 +990,30 @@ __global__ void __launch_bounds__(256) seq_join_kernel(const SeqParams p) {
   const int b = find_seq(p.cu, p.B, p.T, t0, tc, tid & 63);
   if (t >= p.T) return;
   float k[8] = {}, v[8] = {};
-  const int64_t at = ((int64_t)t * p.Hkv + kvh) * D + c, step = (int64_t)p.T * p.Hkv * D;
+  const int64_t at = ((int64_t)t * p.Hkv + kvh) * D + c;
+  const int start = cu_at(p.cu, b, p.T);
+  const bool sinks = WIN && p.sink_parts && b < p.B && t - start < 64 * p.sink_tiles;
+  if (WIN && !sinks && p.parts == 1) return;   // (complete)
   if (b < p.B) {
-    for (int i = 0; i < p.parts; ++i) {
+    const float* pk = p.pk + at;
+    const float* pv = p.pv + at;
+    int64_t step = (int64_t)p.T * p.Hkv * D;
+    if (sinks) {
+      const int64_t from = (((int64_t)b * p.sink_tiles * 64 + t - start) * p.Hkv + kvh) * D + c;
+      pk = p.spk + from;
+      pv = p.spv + from;
+      step = (int64_t)p.B * p.sink_tiles * 64 * p.Hkv * D;
+    }
+    const int parts = sinks ? p.sink_parts : p.parts;
+    for (int i = 0; i < parts; ++i) {
       float x[8], y[8];
-      load8<float>(p.pk + i * step + at, 1, true, x);
-      load8<float>(p.pv + i * step + at, 1, true, y);
+      load8<float>(pk + i * step, 1, true, x);
+      load8<float>(pv + i * step, 1, true, y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) { k[e] += x[e]; v[e] += y[e]; }
     }
-    const int start = cu_at(p.cu, b, p.T);
     const int row = table_row(p.positions ? p.positions[t] : t - start - p.has_cls, p.n_pos);
-    const float factor = dk_factor(p, cu_at(p.cu, b + 1, p.T) - start);
+    const float factor = dk_factor<WIN>(p, cu_at(p.cu, b + 1, p.T) - start);
     float cs[8];
     table_load4(p.cosp, p.sinp, row, D / 2, c / 2, cs);
 #pragma unroll
@@ -901,7 +1031,22 @@ template <typename S, int D, int QT, bool ROT>
 static hipError_t dq(const SeqParams& p0, hipStream_t st) {
   SeqParams p = p0;
   p.slots = (int)seq_slots(p.T, p.B, QT == 2 ? 7 : 6);
-  hipLaunchKernelGGL((seq_dq_kernel<S, D, QT, ROT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
+  const dim3 grid((unsigned)p.slots * p.H);
+  if (p.window) hipLaunchKernelGGL((seq_dq_kernel<S, D, QT, ROT, true>), grid, dim3(kSeqThreads), 0, st, p);
+  else hipLaunchKernelGGL((seq_dq_kernel<S, D, QT, ROT, false>), grid, dim3(kSeqThreads), 0, st, p);
+  return hipGetLastError();
+}
+template <typename S, int D, bool WIN>
+static hipError_t dkdv(const SeqParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)p.slots * p.Hkv * p.parts + (WIN ? (unsigned)p.B * p.sink_tiles * p.sink_parts * p.Hkv : 0u));
+  if constexpr (sizeof(S) == 2 && D == 128)
+    hipLaunchKernelGGL((seq_dkdv_shared_kernel<S, WIN>), grid, dim3(kSeqThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL((seq_dkdv_kernel<S, D, WIN>), grid, dim3(kSeqThreads), 0, st, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || (p.parts == 1 && !(WIN && p.sink_parts))) return e;
+  constexpr int rows = 256 / (D / 8);
+  hipLaunchKernelGGL((seq_join_kernel<S, D, WIN>), dim3((unsigned)((p.T + rows - 1) / rows) * p.Hkv), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 template <typename S, int D>
@@ -912,7 +1057,7 @@ static hipError_t bwd(const SeqParams& p0, hipStream_t st) {
     e = launch_seq_prep(p, std::is_same<S, bf16>::value ? DT_BF16 : std::is_same<S, f16>::value ? DT_F16 : DT_F32, D, true, st);
     if (e != hipSuccess) return e;
     if constexpr (sizeof(S) == 2)
-      e = seq_tile_rows(p.T, p.B, p.H, D, false) == 128 ? dq<S, D, 2, false>(p, st) : dq<S, D, 1, false>(p, st);
+      e = seq_tile_rows(p.T, p.B, p.H, D, false, p.window) == 128 ? dq<S, D, 2, false>(p, st) : dq<S, D, 1, false>(p, st);
     else
       e = dq<S, D, 1, false>(p, st);
   } else if constexpr (D <= 128) {
@@ -920,16 +1065,7 @@ static hipError_t bwd(const SeqParams& p0, hipStream_t st) {
   }
   if (e != hipSuccess) return e;
   p.slots = (int)seq_slots(p.T, p.B, 6);
-  const dim3 grid((unsigned)p.slots * p.Hkv * p.parts);
-  if constexpr (sizeof(S) == 2 && D == 128)
-    hipLaunchKernelGGL((seq_dkdv_shared_kernel<S>), grid, dim3(kSeqThreads), 0, st, p);
-  else
-    hipLaunchKernelGGL((seq_dkdv_kernel<S, D>), grid, dim3(kSeqThreads), 0, st, p);
-  e = hipGetLastError();
-  if (e != hipSuccess || p.parts == 1) return e;
-  constexpr int rows = 256 / (D / 8);
-  hipLaunchKernelGGL((seq_join_kernel<S, D>), dim3((unsigned)((p.T + rows - 1) / rows) * p.Hkv), dim3(256), 0, st, p);
-  return hipGetLastError();
+  return p.window ? dkdv<S, D, true>(p, st) : dkdv<S, D, false>(p, st);
 }
 template <typename S>
 static hipError_t bwd_d(const SeqParams& p, int D, hipStream_t st) {

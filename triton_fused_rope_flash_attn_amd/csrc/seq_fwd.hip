@@ -31,7 +31,7 @@ template <typename S, int D> constexpr int kFwdRows = sizeof(S) == 2 && D == 128
 // a quarter of a microsecond a key), a channel of NaN throughout to 156.  What
 // finds such rows costs (us, without / with) 24 up to 2048 (mean 943), 16 heads, D 128 173 / 175, 64 up to 577, 12
 // heads, D 64 40.3 / 40.6, one of 16384, D 128 553 / 549.
-template <typename S, int D, bool ROT>
+template <typename S, int D, bool ROT, bool WIN>
 __device__ __forceinline__ void row_again(const SeqParams& p, const SeqTile& tl, int head, int kvh, int i, float m, float l, int lane) {
   constexpr int NP = D > 128 ? D / 128 : 1, AHEAD = 4;
   typedef float f2 __attribute__((ext_vector_type(2)));
@@ -51,40 +51,45 @@ __device__ __forceinline__ void row_again(const SeqParams& p, const SeqTile& tl,
     q[n] = f2{(float)(S)x[0], (float)(S)x[1]};
     acc[n] = f2{0.f, 0.f};
   }
-  for (int j0 = 0; j0 <= i; j0 += AHEAD) {
-    float s[AHEAD];
-    f2 v[AHEAD][NP];
+  auto keys = [&](int first, int end) __attribute__((always_inline)) {
+    for (int j0 = first; j0 < end; j0 += AHEAD) {
+      float s[AHEAD];
+      f2 v[AHEAD][NP];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int j = j0 + u <= i ? j0 + u : i;
-      const int64_t tok = tl.start + j;
-      s[u] = 0.f;
+      for (int u = 0; u < AHEAD; ++u) {
+        const int j = j0 + u < end ? j0 + u : end - 1;
+        const int64_t tok = tl.start + j;
+        s[u] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NP; ++n) {
-        const int c = on ? 2 * (lane + 64 * n) : 0;
-        f2 k;
-        if constexpr (ROT) {
-          k = turned(p.k, p.sk, tok, kvh, j, c) * p.c2;
-          k = f2{(float)(S)k[0], (float)(S)k[1]};
-        } else {
-          const S* const x = static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c;
-          k = f2{(float)x[0], (float)x[1]};
+        for (int n = 0; n < NP; ++n) {
+          const int c = on ? 2 * (lane + 64 * n) : 0;
+          f2 k;
+          if constexpr (ROT) {
+            k = turned(p.k, p.sk, tok, kvh, j, c) * p.c2;
+            k = f2{(float)(S)k[0], (float)(S)k[1]};
+          } else {
+            const S* const x = static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tok) * D + c;
+            k = f2{(float)x[0], (float)x[1]};
+          }
+          s[u] += on ? q[n][0] * k[0] + q[n][1] * k[1] : 0.f;
+          const S* const y = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1] + c * p.sv[2];
+          v[u][n] = f2{(float)y[0], (float)y[p.sv[2]]};
         }
-        s[u] += on ? q[n][0] * k[0] + q[n][1] * k[1] : 0.f;
-        const S* const y = static_cast<const S*>(p.v) + tok * p.sv[0] + kvh * p.sv[1] + c * p.sv[2];
-        v[u][n] = f2{(float)y[0], (float)y[p.sv[2]]};
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) s[u] += __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (lane ^ d), __float_as_int(s[u])));
+        const float w = (float)(S)fast_exp2(s[u] - m);
+        if (j0 + u < end)
+#pragma unroll
+          for (int n = 0; n < NP; ++n) acc[n] = f2{acc[n][0] + w * v[u][n][0], acc[n][1] + w * v[u][n][1]};
       }
     }
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) s[u] += __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (lane ^ d), __float_as_int(s[u])));
-      const float w = (float)(S)fast_exp2(s[u] - m);
-      if (j0 + u <= i)
-#pragma unroll
-        for (int n = 0; n < NP; ++n) acc[n] = f2{acc[n][0] + w * v[u][n][0], acc[n][1] + w * v[u][n][1]};
-    }
-  }
+  };
+  const int low = WIN && i + 1 > p.window ? i + 1 - p.window : 0;
+  if (WIN) keys(0, p.sinks < low ? p.sinks : low);
+  keys(low, i + 1);
   S* const o = static_cast<S*>(p.o) + ((int64_t)(tl.start + i) * p.H + head) * D;
   if (on)
 #pragma unroll
@@ -104,7 +109,7 @@ __device__ __forceinline__ void row_again(const SeqParams& p, const SeqTile& tl,
 // Together with O's own rounding (1.6e-3 of its norm in bf16) that leaves 2.8e-3.  P as a pair of
 // values (hi + lo) measured 2.5e-3, Q-hat too 2.1e-3, at (us, one / P / both) 8 x 1024, 16 heads, D 64
 // 40 / 46 / 51, 64 up to 577, 12 heads, D 64 38 / 43 / 46, 16384 tokens, 8 heads, D 128 538 / 700 / 1573.
-template <typename S, int D, int QT, bool ROT>
+template <typename S, int D, int QT, bool ROT, bool WIN>
 __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 : 3)
 seq_fwd_kernel(const SeqParams p) {
   using C = typename SeqComp<S>::C;
@@ -138,14 +143,15 @@ seq_fwd_kernel(const SeqParams p) {
     return;
   }
 
+  const KeyStages<WIN, SR> ks(p, q0, q0 + (1 << LB), tl.len);
   SeqStream<S, D, T::SR> srcK, srcV;
   RotStage<S, D, T::SR> rot;
   if constexpr (ROT) {
-    rot.load(p, tl, kvh, 0, tid);
+    rot.load(p, tl, kvh, ks.at(0), tid);
   } else {
     srcK.lanes(D, wave, lane);
     srcK.base(static_cast<const S*>(p.khat) + ((int64_t)kvh * p.T + tl.start) * D, tl.len);
-    srcK.load(sK0, wave, 0);
+    srcK.load(sK0, wave, ks.at(0) * SR);
   }
   if (!ROT && p.vcopy) {
     srcV.lanes(D, wave, lane);
@@ -154,7 +160,7 @@ seq_fwd_kernel(const SeqParams p) {
     srcV.lanes(p.sv[0], wave, lane);
     srcV.base(static_cast<const S*>(p.v) + tl.start * p.sv[0] + kvh * p.sv[1], tl.len);
   }
-  srcV.load(sV0, wave, 0);
+  srcV.load(sV0, wave, ks.at(0) * SR);
 
   Frag qf[QT][KS];
   int seen[QT];   // keys that the subtile's row of this lane sees
@@ -178,8 +184,7 @@ seq_fwd_kernel(const SeqParams p) {
   // every row of the wave sees keys below lo, none sees keys from hi on
   const int lo = p.causal ? w0 + 1 : tl.len;
   const int hi = p.causal && w0 + 16 * QT < tl.len ? w0 + 16 * QT : tl.len;
-  const int last = p.causal && q0 + (1 << LB) < tl.len ? q0 + (1 << LB) : tl.len;
-  const int ns = (last + SR - 1) / SR;
+  const int ns = ks.n;
 
   f32x4 acc[QT][DT];
   float m_run[QT], l_run[QT];   // the running max (less kWeightUp) and sum
@@ -219,7 +224,11 @@ seq_fwd_kernel(const SeqParams p) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sacc[j][t][h][i] = 32 * j + 16 * h + i < lim ? sacc[j][t][h][i] : -INFINITY;
+            for (int i = 0; i < 4; ++i) {
+              const int e = 32 * j + 16 * h + i;
+              const bool in = e < lim && (!WIN || e >= lim - p.window || e < p.sinks - k0 - 4 * lg);
+              sacc[j][t][h][i] = in ? sacc[j][t][h][i] : -INFINITY;
+            }
       }
     }
     float mx[QT], mxx = -INFINITY;
@@ -241,7 +250,9 @@ seq_fwd_kernel(const SeqParams p) {
       for (int t = 0; t < QT; ++t) {
         const float old = m_run[t] == -INFINITY ? 0.f : m_run[t];
         const float mnew = fmaxf(m_run[t], group4_max(mx[t]) + old - kWeightUp<S>);
-        const float alpha = fast_exp2(m_run[t] - mnew), sh = old - mnew;
+        const bool none = WIN && mnew == -INFINITY;   // the row has seen nothing yet: its first key is to rescale
+        const float alpha = none ? 1.f : fast_exp2(m_run[t] - mnew), sh = none ? 0.f : old - mnew, nm = none ? 0.f : -mnew;
+        if (none) thr = -INFINITY;
         m_run[t] = mnew;
         l_run[t] *= alpha;
 #pragma unroll
@@ -250,7 +261,7 @@ seq_fwd_kernel(const SeqParams p) {
         for (int j = 0; j < NB; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) sacc[j][t][h] += sh;
-        nm4[t] = f32x4{-mnew, -mnew, -mnew, -mnew};
+        nm4[t] = f32x4{nm, nm, nm, nm};
       }
     }
 #pragma unroll
@@ -278,12 +289,17 @@ seq_fwd_kernel(const SeqParams p) {
       __attribute__((always_inline)) {
     seq_stage_barrier();
     if (st + 1 < ns) {
-      if constexpr (ROT) rot.load(p, tl, kvh, st + 1, tid);
-      else srcK.load(kn, wave, (st + 1) * SR);
-      srcV.load(vn, wave, (st + 1) * SR);
+      if constexpr (ROT) rot.load(p, tl, kvh, ks.at(st + 1), tid);
+      else srcK.load(kn, wave, ks.at(st + 1) * SR);
+      srcV.load(vn, wave, ks.at(st + 1) * SR);
     }
-    const int k0 = st * SR;
-    if (active && k0 < hi) blocks(k0 + SR > lo, k0, k, v);
+    const int k0 = ks.at(st) * SR;
+    if constexpr (WIN) {   // (keys before all windows of the wave's rows, and some that are before one's)
+      const bool seen_by_some = k0 < hi && (k0 + SR > w0 + 1 - p.window || k0 < p.sinks);
+      if (active && seen_by_some) blocks(k0 + SR > lo || past_window(p, k0, SR, hi - p.window), k0, k, v);
+    } else {
+      if (active && k0 < hi) blocks(k0 + SR > lo, k0, k, v);
+    }
     if (ROT && st + 1 < ns) rot.store(p, kn, tid);   // (read in the stage before this one)
   };
   if constexpr (ROT) rot.store(p, sK0, tid);
@@ -351,10 +367,15 @@ seq_fwd_kernel(const SeqParams p) {
   auto v_bits = [&](int j, int c) {
     return magnitude_bits((float)static_cast<const S*>(p.v)[(tl.start + j) * p.sv[0] + kvh * p.sv[1] + c * p.sv[2]]);
   };
-  bool odd = false, some = false;
+  bool odd = false, some = WIN;
   for (int c = lane; c < D; c += 64) {
-    some |= v_bits(w0, c) <= kInfBits;
-    for (int j = w0 + 1; j < ns * SR && j < tl.len; ++j) odd |= v_bits(j, c) >= kInfBits;
+    if constexpr (WIN) {
+      for (int st = 0; st < ns; ++st)
+        for (int j = ks.at(st) * SR; j < ks.at(st) * SR + SR && j < tl.len; ++j) odd |= v_bits(j, c) >= kInfBits;
+    } else {
+      some |= v_bits(w0, c) <= kInfBits;
+      for (int j = w0 + 1; j < ns * SR && j < tl.len; ++j) odd |= v_bits(j, c) >= kInfBits;
+    }
   }
   if (!__any(odd) || !__any(some)) return;
   __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the rows as stored above come first
@@ -364,7 +385,7 @@ seq_fwd_kernel(const SeqParams p) {
     const float l = group4_sum(l_run[t]);
     for (unsigned left = again[t]; left; left &= left - 1) {
       const int r = __builtin_ctz(left);
-      row_again<S, D, ROT>(p, tl, head, kvh, w0 + 16 * t + r, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run[t]), r)),
+      row_again<S, D, ROT, WIN>(p, tl, head, kvh, w0 + 16 * t + r, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run[t]), r)),
                            __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l), r)), lane);
     }
   }
@@ -374,7 +395,9 @@ template <typename S, int D, int QT, bool ROT>
 static hipError_t fwd(const SeqParams& p0, hipStream_t st) {
   SeqParams p = p0;
   p.slots = (int)seq_slots(p.T, p.B, QT == 2 ? 7 : 6);
-  hipLaunchKernelGGL((seq_fwd_kernel<S, D, QT, ROT>), dim3((unsigned)p.slots * p.H), dim3(kSeqThreads), 0, st, p);
+  const dim3 grid((unsigned)p.slots * p.H);
+  if (p.window) hipLaunchKernelGGL((seq_fwd_kernel<S, D, QT, ROT, true>), grid, dim3(kSeqThreads), 0, st, p);
+  else hipLaunchKernelGGL((seq_fwd_kernel<S, D, QT, ROT, false>), grid, dim3(kSeqThreads), 0, st, p);
   return hipGetLastError();
 }
 template <typename S, int D>
@@ -382,7 +405,7 @@ static hipError_t fwd_rows(const SeqParams& p, hipStream_t st) {
   if constexpr (D <= 128)
     if (!p.khat) return fwd<S, D, 1, true>(p, st);
   if constexpr (sizeof(S) == 2)
-    if (seq_tile_rows(p.T, p.B, p.H, D, false) == 128) return fwd<S, D, 2, false>(p, st);
+    if (seq_tile_rows(p.T, p.B, p.H, D, false, p.window) == 128) return fwd<S, D, 2, false>(p, st);
   return fwd<S, D, 1, false>(p, st);
 }
 template <typename S>

@@ -40,6 +40,11 @@ struct SeqParams {
   float* pk;                         // [parts, T, Hkv, D]: sums of the parts of dK / scale (rotated), parts > 1
   float* pv;                         // and of dV
   int parts;                         // parts of a key tile's queries
+  float* spk;                        // [sink_parts, B, sink_tiles * 64, Hkv, D]: the same of the tiles with sinks
+  float* spv;
+  int sink_parts;                    // parts of their queries (0: they are as the other tiles)
+  int sink_tiles;                    // key tiles of a sequence that hold sinks
+  int window, sinks;                 // token i sees j <= i with i - j < window or j < sinks; window 0: all j <= i
   int T, B, H, Hkv, n_pos, has_cls, causal;
   float scale, c2;                   // softmax scale; times log2 e
   int slots;                         // row slots of the launch (set by the launcher)
@@ -59,7 +64,7 @@ inline int64_t seq_slots(int T, int B, int lb) { return (int64_t)(T >> lb) + B +
 // 235 / 214, 4 x 2048, 8 [512] 34.8 / 36.3.  D 256, forward and backward: 2 x 4096, 8 [512] 1242 / 1173, 16 x
 // 512, 8 [512] 333 / 331, 4 x 1024, 8 [256] 268 / 302, 64 up to 200 (77), 12 [462] 296 / 368, 125 up to 149 (54),
 // 8 [423] 292 / 365.
-inline int seq_tile_rows(int T, int B, int H, int D, bool f32) {
+inline int seq_tile_rows(int T, int B, int H, int D, bool f32, int window) {
   const int64_t tiles = (int64_t)T * H / 128, mean = T / B;
   if (f32) return 64;
   if (D == 256) return tiles >= 2 * 256 && mean >= 256 ? 128 : 64;
@@ -74,8 +79,8 @@ inline int seq_tile_rows(int T, int B, int H, int D, bool f32) {
 // up to 2048 (1124), 16 103 / 98, 8 x 1024, 16 43.8 / 41.7, 64 up to 577 (223), 12 40 / 49.  Forward
 // and backward: 1020 / 894, 2496 / 2115, 203 / 187, 426 / 421, 149 / 154; 200 up to 600 (224), 8 324 / 344.
 constexpr int kOrderSeqs = 256;   // (four sequences per lane of the search)
-inline int seq_order(int T, int B, int D, int causal) {
-  return causal && B > 1 && B <= kOrderSeqs && T / B >= (D >= 128 ? 128 : 512);
+inline int seq_order(int T, int B, int D, int causal, int window) {   // (with a window the tiles' work is alike)
+  return causal && !window && B > 1 && B <= kOrderSeqs && T / B >= (D >= 128 ? 128 : 512);
 }
 
 hipError_t launch_seq_prep(const SeqParams& p, int dt, int D, bool backward, hipStream_t st);

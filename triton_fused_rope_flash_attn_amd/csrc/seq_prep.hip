@@ -72,8 +72,8 @@ __global__ void __launch_bounds__(256) seq_prep_kernel(const SeqParams p, const 
 template <typename S, int D>
 static hipError_t prep(const SeqParams& p, bool backward, hipStream_t st) {
   SeqMaps m{};
-  m.order = seq_order(p.T, p.B, D, p.causal);
-  m.lb_q = seq_tile_rows(p.T, p.B, p.H, D, sizeof(S) == 4) == 128 ? 7 : 6;
+  m.order = seq_order(p.T, p.B, D, p.causal, p.window);
+  m.lb_q = seq_tile_rows(p.T, p.B, p.H, D, sizeof(S) == 4, p.window) == 128 ? 7 : 6;
   m.slots_q = (int)seq_slots(p.T, p.B, m.lb_q);
   m.slots_k = backward ? (int)seq_slots(p.T, p.B, 6) : 0;
   m.blocks = (m.slots_q + m.slots_k + 3) / 4;

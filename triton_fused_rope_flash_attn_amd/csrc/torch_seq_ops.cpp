@@ -1,5 +1,5 @@
 // Native kernels of the torch ops over packed sequences and over a paged cache:
-// farope::seq_fwd, seq_bwd, cache_append, cache_attn, cache_tree (defined in sequences.py),
+// farope::seq_fwd, seq_bwd, seq_window_fwd, seq_window_bwd, cache_append, cache_attn, cache_tree (defined in sequences.py),
 // cache_accept and cache_fork (pages.py), which also refuse CPU tensors.  As in torch_ops.cpp: argument checks,
 // allocation and the C ABI call without the interpreter, and a native autograd
 // node.  Nothing is read back from the device: sequence starts, lengths and page
@@ -92,15 +92,24 @@ void check_seq(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& 
   if (positions) check_ints(*positions, "positions", q.size(0), q);
 }
 
-Two seq_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cosp, const Tensor& sinp, const Tensor& cu,
-            const Opt& positions, bool causal, bool has_cls, double scale) {
+// (window 0: none)
+Two seq_fwd_rows(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cosp, const Tensor& sinp, const Tensor& cu,
+            const Opt& positions, bool causal, bool has_cls, double scale, int64_t window, int64_t sinks) {
   check_seq(q, k, v, cosp, sinp, cu, positions);
   const c10::DeviceGuard guard(q.device());
   const farope_seq_desc d = make_desc(q.size(0), cu.size(0) - 1, q.size(1), k.size(1), q, cosp, causal, has_cls, scale);
   const Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   const Tensor lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
   if (d.tokens == 0) return {o, lse};
-  const Tensor ws = workspace(q, farope_seq_workspace_elems(&d, 0, farope_seq_streams(&d, v.data_ptr(), strides(v)), 1));
+  const int32_t win = to32(window), first = to32(sinks), vs = farope_seq_streams(&d, v.data_ptr(), strides(v));
+  const Tensor ws = workspace(q, win ? farope_seq_window_workspace_elems(&d, win, first, 0, vs, 1) : farope_seq_workspace_elems(&d, 0, vs, 1));
+  if (win) {
+    check_rc(farope_seq_window_fwd(&d, win, first, q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v),
+                                   floats(cosp), floats(sinp), ints(positions), cu.data_ptr<int32_t>(), o.data_ptr(),
+                                   lse.data_ptr<float>(), floats(ws), ws.defined() ? ws.numel() : 0, stream_of(q)),
+             "farope_seq_window_fwd");
+    return {o, lse};
+  }
   check_rc(farope_seq_fwd(&d, q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v), floats(cosp),
                           floats(sinp), ints(positions), cu.data_ptr<int32_t>(), o.data_ptr(), lse.data_ptr<float>(),
                           floats(ws), ws.defined() ? ws.numel() : 0, stream_of(q)),
@@ -108,9 +117,9 @@ Two seq_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos
   return {o, lse};
 }
 
-Three seq_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse,
+Three seq_bwd_rows(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse,
               const Tensor& cosp, const Tensor& sinp, const Tensor& cu, const Opt& positions, bool causal, bool has_cls,
-              double scale) {
+              double scale, int64_t window, int64_t sinks) {
   check_seq(q, k, v, cosp, sinp, cu, positions);
   TORCH_CHECK_VALUE(dout.sizes() == q.sizes() && o.sizes() == q.sizes() && o.is_contiguous(),
                     "farope: dO and O must have Q's shape, O contiguous");
@@ -126,14 +135,44 @@ Three seq_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor
   const auto dense = [](const Tensor& t) { return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)); };
   const Tensor dq = dense(q), dk = dense(k), dv = dense(v);
   if (d.tokens == 0) return {dq, dk, dv};
-  const Tensor ws = workspace(q, farope_seq_workspace_elems(&d, 1, farope_seq_streams(&d, v.data_ptr(), strides(v)),
-                                                            farope_seq_streams(&d, g.data_ptr(), strides(g))));
+  const int32_t win = to32(window), first = to32(sinks), vs = farope_seq_streams(&d, v.data_ptr(), strides(v));
+  const int32_t gs = farope_seq_streams(&d, g.data_ptr(), strides(g));
+  const Tensor ws = workspace(q, win ? farope_seq_window_workspace_elems(&d, win, first, 1, vs, gs) : farope_seq_workspace_elems(&d, 1, vs, gs));
+  if (win) {
+    check_rc(farope_seq_window_bwd(&d, win, first, q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v),
+                                   o.data_ptr(), g.data_ptr(), strides(g), lse.data_ptr<float>(), floats(cosp), floats(sinp),
+                                   ints(positions), cu.data_ptr<int32_t>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), floats(ws),
+                                   ws.defined() ? ws.numel() : 0, stream_of(q)),
+             "farope_seq_window_bwd");
+    return {dq, dk, dv};
+  }
   check_rc(farope_seq_bwd(&d, q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v), o.data_ptr(),
                           g.data_ptr(), strides(g), lse.data_ptr<float>(), floats(cosp), floats(sinp), ints(positions),
                           cu.data_ptr<int32_t>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), floats(ws),
                           ws.defined() ? ws.numel() : 0, stream_of(q)),
            "farope_seq_bwd");
   return {dq, dk, dv};
+}
+
+Two seq_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cosp, const Tensor& sinp, const Tensor& cu,
+            const Opt& positions, bool causal, bool has_cls, double scale) {
+  return seq_fwd_rows(q, k, v, cosp, sinp, cu, positions, causal, has_cls, scale, 0, 0);
+}
+Two seq_window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cosp, const Tensor& sinp, const Tensor& cu,
+                   const Opt& positions, bool has_cls, double scale, int64_t window, int64_t sinks) {
+  check_window(window, sinks);
+  return seq_fwd_rows(q, k, v, cosp, sinp, cu, positions, true, has_cls, scale, window, sinks);
+}
+Three seq_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse,
+              const Tensor& cosp, const Tensor& sinp, const Tensor& cu, const Opt& positions, bool causal, bool has_cls,
+              double scale) {
+  return seq_bwd_rows(dout, q, k, v, o, lse, cosp, sinp, cu, positions, causal, has_cls, scale, 0, 0);
+}
+Three seq_window_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse,
+                     const Tensor& cosp, const Tensor& sinp, const Tensor& cu, const Opt& positions, bool has_cls, double scale,
+                     int64_t window, int64_t sinks) {
+  check_window(window, sinks);
+  return seq_bwd_rows(dout, q, k, v, o, lse, cosp, sinp, cu, positions, true, has_cls, scale, window, sinks);
 }
 
 farope_cache_desc check_cache(const Tensor& kc, const Tensor& vc, const Tensor& pages, const Tensor& lengths, int64_t kv_heads,
@@ -424,6 +463,82 @@ Three seq_bwd_autograd(const Tensor& dout, const Tensor& q, const Tensor& k, con
   return bwd_op().call(dout, q, k, v, o, lse, cosp, sinp, cu, positions, causal, has_cls, scale);
 }
 
+// The same with a window.
+using WindowFwdSig = Two(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Opt&, bool,
+                         double, int64_t, int64_t);
+using WindowBwdSig = Three(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                           const Tensor&, const Tensor&, const Opt&, bool, double, int64_t, int64_t);
+const c10::TypedOperatorHandle<WindowFwdSig>& window_fwd_op() {
+  static const auto op = find<WindowFwdSig>("farope::seq_window_fwd");
+  return op;
+}
+const c10::TypedOperatorHandle<WindowBwdSig>& window_bwd_op() {
+  static const auto op = find<WindowBwdSig>("farope::seq_window_bwd");
+  return op;
+}
+struct WindowFwdNode : torch::autograd::Function<WindowFwdNode> {
+  static variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const Tensor& cosp, const Tensor& sinp, const Tensor& cu, const Opt& positions, bool has_cls,
+                               double scale, int64_t window, int64_t sinks) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Two r = window_fwd_op().call(q, k, v, cosp, sinp, cu, positions, has_cls, scale, window, sinks);
+    const auto& [o, lse] = r;
+    ctx->mark_non_differentiable({lse});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, v, o, lse, cosp, sinp, cu, positions ? *positions : Tensor()});
+    ctx->saved_data["has_cls"] = has_cls;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    return {o, lse};
+  }
+  static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list grads) {
+    variable_list out(11);
+    if (!grads[0].defined()) return out;   // O received no gradient
+    const variable_list s = ctx->get_saved_variables();
+    std::tie(out[0], out[1], out[2]) =
+        window_bwd_op().call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8].defined() ? Opt(s[8]) : Opt(),
+                             ctx->saved_data["has_cls"].toBool(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["window"].toInt(),
+                             ctx->saved_data["sinks"].toInt());
+    return out;
+  }
+};
+Two seq_window_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cosp, const Tensor& sinp,
+                            const Tensor& cu, const Opt& positions, bool has_cls, double scale, int64_t window, int64_t sinks) {
+  refuse_tangents("seq_window_fwd", {&q, &k, &v, &cosp, &sinp});
+  if (at::GradMode::is_enabled() && any_requires_grad({&q, &k, &v})) {
+    const variable_list r = WindowFwdNode::apply(q, k, v, cosp, sinp, cu, positions, has_cls, scale, window, sinks);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return window_fwd_op().call(q, k, v, cosp, sinp, cu, positions, has_cls, scale, window, sinks);
+}
+struct WindowBwdNode : torch::autograd::Function<WindowBwdNode> {
+  static variable_list forward(torch::autograd::AutogradContext*, const Tensor& dout, const Tensor& q, const Tensor& k,
+                               const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& cosp, const Tensor& sinp,
+                               const Tensor& cu, const Opt& positions, bool has_cls, double scale, int64_t window, int64_t sinks) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Three r = window_bwd_op().call(dout, q, k, v, o, lse, cosp, sinp, cu, positions, has_cls, scale, window, sinks);
+    return {std::get<0>(r), std::get<1>(r), std::get<2>(r)};
+  }
+  static variable_list backward(torch::autograd::AutogradContext*, variable_list) {
+    TORCH_CHECK(false,
+                "Trying to backward through farope.seq_window_bwd.default but no autograd formula was registered "
+                "(the attention's gradients are not differentiable again).");
+  }
+};
+Three seq_window_bwd_autograd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
+                              const Tensor& lse, const Tensor& cosp, const Tensor& sinp, const Tensor& cu, const Opt& positions,
+                              bool has_cls, double scale, int64_t window, int64_t sinks) {
+  refuse_tangents("seq_window_bwd", {&dout, &q, &k, &v, &o, &lse, &cosp, &sinp});
+  if (at::GradMode::is_enabled() && any_requires_grad({&dout, &q, &k, &v, &o, &lse})) {
+    const variable_list r = WindowBwdNode::apply(dout, q, k, v, o, lse, cosp, sinp, cu, positions, has_cls, scale, window, sinks);
+    return {r[0], r[1], r[2]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return window_bwd_op().call(dout, q, k, v, o, lse, cosp, sinp, cu, positions, has_cls, scale, window, sinks);
+}
+
 void bump(std::initializer_list<Tensor*> ts) {
   for (Tensor* t : ts)
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
@@ -536,6 +651,8 @@ Tensor cache_tree_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, 
 TORCH_LIBRARY_IMPL(farope, CUDA, m) {
   m.impl("seq_fwd", seq_fwd);
   m.impl("seq_bwd", seq_bwd);
+  m.impl("seq_window_fwd", seq_window_fwd);
+  m.impl("seq_window_bwd", seq_window_bwd);
   m.impl("cache_append", cache_append);
   m.impl("cache_attn", cache_attn);
   m.impl("cache_attn_window", cache_attn_window);
@@ -547,6 +664,8 @@ TORCH_LIBRARY_IMPL(farope, CUDA, m) {
 TORCH_LIBRARY_IMPL(farope, AutogradCUDA, m) {
   m.impl("seq_fwd", seq_fwd_autograd);
   m.impl("seq_bwd", seq_bwd_autograd);
+  m.impl("seq_window_fwd", seq_window_fwd_autograd);
+  m.impl("seq_window_bwd", seq_window_bwd_autograd);
   m.impl("cache_append", cache_append_autograd);
   m.impl("cache_attn", cache_attn_autograd);
   m.impl("cache_attn_window", cache_attn_window_autograd);

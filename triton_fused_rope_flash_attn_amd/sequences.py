@@ -23,7 +23,7 @@ the device, and a captured call reads their new values when it is replayed.
 Their values are therefore not refused; each function says what it does with
 those that make no sense, and none reads or writes outside its tensors.
 
-The work is done by five ``torch.library`` ops with native GPU kernels
+The work is done by ``torch.library`` ops with native GPU kernels
 (csrc/torch_seq_ops.cpp), one call into libfarope.so each, on the current stream of
 the tensors' device.  There is no CPU fallback: CPU tensors raise.
 """
@@ -191,6 +191,60 @@ def _seq_backward(ctx, do, _dlse):
 _seq_fwd.register_autograd(_seq_backward, setup_context=_seq_setup_context)
 
 
+@torch.library.custom_op("farope::seq_window_fwd", mutates_args=())
+def _seq_window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cosp: torch.Tensor, sinp: torch.Tensor, cu: torch.Tensor,
+                    positions: Optional[torch.Tensor], has_cls: bool, softmax_scale: float, window: int,
+                    sinks: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """-> (O [T, H, D], LSE [H, T])."""
+    _check_window(window, sinks)
+    _check_seq(q, k, v, cosp, sinp, cu, positions)
+    _check_device(q)
+    _lib.require_torch_ops()
+
+
+@_seq_window_fwd.register_fake
+def _seq_window_fwd_fake(q, k, v, cosp, sinp, cu, positions, has_cls, softmax_scale, window, sinks):
+    _check_window(window, sinks)
+    return _seq_fwd_fake(q, k, v, cosp, sinp, cu, positions, True, has_cls, softmax_scale)
+
+
+@torch.library.custom_op("farope::seq_window_bwd", mutates_args=())
+def _seq_window_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                    cosp: torch.Tensor, sinp: torch.Tensor, cu: torch.Tensor, positions: Optional[torch.Tensor], has_cls: bool,
+                    softmax_scale: float, window: int, sinks: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """-> (dQ, dK, dV)."""
+    _check_window(window, sinks)
+    _check_seq(q, k, v, cosp, sinp, cu, positions)
+    _check_device(q)
+    _lib.require_torch_ops()
+
+
+@_seq_window_bwd.register_fake
+def _seq_window_bwd_fake(do, q, k, v, o, lse, cosp, sinp, cu, positions, has_cls, softmax_scale, window, sinks):
+    return q.new_empty(tuple(q.shape)), k.new_empty(tuple(k.shape)), v.new_empty(tuple(v.shape))
+
+
+def _seq_window_setup_context(ctx, inputs, output):
+    q, k, v, cosp, sinp, cu, positions, ctx.has_cls, ctx.softmax_scale, ctx.window, ctx.sinks = inputs
+    o, lse = output
+    ctx.mark_non_differentiable(lse)
+    ctx.set_materialize_grads(False)
+    ctx.has_positions = positions is not None
+    ctx.save_for_backward(q, k, v, o, lse, cosp, sinp, cu, *([positions] if ctx.has_positions else []))
+
+
+def _seq_window_backward(ctx, do, _dlse):
+    if do is None:
+        return (None,) * 11
+    q, k, v, o, lse, cosp, sinp, cu, *rest = ctx.saved_tensors
+    grads = _seq_window_bwd(do, q, k, v, o, lse, cosp, sinp, cu, rest[0] if ctx.has_positions else None, ctx.has_cls,
+                            ctx.softmax_scale, ctx.window, ctx.sinks)
+    return (*grads, None, None, None, None, None, None, None, None)
+
+
+_seq_window_fwd.register_autograd(_seq_window_backward, setup_context=_seq_window_setup_context)
+
+
 @torch.library.custom_op("farope::cache_append", mutates_args=("k_cache", "v_cache"))
 def _cache_append(k: torch.Tensor, v: torch.Tensor, cosp: torch.Tensor, sinp: torch.Tensor, k_cache: torch.Tensor,
                   v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor],
@@ -308,6 +362,7 @@ def _cache_tree_fake(q, k_cache, v_cache, cosp, sinp, page_table, lengths, cu, t
 
 _lib.load_torch_ops()   # (their kernels for GPU tensors, as in attention.py)
 _seq_fwd_op = torch.ops.farope.seq_fwd.default
+_seq_window_fwd_op = torch.ops.farope.seq_window_fwd.default
 _append_op = torch.ops.farope.cache_append.default
 _attn_op = torch.ops.farope.cache_attn.default
 _attn_window_op = torch.ops.farope.cache_attn_window.default
@@ -338,6 +393,8 @@ def sdpa_rope_varlen(
     causal: bool = True,
     has_cls: bool = True,
     positions: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> torch.Tensor:
     """Rotary attention within packed sequences, forward and gradients.
 
@@ -352,16 +409,23 @@ def sdpa_rope_varlen(
     causal: token i of a sequence sees its tokens 0 .. i, else all of them.  What it does not
     see does not reach O, infinities and NaN included.  (Gradients: an infinity or NaN of Q,
     K or dO within 63 tokens of a row that has no part in it may reach it as 0 * NaN.)
+    window, sinks: of the tokens 0 .. i, token i sees the last ``window`` (at least 1: itself) and those
+    below ``sinks`` alone (causal only; without a window ``sinks`` makes no difference).
     positions: int32 ``[T]`` table rows, instead of ``i - has_cls``.
 
     Returns O ``[T, H, D]`` of Q's dtype.  Gradients come back for Q, K and V.
     """
+    if window is not None and not causal:
+        raise ValueError("farope: a window is causal")
     cosp, sinp = _tables(cos_sin)
     dtype = Q.dtype
     if torch.is_autocast_enabled():
         comp = _sdpa_comp_dtype(Q)
         Q, K, V = Q.to(comp), K.to(comp), V.to(comp)
-    O = _seq_fwd_op(Q, K, V, cosp, sinp, cu_seqlens, positions, causal, has_cls, _scale(Q.shape[-1]))[0]
+    if window is None:
+        O = _seq_fwd_op(Q, K, V, cosp, sinp, cu_seqlens, positions, causal, has_cls, _scale(Q.shape[-1]))[0]
+    else:
+        O = _seq_window_fwd_op(Q, K, V, cosp, sinp, cu_seqlens, positions, has_cls, _scale(Q.shape[-1]), window, sinks)[0]
     return O if O.dtype == dtype else O.to(dtype)
 
 
