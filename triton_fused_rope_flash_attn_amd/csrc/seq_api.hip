@@ -562,7 +562,9 @@ int farope_tree(const farope_seq_desc* desc, const void* q, const int64_t q_stri
   if (positions) FAROPE_TRY(check_ptr(positions, 4));
   FAROPE_TRY(check_cache(desc, cache, page_table, lengths));
   FAROPE_TRY(check_ptr(cu, 4));
-  if (tree && (tree_cols < 0 || tree_stride < 0)) return FAROPE_ERR_SHAPE;
+  // (the rows of a sequence's tree are reached by 32-bit offsets)
+  if (tree && (tree_cols < 0 || tree_stride < 0 || tree_stride > INT32_MAX || tree_stride * desc->tokens + tree_cols > INT32_MAX))
+    return FAROPE_ERR_SHAPE;
   FAROPE_TRY(check_ptr(o, 16));
   const TreeWs w = tree_ws(desc, cache);
   if (w.total) {
@@ -581,6 +583,19 @@ int farope_tree(const farope_seq_desc* desc, const void* q, const int64_t q_stri
   p.stats = ws + w.stats;
   p.owners = reinterpret_cast<int*>(ws + w.owners);
   p.T = desc->tokens; p.B = desc->seqs; p.H = desc->heads; p.Hkv = desc->kv_heads; p.n_pos = desc->n_pos; p.has_cls = desc->has_cls;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t k = cache->k_stride[i] * es / 16, v = cache->v_stride[i] * es / 16;
+    if (k < 0 || v < 0 || k > UINT32_MAX || v > UINT32_MAX) return FAROPE_ERR_SHAPE;
+    p.k16[i] = (uint32_t)k;
+    p.v16[i] = (uint32_t)v;
+  }
+  p.alike = p.k16[0] == p.v16[0] && p.k16[1] == p.v16[1];
+  // With 2^(l-1) < page <= 2^l, m = floor(2^(31+l) / page) + 1 and e = m page - 2^(31+l) in (0, page]: x m / 2^(31+l) =
+  // x / page + x e / (page 2^(31+l)), and x e < 2^31 2^l, so the second part is less than 1 / page.
+  int l = 0;
+  while (l < 31 && (int64_t(1) << l) < cache->page_rows) ++l;
+  p.page_mul = (uint32_t)(((uint64_t(1) << (31 + l)) / (uint64_t)cache->page_rows + 1));
+  p.page_shift = 31 + l;
   p.rows = tree_rows(desc);
   // (rows of a key head in 32 bits, with a tile's more; workgroups of the join: 16 rows each)
   if ((int64_t)p.T * p.H > INT32_MAX - 256 || tree_slots(desc) * p.Hkv * (p.rows / 16) > kMaxWorkgroups) return FAROPE_ERR_SHAPE;

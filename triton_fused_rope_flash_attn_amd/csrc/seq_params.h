@@ -152,6 +152,10 @@ struct TreeParams {
   float* stats;          // [2 * workers, Hkv, rows, 2]: their max logit (log2 units) and row sum
   int* owners;           // [slots, 4]: a tile's first worker, how many have a part of it, which piece the first one's is
   int T, B, H, Hkv, n_pos, has_cls;
+  unsigned k16[2], v16[2];   // the caches' strides of a page and of a row, in 16 bytes
+  int alike;                 // both caches' are the same
+  unsigned page_mul;         // x / page = x * page_mul >> page_shift for 0 <= x < 2^31
+  int page_shift;
   int rows;              // of a tile: 64 or 128
   int slots;             // row slots of the call
   int workers;           // workgroups of a key head

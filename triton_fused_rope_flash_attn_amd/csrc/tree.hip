@@ -39,6 +39,16 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
   return s;
 }
 
+__device__ __forceinline__ TreeSeq uniform(TreeSeq s) {
+  s.start = __builtin_amdgcn_readfirstlane(s.start);
+  s.m = __builtin_amdgcn_readfirstlane(s.m);
+  s.len = __builtin_amdgcn_readfirstlane(s.len);
+  s.n = __builtin_amdgcn_readfirstlane(s.n);
+  s.tiles = __builtin_amdgcn_readfirstlane(s.tiles);
+  s.blocks = __builtin_amdgcn_readfirstlane(s.blocks);
+  return s;
+}
+
 __device__ __forceinline__ int64_t wave_scan64(int64_t x, int lane) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -66,7 +76,19 @@ __device__ __forceinline__ void find_rows(const TreeParams& p, int lb, int slot,
   tile = slot - (((cu_at(p.cu, seq, p.T) * group) >> lb) + seq);
 }
 
-// 16 bytes per lane from memory straight into LDS (lane l lands at lds + 16 l); off lanes write nothing.
+__device__ const float kZeros[4] __attribute__((aligned(16))) = {0.f, 0.f, 0.f, 0.f};
+
+// One byte of a buffer (a plain function, as lds_dma16).
+__device__ __forceinline__ uint8_t buf_load1(__amdgpu_buffer_rsrc_t r, unsigned voff) {
+  return __builtin_amdgcn_raw_buffer_load_b8(r, voff, 0, 0);
+}
+
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// 16 bytes per lane from memory straight into LDS (lane l lands at lds + 16 l).
 __device__ __forceinline__ void gather16(const void* from, void* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)from,
                                    (__attribute__((address_space(3))) unsigned*)lds, 16, 0, 0);
@@ -141,7 +163,6 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
 
   const int tid = thread_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int lr = lane & 15, lg = lane >> 4;
   const int worker = block_id() / p.Hkv, kvh = block_id() % p.Hkv, group = p.H / p.Hkv;
 
   // this worker's stages [at, stop) of all, from stage `first` of tile `tile` of sequence b on; `before`: the
@@ -171,7 +192,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
       sum = wave_scan64(n, lane);
       all += lane64(sum, 63);
     }
-    const int64_t even = (all + p.workers - 1) / p.workers;
+    const int64_t even = lane64((all + p.workers - 1) / p.workers, 0);
     size = even > kTreeLeast ? even : kTreeLeast;
     at = worker * size;
     if (at >= all) return;
@@ -196,17 +217,19 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
       before += lane64(sum, 63);
     }
     if (b < 0) return;
-    const TreeSeq s = tree_seq<ROWS, SR>(p, b);
-    tile = (int)((at - before) / s.blocks);
+    const TreeSeq s = uniform(tree_seq<ROWS, SR>(p, b));
+    tile = __builtin_amdgcn_readfirstlane((int)((at - before) / s.blocks));
     before += (int64_t)tile * s.blocks;
     first = (int)(at - before);
   }
 
-  FragAt<S, D> frag;
-  frag.init(lr, lg);
-
   for (;;) {
-    const TreeSeq s = tree_seq<ROWS, SR>(p, b);
+    // (a lane number that the compiler takes as new for each piece: what follows from it, computed once for all of
+    // them, filled the registers)
+    const int lane = fresh(tid & 63), lr = lane & 15, lg = lane >> 4;
+    FragAt<S, D> frag;
+    frag.init(lr, lg);
+    const TreeSeq s = uniform(tree_seq<ROWS, SR>(p, b));
     const int stages = p.direct || stop - at > s.blocks - first ? s.blocks : first + (int)(stop - at);   // this piece: [first, stages)
     const int r0 = tile * ROWS, rows = s.m * group - r0 < ROWS ? s.m * group - r0 : ROWS;
     const bool chain = !p.tree;
@@ -215,7 +238,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
       const int64_t x = chain ? (int64_t)s.len + (r0 + row) / group + 1 : s.n;
       return x < s.n ? (int)x : s.n;
     };
-    const int last = (seen_by(rows - 1) + SR - 1) / SR, end = stages < last ? stages : last;
+    const int last = (__builtin_amdgcn_readfirstlane(seen_by(rows - 1)) + SR - 1) / SR, end = stages < last ? stages : last;
 
     // lane l: row l of a stage: page and row in it
     const int* const pages = p.c.pages + b * p.c.spages;
@@ -224,7 +247,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
       Ids id{-1, 0};
       const int64_t r = (int64_t)st * SR + lane;
       if (st < end && lane < SR && r < s.n) {
-        const unsigned place = (unsigned)r / (unsigned)p.c.page;
+        const unsigned place = (unsigned)((uint64_t)(unsigned)r * p.page_mul >> p.page_shift);   // r / page
         id.page = pages[place];
         id.row = (int)((unsigned)r - place * (unsigned)p.c.page);
       }
@@ -234,38 +257,33 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
     auto load = [&](const Ids& id, S* __restrict__ kd, S* __restrict__ vd) __attribute__((always_inline)) {
       const bool in = id.page >= 0 && id.page < p.c.n_pages;
       rows_in = __builtin_amdgcn_ballot_w64(in);
-      const int64_t g = in ? id.page : 0, r = in ? id.row : 0;   // (the others read page 0's first row)
-      const int64_t ko = g * p.c.skc[0] + r * p.c.skc[1], vo = g * p.c.svc[0] + r * p.c.svc[1];
-      const S* const kb = static_cast<const S*>(p.c.kc) + kvh * p.c.skc[2];
-      const S* const vb = static_cast<const S*>(p.c.vc) + kvh * p.c.svc[2];
+      // (strides in 16 bytes; K rows that do not exist: page 0's first; they are masked)
+      const unsigned g = in ? (unsigned)id.page : 0u, r = in ? (unsigned)id.row : 0u;
+      const int64_t ko = (int64_t)((uint64_t)g * p.k16[0] + (uint64_t)r * p.k16[1]);
+      const int64_t vo = p.alike ? ko : (int64_t)((uint64_t)g * p.v16[0] + (uint64_t)r * p.v16[1]);
+      const char* const kb = static_cast<const char*>(p.c.kc) + kvh * p.c.skc[2] * (int)sizeof(S);
+      const char* const vb = static_cast<const char*>(p.c.vc) + kvh * p.c.svc[2] * (int)sizeof(S);
+      const int ln = fresh(lane);
 #pragma unroll
       for (int i = 0; i < T::NI; ++i) {
-        const int rw = (i * kSeqNW + wave) * T::RPI + lane / T::CPR, ch = ((lane % T::CPR) ^ T::chunk_xor(rw)) * T::EPC;
-        gather16(kb + shfl64(ko, rw) + ch, kd + (i * kSeqNW + wave) * T::RPI * D);
-      }
-#pragma unroll
-      for (int i = 0; i < T::NI; ++i) {
-        const int rw = (i * kSeqNW + wave) * T::RPI + lane / T::CPR, ch = ((lane % T::CPR) ^ T::chunk_xor(rw)) * T::EPC;
-        S* const to = vd + (i * kSeqNW + wave) * T::RPI * D;
-        const S* const from = vb + shfl64(vo, rw) + ch;
-        if (rows_in == kAll) {   // uniform
-          gather16(from, to);
-        } else if (rows_in >> rw & 1) {
-          gather16(from, to);
-        } else {   // V rows that do not exist are zeros: their weights are
-          *reinterpret_cast<u32x4*>(to + lane * T::EPC) = u32x4{0u, 0u, 0u, 0u};
-        }
+        const int rw = (i * kSeqNW + wave) * T::RPI + ln / T::CPR, ch = (ln % T::CPR) ^ T::chunk_xor(rw);
+        const int64_t kr = shfl64(ko, rw) + ch, vr = p.alike ? kr : shfl64(vo, rw) + ch;   // (uniform)
+        gather16(kb + 16 * kr, kd + (i * kSeqNW + wave) * T::RPI * D);
+        const char* const from = vb + 16 * vr;   // V rows that do not exist are zeros: their weights are
+        gather16(rows_in >> rw & 1 ? from : reinterpret_cast<const char*>(kZeros), vd + (i * kSeqNW + wave) * T::RPI * D);
       }
     };
 
+    const auto rTree = make_rsrc(p.tree + (chain ? 0 : s.start * p.stree), chain ? 0u : (unsigned)((s.m - 1) * (int)p.stree + p.cols));
     const int row0 = wave * 16 * QT + lr;   // of the tile; subtile t: + 16 t
     const int w0 = wave * 16 * QT, w1 = w0 + 16 * QT < rows ? w0 + 16 * QT - 1 : rows - 1;
     const bool active = w0 < rows;
     // every row of the wave sees rows below lo of the cache, none sees rows from hi on
-    const int lo = chain ? seen_by(active ? w0 : 0) : s.len < s.n ? s.len : s.n, hi = seen_by(active ? w1 : 0);
+    const int lo = chain ? __builtin_amdgcn_readfirstlane(seen_by(active ? w0 : 0)) : s.len < s.n ? s.len : s.n;
+    const int hi = __builtin_amdgcn_readfirstlane(seen_by(active ? w1 : 0));
     Frag qf[QT][KS];
     int seen[QT];                // chain: rows that the lane's row of the subtile sees
-    const uint8_t* sees[QT];     // tree: its row of the tree
+    int tok[QT];                 // its token of the sequence
     f32x4 acc[QT][DT];
     float m_run[QT], l_run[QT];
     {
@@ -276,11 +294,11 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           const int r = row0 + 16 * t < rows ? row0 + 16 * t : rows - 1, j = (r0 + r) / group, h = kvh * group + (r0 + r) % group;
-          const int64_t tok = s.start + j, index = (int64_t)s.len + j - p.has_cls;
+          const int64_t at_tok = s.start + j, index = (int64_t)s.len + j - p.has_cls;
           seen[t] = seen_by(r);
-          sees[t] = p.tree + tok * p.stree;
-          const int tr = table_row(p.positions ? p.positions[tok] : (int)(index < INT32_MAX ? index : INT32_MAX), p.n_pos);
-          const S* const qp = static_cast<const S*>(p.q) + tok * p.sq[0] + h * p.sq[1];
+          tok[t] = j;
+          const int tr = table_row(p.positions ? p.positions[at_tok] : (int)(index < INT32_MAX ? index : INT32_MAX), p.n_pos);
+          const S* const qp = static_cast<const S*>(p.q) + at_tok * p.sq[0] + h * p.sq[1];
 #pragma unroll
           for (int c = 0; c < KS; ++c) {
             float x[8], cs[8];
@@ -319,19 +337,32 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
         if (tail) {   // uniform: some row of the wave does not see all of these rows
 #pragma unroll
           for (int t = 0; t < QT; ++t) {
+            const int g4 = fresh(4 * lg), lim = (chain ? seen[t] : s.len) - k0 - g4;
+            unsigned more = 0;   // bit 8 j + 4 h + i: the lane's row sees row 32 j + 16 h + 4 lg + i of the stage, a new token's
+            if (!chain && k0 + SR > s.len && p.cols > 0) {   // (uniform) the bytes of its row of the tree, all loads in flight together
+              const int d0 = -lim;
+              const int at_row = tok[t] * (int)p.stree;
+              uint8_t x[8 * NB];
+#pragma unroll
+              for (int e = 0; e < 8 * NB; ++e) {   // (what lies behind the sequence's rows reads as 0)
+                const int d = d0 + 32 * (e >> 3) + 16 * (e >> 2 & 1) + (e & 3);
+                x[e] = buf_load1(rTree, (unsigned)(at_row + (d > 0 ? d : 0)));
+              }
+#pragma unroll
+              for (int e = 0; e < 8 * NB; ++e) {
+                const int d = d0 + 32 * (e >> 3) + 16 * (e >> 2 & 1) + (e & 3);
+                more |= d >= 0 && d < p.cols && x[e] != 0 ? 1u << e : 0u;
+              }
+            }
+            const uint64_t there = have >> g4;
 #pragma unroll
             for (int j = 0; j < NB; ++j)
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  const int e = 32 * j + 16 * h + 4 * lg + i, key = k0 + e;
-                  bool in = have >> e & 1;
-                  if (chain) {
-                    in = in && key < seen[t];
-                  } else if (in && key >= s.len) {
-                    in = key - s.len < p.cols && sees[t][key - s.len] != 0;
-                  }
+                  const int e = 32 * j + 16 * h + i;
+                  const bool in = (e < lim || (more >> (8 * j + 4 * h + i) & 1)) && (there >> e & 1);
                   sacc[j][t][h][i] = in ? sacc[j][t][h][i] : -INFINITY;
                 }
           }
@@ -408,6 +439,8 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
     }
 
     const bool whole = first == 0 && stages == s.blocks;   // the tile is this worker's alone
+    {
+    const int lane = fresh(tid & 63), lr = lane & 15, lg = lane >> 4, row0 = wave * 16 * QT + lr;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       const int row = row0 + 16 * t;
@@ -487,6 +520,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
                                out, whole, lane);
         }
       }
+    }
     }
     if (p.direct) return;
     // the join's: the tile's first worker, how many have a part of it, and which piece the first one's is
