@@ -381,7 +381,7 @@ int tree_rows(const farope_seq_desc* d) {
   return d->dtype != FAROPE_F32 && (int64_t)d->tokens * tree_group(d) / d->seqs > 64 ? 128 : 64;
 }
 int64_t tree_slots(const farope_seq_desc* d) { return (int64_t)d->tokens * tree_group(d) / tree_rows(d) + d->seqs + 1; }
-int tree_stage(const farope_seq_desc* d) { return d->head_dim * elem_size(d->dtype) <= 256 ? 64 : 32; }
+int tree_stage(const farope_seq_desc* d) { return d->head_dim * elem_size(d->dtype) <= 128 ? 64 : 32; }   // (kTreeRows of tree.hip)
 bool tree_direct(const farope_seq_desc* d, const farope_cache_desc* c) {
   return (int64_t)c->max_pages * c->page_rows <= 512;
 }

@@ -20,6 +20,10 @@
 
 namespace farope {
 
+// Rows of a stage and stages in LDS: three are on their way while one is read, but for rows of 1 KB.
+template <typename S, int D> constexpr int kTreeRows = D * sizeof(S) <= 128 ? 64 : 32;
+template <typename S, int D> constexpr int kTreeBufs = D * sizeof(S) <= 512 ? 4 : 2;
+
 // What a sequence has: its tokens, rows cached before them, rows in the cache with them, tiles, stages of a tile.
 struct TreeSeq {
   int start, m, len, n, tiles, blocks;
@@ -81,6 +85,16 @@ __device__ const float kZeros[4] __attribute__((aligned(16))) = {0.f, 0.f, 0.f, 
 // One byte of a buffer (a plain function, as lds_dma16).
 __device__ __forceinline__ uint8_t buf_load1(__amdgpu_buffer_rsrc_t r, unsigned voff) {
   return __builtin_amdgcn_raw_buffer_load_b8(r, voff, 0, 0);
+}
+
+// Every wave is here, with at most N of its loads still on their way and none of its LDS accesses.  (Without the
+// fences of lds_barrier, which wait for all loads to LDS.)
+template <int N> __device__ __forceinline__ void loads_barrier() {
+  static_assert(N < 64, "");
+  asm volatile("" : : : "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" : : : "memory");
 }
 
 __device__ __forceinline__ int fresh(int x) {
@@ -156,10 +170,13 @@ template <typename S, int D, int QT>
 __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tree_kernel(const TreeParams p) {
   using C = typename SeqComp<S>::C;
   using Frag = typename C::Frag;
-  using T = Tile<S, D>;
+  using T = Tile<S, D, kTreeRows<S, D>>;
+  constexpr int BUFS = kTreeBufs<S, D>, AHEAD = BUFS - 1, LOADS = 2 * T::NI;   // (LOADS: of a wave and stage)
   constexpr int KS = D / 32, DT = D / 16, SR = T::SR, NB = SR / 32, ROWS = 64 * QT, LB = QT == 2 ? 7 : 6;
   constexpr uint64_t kAll = SR == 64 ? ~0ull : 0xffffffffull;
-  __shared__ __attribute__((aligned(16))) S sK0[SR * D], sK1[SR * D], sV0[SR * D], sV1[SR * D];
+  constexpr int MORE = BUFS > 2 ? SR * D : 8;
+  __shared__ __attribute__((aligned(16))) S sK0[SR * D], sK1[SR * D], sK2[MORE], sK3[MORE];
+  __shared__ __attribute__((aligned(16))) S sV0[SR * D], sV1[SR * D], sV2[MORE], sV3[MORE];
 
   const int tid = thread_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -242,36 +259,42 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
 
     // lane l: row l of a stage: page and row in it
     const int* const pages = p.c.pages + b * p.c.spages;
-    struct Ids { int page, row; };
+    struct Ids { int page, row; };   // (row -1: there is none)
     auto fetch = [&](int st) __attribute__((always_inline)) {
-      Ids id{-1, 0};
-      const int64_t r = (int64_t)st * SR + lane;
-      if (st < end && lane < SR && r < s.n) {
-        const unsigned place = (unsigned)((uint64_t)(unsigned)r * p.page_mul >> p.page_shift);   // r / page
-        id.page = pages[place];
-        id.row = (int)((unsigned)r - place * (unsigned)p.c.page);
-      }
+      const unsigned r = (unsigned)st * SR + (unsigned)lane;   // (below 2^31: stages end at s.n, with a few behind)
+      unsigned place = (unsigned)((uint64_t)r * p.page_mul >> p.page_shift);   // r / page
+      Ids id;
+      id.row = st < end && lane < SR && r < (unsigned)s.n ? (int)(r - place * (unsigned)p.c.page) : -1;
+      place = place < (unsigned)p.c.max_pages ? place : (unsigned)p.c.max_pages - 1u;
+      id.page = pages[place];   // (one load whatever there is, so that the number of loads on their way is known)
       return id;
     };
-    uint64_t rows_in = 0;   // rows (bits) of the loaded stage that exist
-    auto load = [&](const Ids& id, S* __restrict__ kd, S* __restrict__ vd) __attribute__((always_inline)) {
-      const bool in = id.page >= 0 && id.page < p.c.n_pages;
-      rows_in = __builtin_amdgcn_ballot_w64(in);
+    auto load = [&](Ids id, S* __restrict__ kd, S* __restrict__ vd) __attribute__((always_inline)) {
+      id.page = fresh(id.page);   // (not looked at before the barrier, where other loads would have to be waited for)
+      const bool in = id.row >= 0 && id.page >= 0 && id.page < p.c.n_pages;
+      const uint64_t rows_in = __builtin_amdgcn_ballot_w64(in);
       // (strides in 16 bytes; K rows that do not exist: page 0's first; they are masked)
       const unsigned g = in ? (unsigned)id.page : 0u, r = in ? (unsigned)id.row : 0u;
       const int64_t ko = (int64_t)((uint64_t)g * p.k16[0] + (uint64_t)r * p.k16[1]);
-      const int64_t vo = p.alike ? ko : (int64_t)((uint64_t)g * p.v16[0] + (uint64_t)r * p.v16[1]);
+      const int64_t vo = (int64_t)((uint64_t)g * p.v16[0] + (uint64_t)r * p.v16[1]);
       const char* const kb = static_cast<const char*>(p.c.kc) + kvh * p.c.skc[2] * (int)sizeof(S);
       const char* const vb = static_cast<const char*>(p.c.vc) + kvh * p.c.svc[2] * (int)sizeof(S);
-      const int ln = fresh(lane);
+      const unsigned ln = (unsigned)fresh(lane) & 63u;
+      int64_t kr[T::NI], vr[T::NI];
+#pragma unroll
+      for (int i = 0; i < T::NI; ++i) vr[i] = kr[i] = shfl64(ko, (i * kSeqNW + wave) * T::RPI + (int)(ln / T::CPR));
+      if (!p.alike) {   // (uniform)
+#pragma unroll
+        for (int i = 0; i < T::NI; ++i) vr[i] = shfl64(vo, (i * kSeqNW + wave) * T::RPI + (int)(ln / T::CPR));
+      }
 #pragma unroll
       for (int i = 0; i < T::NI; ++i) {
-        const int rw = (i * kSeqNW + wave) * T::RPI + ln / T::CPR, ch = (ln % T::CPR) ^ T::chunk_xor(rw);
-        const int64_t kr = shfl64(ko, rw) + ch, vr = p.alike ? kr : shfl64(vo, rw) + ch;   // (uniform)
-        gather16(kb + 16 * kr, kd + (i * kSeqNW + wave) * T::RPI * D);
-        const char* const from = vb + 16 * vr;   // V rows that do not exist are zeros: their weights are
+        const int rw = (i * kSeqNW + wave) * T::RPI + (int)(ln / T::CPR), ch = (int)(ln % T::CPR) ^ T::chunk_xor(rw);
+        gather16(kb + 16 * (kr[i] + ch), kd + (i * kSeqNW + wave) * T::RPI * D);
+        const char* const from = vb + 16 * (vr[i] + ch);   // V rows that do not exist are zeros: their weights are
         gather16(rows_in >> rw & 1 ? from : reinterpret_cast<const char*>(kZeros), vd + (i * kSeqNW + wave) * T::RPI * D);
       }
+      return rows_in;   // the stage's rows (bits) that exist
     };
 
     const auto rTree = make_rsrc(p.tree + (chain ? 0 : s.start * p.stree), chain ? 0u : (unsigned)((s.m - 1) * (int)p.stree + p.cols));
@@ -287,9 +310,20 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
     f32x4 acc[QT][DT];
     float m_run[QT], l_run[QT];
     {
-      Ids next = fetch(first);
-      if (first < end) load(next, sK0, sV0);
-      next = fetch(first + 1);
+      // ids[i] and rows_in[i]: of the stages that are first + i but for a multiple of 4.  Page numbers are read AHEAD
+      // stages before their rows, so that to wait for them is not to wait for rows.  Stages behind the piece's
+      // end are loaded too (V as zeros, K from one row), and not used.
+      Ids ids[4];
+      uint64_t rows_in[4];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) ids[i] = fetch(first + i);
+      rows_in[0] = load(ids[0], sK0, sV0);
+      if constexpr (AHEAD > 1) {
+        rows_in[1] = load(ids[1], sK1, sV1);
+        rows_in[2] = load(ids[2], sK2, sV2);
+      }
+#pragma unroll
+      for (int i = AHEAD; i < 2 * AHEAD; ++i) ids[i & 3] = fetch(first + i);
       {
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
@@ -413,28 +447,42 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
             l_run[t] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             pf[t] = C::make(x);   // (16-bit tensors: P rounded to their type for the O product; the row sum is not)
           }
+          Frag a[3];   // (two fragments ahead)
+          a[0] = frag.col(v + 32 * j * D, 0);
+          a[1] = frag.col(v + 32 * j * D, 1);
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            const Frag a = frag.col(v + 32 * j * D, d);
+            if (d + 2 < DT) a[(d + 2) % 3] = frag.col(v + 32 * j * D, d + 2);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) acc[t][d] = C::mma(a, pf[t], acc[t][d]);
+            for (int t = 0; t < QT; ++t) acc[t][d] = C::mma(a[d % 3], pf[t], acc[t][d]);
           }
         }
       };
-      auto stage = [&](int st, const S* __restrict__ k, const S* __restrict__ v, S* __restrict__ kn, S* __restrict__ vn)
+      auto stage = [&](auto slot, int st, const S* __restrict__ k, const S* __restrict__ v, S* __restrict__ kn, S* __restrict__ vn)
           __attribute__((always_inline)) {
-        seq_stage_barrier();
-        const uint64_t have = rows_in;
-        if (st + 1 < end) {
-          load(next, kn, vn);
-          next = fetch(st + 2);
-        }
+        constexpr int U = decltype(slot)::value;
+        // The stage's own loads have landed: those of the AHEAD - 1 stages behind it are the last that were issued, LOADS
+        // each at least (page numbers come on top).
+        loads_barrier<(AHEAD - 1) * LOADS>();
+        const uint64_t have = rows_in[U];
+        rows_in[(U + AHEAD) & 3] = load(ids[(U + AHEAD) & 3], kn, vn);
+        ids[(U + 2 * AHEAD) & 3] = fetch(st + 2 * AHEAD);
         const int k0 = st * SR;
-        if (active && k0 < hi) blocks(have != kAll || k0 + SR > lo, have, k0, k, v);
+        if (active && st < end && k0 < hi) blocks(have != kAll || k0 + SR > lo, have, k0, k, v);
       };
-      for (int st = first; st < end; st += 2) {
-        stage(st, sK0, sV0, sK1, sV1);
-        if (st + 1 < end) stage(st + 1, sK1, sV1, sK0, sV0);
+      using std::integral_constant;
+      for (int st = first; st < end; st += 4) {
+        if constexpr (BUFS == 4) {
+          stage(integral_constant<int, 0>{}, st, sK0, sV0, sK3, sV3);
+          stage(integral_constant<int, 1>{}, st + 1, sK1, sV1, sK0, sV0);
+          stage(integral_constant<int, 2>{}, st + 2, sK2, sV2, sK1, sV1);
+          stage(integral_constant<int, 3>{}, st + 3, sK3, sV3, sK2, sV2);
+        } else {
+          stage(integral_constant<int, 0>{}, st, sK0, sV0, sK1, sV1);
+          stage(integral_constant<int, 1>{}, st + 1, sK1, sV1, sK0, sV0);
+          stage(integral_constant<int, 2>{}, st + 2, sK0, sV0, sK1, sV1);
+          stage(integral_constant<int, 3>{}, st + 3, sK1, sV1, sK0, sV0);
+        }
       }
     }
 
@@ -541,7 +589,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
         if (++b == p.B) return;
       } while (cu_at(p.cu, b + 1, p.T) <= cu_at(p.cu, b, p.T));
     }
-    lds_barrier();   // (the last stage has been read)
+    loads_barrier<0>();   // (the last stages have been read, and nothing is on its way to LDS)
   }
 }
 
