@@ -618,14 +618,35 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     if (row >= rows) break;
     auto at = [&](int i) { return ((int64_t)(2 * (w0 + i) + (i ? 0 : which)) * p.Hkv + kvh) * ROWS + row; };
     float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, p.stats[2 * at(i)]);
     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < n; ++i) {
-      const float mi = p.stats[2 * at(i)];
-      if (mi == -INFINITY) continue;
-      const float a = fmaxf(fast_exp2(mi - m), 0x1p-126f);   // (an infinite sum stays one)
-      l += a * p.stats[2 * at(i) + 1];
-      x += a * *reinterpret_cast<const f32x4*>(p.sums + at(i) * D + c);
+    constexpr int PER = 4;   // parts whose loads are on their way together
+    for (int i0 = 0; i0 < n; i0 += PER) {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+      f2 st[PER];
+      f32x4 y[PER];
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const int64_t a = at(i0 + u < n ? i0 + u : n - 1);
+        st[u] = *reinterpret_cast<const f2*>(p.stats + 2 * a);
+        y[u] = *reinterpret_cast<const f32x4*>(p.sums + a * D + c);
+      }
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) top = fmaxf(top, st[u][0]);
+      if (top == -INFINITY) continue;   // (such parts have seen nothing and have no sums)
+      const float keep = m == -INFINITY ? 0.f : fmaxf(fast_exp2(m - top), 0x1p-126f);   // (an infinite sum stays one)
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = m == -INFINITY ? 0.f : x[e] * keep;
+      m = top;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const bool in = i0 + u < n && st[u][0] != -INFINITY;
+        const float a = fmaxf(fast_exp2(st[u][0] - top), 0x1p-126f);
+        l += in ? a * st[u][1] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += in ? a * y[u][e] : 0.f;
+      }
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const int r = tile * ROWS + row;
