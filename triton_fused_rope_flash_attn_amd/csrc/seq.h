@@ -276,22 +276,33 @@ __device__ __forceinline__ SeqTile ordered_tile(const int* __restrict__ cu, int 
   return t;
 }
 // Stages of SR keys that a tile of queries [q0, end) reads: with a window (WIN) the ones that hold sinks,
-// then, `gap` further on, those of its rows' windows.
+// then those of its rows' windows.  These in an order that goes by their number modulo how many there are,
+// whatever the tile: tiles that run side by side, whose windows are shifted, then read the same keys at a time, which come
+// from L2 once they are there.
 template <bool WIN, int SR> struct KeyStages {
-  int n, sink, gap;
+  int n, sink, low, near, turn;
   __device__ __forceinline__ KeyStages(const SeqParams& p, int q0, int end, int len) {
     const int last = p.causal && end < len ? end : len;
     n = (last + SR - 1) / SR;
-    sink = gap = 0;
+    sink = low = turn = 0;
+    near = n;
     if constexpr (WIN) {
-      const int low = q0 + 1 > p.window ? q0 + 1 - p.window : 0;   // the first key of the first row's window
-      sink = ((p.sinks < low ? p.sinks : low) + SR - 1) / SR;
-      gap = low / SR > sink ? low / SR - sink : 0;
-      n -= gap;
+      const int from = q0 + 1 > p.window ? q0 + 1 - p.window : 0;   // the first key of the first row's window
+      sink = ((p.sinks < from ? p.sinks : from) + SR - 1) / SR;
+      low = from / SR > sink ? from / SR : sink;
+      near = n - low;
+      n = sink + near;
+      turn = near - low % near;
+      if (turn == near) turn = 0;
     }
   }
   // stage st of the tile: which of the sequence's
-  __device__ __forceinline__ int at(int st) const { return WIN && st >= sink ? st + gap : st; }
+  __device__ __forceinline__ int at(int st) const {
+    if (!WIN) return st;
+    if (st < sink) return st;
+    const int x = st - sink + turn;   // the one of the tile's last `near` whose number is st - sink modulo near
+    return low + (x < near ? x : x - near);
+  }
 };
 // Whether some key of [k0, k0 + n) is none that a row with the window [from, ..] sees
 __device__ __forceinline__ bool past_window(const SeqParams& p, int k0, int n, int from) { return k0 < from && k0 + n > p.sinks; }

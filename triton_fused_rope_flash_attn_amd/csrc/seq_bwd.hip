@@ -252,7 +252,7 @@ seq_dq_kernel(const SeqParams p) {
   auto sees = [&](int e, int lim, int k0) __attribute__((always_inline)) {
     return e < lim && (!WIN || e >= lim - p.window || e < p.sinks - k0 - 4 * lg);
   };
-  auto block = [&](bool tail, int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
+  auto block = [&](bool tail, bool edge, int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
     f32x4 sacc[QT][2], pacc[QT][2];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -280,8 +280,15 @@ seq_dq_kernel(const SeqParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float y = fast_exp2(sacc[t][h][i]) * pacc[t][h][i];
-          ds[4 * h + i] = !tail || sees(16 * h + i, lim, k0) ? y : 0.f;
+          ds[4 * h + i] = !tail || 16 * h + i < lim ? y : 0.f;
         }
+      if (WIN && edge) {
+        const int from = seen[t] - p.window - k0 - 4 * lg, sinks = p.sinks - k0 - 4 * lg;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ds[4 * h + i] = 16 * h + i >= from || 16 * h + i < sinks ? ds[4 * h + i] : 0.f;
+      }
       if constexpr (kFitDs<S>) {
         const float most = amax8(0.f, ds);
         if (__any(most > kDsMost)) {   // rows that pass it start again from 2^12
@@ -337,11 +344,11 @@ seq_dq_kernel(const SeqParams p) {
     }
     const int k0 = ks.at(st) * SR;
     if (active && k0 < hi && (!WIN || k0 + SR > w0 + 1 - p.window || k0 < p.sinks)) {
-      const bool tail = k0 + SR > lo || (WIN && past_window(p, k0, SR, hi - p.window));
+      const bool tail = k0 + SR > lo || sees_itself<WIN>(p), edge = WIN && past_window(p, k0, SR, hi - p.window);
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         if (WIN && sums) sum_block(k0 + 32 * j, k + 32 * j * D, v + 32 * j * D);
-        else block(tail, k0 + 32 * j, k + 32 * j * D, v + 32 * j * D);
+        else block(tail, edge, k0 + 32 * j, k + 32 * j * D, v + 32 * j * D);
       }
     }
     if (ROT && st + 1 < ns) rot.store(p, kn, tid);   // (read in the stage before this one)
@@ -430,7 +437,7 @@ seq_dq_kernel(const SeqParams p) {
       if (active) whole(k, v);
     } else if (active) {
 #pragma unroll 1
-      for (int j = 0; j < 2 * NB && 32 * j < hi; ++j) block(true, 32 * j, at_block(sK0, sK1, j), at_block(sV0, sV1, j));
+      for (int j = 0; j < 2 * NB && 32 * j < hi; ++j) block(true, false, 32 * j, at_block(sK0, sK1, j), at_block(sV0, sV1, j));
     }
     from = 2;
     if (ns > 2) {

@@ -203,7 +203,7 @@ seq_fwd_kernel(const SeqParams p) {
 
   // One stage's keys: the logit products, one test of the running max, then the
   // probabilities and O products of its 32-key blocks.
-  auto blocks = [&](bool tail, int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
+  auto blocks = [&](bool tail, bool edge, int k0, const S* __restrict__ k, const S* __restrict__ v) __attribute__((always_inline)) {
     f32x4 sacc[NB][QT][2];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -215,7 +215,7 @@ seq_fwd_kernel(const SeqParams p) {
 #pragma unroll
           for (int t = 0; t < QT; ++t) sacc[j][t][h] = C::mma(a, qf[t][s], s == 0 ? nm4[t] : sacc[j][t][h]);
         }
-    if (tail) {   // uniform: some row of the wave does not see all of these keys
+    if (tail) {   // uniform: some of these keys are behind a row of the wave
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         const int lim = seen[t] - k0 - 4 * lg;
@@ -224,10 +224,21 @@ seq_fwd_kernel(const SeqParams p) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
+            for (int i = 0; i < 4; ++i) sacc[j][t][h][i] = 32 * j + 16 * h + i < lim ? sacc[j][t][h][i] : -INFINITY;
+      }
+    }
+    if (WIN && edge) {   // uniform: some are before a row's window
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const int from = seen[t] - p.window - k0 - 4 * lg, sinks = p.sinks - k0 - 4 * lg;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int e = 32 * j + 16 * h + i;
-              const bool in = e < lim && (!WIN || e >= lim - p.window || e < p.sinks - k0 - 4 * lg);
-              sacc[j][t][h][i] = in ? sacc[j][t][h][i] : -INFINITY;
+              sacc[j][t][h][i] = e >= from || e < sinks ? sacc[j][t][h][i] : -INFINITY;
             }
       }
     }
@@ -296,9 +307,9 @@ seq_fwd_kernel(const SeqParams p) {
     const int k0 = ks.at(st) * SR;
     if constexpr (WIN) {   // (keys before all windows of the wave's rows, and some that are before one's)
       const bool seen_by_some = k0 < hi && (k0 + SR > w0 + 1 - p.window || k0 < p.sinks);
-      if (active && seen_by_some) blocks(k0 + SR > lo || past_window(p, k0, SR, hi - p.window), k0, k, v);
+      if (active && seen_by_some) blocks(k0 + SR > lo, past_window(p, k0, SR, hi - p.window), k0, k, v);
     } else {
-      if (active && k0 < hi) blocks(k0 + SR > lo, k0, k, v);
+      if (active && k0 < hi) blocks(k0 + SR > lo, false, k0, k, v);
     }
     if (ROT && st + 1 < ns) rot.store(p, kn, tid);   // (read in the stage before this one)
   };
