@@ -97,8 +97,8 @@ def test_c_workspaces():
     assert a == b                    # the forward's rows are the same
     none, _ = seq(128, 0)
     some, _ = seq(128, 65)
-    # 4096 / (128 + 128) = 16 parts of two tiles' sums, for K and V
-    assert some - none == 2 * 16 * 2 * 64 * 2 * 64
+    # the sinks' tiles have 2 heads of 65 stages; other tiles 8, in 4 parts of 2: 65 parts of two tiles' sums, for K and V
+    assert some - none == 2 * 65 * 2 * 64 * 2 * 64
     short, _ = seq(4000, 65)
     none, _ = seq(4000, 0)
     assert short == none             # the sinks' tiles have no more to do than others

@@ -99,11 +99,38 @@ struct SeqWs {
 // [264] 713 / 523 / 432, 1024, 4 [72] 181 / 129 / 105, 8 x 1024, 8 [1096] 208 / 239 / 311; D 64:
 // 2048, 2 [68] 204 / 138 / 105, 4 x 2048, 8 [1064] 180 / 179 / 196; D 256: 2 x 4096, 8 [1048] 1251 /
 // 1347 / 1525; fp32, D 64: 3 up to 257, 4 [44] 100 / 79 / 72.
+// With a window key tiles have like work, so the chip should end its last round of workgroups full: the parts with the
+// fewest stages one after the other, a part's sums, written and read, counted in stages too (at 4.9 TB/s, of 2.7 us).
+// Measured (us, forward and backward, 1 / 2 / 3 / 4 parts), D 128: 16384 tokens, 2 key heads, window 1024 450 / 475 / 498 / 506; fp32, D 64: 3 up
+// to 513, 4, window 100 149 / 105 / 90 / 86.
+int64_t dkdv_resident(const farope_seq_desc* d) {   // workgroups of seq_dkdv_kernel, by its registers and LDS
+  const int row = d->head_dim * elem_size(d->dtype);
+  return (int64_t)kCus * (d->dtype == FAROPE_F32 ? row <= 256 ? 2 : 1 : row <= 128 ? 4 : row == 256 ? 2 : 1);
+}
+int64_t window_stages(const farope_seq_desc* d, Window win) {
+  const int64_t mean = d->tokens / d->seqs;
+  return (int64_t)(d->heads / d->kv_heads) * ((mean < win.window ? mean : win.window) / 64 + 2);
+}
+int window_parts(const farope_seq_desc* d, Window win) {
+  // (tiles, not slots: a sequence ends half a tile before its last one's end)
+  const int64_t wgs = (d->tokens / 64 + (d->seqs + 1) / 2 * (d->seqs > 1)) * d->kv_heads, slots = dkdv_resident(d), stages = window_stages(d, win);
+  const double sums = (double)d->tokens * d->kv_heads * d->head_dim * 1.2e-6;
+  int best = 1;
+  double least = 0;
+  for (int parts = 1; parts <= kMaxParts && parts <= stages; ++parts) {
+    const int64_t rounds = (wgs * parts + slots - 1) / slots;
+    const double cost = (double)stages * (rounds < 1 ? 1 : rounds) / parts + (parts > 1 ? parts * sums : 0.);
+    if (parts == 1 || cost < least) {
+      best = parts;
+      least = cost;
+    }
+  }
+  return best;
+}
 int dkdv_parts(const farope_seq_desc* d, Window win) {
   const int64_t wgs = seq_slots(d->tokens, d->seqs, 6) * d->kv_heads;
-  int64_t rows = d->tokens / d->seqs;   // queries that see a key
-  if (win.window && rows > win.window) rows = win.window;
-  const int64_t stages = (int64_t)(d->heads / d->kv_heads) * (rows / 64 + 1);
+  if (win.window) return window_parts(d, win);
+  const int64_t stages = (int64_t)(d->heads / d->kv_heads) * (d->tokens / d->seqs / 64 + 1);
   int64_t parts = (4 * kCus + wgs / 2) / wgs;
   if (parts > kMaxParts) parts = kMaxParts;
   if (parts > stages) parts = stages;
@@ -123,13 +150,19 @@ bool rotates_itself(const farope_seq_desc* d, bool v_streams) {
   if (d->head_dim == 128) return d->tokens <= 128;
   return mean <= 128 || (mean <= 256 && d->tokens <= 1024);
 }
-// Key tiles with sinks, which every later query sees: parts of their queries, so that one has about the
-// work of another tile, whose queries are those of a window (0: they are not divided).
-constexpr int kMaxSinkParts = 64;
+// Key tiles with sinks, which every later query sees: where that is more than half as much again as other tiles have,
+// parts of their queries of 8 stages, or of a workgroup's for other tiles where these are fewer (0: they are not
+// divided).  Measured (us, forward and backward of 16384 tokens, 8 heads, 2 of keys, D 128, window 1024, 4 sinks):
+// parts as large as the other workgroups' and at the launch's front 504, of 16 stages and at its end 473, of 8 450.
+constexpr int kMaxSinkParts = 128;
 int sink_tiles(Window win) { return win.window ? (int)(((int64_t)win.sinks + 63) / 64) : 0; }
 int sink_parts(const farope_seq_desc* d, Window win) {
   if (!sink_tiles(win)) return 0;
-  const int64_t n = d->tokens / d->seqs / ((int64_t)win.window + 128);
+  const int64_t all = (int64_t)(d->heads / d->kv_heads) * (d->tokens / d->seqs / 64 + 1);
+  if (2 * all <= 3 * window_stages(d, win)) return 0;
+  int64_t part = window_stages(d, win) / window_parts(d, win);
+  part = part > 8 ? 8 : part < 1 ? 1 : part;
+  const int64_t n = (all + part - 1) / part;
   return n < 2 ? 0 : n < kMaxSinkParts ? (int)n : kMaxSinkParts;
 }
 int64_t sink_workgroups(const farope_seq_desc* d, Window win) {
@@ -254,7 +287,10 @@ int seq_bwd_call(const farope_seq_desc* desc, Window win, const void* q, const i
   FAROPE_TRY(check_ptr(dv, 16));
   FAROPE_TRY(check_ptr(ws, 16));
   const bool vs = streams(desc, v, v_stride), gs = streams(desc, dout, dout_stride);
-  if (seq_slots(desc->tokens, desc->seqs, 6) * desc->kv_heads * kMaxParts + sink_workgroups(desc, win) > INT32_MAX) return FAROPE_ERR_SHAPE;
+  // (with 64 tokens a workgroup of the tiles that hold sinks, where their sums are added)
+  if (seq_slots(desc->tokens, desc->seqs, 6) * desc->kv_heads * kMaxParts + sink_workgroups(desc, win) > INT32_MAX ||
+      (int64_t)desc->seqs * 64 * sink_tiles(win) * desc->kv_heads > kMaxWorkgroups)
+    return FAROPE_ERR_SHAPE;
   const SeqWs w = seq_ws(desc, true, vs, gs, win);
   if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
   SeqParams p{};

@@ -493,8 +493,8 @@ __device__ __forceinline__ int key_reach(const SeqParams& p, int len, int first,
 }
 
 // A workgroup's key tile, key head and part of the queries.  With a window all queries behind them see the sinks, so
-// their tiles have many times the others' work: the workgroups of the launch's front divide it into parts
-// of their own, and the others leave it to them.
+// their tiles have many times the others' work: workgroups of the launch's end divide it into parts
+// of their own, small ones that fill the chip while the last tiles are worked on, and the others leave it to them.
 template <bool WIN> struct KeyTile {
   SeqTile tl;
   int part, parts, kvh;
@@ -504,8 +504,9 @@ template <bool WIN> struct KeyTile {
     int id = block_id();
     sinks = false;
     if constexpr (WIN) {
-      const int front = p.B * p.sink_tiles * p.sink_parts * p.Hkv;
-      if (id < front) {
+      const int tiles = p.slots * p.Hkv * p.parts;
+      if (id >= tiles) {
+        id -= tiles;
         sinks = sums = true;
         parts = p.sink_parts;
         part = id % parts;
@@ -521,7 +522,6 @@ template <bool WIN> struct KeyTile {
         if (tl.tile >= tl.tiles) tl.tile = -1;
         return;
       }
-      id -= front;
     }
     parts = p.parts;
     sums = parts > 1;
@@ -999,23 +999,13 @@ __global__ void __launch_bounds__(256) seq_join_kernel(const SeqParams p) {
   float k[8] = {}, v[8] = {};
   const int64_t at = ((int64_t)t * p.Hkv + kvh) * D + c;
   const int start = cu_at(p.cu, b, p.T);
-  const bool sinks = WIN && p.sink_parts && b < p.B && t - start < 64 * p.sink_tiles;
-  if (WIN && !sinks && p.parts == 1) return;   // (complete)
+  if (WIN && p.sink_parts && b < p.B && t - start < 64 * p.sink_tiles) return;   // (sink_join_kernel's)
+  const int64_t step = (int64_t)p.T * p.Hkv * D;
   if (b < p.B) {
-    const float* pk = p.pk + at;
-    const float* pv = p.pv + at;
-    int64_t step = (int64_t)p.T * p.Hkv * D;
-    if (sinks) {
-      const int64_t from = (((int64_t)b * p.sink_tiles * 64 + t - start) * p.Hkv + kvh) * D + c;
-      pk = p.spk + from;
-      pv = p.spv + from;
-      step = (int64_t)p.B * p.sink_tiles * 64 * p.Hkv * D;
-    }
-    const int parts = sinks ? p.sink_parts : p.parts;
-    for (int i = 0; i < parts; ++i) {
+    for (int i = 0; i < p.parts; ++i) {
       float x[8], y[8];
-      load8<float>(pk + i * step, 1, true, x);
-      load8<float>(pv + i * step, 1, true, y);
+      load8<float>(p.pk + i * step + at, 1, true, x);
+      load8<float>(p.pv + i * step + at, 1, true, y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) { k[e] += x[e]; v[e] += y[e]; }
     }
@@ -1034,6 +1024,51 @@ __global__ void __launch_bounds__(256) seq_join_kernel(const SeqParams p) {
   put_row8<S>(static_cast<S*>(p.dv) + at, v);
 }
 
+// The same of the tiles with sinks, whose parts are many: a workgroup takes one token and key head, its threads 8 channels
+// of every so manieth part, and the threads' sums are added in order.
+template <typename S, int D>
+__global__ void __launch_bounds__(256) sink_join_kernel(const SeqParams p) {
+  constexpr int CPR = D / 8, L = 256 / CPR;
+  __shared__ __attribute__((aligned(16))) float sums[2][L][D];
+  const int tid = thread_id(), c = 8 * (tid % CPR), l = tid / CPR;
+  const int kvh = block_id() % p.Hkv, at = block_id() / p.Hkv, rows = 64 * p.sink_tiles, b = at / rows, j = at % rows;
+  const int start = cu_at(p.cu, b, p.T), len = cu_at(p.cu, b + 1, p.T) - start;
+  if (j >= len) return;
+  float k[8] = {}, v[8] = {};
+  const int64_t step = (int64_t)p.B * rows * p.Hkv * D, from = ((int64_t)at * p.Hkv + kvh) * D + c;
+  for (int i = l; i < p.sink_parts; i += L) {
+    float x[8], y[8];
+    load8<float>(p.spk + i * step + from, 1, true, x);
+    load8<float>(p.spv + i * step + from, 1, true, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { k[e] += x[e]; v[e] += y[e]; }
+  }
+  put_row8<float>(&sums[0][l][c], k);
+  put_row8<float>(&sums[1][l][c], v);
+  lds_barrier();
+  if (l >= 2) return;
+  float x[8] = {};
+  for (int i = 0; i < L; ++i) {
+    float y[8];
+    load8<float>(&sums[l][i][c], 1, true, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += y[e];
+  }
+  const int64_t t = start + j, to = (t * p.Hkv + kvh) * D + c;
+  if (l == 0) {
+    const float factor = dk_factor<true>(p, len);
+    float cs[8];
+    table_load4(p.cosp, p.sinp, table_row(p.positions ? p.positions[t] : j - p.has_cls, p.n_pos), D / 2, c / 2, cs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float e = x[2 * i] * factor, o = x[2 * i + 1] * factor;
+      x[2 * i] = e * cs[2 * i] + o * cs[2 * i + 1];
+      x[2 * i + 1] = o * cs[2 * i] - e * cs[2 * i + 1];
+    }
+  }
+  put_row8<S>(static_cast<S*>(l ? p.dv : p.dk) + to, x);
+}
+
 template <typename S, int D, int QT, bool ROT>
 static hipError_t dq(const SeqParams& p0, hipStream_t st) {
   SeqParams p = p0;
@@ -1050,10 +1085,16 @@ static hipError_t dkdv(const SeqParams& p, hipStream_t st) {
     hipLaunchKernelGGL((seq_dkdv_shared_kernel<S, WIN>), grid, dim3(kSeqThreads), 0, st, p);
   else
     hipLaunchKernelGGL((seq_dkdv_kernel<S, D, WIN>), grid, dim3(kSeqThreads), 0, st, p);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || (p.parts == 1 && !(WIN && p.sink_parts))) return e;
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
   constexpr int rows = 256 / (D / 8);
-  hipLaunchKernelGGL((seq_join_kernel<S, D, WIN>), dim3((unsigned)((p.T + rows - 1) / rows) * p.Hkv), dim3(256), 0, st, p);
+  if (p.parts > 1)
+    hipLaunchKernelGGL((seq_join_kernel<S, D, WIN>), dim3((unsigned)((p.T + rows - 1) / rows) * p.Hkv), dim3(256), 0, st, p);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if constexpr (WIN)
+    if (p.sink_parts)
+      hipLaunchKernelGGL((sink_join_kernel<S, D>), dim3((unsigned)p.B * 64u * (unsigned)p.sink_tiles * p.Hkv), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 template <typename S, int D>
