@@ -3,7 +3,9 @@
 // sequences, sharing, copying, reserving and freeing pages.
 //
 // Both are copies of whole rows and bound by memory, small calls by the round
-// trips of their page numbers and by the launches.
+// trips of their page numbers and by the launches.  Measured (us a call): accepted tokens of one tree of 8, 12 heads, D 64
+// 5.7, of 128 trees of 64, 8 heads, D 128 7.7; 4 places of one prompt forked 9.8, 256 places, 8 a prompt, pages of 128
+// rows, 8 heads, D 128, fp16 35 (122 MB read and written, 3.5 TB/s with both launches).
 #include "seq.h"
 
 namespace farope {

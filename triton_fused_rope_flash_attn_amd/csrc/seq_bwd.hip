@@ -10,6 +10,10 @@
 //   seq_dq_kernel     query tiles: dQ; also -delta, -LSE * log2 e and the rotated Q rows (fp16, D 128: dO's norms)
 //   seq_dkdv_kernel   key tiles: dK, dV, one pass over the group's query heads, so the
 //                     sums of shared key heads stay in registers and in one order
+// With a window (WIN) a key tile's queries end with its last key's window, but for tiles with sinks, whose queries
+// are divided (KeyTile) and joined by sink_join_kernel; and rows that see 64 keys at most, which may be anywhere, have their
+// delta from a pass of its own over the tile's keys (two of its four products: one of 16384 tokens, 8 heads, D 128, window
+// 1024: dQ 166 us, dK/dV 218).
 // Both tile kernels stream their rows as the forward does (seq_fwd.hip).  No row of a
 // sequence reads another's: streams end at the sequence's last row.
 //

@@ -7,20 +7,27 @@
 //
 // A key head's query rows (tokens times the heads of its group, head fastest) are taken in tiles of
 // 64 or 128, whose 4 waves have 16 or 32 of them each, and the cache's rows in stages, gathered through the page
-// table from memory straight to LDS, double-buffered, one barrier a stage.  The stages of all tiles of all
+// table from memory straight to LDS, three stages ahead, one barrier a stage.  The stages of all tiles of all
 // sequences are divided evenly over the workers (workgroups) of a key head, as in decode.hip: a
 // worker's share may end inside a tile and run on in the next; of tiles that several workers share
 // these leave unnormalised sums, which tree_join_kernel joins.
 //
 // Few rows are bound by memory (the cache is read once a tile), many by the issue of matrix and vector
-// instructions, as the forward over packed sequences.
+// instructions and by the last-level cache, from which every tile has its rows.  Measured (us a call, both launches): 32
+// sequences up to 8192 rows with up to 32 drafted tokens, 32 heads of 8, D 128, bf16 150 (497 MB; without the
+// products 122); 4 up to 8192 with up to 1024 new tokens, fp16 330 (670 TFLOP/s; without 205); one of 1024
+// with 8, 12 heads, D 64 14.6, the chain of lengths, page numbers, rows and the join.
+//
+// 16-bit tensors: q-hat (with the scale) and P are rounded once to their type, as the products' operands; with O's own
+// rounding that leaves 2.8e-3 of O's norm in bf16 (the storing alone 1.7e-3).
 #include <type_traits>
 
 #include "seq.h"
 
 namespace farope {
 
-// Rows of a stage and stages in LDS: three are on their way while one is read, but for rows of 1 KB.
+// Rows of a stage and stages in LDS: three are on their way while one is read, but for rows of 1 KB.  (One stage of 64 rows
+// on its way: 152 us and 337 for the first two calls above; two stages and three workgroups a CU 158 and 340.)
 template <typename S, int D> constexpr int kTreeRows = D * sizeof(S) <= 128 ? 64 : 32;
 template <typename S, int D> constexpr int kTreeBufs = D * sizeof(S) <= 512 ? 4 : 2;
 
