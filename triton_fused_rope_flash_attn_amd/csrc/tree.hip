@@ -493,6 +493,10 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
       }
     }
 
+    // The loads of the stages behind the end have landed: none is on its way to LDS when a workgroup ends, and another has its LDS.
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+    asm volatile("" : : : "memory");
+
     const bool whole = first == 0 && stages == s.blocks;   // the tile is this worker's alone
     {
     const int lane = fresh(tid & 63), lr = lane & 15, lg = lane >> 4, row0 = wave * 16 * QT + lr;
@@ -596,7 +600,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
         if (++b == p.B) return;
       } while (cu_at(p.cu, b + 1, p.T) <= cu_at(p.cu, b, p.T));
     }
-    loads_barrier<0>();   // (the last stages have been read, and nothing is on its way to LDS)
+    loads_barrier<0>();   // (the last stages have been read)
   }
 }
 
