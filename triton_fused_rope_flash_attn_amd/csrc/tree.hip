@@ -325,8 +325,10 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) ids[i] = fetch(first + i);
       rows_in[0] = load(ids[0], sK0, sV0);
-      if constexpr (AHEAD > 1) {
+      if constexpr (AHEAD > 1) {   // (one stage's loads after the other's: the waits count on it)
+        asm volatile("" : : : "memory");
         rows_in[1] = load(ids[1], sK1, sV1);
+        asm volatile("" : : : "memory");
         rows_in[2] = load(ids[2], sK2, sV2);
       }
 #pragma unroll
