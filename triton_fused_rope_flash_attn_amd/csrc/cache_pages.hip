@@ -4,8 +4,8 @@
 //
 // Both are copies of whole rows and bound by memory, small calls by the round
 // trips of their page numbers and by the launches.  Measured (us a call): accepted tokens of one tree of 8, 12 heads, D 64
-// 5.7, of 128 trees of 64, 8 heads, D 128 7.7; 4 places of one prompt forked 9.8, 256 places, 8 a prompt, pages of 128
-// rows, 8 heads, D 128, fp16 35 (122 MB read and written, 3.5 TB/s with both launches).
+// 5.7, of 128 trees of 64, 8 heads, D 128 7.7; 4 places of one prompt forked 8.9, 256 places, 8 a prompt, pages of 128
+// rows, 8 heads, D 128, fp16 27 (122 MB read and written, 4.5 TB/s with both launches).
 #include "seq.h"
 
 namespace farope {
@@ -179,7 +179,9 @@ __device__ __forceinline__ int find_free(const ForkParams& p, int rank, int lane
   return chunk * kForkChunk + 64 * l + __builtin_ctzll(bits);
 }
 
-constexpr int kCopyChunks = 8;   // 16-byte chunks a thread copies
+// 16-byte chunks a thread copies.  Each workgroup finds its place's page by itself, a chain of dependent
+// reads, so few workgroups with much to copy are better: 8 chunks take 35 us for the 256 places above, 16 take 27.
+constexpr int kCopyChunks = 16;
 
 __global__ void __launch_bounds__(256) cache_fork_kernel(const ForkParams p, int copies) {
   __shared__ int share[4];
@@ -188,7 +190,10 @@ __global__ void __launch_bounds__(256) cache_fork_kernel(const ForkParams p, int
   const bool tables = block_id() < p.B;
   const int b = tables ? block_id() : (block_id() - p.B) / copies;
   const int src = p.from[b];
-  if (!tables && src < 0) return;
+  const int n = p.len[b], row_chunks = p.Hkv * p.cpr;
+  const int64_t all = (int64_t)(n % p.c.page) * row_chunks;   // 16-byte chunks of one cache to be copied
+  const int64_t at = (int64_t)(tables ? 0 : (block_id() - p.B) % copies) * (256 * kCopyChunks) + tid;
+  if (!tables && (src < 0 || at - tid >= 2 * all)) return;
   int first = 0;   // pages that the places before want
   for (int i = tid; i < b; i += 256) first += p.wanted[i];
   first = block_sum(first, share, tid);
@@ -196,9 +201,6 @@ __global__ void __launch_bounds__(256) cache_fork_kernel(const ForkParams p, int
   if (!tables) {
     const int dst = find_free(p, first, lane);   // (entry `full` is the first that wants one)
     if (dst < 0) return;
-    const int n = p.len[b], rows = n % p.c.page, row_chunks = p.Hkv * p.cpr;
-    const int64_t all = (int64_t)rows * row_chunks;
-    const int64_t at = (int64_t)((block_id() - p.B) % copies) * (256 * kCopyChunks) + tid;
     u32x4 x[kCopyChunks];
     int64_t to[kCopyChunks];
 #pragma unroll
