@@ -413,14 +413,23 @@ int decode_call(const farope_seq_desc* desc, int32_t window, int32_t sinks, cons
 // Several new tokens per sequence over a cache (tree.hip).  The host knows the sequences' number, their
 // mean of new tokens and their room alone.
 int tree_group(const farope_seq_desc* d) { return d->heads / d->kv_heads; }
+// Rows of a tile: 128 read the cache half as often, once a sequence's rows do not fit 64.  Measured, us with 64 and
+// with 128 (32 sequences of 8192 rows, 32 heads of 8, D 128, bf16): 16 new tokens each (64 rows) 243, 249; 20 279, 250;
+// 32 283, 256; 48 638, 345.
 int tree_rows(const farope_seq_desc* d) {
   return d->dtype != FAROPE_F32 && (int64_t)d->tokens * tree_group(d) / d->seqs > 64 ? 128 : 64;
 }
 int64_t tree_slots(const farope_seq_desc* d) { return (int64_t)d->tokens * tree_group(d) / tree_rows(d) + d->seqs + 1; }
 int tree_stage(const farope_seq_desc* d) { return d->head_dim * elem_size(d->dtype) <= 128 ? 64 : 32; }   // (kTreeRows of tree.hip)
+// A workgroup a tile instead of even shares and a join: where sequences are short their lengths differ by little, and
+// the join's launch is what costs.  Measured, us with shares and alone (8 new tokens, 12 heads, D 64, bf16): one sequence of
+// 120 rows 12.4, 9.2, of 500 13.4, 12.9, of 1000 14.4, 18.9; 64 of 500 43, 32.  32 new tokens, 32 heads of 8, D 128: 32 of 480
+// 43, 34, but 64 of 250 41, 51 (a second round of workgroups, mostly their starts); 32 of unlike lengths up to 8192 150, 254.
 bool tree_direct(const farope_seq_desc* d, const farope_cache_desc* c) {
   return (int64_t)c->max_pages * c->page_rows <= 512;
 }
+// Workgroups of a key head: one resident round.  Measured, us with half of it, all, two (32 heads of 8, D 128, bf16): 8
+// sequences of 4096 rows, 16 new tokens 50, 48, 61; 32 of 8192, 32 new 264, 259, 289.
 int tree_workers(const farope_seq_desc* d, const farope_cache_desc* c) {
   const int64_t room = ((int64_t)c->max_pages * c->page_rows + tree_stage(d) - 1) / tree_stage(d);
   const int64_t wgs = (int64_t)kCus * (d->head_dim * elem_size(d->dtype) <= 256 ? 2 : 1);
