@@ -4,8 +4,8 @@
 //
 // Both are copies of whole rows and bound by memory, small calls by the round
 // trips of their page numbers and by the launches.  Measured (us a call): accepted tokens of one tree of 8, 12 heads, D 64
-// 5.7, of 128 trees of 64, 8 heads, D 128 7.7; 4 places of one prompt forked 8.9, 256 places, 8 a prompt, pages of 128
-// rows, 8 heads, D 128, fp16 27 (122 MB read and written, 4.5 TB/s with both launches).
+// 5.7, of 128 trees of 64, 8 heads, D 128 7.7; 4 places of one prompt forked 9 to 10, 256 places, 8 a prompt, pages of 128
+// rows, 8 heads, D 128, fp16 26 to 27 (122 MB read and written, 4.6 TB/s with both launches).
 #include "seq.h"
 
 namespace farope {
@@ -180,7 +180,8 @@ __device__ __forceinline__ int find_free(const ForkParams& p, int rank, int lane
 }
 
 // 16-byte chunks a thread copies.  Each workgroup finds its place's page by itself, a chain of dependent
-// reads, so few workgroups with much to copy are better: 8 chunks take 35 us for the 256 places above, 16 take 27.
+// reads, so few workgroups with much to copy are better: 8 chunks take 35 us for the 256 places above, 16 take 26 to 27
+// (the 4 places: no difference).
 constexpr int kCopyChunks = 16;
 
 __global__ void __launch_bounds__(256) cache_fork_kernel(const ForkParams p, int copies) {
