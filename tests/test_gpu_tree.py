@@ -398,6 +398,31 @@ def test_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(out, step())), i
 
 
+def test_two_graphs_at_once():
+    """Each has partial sums of its own: replayed on two streams together they give what each gives alone."""
+    page, D = 16, 64
+    table = seq_ref.Table(2100, D, DEV)
+    sides = []
+    for seed in (1, 2):
+        pages, n = page_table(2, 130, seed=seed)
+        kc, vc = caches(n, page, 2, D, BF16)
+        q = randn(40, 8, D, dtype=BF16, seed=seed)
+        args = (q, kc, vc, table, pages, ints([2000, 300 * seed]), ints([0, 30, 40]))
+        want, stream, graph = sdpa_rope_tree(*args), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            out = sdpa_rope_tree(*args)
+        sides.append((want, stream, graph, out, args))
+    for _ in range(5):
+        torch.cuda.synchronize()
+        for _, stream, graph, out, _ in sides:
+            with torch.cuda.stream(stream):
+                out.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for want, _, _, out, _ in sides)
+
+
 def test_another_stream():
     page, D = 16, 128
     pages, n = page_table(2, 100)
