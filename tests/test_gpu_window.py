@@ -538,3 +538,17 @@ def test_decode_opcheck_and_gradients_refused():
     torch.library.opcheck(torch.ops.farope.cache_attn_window.default, (q, kc, vc, *table.tables(), pages, ints([40, 3]), None, True, 0.125, 9, 2))
     with pytest.raises(RuntimeError, match="no autograd formula"):
         sdpa_rope_decode(q.requires_grad_(), kc, vc, table, pages, ints([40, 3]), window=9).sum().backward()
+
+
+# ---------------------------------------------------------------------------
+# sinks as many as tokens, ragged packs
+# ---------------------------------------------------------------------------
+def test_many_short_sequences_with_more_sinks_than_tokens():
+    """Their key tiles all hold sinks; the backward takes what the forward does."""
+    rng = random.Random(6)
+    lens = [rng.choice([1, 20, 30, 40, 65]) for _ in range(300)]
+    q, k, v, do = inputs(sum(lens), 8, 8, 32, BF16, seed=4)
+    table = seq_ref.Table(65, 32, DEV)
+    for window, sinks in ((8, 2 ** 31 - 1), (8, 20)):
+        got = grads(q, k, v, do, table, starts(lens), window=window, sinks=sinks)
+        compare(f"300 sequences, {sinks} sinks", got, varlen(q, k, v, do, table, starts(lens), window, sinks), BF16)

@@ -112,3 +112,20 @@ def test_c_workspaces():
     assert decode(0, 0)[0] == 0 and decode(100, 4)[0] == 0 and decode(100, 4)[1] > 0   # (a worker a sequence)
     assert decode(16000, 0)[0] == decode(16000, 0)[1]
     assert 0 < decode(2000, 4)[0] < decode(16000, 0)[1]
+
+
+# (the divided form of the sinks' tiles fits no launch, or is not taken: that is no reason to refuse)
+@pytest.mark.parametrize("window,sinks,kw", [
+    (128, 4096, dict(tokens=65536, seqs=256, heads=16, kv_heads=16)),
+    (64, 4, dict(tokens=300000, seqs=40000, heads=8, kv_heads=8)),
+    (64, 1024, dict(tokens=262144, seqs=4096, heads=8, kv_heads=8)),
+    (512, 2 ** 31 - 1, dict(tokens=65536, seqs=16, heads=16, kv_heads=16)),
+    (64, 4, dict(tokens=24000000, seqs=40000, heads=8, kv_heads=8, head_dim=32)),
+    (2, 1, dict(tokens=16000000, seqs=260000, heads=1, kv_heads=1)),
+])
+def test_the_backward_takes_what_the_forward_takes(window, sinks, kw):
+    """(nothing is launched: the forward's LSE is not aligned, the backward's workspace too short; both are looked at after the sizes)"""
+    lib, s, d = _lib.load(), (ctypes.c_int64 * 3)(8, 8, 1), _desc(**{**dict(n_pos=10), **kw})
+    fwd = lib.farope_seq_window_fwd(ctypes.byref(d), window, sinks, 16, s, 16, s, 16, s, 16, 16, None, 4, 16, 6, 16, 1, None)
+    bwd = lib.farope_seq_window_bwd(ctypes.byref(d), window, sinks, 16, s, 16, s, 16, s, 16, 16, s, 4, 16, 16, None, 4, 16, 16, 16, 16, 1, None)
+    assert (fwd, bwd) == (_lib.ERR_ALIGN, _lib.ERR_SCRATCH)

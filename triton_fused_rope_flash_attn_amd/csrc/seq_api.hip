@@ -111,6 +111,11 @@ int64_t window_stages(const farope_seq_desc* d, Window win) {
   const int64_t mean = d->tokens / d->seqs;
   return (int64_t)(d->heads / d->kv_heads) * ((mean < win.window ? mean : win.window) / 64 + 2);
 }
+// Parts of the key tiles' queries that the launches of seq_dkdv_kernel and seq_join_kernel hold.
+bool parts_fit(const farope_seq_desc* d, int64_t parts) {
+  return seq_slots(d->tokens, d->seqs, 6) * d->kv_heads * parts <= kMaxWorkgroups &&
+         ((int64_t)d->tokens * d->head_dim / 2048 + 1) * d->kv_heads <= kMaxWorkgroups;
+}
 int window_parts(const farope_seq_desc* d, Window win) {
   // (tiles, not slots: a sequence ends half a tile before its last one's end)
   const int64_t wgs = (d->tokens / 64 + (d->seqs + 1) / 2 * (d->seqs > 1)) * d->kv_heads, slots = dkdv_resident(d), stages = window_stages(d, win);
@@ -118,6 +123,7 @@ int window_parts(const farope_seq_desc* d, Window win) {
   int best = 1;
   double least = 0;
   for (int parts = 1; parts <= kMaxParts && parts <= stages; ++parts) {
+    if (parts > 1 && !parts_fit(d, parts)) break;
     const int64_t rounds = (wgs * parts + slots - 1) / slots;
     const double cost = (double)stages * (rounds < 1 ? 1 : rounds) / parts + (parts > 1 ? parts * sums : 0.);
     if (parts == 1 || cost < least) {
@@ -162,8 +168,12 @@ int sink_parts(const farope_seq_desc* d, Window win) {
   if (2 * all <= 3 * window_stages(d, win)) return 0;
   int64_t part = window_stages(d, win) / window_parts(d, win);
   part = part > 8 ? 8 : part < 1 ? 1 : part;
-  const int64_t n = (all + part - 1) / part;
-  return n < 2 ? 0 : n < kMaxSinkParts ? (int)n : kMaxSinkParts;
+  int64_t n = (all + part - 1) / part;
+  if (n > kMaxSinkParts) n = kMaxSinkParts;
+  // (and where the launches do not hold them: sink_join_kernel has a workgroup a token of these tiles)
+  const int64_t tiles = (int64_t)d->seqs * sink_tiles(win) * d->kv_heads;
+  const int64_t others = seq_slots(d->tokens, d->seqs, 6) * d->kv_heads * window_parts(d, win);
+  return n < 2 || 64 * tiles > kMaxWorkgroups || others + tiles * n > kMaxWorkgroups ? 0 : (int)n;
 }
 int64_t sink_workgroups(const farope_seq_desc* d, Window win) {
   return (int64_t)d->seqs * sink_tiles(win) * sink_parts(d, win) * d->kv_heads;
@@ -287,10 +297,6 @@ int seq_bwd_call(const farope_seq_desc* desc, Window win, const void* q, const i
   FAROPE_TRY(check_ptr(dv, 16));
   FAROPE_TRY(check_ptr(ws, 16));
   const bool vs = streams(desc, v, v_stride), gs = streams(desc, dout, dout_stride);
-  // (with 64 tokens a workgroup of the tiles that hold sinks, where their sums are added)
-  if (seq_slots(desc->tokens, desc->seqs, 6) * desc->kv_heads * kMaxParts + sink_workgroups(desc, win) > INT32_MAX ||
-      (int64_t)desc->seqs * 64 * sink_tiles(win) * desc->kv_heads > kMaxWorkgroups)
-    return FAROPE_ERR_SHAPE;
   const SeqWs w = seq_ws(desc, true, vs, gs, win);
   if ((int64_t)ws_elems < w.total) return FAROPE_ERR_SCRATCH;
   SeqParams p{};
