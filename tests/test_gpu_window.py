@@ -552,3 +552,13 @@ def test_many_short_sequences_with_more_sinks_than_tokens():
     for window, sinks in ((8, 2 ** 31 - 1), (8, 20)):
         got = grads(q, k, v, do, table, starts(lens), window=window, sinks=sinks)
         compare(f"300 sequences, {sinks} sinks", got, varlen(q, k, v, do, table, starts(lens), window, sinks), BF16)
+
+
+@pytest.mark.parametrize("lens,H,Hkv,window,sinks", [([3000, 2800], 2, 2, 100, 600), ([4000], 4, 1, 70, 3000), ([2500] + [50] * 40, 4, 2, 90, 3),
+                                                     ([900] * 6, 16, 16, 64, 70)])
+def test_many_sinks_and_ragged_packs(lens, H, Hkv, window, sinks):
+    """Sinks over many key tiles, in few parts or undivided, and of one long sequence beside many short ones."""
+    q, k, v, do = inputs(sum(lens), H, Hkv, 64, BF16, seed=9)
+    table = seq_ref.Table(max(lens), 64, DEV)
+    got = grads(q, k, v, do, table, starts(lens), window=window, sinks=sinks)
+    compare(f"{len(lens)} up to {max(lens)}, {sinks} sinks", got, varlen(q, k, v, do, table, starts(lens), window, sinks), BF16)

@@ -129,3 +129,16 @@ def test_the_backward_takes_what_the_forward_takes(window, sinks, kw):
     fwd = lib.farope_seq_window_fwd(ctypes.byref(d), window, sinks, 16, s, 16, s, 16, s, 16, 16, None, 4, 16, 6, 16, 1, None)
     bwd = lib.farope_seq_window_bwd(ctypes.byref(d), window, sinks, 16, s, 16, s, 16, s, 16, 16, s, 4, 16, 16, None, 4, 16, 16, 16, 16, 1, None)
     assert (fwd, bwd) == (_lib.ERR_ALIGN, _lib.ERR_SCRATCH)
+
+
+@pytest.mark.parametrize("dtype,D", [(_lib.BF16, 32), (_lib.F16, 64), (_lib.BF16, 128), (_lib.F16, 256), (_lib.F32, 64), (_lib.F32, 256)])
+@pytest.mark.parametrize("tokens,seqs,heads,kv,window,sinks", [
+    (16384, 1, 32, 8, 1024, 4), (16384, 1, 32, 8, 1024, 1024), (16384, 1, 32, 8, 1024, 4096), (131072, 32, 32, 8, 512, 2048),
+    (16384, 8, 32, 8, 512, 1024), (131072, 8, 32, 8, 1024, 4), (65536, 64, 8, 8, 64, 4), (65536, 16, 16, 16, 512, 2 ** 31 - 1),
+])
+def test_many_sinks_need_no_more_workspace(dtype, D, tokens, seqs, heads, kv, window, sinks):
+    """The sinks' sums are those of one resident round of workgroups at most, 2 * 64 * D each: 32 MB whatever the call."""
+    lib = _lib.load()
+    d = _desc(tokens=tokens, seqs=seqs, heads=heads, kv_heads=kv, head_dim=D, dtype=dtype, n_pos=10)
+    with_, none = (lib.farope_seq_window_workspace_elems(ctypes.byref(d), window, s, 1, 1, 1) for s in (sinks, 0))
+    assert 0 <= (with_ - none) * 4 <= 32 << 20

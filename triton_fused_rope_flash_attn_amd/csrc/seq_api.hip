@@ -160,6 +160,11 @@ bool rotates_itself(const farope_seq_desc* d, bool v_streams) {
 // parts of their queries of 8 stages, or of a workgroup's for other tiles where these are fewer (0: they are not
 // divided).  Measured (us, forward and backward of 16384 tokens, 8 heads, 2 of keys, D 128, window 1024, 4 sinks):
 // parts as large as the other workgroups' and at the launch's front 504, of 16 stages and at its end 473, of 8 450.
+// No more parts than one resident round of workgroups: many tiles fill the chip by themselves, and each part has its sums,
+// 2 * 64 * D in fp32, in the workspace, 32 MB of them at most.  Measured (us, one round / two / four / no such bound; 32 heads, 8 of
+// keys, D 128): 16384 tokens, window 1024, 4 sinks 1557 / 1554 / 1555 / 1551, 1024 2501 / 2535 / 2588 / 3072, 4096 4970 / 5026 /
+// 5096 / 7575; 32 x 4096, window 512, 256 sinks 9416 / 9470 / 9211 / 10230, 2048 18200 / 18200 / 18240 / 28000; 64 x 1024, 8 heads, D 64,
+// window 64, 4 sinks 473 / 481 / 491 / 492.
 constexpr int kMaxSinkParts = 128;
 int sink_tiles(Window win) { return win.window ? (int)(((int64_t)win.sinks + 63) / 64) : 0; }
 int sink_parts(const farope_seq_desc* d, Window win) {
@@ -170,8 +175,9 @@ int sink_parts(const farope_seq_desc* d, Window win) {
   part = part > 8 ? 8 : part < 1 ? 1 : part;
   int64_t n = (all + part - 1) / part;
   if (n > kMaxSinkParts) n = kMaxSinkParts;
-  // (and where the launches do not hold them: sink_join_kernel has a workgroup a token of these tiles)
   const int64_t tiles = (int64_t)d->seqs * sink_tiles(win) * d->kv_heads;
+  if (n > dkdv_resident(d) / tiles) n = dkdv_resident(d) / tiles;
+  // (and where the launches do not hold them: sink_join_kernel has a workgroup a token of these tiles)
   const int64_t others = seq_slots(d->tokens, d->seqs, 6) * d->kv_heads * window_parts(d, win);
   return n < 2 || 64 * tiles > kMaxWorkgroups || others + tiles * n > kMaxWorkgroups ? 0 : (int)n;
 }
