@@ -562,3 +562,43 @@ def test_many_sinks_and_ragged_packs(lens, H, Hkv, window, sinks):
     table = seq_ref.Table(max(lens), 64, DEV)
     got = grads(q, k, v, do, table, starts(lens), window=window, sinks=sinks)
     compare(f"{len(lens)} up to {max(lens)}, {sinks} sinks", got, varlen(q, k, v, do, table, starts(lens), window, sinks), BF16)
+
+
+@pytest.mark.parametrize("dtype,D,H,Hkv,lens", [(BF16, 64, 2, 1, [300, 200]), (BF16, 128, 4, 2, [700, 130]), (F16, 128, 4, 4, [700, 130]),
+                                                (F16, 64, 4, 2, [1700, 30]), (BF16, 256, 2, 1, [500]), (F32, 64, 2, 1, [400, 33]),
+                                                (BF16, 32, 16, 16, [1300, 600]), (F32, 128, 2, 2, [400]),
+                                                # (key tiles with sinks that are not divided)
+                                                (BF16, 128, 16, 16, [330] * 33), (F16, 64, 32, 32, [330] * 33)])
+@pytest.mark.parametrize("what", ["dO", "Q"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_gradients_do_not_feel_rows_far_from_theirs(dtype, D, H, Hkv, lens, what, value):
+    """dO or Q of a token that is not finite reach dK and dV of the keys that it sees, and none whose own queries all are more than
+    126 tokens from it: not those in a tile with the sinks either."""
+    window, sinks = 50, 2
+    q, k, v, do = inputs(sum(lens), H, Hkv, D, dtype, seed=17)
+    table, cu = seq_ref.Table(max(lens), D, DEV), starts(lens)
+    clean = grads(q, k, v, do, table, cu, window=window, sinks=sinks)
+    bad_q, bad_do = q.clone(), do.clone()
+    sees, near = (torch.zeros(sum(lens), dtype=torch.bool) for _ in range(2))
+    for a, n in zip(cu.tolist(), lens):
+        i = n - 20
+        (bad_q if what == "Q" else bad_do)[a + i] = value
+        seen = visible(n, window, sinks)
+        sees[a:a + n] = seen[i]
+        near[a:a + n] = seen[max(0, i - 126):i + 127].any(0)
+    got = grads(bad_q, k, v, bad_do, table, cu, window=window, sinks=sinks)
+    sees, far = sees.to(DEV), ~near.to(DEV)
+    assert far.sum() > 60
+    for name in ("dk", "dv"):
+        assert torch.isfinite(got[name][far]).all(), name
+        units = seq_ref.FP32_UNITS if dtype == F32 else seq_ref.ROUNDINGS
+        tol = 4 * units[name] * seq_ref.U[dtype]
+        off = (got[name][far].double() - clean[name][far].double()).norm(dim=-1)
+        size = clean[name][far].double().norm(dim=-1)
+        assert (off <= tol * (size + clean[name].double().norm(dim=-1).square().mean().sqrt())).all(), name
+        if value != value:
+            assert not torch.isfinite(got[name][sees]).any(), name
+    rest = torch.ones(sum(lens), dtype=torch.bool, device=DEV)
+    for a, n in zip(cu.tolist(), lens):
+        rest[a + n - 20] = False
+    assert torch.isfinite(got["dq"][rest]).all()

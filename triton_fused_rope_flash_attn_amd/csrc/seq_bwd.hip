@@ -542,6 +542,28 @@ template <bool WIN> struct KeyTile {
   }
 };
 
+// The order of a key tile's stages of queries: head by head, the last queries first, as far back as the tile's first key when
+// causal.  (Every tile of a sequence then begins with the same rows, which come from L2.  Measured (us, forward and backward,
+// first / last queries first): 16 sequences up to 2048 tokens, 16 heads (4 of keys), D 64 406 / 390, 64 up to 577, 12
+// 143 / 140, 8 x 1024, 8, D 128 159 / 156, one sequence of 16384 2510 / 2494 (HBM reads of the kernel 1716 / 419 MB).)
+// With a window the far queries, which see of the tile's keys the sinks alone, come first in all heads: behind them the sums of
+// the other keys, of weights that are 0, begin again from 0 (drop).  A query that is not finite, far from every query that sees such
+// a key, so does not reach it as 0 * NaN.  (What this costs, us without / with, window 1024 or 512, 4 sinks, D 64 267 / 269, D 128 457 / 456,
+// fp32 892 / 903, D 256 3635 / 3690, fp32 1858 / 1930: registers that the drop's results are moved through.)
+template <bool WIN> struct QueryStages {
+  int first, near, far;   // the first stage; stages of a head that are near (without a window: all) and far
+  __device__ __forceinline__ QueryStages(const SeqParams& p, int k0, int len, int sr) {
+    first = p.causal ? k0 / sr : 0;
+    near = (key_reach<WIN>(p, len, k0, k0 + 63) + sr - 1) / sr - first;
+    far = 0;
+    if (WIN && k0 < p.sinks && k0 + 64 > p.sinks) {
+      const int all = near;
+      near = (key_reach<WIN>(p, len, p.sinks, k0 + 63) + sr - 1) / sr - first;
+      far = all - near;
+    }
+  }
+};
+
 // ---------------------------------------------------------------------------
 // dK and dV of 64 key rows of one key head.  Wave w owns 16 of them: their K-hat and
 // V rows are operands in registers, dK-hat and dV accumulate in registers over the
@@ -577,23 +599,26 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
     return;
   }
 
-  // stages of a query head, back to the tile's first key when causal; this part's share of all heads'.
-  // Last queries first: every tile of a sequence begins with the same rows, which then come from
-  // L2.  Measured (us, forward and backward, first / last queries first): 16 sequences up to 2048
-  // tokens, 16 heads (4 of keys), D 64 406 / 390, 64 up to 577, 12 143 / 140, 8 x 1024, 8, D 128 159 / 156,
-  // one sequence of 16384 2510 / 2494
-  // (HBM reads of the kernel 1716 / 419 MB).
-  const int first = p.causal ? k0 / SR : 0, per = (key_reach<WIN>(p, tl.len, k0, k0 + 63) + SR - 1) / SR - first;
-  const int64_t all = (int64_t)per * group;
-  const int begin = (int)(all * part / parts), ns = (int)(all * (part + 1) / parts) - begin;
+  // this part's share of all heads' stages, the far ones first; `run` of a head, the last of them `top`
+  const QueryStages<WIN> qs(p, k0, tl.len, SR);
+  const int64_t all = (int64_t)(qs.far + qs.near) * group;
+  const int begin = (int)(all * part / parts), end = (int)(all * (part + 1) / parts);
+  const bool far = WIN && begin < qs.far * group;
+  const int begin_in = WIN && !far ? begin - qs.far * group : begin;   // among the far or near ones
+  int run = far ? qs.far : qs.near, top = qs.first + (far ? qs.far + qs.near : qs.near) - 1;
+  // Stages are numbered from `odd`, 0 or 1, on, so that the first near one behind far ones, `turn`, is even.
+  const int odd = far ? (qs.far * group - begin) & 1 : 0, turn = far ? qs.far * group - begin + odd : 0, ns = end - begin + odd;
   SeqStream<S, D> srcQ, srcG;
   srcQ.lanes(D, wave, lane);
   srcG.lanes(p.gcopy ? D : p.sdo[0], wave, lane);
-  int lh = begin / per - 1, lst = per, cst = begin % per;   // the stage loaded next: head of the group, stage
+  int lh = begin_in / run - 1, lst = run, cst = begin_in % run;   // the stage loaded next: head of the group, stage
+  int from = cst;
   __amdgpu_buffer_rsrc_t rStat = make_rsrc(p.nl, 0u);
+  // (at `turn` the stage before it has been loaded)
   auto load = [&](S* q, S* g, float* l, float* d) __attribute__((always_inline)) {
-    if (lst == per) {
-      lst = lh < begin / per ? cst : 0;
+    if (lst == run) {
+      lst = from;
+      from = 0;
       const int head = kvh * group + ++lh;
       const int64_t hrow = (int64_t)head * p.T + tl.start;
       srcQ.base(static_cast<const S*>(p.qhat) + hrow * D, tl.len);
@@ -601,14 +626,17 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
                         : static_cast<const S*>(p.dout) + tl.start * p.sdo[0] + head * p.sdo[1], tl.len);
       rStat = make_rsrc((wave & 1 ? p.nd : p.nl) + hrow, (unsigned)tl.len * 4u);
     }
-    const int r0 = (first + per - 1 - lst) * SR;
+    const int r0 = (top - lst) * SR;
     srcQ.load(q, wave, r0);
     srcG.load(g, wave, r0);
     // waves 0 and 1 also fetch the stage's -LSE2 and -delta (64 rows, of which SR count)
     if (wave < 2) seq_dma4(rStat, wave ? d : l, (unsigned)lane * 4u, (unsigned)r0 * 4u);
     ++lst;
   };
-  if (ns > 0) load(sQ0, sG0, sL0, sD0);
+  if (end > begin) {
+    if (WIN && odd) load(sQ1, sG1, sL1, sD1);
+    else load(sQ0, sG0, sL0, sD0);
+  }
 
   const int row0 = wave * 16 + lr;   // of the tile
   Frag kf[KS], vf[KS];
@@ -702,13 +730,28 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
       dk[d] = C::mma(at.col(q, d), dsf, dk[d]);
     }
   };
+  auto drop = [&]() __attribute__((always_inline)) {   // the sums of the lane's key, if it is no sink
+    const bool sink = k0 + row0 < p.sinks;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dv[d][i] = sink ? dv[d][i] : 0.f;
+        dk[d][i] = sink ? dk[d][i] : 0.f;
+      }
+  };
   // (cst: this stage within its head)
   auto stage = [&](int st, const S* __restrict__ q, const S* __restrict__ g, const float* __restrict__ l, const float* __restrict__ dl,
                    S* __restrict__ qn, S* __restrict__ gn, float* __restrict__ ln, float* __restrict__ dn) __attribute__((always_inline)) {
     seq_stage_barrier();
+    const int q0 = (top - cst) * SR;
+    cst = cst + 1 == run ? 0 : cst + 1;
+    if (WIN && st + 1 == turn) {   // (cst is 0, lst run)
+      run = lst = qs.near;
+      top = qs.first + qs.near - 1;
+      lh = -1;
+    }
     if (st + 1 < ns) load(qn, gn, ln, dn);
-    const int q0 = (first + per - 1 - cst) * SR;
-    cst = cst + 1 == per ? 0 : cst + 1;
     if (!active || (p.causal && q0 + SR <= w0) || (WIN && q0 >= qlast)) return;
     const bool tail = q0 + SR > qfull || (p.causal && q0 < w0 + 16);
 #pragma unroll
@@ -716,9 +759,11 @@ __global__ void __launch_bounds__(kSeqThreads, (sizeof(S) == 4 || D == 256) ? 1 
       block(tail, q0 + 32 * j, q + 32 * j * D, g + 32 * j * D, l + 32 * j, dl + 32 * j);
   };
   for (int st = 0; st < ns; st += 2) {
-    stage(st, sQ0, sG0, sL0, sD0, sQ1, sG1, sL1, sD1);
+    if (far && st == turn) drop();
+    if (!WIN || st >= odd) stage(st, sQ0, sG0, sL0, sD0, sQ1, sG1, sL1, sD1);
     if (st + 1 < ns) stage(st + 1, sQ1, sG1, sL1, sD1, sQ0, sG0, sL0, sD0);
   }
+  if (far && turn >= ns) drop();
 
   const float up = pow2(-(int)kWeightUp<S>);   // out of P
   if (kt.sums) {   // sums as they are, for seq_join_kernel
@@ -776,23 +821,28 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
     return;
   }
 
-  const int first = p.causal ? k0 / SR : 0, per = (key_reach<WIN>(p, tl.len, k0, k0 + 63) + SR - 1) / SR - first;
-  const int64_t all = (int64_t)per * group;
-  const int begin = (int)(all * part / parts), ns = (int)(all * (part + 1) / parts) - begin;
+  // this part's share of all heads' stages, the far ones first; `run` of a head, the last of them `top`
+  const QueryStages<WIN> qs(p, k0, tl.len, SR);
+  const int64_t all = (int64_t)(qs.far + qs.near) * group;
+  const int begin = (int)(all * part / parts), end = (int)(all * (part + 1) / parts);
+  const bool far = WIN && begin < qs.far * group;
+  const int begin_in = WIN && !far ? begin - qs.far * group : begin;   // among the far or near ones
+  int run = far ? qs.far : qs.near, top = qs.first + (far ? qs.far + qs.near : qs.near) - 1;
+  // Stages are numbered from `odd`, 0 or 1, on, so that the first near one behind far ones, `turn`, is even.
+  const int odd = far ? (qs.far * group - begin) & 1 : 0, turn = far ? qs.far * group - begin + odd : 0, ns = end - begin + odd;
   SeqStream<S, D> srcQ, srcG;
   srcQ.lanes(D, wave, lane);
   srcG.lanes(p.gcopy ? D : p.sdo[0], wave, lane);
-  int head = kvh * group + begin / per - 1, lst = per;   // of the stage loaded next
-  const int start = begin % per;
-  bool fresh = true;
+  int head = kvh * group + begin_in / run - 1, lst = run, cst = begin_in % run;   // of the stage loaded next
+  int from = cst;
   __amdgpu_buffer_rsrc_t rNl = make_rsrc(p.nl, 0u), rNd = make_rsrc(p.nd, 0u), rNg = make_rsrc(p.nd, 0u);
   const int qh = wave & 1, kh = wave >> 1;   // the wave's halves of the queries and keys
   u32x4 nl_next[2], nd_next[2];              // -LSE2 and -delta of queries 32 qh + 16 h + 4 lg + (0..3)
   unsigned ng_next = 0, na_next = 0;         // kFitDs: |dO| and -delta of query `lane`
   auto load = [&](S* q, S* g) __attribute__((always_inline)) {
-    if (lst == per) {
-      lst = fresh ? start : 0;
-      fresh = false;
+    if (lst == run) {
+      lst = from;
+      from = 0;
       ++head;
       const int64_t hrow = (int64_t)head * p.T + tl.start;
       srcQ.base(static_cast<const S*>(p.qhat) + hrow * D, tl.len);
@@ -802,7 +852,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
       rNd = make_rsrc(p.nd + hrow, (unsigned)tl.len * 4u);
       if constexpr (kFitDs<S>) rNg = make_rsrc(p.ng + hrow, (unsigned)tl.len * 4u);
     }
-    const int r0 = (first + per - 1 - lst) * SR;
+    const int r0 = (top - lst) * SR;
     srcQ.load(q, wave, r0);
     srcG.load(g, wave, r0);
     if constexpr (kFitDs<S>) {
@@ -817,7 +867,10 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
     }
     ++lst;
   };
-  if (ns > 0) load(sQ0, sG0);
+  if (end > begin) {
+    if (WIN && odd) load(sQ1, sG1);
+    else load(sQ0, sG0);
+  }
 
   Frag kf[2][KS], vf[2][KS];   // key 32 kh + 16 u + lr
   float vmax = 0.f;            // kFitDs: the largest |V_j| of the tile
@@ -883,7 +936,20 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
   for (int u = 0; u < 2; ++u) qend[u] = key_reach<WIN>(p, tl.len, k0 + 32 * kh + 16 * u + lr, k0 + 32 * kh + 16 * u + lr);
   // ... some of the tile's keys
   const int qfull = WIN ? k0 + 64 <= p.sinks ? tl.len : key_reach<WIN>(p, tl.len, p.sinks > k0 ? p.sinks : k0, k0) : tl.len;
-  int cst = start;   // this stage within its head
+  auto drop = [&]() __attribute__((always_inline)) {   // the sums of keys that are no sinks
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool sink = k0 + 16 * u + lr < p.sinks;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          dv[u][d][i] = sink ? dv[u][d][i] : 0.f;
+          dk[u][d][i] = sink ? dk[u][d][i] : 0.f;
+        }
+    }
+  };
+  // (cst: this stage within its head)
   auto stage = [&](int st, const S* __restrict__ q, const S* __restrict__ g, S* __restrict__ qn, S* __restrict__ gn)
       __attribute__((always_inline)) {
     seq_stage_barrier();
@@ -906,9 +972,14 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
         fit = pow2(ex);
       }
     }
+    const int q0 = (top - cst) * SR;
+    cst = cst + 1 == run ? 0 : cst + 1;
+    if (WIN && st + 1 == turn) {   // (cst is 0, lst run)
+      run = lst = qs.near;
+      top = qs.first + qs.near - 1;
+      head = kvh * group - 1;
+    }
     if (st + 1 < ns) load(qn, gn);
-    const int q0 = (first + per - 1 - cst) * SR;
-    cst = cst + 1 == per ? 0 : cst + 1;
     const bool tail = q0 + SR > qfull || (p.causal && q0 < k0 + 64);   // uniform
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -961,9 +1032,11 @@ __global__ void __launch_bounds__(kSeqThreads, 2) seq_dkdv_shared_kernel(const S
     }
   };
   for (int st = 0; st < ns; st += 2) {
-    stage(st, sQ0, sG0, sQ1, sG1);
+    if (far && st == turn) drop();
+    if (!WIN || st >= odd) stage(st, sQ0, sG0, sQ1, sG1);
     if (st + 1 < ns) stage(st + 1, sQ1, sG1, sQ0, sG0);
   }
+  if (far && turn >= ns) drop();
 
   // lane holds key 16 u + lr, channels 16 (d0 + d) + 4lg + (0..3)
   const float up = pow2(-(int)kWeightUp<S>);   // out of P

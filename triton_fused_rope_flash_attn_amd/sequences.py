@@ -407,9 +407,8 @@ def sdpa_rope_varlen(
     The first start counts as 0, the others are cut to 0 .. T; where they do not ascend,
     the rows concerned hold no defined values.
     causal: token i of a sequence sees its tokens 0 .. i, else all of them.  What it does not
-    see does not reach O, infinities and NaN included.  (Gradients: an infinity or NaN of Q,
-    K or dO within 63 tokens of a row that has no part in it, with a window within 126 of what it sees,
-    may reach it as 0 * NaN.)
+    see does not reach O, infinities and NaN included.  (Gradients: an infinity or NaN of Q, K or dO may reach
+    a row that it has no part in as 0 * NaN, if it is within 63 tokens of one that has, with a window within 126.)
     window, sinks: of the tokens 0 .. i, token i sees the last ``window`` (at least 1: itself) and those
     below ``sinks`` alone (causal only; without a window ``sinks`` makes no difference).
     positions: int32 ``[T]`` table rows, instead of ``i - has_cls``.
