@@ -248,6 +248,27 @@ def test_nothing_that_is_not_seen_reaches_a_row(dtype, D):
                     at += m
 
 
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (F32, 32), (BF16, 256), (F32, 256)])
+def test_nan_queries_give_nan(dtype, D):
+    """Of the tokens whose queries they are, and of no others, however many workers share their rows."""
+    page, lens, new = 16, [500, 3, 700], [4, 2, 40]
+    table = seq_ref.Table(800, D, DEV)
+    for per in (48, 20, 120):
+        pages, n = page_table(3, per)
+        kc, vc = caches(n, page, 2, D, dtype)
+        q = randn(sum(new), 4, D, dtype=dtype, seed=3)
+        bad = q.clone()
+        rows = [1, 5, 9, 44]
+        bad[rows] = float("nan")
+        sees, _ = draft(new, 7)
+        for kw in ({}, dict(tree=sees)):
+            want = sdpa_rope_tree(q, kc, vc, table, pages, ints(lens), starts(new), **kw)
+            got = sdpa_rope_tree(bad, kc, vc, table, pages, ints(lens), starts(new), **kw)
+            rest = [i for i in range(sum(new)) if i not in rows]
+            assert torch.equal(got[rest], want[rest])
+            assert torch.isnan(got[rows]).all()
+
+
 def test_infinite_values_of_light_rows():
     """An infinite value whose weight is 2^-200 of the largest is infinite in O all the same."""
     page, D = 16, 64

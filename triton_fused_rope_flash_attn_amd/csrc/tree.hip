@@ -542,12 +542,14 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
       } else if (row < rows) {
         // (the first piece of a share and its last one: no other piece is a part of a tile)
         const int64_t at_row = ((int64_t)(2 * worker + which) * p.Hkv + kvh) * ROWS + row;
-        if (m_run[t] > -INFINITY) {
+        // (a maximum passes over NaN: a row whose logits are all NaN has sums all the same, NaN as its weights')
+        const float m = m_run[t] == -INFINITY && magnitude_bits(l) > kInfBits ? 0.f : m_run[t];
+        if (m > -INFINITY) {
 #pragma unroll
           for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.sums + at_row * D + 16 * d + 4 * lg) = acc[t][d];
         }
         if (lg == 0) {
-          p.stats[2 * at_row] = m_run[t];
+          p.stats[2 * at_row] = m;
           p.stats[2 * at_row + 1] = l;
         }
       }
