@@ -269,6 +269,23 @@ def test_nan_queries_give_nan(dtype, D):
             assert torch.isnan(got[rows]).all()
 
 
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (F32, 32), (BF16, 256)])
+def test_rows_that_see_nothing_feel_nothing(dtype, D):
+    """Zeros, whatever the new tokens' rows hold, and on pages that are none."""
+    page, lens, new = 16, [0, 0, 30], [6, 70, 4]
+    table = seq_ref.Table(120, D, DEV)
+    for per in (7, 80):
+        pages, n = page_table(3, per)
+        kc, vc = (torch.full((n, page, 2, D), x, dtype=dtype, device=DEV) for x in (float("nan"), float("inf")))
+        q = randn(sum(new), 4, D, dtype=dtype, seed=3)
+        tree = torch.zeros(sum(new), 70, dtype=torch.bool, device=DEV)
+        got = sdpa_rope_tree(q, kc, vc, table, pages, ints(lens), starts(new), tree=tree)
+        assert (got[:76] == 0).all()
+        pages[2] = -1
+        got = sdpa_rope_tree(q, kc, vc, table, pages, ints(lens), starts(new), tree=tree)
+        assert (got == 0).all()
+
+
 def test_infinite_values_of_light_rows():
     """An infinite value whose weight is 2^-200 of the largest is infinite in O all the same."""
     page, D = 16, 64

@@ -508,6 +508,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
       const float l = group4_sum(l_run[t]);
       if (whole) {
         const float inv = l > 0.f ? 1.f / l : 0.f;
+        const bool none = magnitude_bits(l) == 0;   // the row sees nothing: 0, whatever V holds in rows that it does not see
         const int j = (r0 + row) / group, h = kvh * group + (r0 + row) % group;
         S* const o = static_cast<S*>(p.o) + ((int64_t)(s.start + j) * p.H + h) * D;
 #pragma unroll
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
           if constexpr (sizeof(S) == 4) {
 #pragma unroll
             for (int d = d0; d < d0 + 2; ++d) {
-              const f32x4 x = acc[t][d] * inv;
+              const f32x4 x = none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[t][d] * inv;
               if (row < rows) *reinterpret_cast<f32x4*>(o + 16 * d + 4 * lg) = x;
             }
           } else {
@@ -526,7 +527,7 @@ __global__ void __launch_bounds__(kSeqThreads, D * sizeof(S) <= 256 ? 2 : 1) tre
               typedef S s4 __attribute__((ext_vector_type(4)));
               s4 a;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) a[e] = (S)(acc[t][d0 + k][e] * inv);
+              for (int e = 0; e < 4; ++e) a[e] = (S)(none ? 0.f : acc[t][d0 + k][e] * inv);
               __builtin_memcpy(&w[k], &a, 8);
             }
             u32x4 x;
