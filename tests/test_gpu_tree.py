@@ -476,6 +476,18 @@ def test_another_stream():
     assert all(torch.equal(x, want) for x in got)
 
 
+def test_more_rows_than_a_join_could_take():
+    """2^28 query rows and more over short tables, where nothing is joined."""
+    B, m, H, page, D = 16384, 257, 64, 64, 32
+    kc, vc = caches(8, page, 1, D, BF16)
+    table, q = seq_ref.Table(1024, D, DEV), randn(1, H, D, dtype=BF16, seed=3)
+    pages, lengths = ints([[3, 1, 4, 0, 5]]).expand(B, 5), ints([40] * B)
+    got = sdpa_rope_tree(q.expand(B * m, H, D), kc, vc, table, pages, lengths, torch.arange(B + 1, dtype=torch.int32, device=DEV) * m)
+    want = run("one of many", q.expand(m, H, D), kc, vc, table, pages[:1], lengths[:1], ints([0, m]))
+    for b in (0, 1, B // 2 + 1, B - 1):
+        assert torch.equal(got[b * m:(b + 1) * m], want), b
+
+
 def test_cache_past_32_bits():
     Hkv, D, page = 8, 128, 64
     n = (1 << 31) // (Hkv * D * page) + 3

@@ -654,8 +654,9 @@ int farope_tree(const farope_seq_desc* desc, const void* q, const int64_t q_stri
   p.page_mul = (uint32_t)(((uint64_t(1) << (31 + l)) / (uint64_t)cache->page_rows + 1));
   p.page_shift = 31 + l;
   p.rows = tree_rows(desc);
-  // (rows of a key head in 32 bits, with a tile's more; workgroups of the join: 16 rows each)
-  if ((int64_t)p.T * p.H > INT32_MAX - 256 || tree_slots(desc) * p.Hkv * (p.rows / 16) > kMaxWorkgroups) return FAROPE_ERR_SHAPE;
+  // (rows of a key head in 32 bits, with a tile's more; workgroups: a tile each, and in the join 16 rows each)
+  const int64_t join = w.total ? p.rows / 16 : 1;
+  if ((int64_t)p.T * p.H > INT32_MAX - 256 || tree_slots(desc) * p.Hkv * join > kMaxWorkgroups) return FAROPE_ERR_SHAPE;
   p.slots = (int)tree_slots(desc);
   p.workers = tree_workers(desc, cache);
   p.direct = w.total == 0;
