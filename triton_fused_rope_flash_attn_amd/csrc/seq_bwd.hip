@@ -1182,7 +1182,7 @@ static hipError_t bwd(const SeqParams& p0, hipStream_t st) {
     e = launch_seq_prep(p, std::is_same<S, bf16>::value ? DT_BF16 : std::is_same<S, f16>::value ? DT_F16 : DT_F32, D, true, st);
     if (e != hipSuccess) return e;
     if constexpr (sizeof(S) == 2)
-      e = seq_tile_rows(p.T, p.B, p.H, D, false, p.window) == 128 ? dq<S, D, 2, false>(p, st) : dq<S, D, 1, false>(p, st);
+      e = seq_tile_rows(p.T, p.B, p.H, D, false) == 128 ? dq<S, D, 2, false>(p, st) : dq<S, D, 1, false>(p, st);
     else
       e = dq<S, D, 1, false>(p, st);
   } else if constexpr (D <= 128) {

@@ -420,7 +420,7 @@ static hipError_t fwd_rows(const SeqParams& p, hipStream_t st) {
   if constexpr (D <= 128)
     if (!p.khat) return fwd<S, D, 1, true>(p, st);
   if constexpr (sizeof(S) == 2)
-    if (seq_tile_rows(p.T, p.B, p.H, D, false, p.window) == 128) return fwd<S, D, 2, false>(p, st);
+    if (seq_tile_rows(p.T, p.B, p.H, D, false) == 128) return fwd<S, D, 2, false>(p, st);
   return fwd<S, D, 1, false>(p, st);
 }
 template <typename S>

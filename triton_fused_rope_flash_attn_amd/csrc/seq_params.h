@@ -64,7 +64,7 @@ inline int64_t seq_slots(int T, int B, int lb) { return (int64_t)(T >> lb) + B +
 // 235 / 214, 4 x 2048, 8 [512] 34.8 / 36.3.  D 256, forward and backward: 2 x 4096, 8 [512] 1242 / 1173, 16 x
 // 512, 8 [512] 333 / 331, 4 x 1024, 8 [256] 268 / 302, 64 up to 200 (77), 12 [462] 296 / 368, 125 up to 149 (54),
 // 8 [423] 292 / 365.
-inline int seq_tile_rows(int T, int B, int H, int D, bool f32, int window) {
+inline int seq_tile_rows(int T, int B, int H, int D, bool f32) {
   const int64_t tiles = (int64_t)T * H / 128, mean = T / B;
   if (f32) return 64;
   if (D == 256) return tiles >= 2 * 256 && mean >= 256 ? 128 : 64;

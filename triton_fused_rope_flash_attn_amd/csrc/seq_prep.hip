@@ -73,7 +73,7 @@ template <typename S, int D>
 static hipError_t prep(const SeqParams& p, bool backward, hipStream_t st) {
   SeqMaps m{};
   m.order = seq_order(p.T, p.B, D, p.causal, p.window);
-  m.lb_q = seq_tile_rows(p.T, p.B, p.H, D, sizeof(S) == 4, p.window) == 128 ? 7 : 6;
+  m.lb_q = seq_tile_rows(p.T, p.B, p.H, D, sizeof(S) == 4) == 128 ? 7 : 6;
   m.slots_q = (int)seq_slots(p.T, p.B, m.lb_q);
   m.slots_k = backward ? (int)seq_slots(p.T, p.B, 6) : 0;
   m.blocks = (m.slots_q + m.slots_k + 3) / 4;
