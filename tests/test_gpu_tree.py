@@ -9,7 +9,7 @@ import torch
 
 from tests import seq_ref
 from tests._report import LINES
-from triton_fused_rope_flash_attn_amd import (rope_cache_accept, rope_cache_append, sdpa_rope_decode, sdpa_rope_tree,
+from triton_fused_rope_flash_attn_amd import (rope_cache_accept, rope_cache_append, rope_cache_fork, sdpa_rope_decode, sdpa_rope_tree,
                                               sdpa_rope_varlen)
 
 pytestmark = pytest.mark.gpu
@@ -510,3 +510,33 @@ def test_op_passes_opcheck():
     torch.library.opcheck(torch.ops.farope.cache_tree.default, (*args, None, ints([0] * 5), True, 0.125))
     with pytest.raises(RuntimeError, match="no autograd formula"):
         sdpa_rope_tree(q.requires_grad_(), kc, vc, table, *args[5:]).sum().backward()
+
+
+def test_compiled_steps():
+    """Append, tree, accept, fork and windowed decode as one compiled graph, against the same calls."""
+    page, D = 16, 64
+    table = seq_ref.Table(200, D, DEV)
+    new, lens = [4, 6], [30, 3]
+    sees, depths = draft(new, 3)
+    positions = ints([x + d - 1 for x, row in zip(lens, depths) for d in row])
+    q, k, v = (randn(sum(new), h, D, dtype=BF16, seed=s) for s, h in enumerate((4, 2, 2)))
+    path, parents, room = ints([[0, 2, -1], [1, 3, 5]]), ints([1, 1]), ints([20, 5])
+
+    def step(kc, vc, pages, lengths, refs, cu):
+        rope_cache_append(k, v, table, kc, vc, pages, lengths, cu_seqlens=cu, positions=positions)
+        out = sdpa_rope_tree(q, kc, vc, table, pages, lengths, cu, tree=sees, positions=positions)
+        chain = sdpa_rope_tree(q, kc, vc, table, pages, lengths, cu)
+        lengths.copy_(rope_cache_accept(kc, vc, pages, lengths, path))
+        missing = rope_cache_fork(kc, vc, pages, lengths, refs, parents, room=room)
+        one = sdpa_rope_decode(q[:2], kc, vc, table, pages, lengths, window=9, sinks=2)
+        return out, chain, missing, one
+
+    results = []
+    for fn in (step, torch.compile(step, fullgraph=True, backend="aot_eager")):
+        kc, vc = caches(20, page, 2, D, BF16)
+        state = (kc, vc, ints([[3, 1, 7, -1, -1], [2, 0, -1, -1, -1]]), ints(lens), ints([1, 1, 1, 1, 0, 0, 0, 1] + [0] * 12), starts(new))
+        results.append((*fn(*state), *state))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    # (both go on from place 1, 6 rows of one page: the first keeps it and room for 26 rows, the other copies it)
+    assert results[0][7].tolist() == [6, 6] and results[0][6].tolist() == [[2, 0, -1, -1, -1], [4, -1, -1, -1, -1]]
