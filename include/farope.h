@@ -386,7 +386,8 @@ int farope_cache_append(const farope_seq_desc* desc, const void* k, const int64_
 
 /* O [B, heads, D] of one query per sequence (tokens = seqs) over the lengths[b] rows of its
  * cache, the last of which is its own: q is rotated by row lengths[b] - 1 - has_cls, or by
- * positions [B].  A sequence with no rows in the cache has O = 0.  desc: causal is not read.
+ * positions [B].  A length past the page table counts as the table's rows.  A sequence with no rows in the
+ * cache has O = 0.  desc: causal is not read.
  * ws: farope_decode_workspace_elems fp32 elements (unnormalised rows of sequences that several
  * workgroups share; 0 where none are), 16-byte aligned. */
 size_t farope_decode_workspace_elems(const farope_seq_desc* desc, const farope_cache_desc* cache);

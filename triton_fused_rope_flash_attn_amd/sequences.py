@@ -489,8 +489,8 @@ def sdpa_rope_decode(
     How the rows are divided goes by the page table's width (lengths stay on the GPU): for short
     sequences a view of its first columns, as many as they need, is faster.
 
-    Returns O ``[B, H, D]``.  A sequence without rows has O = 0; rows past the page table
-    or on a page number that is no page of the cache are left out.  No gradients.
+    Returns O ``[B, H, D]``.  A sequence without rows has O = 0; a length past the page table counts as
+    the table's rows, and rows on a page number that is no page of the cache are left out.  No gradients.
     """
     cosp, sinp = _tables(cos_sin)
     args = (Q, k_cache, v_cache, cosp, sinp, page_table, lengths, positions, has_cls, _scale(Q.shape[-1]))
@@ -523,6 +523,10 @@ def sdpa_rope_tree(
     Q is rotated by table row ``lengths[b] + j - has_cls`` for the j-th token, or by positions[t] (int32
     ``[T]``): a tree's tokens take the rows of their depths, so that accepted ones (``rope_cache_accept``)
     are where a chain would have put them.
+
+    bf16 and fp16: the rotated Q and the softmax weights are rounded to their type for the products, as in
+    ``sdpa_rope_varlen``; ``sdpa_rope_decode`` keeps more of both, so a token's O may differ from its there by
+    about the type's rounding.
 
     Returns O ``[T, H, D]``.  A token that sees no row has O = 0, and so have tokens behind the last
     sequence and those of a sequence of negative length; rows past the page table or on a page number that is no page
