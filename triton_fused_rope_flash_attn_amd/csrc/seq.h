@@ -64,9 +64,10 @@ constexpr float kSeqSlack = 8.0f;
 
 // ---------------------------------------------------------------------------
 // Streamed tiles: rows of D elements, unpadded, their 16-byte chunks XOR-swizzled
-// per row with period 16 (as in stream.h: 16-byte reads of 16 rows and the
-// transposed reads are free of bank conflicts).  A stage holds SR rows; a
-// 16-byte-per-lane load to LDS fills RPI of them.
+// per row with period 16, as in stream.h.  Rows of 128 bytes: 16-byte reads of 16 rows and the
+// transposed reads are free of bank conflicts.  Rows of 256: SQ_LDS_BANK_CONFLICT counts 4 cycles more than the 4
+// of a 16-byte read in a row, 2 for a transposed one (a loop of such reads alone takes as long as one of reads in a row, 14
+// cycles each).  A stage holds SR rows; a 16-byte-per-lane load to LDS fills RPI of them.
 // ---------------------------------------------------------------------------
 template <typename S, int D> constexpr int kStageRowsOf = D * sizeof(S) <= 256 ? 64 : 32;
 template <typename S, int D, int ROWS = kStageRowsOf<S, D>> struct Tile {

@@ -159,7 +159,10 @@ bool rotates_itself(const farope_seq_desc* d, bool v_streams) {
 // Key tiles with sinks, which every later query sees: where that is more than half as much again as other tiles have,
 // parts of their queries of 8 stages, or of a workgroup's for other tiles where these are fewer (0: they are not
 // divided).  Measured (us, forward and backward of 16384 tokens, 8 heads, 2 of keys, D 128, window 1024, 4 sinks):
-// parts as large as the other workgroups' and at the launch's front 504, of 16 stages and at its end 473, of 8 450.
+// parts as large as the other workgroups' and at the launch's front 504, of 16 stages and at its end 473, of 8 450.  Undivided / divided,
+// the sinks' tile having r times the others' stages: 8 x 2048, 32 heads, 8 of keys, D 128, window 512 [r 3.3] 1157 / 1017, 1024 [1.8]
+// 1392 / 1301, 1300 [1.5] 1512 / 1515, 1536 [1.3] 1550 / 1576; 2 x 4096, 16, 4 of keys, D 64, 1024 [3.6] 307 / 263, 2048 [1.9] 335 / 338, 3000
+// [1.3] 396 / 405; one of 16384, 8, 2 of keys, D 128, few workgroups, 12000 [1.4] 3220 / 2657.
 // No more parts than one resident round of workgroups: many tiles fill the chip by themselves, and each part has its sums,
 // 2 * 64 * D in fp32, in the workspace, 32 MB of them at most.  Measured (us, one round / two / four / no such bound; 32 heads, 8 of
 // keys, D 128): 16384 tokens, window 1024, 4 sinks 1557 / 1554 / 1555 / 1551, 1024 2501 / 2535 / 2588 / 3072, 4096 4970 / 5026 /
@@ -440,8 +443,10 @@ int tree_stage(const farope_seq_desc* d) { return d->head_dim * elem_size(d->dty
 bool tree_direct(const farope_seq_desc* d, const farope_cache_desc* c) {
   return (int64_t)c->max_pages * c->page_rows <= 512;
 }
-// Workgroups of a key head: one resident round.  Measured, us with half of it, all, two (32 heads of 8, D 128, bf16): 8
-// sequences of 4096 rows, 16 new tokens 50, 48, 61; 32 of 8192, 32 new 264, 259, 289.
+// Workgroups of a key head: two a CU, one for rows of more than 256 bytes; that is one resident round from D 64 on.  Measured, us with half
+// of it, all, two (32 heads of 8, D 128, bf16): 8 sequences of 4096 rows, 16 new tokens 50, 48, 61; 32 of 8192, 32 new 264, 259, 289.
+// At D 32 a CU holds three and four; with two, three, four: 32 of 4096, 16 new 53.8, 55.0, 59.2, 8 of 4096 26.5, 29.0, 26.7, 4 of 8192,
+// 512 new, fp16 142.8, 142.7, 139.6.
 int tree_workers(const farope_seq_desc* d, const farope_cache_desc* c) {
   const int64_t room = ((int64_t)c->max_pages * c->page_rows + tree_stage(d) - 1) / tree_stage(d);
   const int64_t wgs = (int64_t)kCus * (d->head_dim * elem_size(d->dtype) <= 256 ? 2 : 1);

@@ -11,9 +11,10 @@
 //   seq_dkdv_kernel   key tiles: dK, dV, one pass over the group's query heads, so the
 //                     sums of shared key heads stay in registers and in one order
 // With a window (WIN) a key tile's queries end with its last key's window, but for tiles with sinks, whose queries
-// are divided (KeyTile) and joined by sink_join_kernel; and rows that see 64 keys at most, which may be anywhere, have their
-// delta from a pass of its own over the tile's keys (two of its four products: one of 16384 tokens, 8 heads, D 128, window
-// 1024: dQ 166 us, dK/dV 218).
+// are divided (KeyTile), joined by sink_join_kernel and taken in an order of their own (QueryStages); and rows that see 64 keys at most,
+// which may be anywhere, have their delta from a pass of its own over the tile's keys (two of its four products).  One of 16384
+// tokens, 8 heads, 2 of keys, D 128, 4 sinks, window 1024: dQ 163 us, dK/dV 216; the whole step with window 20, all rows with that
+// pass, 213, with 64, none but the first tile's, 203.
 // Both tile kernels stream their rows as the forward does (seq_fwd.hip).  No row of a
 // sequence reads another's: streams end at the sequence's last row.
 //

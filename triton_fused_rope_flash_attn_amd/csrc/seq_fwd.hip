@@ -10,8 +10,8 @@
 // such pass: the workgroups rotate K themselves.
 //
 // With a window (WIN) a tile reads the stages that hold sinks and those of its rows' windows (KeyStages in seq.h), and a
-// row may see no key of its first stages: one of 16384 tokens, 8 heads, D 128, window 1024 115 us, 16 up to 4096,
-// 16 heads, D 128, window 512 187 with K-hat's pass.
+// row may see no key of its first stages: one of 16384 tokens, 8 heads, D 128, window 1024 113 us, 16 up to 4096,
+// 16 heads, D 128, window 512 186 with K-hat's pass.
 //
 // Bound by the issue of matrix and vector instructions, which overlap between a SIMD's waves:
 // one sequence of 16384 tokens, 8 heads, D 128, causal 540 us (1020 TFLOP/s; matrix instructions run

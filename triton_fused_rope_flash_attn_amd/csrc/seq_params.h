@@ -55,7 +55,7 @@ inline int64_t seq_slots(int T, int B, int lb) { return (int64_t)(T >> lb) + B +
 
 // Rows per workgroup of the forward and of dQ, 128 (two 16-row subtiles per wave) or 64.  Two
 // subtiles halve the LDS reads per product, but cost workgroups, and products above the
-// diagonal.  ("24 up to 2048": here and beside the kernels lengths drawn down to a 16th of the longest, on a
+// diagonal.  (The same rule with a window.)  ("24 up to 2048": here and beside the kernels lengths drawn down to a 16th of the longest, on a
 // logarithmic scale; these have a mean of 943.)  16-bit tensors; measured (us, forward and backward, 64 / 128 rows; "sequences x
 // tokens, heads" and the call's 128-row tiles), D 128: 24 up to 2048, 16 [2828] 916 / 869, 1 x 16384, 8
 // [1024] 2702 / 2512, 4 up to 4096, 8 [676] 455 / 484, 1 x 4096, 16 [512] 422 / 467, 8 x 1024, 8 [512]
@@ -162,7 +162,9 @@ struct TreeParams {
   int direct;            // a workgroup a slot: nothing is joined
   float c2;
 };
-constexpr int kTreeLeast = 2;   // stages of a worker's share at least
+// Stages of a worker's share at least.  Measured, us with 1, 2, 4 (8 new tokens): 12 heads, D 64, one sequence of 600 rows 14.7, 14.3,
+// 14.0, of 1024 16.4, 15.0, 14.8, of 4096 21.2, 21.3, 17.3; two of 1000, 16 new, 8 heads of 2, D 128, fp32 29.1, 25.5, 26.6.
+constexpr int kTreeLeast = 2;
 hipError_t launch_tree(const TreeParams& p, int dt, int D, hipStream_t st);
 
 // Rows and pages of a cache that are there (cache_pages.hip).  Rows are copied as bytes: es per

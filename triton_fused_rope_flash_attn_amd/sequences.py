@@ -517,7 +517,7 @@ def sdpa_rope_tree(
     cu_seqlens and positions).  Q: ``[T, H, D]`` of the cache's dtype, any strides, packed as
     cu_seqlens (int32 ``[B + 1]``) says; caches and page_table as in ``rope_cache_append``;
     lengths: int32 ``[B]``, the rows of each sequence's cache before the new tokens.
-    tree: bool ``[T, columns]``, rows contiguous: token t sees the i-th new token of its sequence where ``tree[t, i]``
+    tree: bool ``[T, columns]``, rows contiguous, less than 2 GiB with what lies between them: token t sees the i-th new token of its sequence where ``tree[t, i]``
     (its ancestors and itself), and every row before them; without it the new tokens up to itself.  What it does not
     see does not reach O, infinities and NaN included.
     Q is rotated by table row ``lengths[b] + j - has_cls`` for the j-th token, or by positions[t] (int32
