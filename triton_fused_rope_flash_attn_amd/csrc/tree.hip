@@ -18,8 +18,11 @@
 // products 122); 4 up to 8192 with up to 1024 new tokens, fp16 330 (670 TFLOP/s; without 205); one of 1024
 // with 8, 12 heads, D 64 14.6, the chain of lengths, page numbers, rows and the join.
 //
-// 16-bit tensors: q-hat (with the scale) and P are rounded once to their type, as the products' operands; with O's own
-// rounding that leaves 2.8e-3 of O's norm in bf16 (the storing alone 1.7e-3).
+// 16-bit tensors: q-hat (with the scale) and P are rounded once to their type, as the products' operands, as in the forward over
+// packed sequences; with O's own rounding that leaves 2.8e-3 of O's norm in bf16 (the storing alone 1.7e-3).  As pairs of values, as
+// in decode.hip, where a step has 16 rows a key head: P alone 2.4e-3, q-hat alone 2.2e-3, both 1.7e-3; us, one / P / q-hat / both: the
+// three calls above 150 / 156 / 156 / 163, 325 / 439 / 388 / 497, 14.7 / 14.8 / 14.8 / 15.0; 32 of 8192 with 32 new tokens 243 / both 322, 32 of
+// 4096 with 16, D 64 64 / 70 / 68 / 75, 8 of 4096 with 32, 16 heads of 4, D 256 93 / 101 / 149 / 155.
 #include <type_traits>
 
 #include "seq.h"
