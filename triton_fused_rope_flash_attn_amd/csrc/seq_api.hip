@@ -165,7 +165,7 @@ bool rotates_itself(const farope_seq_desc* d, bool v_streams) {
 // [1.3] 396 / 405; one of 16384, 8, 2 of keys, D 128, few workgroups, 12000 [1.4] 3220 / 2657.
 // No more parts than one resident round of workgroups: many tiles fill the chip by themselves, and each part has its sums,
 // 2 * 64 * D in fp32, in the workspace, 32 MB of them at most.  Measured (us, one round / two / four / no such bound; 32 heads, 8 of
-// keys, D 128): 16384 tokens, window 1024, 4 sinks 1557 / 1554 / 1555 / 1551, 1024 2501 / 2535 / 2588 / 3072, 4096 4970 / 5026 /
+// keys, D 128): 16384 tokens, window 1024, 4 sinks 1557 / 1554 / 1555 / 1551, 1024 2501 / 2535 / 2588 / 3070, 4096 4970 / 5026 /
 // 5096 / 7575; 32 x 4096, window 512, 256 sinks 9416 / 9470 / 9211 / 10230, 2048 18200 / 18200 / 18240 / 28000; 64 x 1024, 8 heads, D 64,
 // window 64, 4 sinks 473 / 481 / 491 / 492.
 constexpr int kMaxSinkParts = 128;
