@@ -180,9 +180,9 @@ int sink_parts(const farope_seq_desc* d, Window win) {
   if (n > kMaxSinkParts) n = kMaxSinkParts;
   const int64_t tiles = (int64_t)d->seqs * sink_tiles(win) * d->kv_heads;
   if (n > dkdv_resident(d) / tiles) n = dkdv_resident(d) / tiles;
-  // (and where the launches do not hold them: sink_join_kernel has a workgroup a token of these tiles)
+  // (and none where the launch does not hold them; sink_join_kernel has 64 workgroups a tile, of which there are few here)
   const int64_t others = seq_slots(d->tokens, d->seqs, 6) * d->kv_heads * window_parts(d, win);
-  return n < 2 || 64 * tiles > kMaxWorkgroups || others + tiles * n > kMaxWorkgroups ? 0 : (int)n;
+  return n < 2 || others + tiles * n > kMaxWorkgroups ? 0 : (int)n;
 }
 int64_t sink_workgroups(const farope_seq_desc* d, Window win) {
   return (int64_t)d->seqs * sink_tiles(win) * sink_parts(d, win) * d->kv_heads;
